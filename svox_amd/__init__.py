@@ -2,10 +2,12 @@
 
 Use it where `import svox` was used:  `import svox_amd as svox`.
 """
+from .decoder import gated_ffn, layer_norm
 from .formats import DataFormat, LocalIndex, NDCConfig, Rays
 from .renderer import VolumeRenderer
 from .tree import N3Tree
 from .view import N3TreeView
 
 __version__ = "0.1.0"
-__all__ = ["N3Tree", "N3TreeView", "VolumeRenderer", "NDCConfig", "Rays", "LocalIndex", "DataFormat"]
+__all__ = ["N3Tree", "N3TreeView", "VolumeRenderer", "NDCConfig", "Rays", "LocalIndex", "DataFormat",
+           "layer_norm", "gated_ffn"]

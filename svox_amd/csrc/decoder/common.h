@@ -1,0 +1,135 @@
+// common.h -- scalar types, the matrix-core forms they take, activations and small helpers of the leaf-decoder kernels.
+//
+// The matrix cores multiply 16-bit operands and add in 32 bits.  bfloat16 and float16 go in as they are (one "plane").  A
+// float32 number goes in as three bfloat16 numbers whose sum it is to within 2^-25 of itself,
+//     hi = round(x),  mid = round(x - hi),  lo = round(x - hi - mid)      (8 significant bits each, signs of their own),
+// and a product of two of them as the six products of planes whose weights are at least 2^-16 of the whole,
+//     hi*hi' + hi*mid' + mid*hi' + hi*lo' + lo*hi' + mid*mid';
+// what is left out is below 2^-24 of the product, as much as a 32-bit multiplication rounds away.  Six bfloat16 products cost
+// 6/16 of what the 32-bit matrix instructions cost.  (Infinite inputs give NaN: inf - inf in the second plane.)
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace svox_decoder {
+
+typedef unsigned short u16;
+typedef u16 u16x4 __attribute__((ext_vector_type(4)));
+typedef u16 u16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+typedef __bf16 Bf16;
+typedef _Float16 F16;
+
+constexpr int kWave = 64;
+
+// ---- a type's planes
+template <class T>
+struct Form;
+template <>
+struct Form<Bf16> {
+    static constexpr int planes = 1;
+    static __device__ f32x4 mma(u16x8 a, u16x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ void split(f32x4 v, u16x4* out) { out[0] = __builtin_bit_cast(u16x4, __builtin_convertvector(v, bf16x4)); }
+    static __device__ u16 one() { return 0x3f80; }
+};
+template <>
+struct Form<F16> {
+    static constexpr int planes = 1;
+    static __device__ f32x4 mma(u16x8 a, u16x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ void split(f32x4 v, u16x4* out) { out[0] = __builtin_bit_cast(u16x4, __builtin_convertvector(v, f16x4)); }
+    static __device__ u16 one() { return 0x3c00; }
+};
+template <>
+struct Form<float> {
+    static constexpr int planes = 3;
+    static __device__ f32x4 mma(u16x8 a, u16x8 b, f32x4 c) { return Form<Bf16>::mma(a, b, c); }
+    static __device__ void split(f32x4 v, u16x4* out) {
+        for (int p = 0; p < 3; ++p) {
+            const bf16x4 part = __builtin_convertvector(v, bf16x4);
+            out[p] = __builtin_bit_cast(u16x4, part);
+            if (p < 2) v -= __builtin_convertvector(part, f32x4);
+        }
+    }
+    static __device__ u16 one() { return 0x3f80; }
+};
+
+// the product of two fragments, all planes: the small products first
+template <class T>
+__device__ __forceinline__ f32x4 multiply(const u16x8 (&a)[Form<T>::planes], const u16x8 (&b)[Form<T>::planes], f32x4 c) {
+    if constexpr (Form<T>::planes == 3) {
+        c = Form<T>::mma(a[1], b[1], c);
+        c = Form<T>::mma(a[0], b[2], c);
+        c = Form<T>::mma(a[2], b[0], c);
+        c = Form<T>::mma(a[0], b[1], c);
+        c = Form<T>::mma(a[1], b[0], c);
+    }
+    return Form<T>::mma(a[0], b[0], c);
+}
+
+// ---- a few values of a row at any alignment of the type's own
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Few {
+    typedef T vector __attribute__((ext_vector_type(N)));
+    vector v;
+};
+template <class T, int N>
+__device__ __forceinline__ typename Few<T, N>::vector load_few(const T* at) {
+    return reinterpret_cast<const Few<T, N>*>(at)->v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_few(T* at, typename Few<T, N>::vector v) {
+    reinterpret_cast<Few<T, N>*>(at)->v = v;
+}
+
+// ---- activations
+enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
+
+// exp and the reciprocal: for results that are rounded to 16 bits the hardware's, good to 22 bits
+template <bool accurate>
+__device__ __forceinline__ float sigmoid(float g) {
+    if constexpr (accurate) return 1.0f / (1.0f + expf(-g));
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+}
+// act(g); slope: its derivative too
+template <bool accurate>
+__device__ __forceinline__ float activate(int activation, float g, float* slope) {
+    switch (activation) {
+        case kSilu: {
+            const float s = sigmoid<accurate>(g);
+            if (slope) *slope = s * (1.0f + g * (1.0f - s));
+            return g * s;
+        }
+        case kGelu: {
+            const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+            if (slope) *slope = below + g * (accurate ? expf(-0.5f * g * g) : __expf(-0.5f * g * g)) * 0.3989422804014327f;
+            return g * below;
+        }
+        case kRelu: {
+            // (NaN stays NaN; the derivative at 0 is 0)
+            if (slope) *slope = g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
+            return g < 0.0f ? 0.0f : g;
+        }
+        default: {
+            const float s = sigmoid<accurate>(g);
+            if (slope) *slope = s * (1.0f - s);
+            return s;
+        }
+    }
+}
+
+inline int64_t up_to(int64_t n, int64_t whole) { return (n + whole - 1) / whole * whole; }
+inline int64_t pieces(int64_t n, int64_t size) { return (n + size - 1) / size; }
+
+}  // namespace svox_decoder

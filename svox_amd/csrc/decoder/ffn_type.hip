@@ -1,0 +1,240 @@
+// ffn_type.hip -- the kernels of the gated feed-forward block of one type (SVOX_DECODER_TYPE) and their launches.
+#include "entry.h"
+#include "product_kernels.h"
+
+namespace svox_decoder {
+
+using T = SVOX_DECODER_TYPE;
+
+namespace {
+
+constexpr int kPlanes = Form<T>::planes;
+constexpr int kKT = kPlanes == 1 ? 64 : 32;
+using HiddenShape = Shape<128, 64, kKT, 2, 2>;
+using OutputShape = Shape<128, 128, kKT, 2, 2>;
+using WeightShape = Shape<128, 128, kKT, 2, 2>;
+
+// ---- operands: where they are if the tiles can be read from there, else laid out in the workspace
+bool tiles_read(const void* at, int64_t ld, int64_t cols) {
+    return kPlanes == 1 && (uintptr_t)at % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
+}
+struct Lays {
+    LayArgs<T> args{};
+    int count = 0;
+    int64_t blocks = 0;
+    Planes operand(Room& room, const void* at, int64_t ld, int64_t rows, int64_t cols) {
+        if (tiles_read(at, ld, cols)) return Planes{(const u16*)at, ld, 0, rows, cols};
+        const int64_t wide = up_to(cols, 8);
+        Planes to{nullptr, wide, rows * wide, rows, wide};
+        to.at = room.take<u16>(kPlanes * rows * wide);
+        LayJob<T>& job = args.job[count++];
+        job = LayJob<T>{(const T*)at, ld, to, cols, pieces(rows * wide / 8, kLayThreads)};
+        blocks += job.blocks;
+        return to;
+    }
+    void launch(hipStream_t stream) const {
+        if (blocks > 0) hipLaunchKernelGGL((lay_kernel<T>), dim3((unsigned)blocks), dim3(kLayThreads), 0, stream, args);
+    }
+};
+Planes hidden_numbers(Room& room, const SvoxGatedFfn& s) {
+    const int64_t wide = up_to(s.hidden, 8);
+    Planes h{nullptr, wide, s.rows * wide, s.rows, wide};
+    h.at = room.take<u16>(kPlanes * s.rows * wide);
+    return h;
+}
+
+// ---- what a call keeps in its workspace
+struct Forward {
+    Lays lays;
+    Planes x, w_gate, w_up, w_down, h;
+    int64_t bytes;
+    Forward(const SvoxGatedFfn& s, void* workspace) {
+        Room room(workspace);
+        x = lays.operand(room, s.x, s.x_stride, s.rows, s.dim);
+        w_gate = lays.operand(room, s.w_gate, s.dim, s.hidden, s.dim);
+        w_up = lays.operand(room, s.w_up, s.dim, s.hidden, s.dim);
+        w_down = lays.operand(room, s.w_down, s.hidden, s.out, s.hidden);
+        h = hidden_numbers(room, s);
+        bytes = room.used;
+    }
+};
+
+struct Split {
+    int64_t tiles, each;
+    int splits;
+};
+Split weight_split(const SvoxGatedFfn& s) {
+    using S = WeightShape;
+    const int64_t across = pieces(s.hidden, S::BM) * pieces(s.dim, S::BN);
+    Split w;
+    w.tiles = 2 * across + pieces(s.out, S::BM) * pieces(s.hidden, S::BN);
+    // two blocks a compute unit, of eight stages at least
+    int64_t splits = pieces(512, w.tiles);
+    const int64_t most = pieces(s.rows, 8 * S::KT);
+    if (splits > most) splits = most;
+    w.each = up_to(pieces(s.rows, splits), S::KT);
+    w.splits = (int)pieces(s.rows, w.each);
+    return w;
+}
+int64_t gradient_numbers(const SvoxGatedFfn& s) {
+    return 2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + 2 * (int64_t)s.hidden + s.out;
+}
+
+struct Backward {
+    Lays lays;
+    Planes x, w_gate, w_up, w_down, dy, h, dgate, dup;
+    Split split;
+    float* part;
+    int64_t bytes;
+    Backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, void* workspace, bool any_grad) {
+        Room room(workspace);
+        // (grad_output's address is not known when its workspace is asked for: there is room to lay it out)
+        x = lays.operand(room, s.x, s.x_stride, s.rows, s.dim);
+        w_gate = lays.operand(room, s.w_gate, s.dim, s.hidden, s.dim);
+        w_up = lays.operand(room, s.w_up, s.dim, s.hidden, s.dim);
+        w_down = lays.operand(room, s.w_down, s.hidden, s.out, s.hidden);
+        h = hidden_numbers(room, s);
+        dgate = hidden_numbers(room, s);
+        dup = hidden_numbers(room, s);
+        split = weight_split(s);
+        part = split.splits > 1 ? room.take<float>(split.splits * gradient_numbers(s)) : nullptr;
+        if (any_grad)
+            room.take<u16>(kPlanes * s.rows * up_to(s.out, 8));
+        else
+            dy = lays.operand(room, grad_output, grad_stride, s.rows, s.out);
+        bytes = room.used;
+    }
+};
+
+HiddenArgs<T> hidden_args(const SvoxGatedFfn& s, const Planes& x, const Planes& w_gate, const Planes& w_up, const Planes& h) {
+    HiddenArgs<T> p{};
+    p.x = x;
+    p.w_gate = w_gate;
+    p.w_up = w_up;
+    p.b_gate = (const T*)s.b_gate;
+    p.b_up = (const T*)s.b_up;
+    p.h = const_cast<u16*>(h.at);
+    p.ldh = h.ld;
+    p.plane = h.plane;
+    p.rows = s.rows;
+    p.dim = s.dim;
+    p.hidden = s.hidden;
+    p.out = s.out;
+    p.tiles_m = pieces(s.rows, HiddenShape::BM);
+    p.tiles_n = pieces(h.ld, HiddenShape::BN);
+    p.activation = s.activation;
+    return p;
+}
+
+template <bool along_b>
+void launch_output(OutputArgs<T> p, hipStream_t stream) {
+    p.tiles_m = pieces(p.rows, OutputShape::BM);
+    p.tiles_n = pieces(p.cols, OutputShape::BN);
+    hipLaunchKernelGGL((output_kernel<T, OutputShape, along_b>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(OutputShape::threads), 0, stream, p);
+}
+
+}  // namespace
+
+template <>
+int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
+    return backward ? Backward(s, nullptr, 0, nullptr, true).bytes : Forward(s, nullptr).bytes;
+}
+
+template <>
+int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    const Forward f(s, workspace);
+    f.lays.launch(stream);
+    const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);
+    hipLaunchKernelGGL((hidden_kernel<T, HiddenShape, false>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(HiddenShape::threads), 0, stream, p);
+    OutputArgs<T> o{};
+    o.a[0] = f.h;
+    o.b[0] = f.w_down;
+    o.pairs = 1;
+    o.bias = (const T*)s.b_down;
+    o.residual = (const T*)s.residual;
+    o.residual_ld = s.residual_stride;
+    o.y = (T*)y;
+    o.rows = s.rows;
+    o.cols = s.out;
+    launch_output<true>(o, stream);
+    return check_launch("gated_ffn");
+}
+
+template <>
+int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
+                           hipStream_t stream) {
+    Backward b(s, grad_output, grad_stride, workspace, false);
+    b.lays.launch(stream);
+    HiddenArgs<T> p = hidden_args(s, b.x, b.w_gate, b.w_up, b.h);
+    p.dy = b.dy;
+    p.w_down = b.w_down;
+    p.dgate = const_cast<u16*>(b.dgate.at);
+    p.dup = const_cast<u16*>(b.dup.at);
+    hipLaunchKernelGGL((hidden_kernel<T, HiddenShape, true>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(HiddenShape::threads), 0, stream, p);
+    if (grads.x) {
+        OutputArgs<T> o{};
+        o.a[0] = b.dgate;
+        o.a[1] = b.dup;
+        o.b[0] = b.w_gate;
+        o.b[1] = b.w_up;
+        o.pairs = 2;
+        o.y = (T*)grads.x;
+        o.rows = s.rows;
+        o.cols = s.dim;
+        launch_output<false>(o, stream);
+    }
+    using S = WeightShape;
+    WeightArgs<T> w{};
+    JoinArgs<T> join{};
+    const int64_t H = s.hidden, D = s.dim, O = s.out;
+    float* part = b.part;
+    auto take = [&](int64_t count) {
+        float* const at = part;
+        if (part) part += b.split.splits * count;
+        return at;
+    };
+    // (a gradient that nobody wants is computed with the others and left in the workspace, or not at all)
+    void* const outs[3] = {grads.w_gate, grads.w_up, grads.w_down};
+    void* const sums[3] = {grads.b_gate, grads.b_up, grads.b_down};
+    const Planes left[3] = {b.dgate, b.dup, b.dy}, right[3] = {b.x, b.x, b.h};
+    int64_t blocks = 0;
+    int jobs = 0;
+    for (int j = 0; j < 3; ++j) {
+        if (!outs[j] && !sums[j]) continue;
+        WeightJob<T>& job = w.job[jobs++];
+        job.a = left[j];
+        job.b = right[j];
+        job.m = j < 2 ? H : O;
+        job.n = j < 2 ? D : H;
+        job.tiles_m = pieces(job.m, S::BM);
+        job.tiles_n = pieces(job.n, S::BN);
+        job.out = (T*)outs[j];
+        job.sums_out = (T*)sums[j];
+        job.part = take(job.m * job.n);
+        job.sums_part = take(job.m);
+        blocks += job.tiles_m * job.tiles_n;
+    }
+    if (jobs) {
+        w.rows = s.rows;
+        w.each = b.split.each;
+        w.splits = b.split.splits;
+        hipLaunchKernelGGL((weight_kernel<T, S>), dim3((unsigned)blocks, (unsigned)w.splits), dim3(S::threads), 0, stream, w);
+        if (w.splits > 1) {
+            int64_t join_blocks = 0;
+            int n = 0;
+            for (int j = 0; j < jobs; ++j)
+                for (int which = 0; which < 2; ++which) {
+                    T* const to = which ? w.job[j].sums_out : w.job[j].out;
+                    if (!to) continue;
+                    join.job[n] = {which ? w.job[j].sums_part : w.job[j].part, to, which ? w.job[j].m : w.job[j].m * w.job[j].n};
+                    join.blocks[n] = pieces(join.job[n].count, 4 * kJoinThreads);
+                    join_blocks += join.blocks[n++];
+                }
+            join.splits = w.splits;
+            hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)join_blocks), dim3(kJoinThreads), 0, stream, join);
+        }
+    }
+    return check_launch("gated_ffn_backward");
+}
+
+}  // namespace svox_decoder

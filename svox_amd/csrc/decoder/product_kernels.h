@@ -1,0 +1,358 @@
+// product_kernels.h -- the gated feed-forward block as products of whole matrices, for rows enough to fill tiles.
+//
+// forward   hidden_kernel   h = act(x Wg' + bg) * (x Wu' + bu)            both products of a tile side by side, h alone is stored
+//           output_kernel   y = h Wd' + bd + residual
+// backward  hidden_kernel   gate and up again, dh = dy Wd, then h, dgate = dh up act'(gate), dup = dh act(gate)
+//           output_kernel   dx = dgate Wg + dup Wu
+//           weight_kernel   dWg = dgate' x, dWu = dup' x, dWd = dy' h, the biases' gradients as products with ones; the rows
+//                           are shared out where the tiles are few, and join_kernel adds the parts in their order
+#pragma once
+#include "tile.h"
+
+namespace svox_decoder {
+
+// The shape of a block's work: BM x BN numbers of the result, KT of the reduction at a time, WM x WN wavefronts.
+template <int BM_, int BN_, int KT_, int WM_, int WN_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, KT = KT_, WM = WM_, WN = WN_, threads = WM * WN * kWave;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+};
+
+// NB products of one left operand with NB right ones, a block's tile of each.
+template <class T, class S, bool along_a, bool along_b, int NB>
+struct Product {
+    static constexpr int planes = Form<T>::planes;
+    using A = TileOf<along_a, S::BM, S::KT, S::threads>;
+    using B = TileOf<along_b, S::BN, S::KT, S::threads>;
+    static constexpr int stage = planes * (A::numbers + NB * B::numbers);   // 16-bit numbers
+
+    static __device__ __forceinline__ void load(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds) {
+#pragma unroll
+        for (int p = 0; p < planes; ++p) {
+            A::load(a, a.at + p * a.plane, m0, k, k_end, lds + p * A::numbers);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                B::load(b[i], b[i].at + p * b[i].plane, n0, k, k_end, lds + planes * A::numbers + (p * NB + i) * B::numbers);
+        }
+    }
+    // ones: also the sums of the left operand's columns (over the reduction), in `sums`
+    template <bool ones>
+    static __device__ __forceinline__ void multiply_stage(const u16* lds, int wm, int wn, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
+#pragma unroll
+        for (int step = 0; step < S::KT / 32; ++step) {
+            u16x8 a[S::TM][planes];
+#pragma unroll
+            for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+                for (int p = 0; p < planes; ++p) a[m][p] = A::fragment(lds + p * A::numbers, (wm * S::TM + m) * 16, step);
+            if constexpr (ones) {
+                u16x8 one;
+                for (int i = 0; i < 8; ++i) one[i] = Form<T>::one();
+#pragma unroll
+                for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+                    for (int p = planes; p-- > 0;) sums[m] = Form<T>::mma(one, a[m][p], sums[m]);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int n = 0; n < S::TN; ++n) {
+                    u16x8 b[planes];
+#pragma unroll
+                    for (int p = 0; p < planes; ++p)
+                        b[p] = B::fragment(lds + planes * A::numbers + (p * NB + i) * B::numbers, (wn * S::TN + n) * 16, step);
+#pragma unroll
+                    for (int m = 0; m < S::TM; ++m) acc[i][m][n] = multiply<T>(b, a[m], acc[i][m][n]);
+                }
+        }
+    }
+    // adds the products over [k, k_end) to acc; lds: two stages
+    template <bool ones>
+    static __device__ __forceinline__ void run(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
+                                               f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
+        if (k >= k_end) return;
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), wm = wave % S::WM, wn = wave / S::WM;
+        __syncthreads();   // (another product's last stage may still be read)
+        load(a, b, m0, n0, k, k_end, lds);
+        int at = 0;
+        for (; k < k_end; k += S::KT) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();   // this stage is there, the other one is free
+            if (k + S::KT < k_end) load(a, b, m0, n0, k + S::KT, k_end, lds + (at ^ 1) * stage);
+            multiply_stage<ones>(lds + at * stage, wm, wn, acc, sums);
+            at ^= 1;
+        }
+    }
+};
+
+template <int NB, int TM, int TN>
+__device__ __forceinline__ void clear(f32x4 (&acc)[NB][TM][TN]) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+#pragma unroll
+            for (int n = 0; n < TN; ++n) acc[i][m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// Where a lane's four numbers of a tile lie: row m, columns n..n+3.
+template <class S>
+struct Place {
+    int64_t m0, n0;
+    __device__ Place(int64_t tile_m, int64_t tile_n) {
+        const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+        m0 = tile_m + (wave % S::WM) * S::TM * 16 + (lane & 15);
+        n0 = tile_n + (wave / S::WM) * S::TN * 16 + (lane >> 4) * 4;
+    }
+    __device__ int64_t row(int m) const { return m0 + m * 16; }
+    __device__ int64_t col(int n) const { return n0 + n * 16; }
+};
+
+template <class T>
+__device__ __forceinline__ f32x4 four_of(const T* from, int64_t n, int64_t count) {   // zeros beyond `count`
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!from) return v;
+    if (n + 4 <= count) {
+        const auto f = load_few<T, 4>(from + n);
+        for (int i = 0; i < 4; ++i) v[i] = (float)f[i];
+    } else {
+        for (int i = 0; i < 4; ++i)
+            if (n + i < count) v[i] = (float)from[n + i];
+    }
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void store_four(T* to, f32x4 v, int64_t n, int64_t count) {
+    if (n + 4 <= count) {
+        typename Few<T, 4>::vector f;
+        for (int i = 0; i < 4; ++i) f[i] = (T)v[i];
+        store_few<T, 4>(to + n, f);
+    } else {
+        for (int i = 0; i < 4; ++i)
+            if (n + i < count) to[n + i] = (T)v[i];
+    }
+}
+
+template <class T>
+struct HiddenArgs {
+    Planes x, w_gate, w_up;      // (rows, dim), (hidden, dim) twice
+    Planes dy, w_down;           // backward: (rows, out), (out, hidden)
+    const T *b_gate, *b_up;      // or NULL
+    u16 *h, *dgate, *dup;        // planes of (rows, ldh)
+    int64_t ldh, plane;
+    int64_t rows, dim, hidden, out;
+    int64_t tiles_m, tiles_n;
+    int activation;
+};
+
+template <class T, class S, bool backward>
+__global__ __launch_bounds__(S::threads) void hidden_kernel(HiddenArgs<T> p) {
+    using Forward = Product<T, S, true, true, 2>;
+    using Back = Product<T, S, true, false, 1>;
+    constexpr int planes = Form<T>::planes;
+    static_assert(Back::stage <= Forward::stage, "room");
+    __shared__ __align__(16) u16 lds[2 * Forward::stage];
+    int64_t tm, tn;
+    tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
+    f32x4 acc[2][S::TM][S::TN], dh[1][S::TM][S::TN];
+    clear(acc);
+    const Planes w[2] = {p.w_gate, p.w_up};
+    Forward::template run<false>(p.x, w, m0, n0, 0, p.x.cols, lds, acc, nullptr);
+    if constexpr (backward) {
+        clear(dh);
+        Back::template run<false>(p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
+    }
+    const Place<S> place(m0, n0);
+#pragma unroll
+    for (int n = 0; n < S::TN; ++n) {
+        const int64_t col = place.col(n);
+        if (col >= p.ldh) continue;
+        const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
+#pragma unroll
+        for (int m = 0; m < S::TM; ++m) {
+            const int64_t row = place.row(m);
+            if (row >= p.rows) continue;
+            f32x4 h, dg, du;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float g = acc[0][m][n][i] + bg[i], u = acc[1][m][n][i] + bu[i];
+                float slope;
+                const float a = activate<planes == 3>(p.activation, g, backward ? &slope : nullptr);
+                h[i] = a * u;
+                if constexpr (backward) {
+                    dg[i] = dh[0][m][n][i] * u * slope;
+                    du[i] = dh[0][m][n][i] * a;
+                }
+            }
+            u16x4 part[planes];
+            const int64_t at = row * p.ldh + col;
+            auto keep = [&](f32x4 v, u16* to) {
+                Form<T>::split(v, part);
+                for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(to + q * p.plane + at) = part[q];
+            };
+            keep(h, p.h);
+            if constexpr (backward) {
+                keep(dg, p.dgate);
+                keep(du, p.dup);
+            }
+        }
+    }
+}
+
+template <class T>
+struct OutputArgs {
+    Planes a[2], b[2];     // y = sum over `pairs` of a[i] times b[i]
+    int pairs;
+    const T *bias, *residual;
+    int64_t residual_ld;
+    T* y;                  // (rows, cols), dense
+    int64_t rows, cols;
+    int64_t tiles_m, tiles_n;
+};
+
+// along_b: b is (cols, reduction), else (reduction, cols)
+template <class T, class S, bool along_b>
+__global__ __launch_bounds__(S::threads) void output_kernel(OutputArgs<T> p) {
+    using P = Product<T, S, true, along_b, 1>;
+    __shared__ __align__(16) u16 lds[2 * P::stage];
+    int64_t tm, tn;
+    tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
+    f32x4 acc[1][S::TM][S::TN];
+    clear(acc);
+    for (int i = 0; i < p.pairs; ++i) P::template run<false>(p.a[i], &p.b[i], m0, n0, 0, p.a[i].cols, lds, acc, nullptr);
+    const Place<S> place(m0, n0);
+#pragma unroll
+    for (int n = 0; n < S::TN; ++n) {
+        const int64_t col = place.col(n);
+        if (col >= p.cols) continue;
+        const f32x4 bias = four_of(p.bias, col, p.cols);
+#pragma unroll
+        for (int m = 0; m < S::TM; ++m) {
+            const int64_t row = place.row(m);
+            if (row >= p.rows) continue;
+            f32x4 v = acc[0][m][n] + bias;
+            if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, p.cols);
+            store_four(p.y + row * p.cols, v, col, p.cols);
+        }
+    }
+}
+
+// One weight's gradient: a' b over the rows, (m, n), and the sums of a's columns.
+template <class T>
+struct WeightJob {
+    Planes a, b;
+    int64_t m, n, tiles_m, tiles_n;
+    float *part, *sums_part;   // [splits][m][n], [splits][m]; unused with one split
+    T *out, *sums_out;         // sums_out NULL: no bias
+};
+template <class T>
+struct WeightArgs {
+    WeightJob<T> job[3];
+    int64_t rows, each;        // rows of a split: a whole number of KT
+    int splits;
+};
+
+template <class T, class S>
+__global__ __launch_bounds__(S::threads) void weight_kernel(WeightArgs<T> p) {
+    using P = Product<T, S, false, false, 1>;
+    __shared__ __align__(16) u16 lds[2 * P::stage];
+    int64_t block = blockIdx.x;
+    int j = 0;
+    while (j < 2 && block >= p.job[j].tiles_m * p.job[j].tiles_n) {
+        block -= p.job[j].tiles_m * p.job[j].tiles_n;
+        ++j;
+    }
+    const WeightJob<T> job = p.job[j];
+    const int64_t m0 = block / job.tiles_n * S::BM, n0 = block % job.tiles_n * S::BN, split = blockIdx.y;
+    const int64_t k = split * p.each, k_end = k + p.each < p.rows ? k + p.each : p.rows;
+    f32x4 acc[1][S::TM][S::TN], sums[S::TM];
+    clear(acc);
+    for (int m = 0; m < S::TM; ++m) sums[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const bool with_sums = job.sums_out && n0 == 0;
+    if (with_sums)
+        P::template run<true>(job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
+    else
+        P::template run<false>(job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
+    const Place<S> place(m0, n0);
+#pragma unroll
+    for (int m = 0; m < S::TM; ++m) {
+        const int64_t row = place.row(m);
+        if (row >= job.m) continue;
+#pragma unroll
+        for (int n = 0; n < S::TN; ++n) {
+            const int64_t col = place.col(n);
+            if (col >= job.n) continue;
+            if (!job.out) continue;
+            if (p.splits > 1)
+                store_four(job.part + (split * job.m + row) * job.n, acc[0][m][n], col, job.n);
+            else
+                store_four(job.out + row * job.n, acc[0][m][n], col, job.n);
+        }
+        if (with_sums && place.n0 == 0) {   // (every column of the product with ones is the sum)
+            if (p.splits > 1)
+                job.sums_part[split * job.m + row] = sums[m][0];
+            else
+                job.sums_out[row] = (T)sums[m][0];
+        }
+    }
+}
+
+// out = the sum of the parts, in their order
+template <class T>
+struct JoinArgs {
+    struct Job {
+        const float* part;
+        T* out;
+        int64_t count;
+    } job[6];
+    int64_t blocks[6];   // of every job
+    int splits;
+};
+constexpr int kJoinThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
+    int64_t block = blockIdx.x;
+    int j = 0;
+    while (j < 5 && block >= p.blocks[j]) block -= p.blocks[j++];
+    const auto job = p.job[j];
+    const int64_t i = (block * kJoinThreads + threadIdx.x) * 4;
+    if (i >= job.count) return;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < p.splits; ++s) sum += four_of(job.part + s * job.count, i, job.count);
+    store_four(job.out, sum, i, job.count);
+}
+
+// Matrices laid out for TileOf: rows of whole 8 numbers, zeros beyond the columns, planes for float32.
+template <class T>
+struct LayJob {
+    const T* from;
+    int64_t ld;          // of `from`
+    Planes to;
+    int64_t cols;        // of `from`
+    int64_t blocks;
+};
+template <class T>
+struct LayArgs {
+    LayJob<T> job[5];
+};
+constexpr int kLayThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kLayThreads) void lay_kernel(LayArgs<T> p) {
+    int64_t block = blockIdx.x;
+    int j = 0;
+    while (j < 4 && block >= p.job[j].blocks) block -= p.job[j++].blocks;
+    const LayJob<T> job = p.job[j];
+    const int64_t each = job.to.cols / 8, i = block * kLayThreads + threadIdx.x;
+    if (i >= job.to.rows * each) return;
+    const int64_t row = i / each, col = i % each * 8;
+    u16* const to = const_cast<u16*>(job.to.at) + row * job.to.ld + col;
+    for (int half = 0; half < 2; ++half) {
+        u16x4 part[Form<T>::planes];
+        Form<T>::split(four_of(job.from + row * job.ld, col + half * 4, job.cols), part);
+        for (int q = 0; q < Form<T>::planes; ++q) *reinterpret_cast<u16x4*>(to + q * job.to.plane + half * 4) = part[q];
+    }
+}
+
+}  // namespace svox_decoder
