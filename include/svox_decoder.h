@@ -71,7 +71,7 @@ typedef struct SvoxGatedFfn {
     const void* residual;   /* (rows, out), rows residual_stride numbers apart, or NULL: 0 */
     int64_t rows;           /* >= 0 */
     int64_t x_stride, residual_stride;
-    int32_t dim, hidden, out;   /* >= 1 */
+    int32_t dim, hidden, out;   /* 1 .. 2^22 */
     int32_t dtype;
     int32_t activation;
 } SvoxGatedFfn;

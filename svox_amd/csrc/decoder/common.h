@@ -129,6 +129,7 @@ __device__ __forceinline__ float activate(int activation, float g, float* slope)
     }
 }
 
+__host__ __device__ inline int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
 inline int64_t up_to(int64_t n, int64_t whole) { return (n + whole - 1) / whole * whole; }
 inline int64_t pieces(int64_t n, int64_t size) { return (n + size - 1) / size; }
 

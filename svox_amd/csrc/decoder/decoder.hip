@@ -62,12 +62,15 @@ int check_norm(const SvoxLayerNorm* s) {
     return check_matrix("x", s->x, s->rows, s->dim, s->x_stride);
 }
 
+constexpr int kMostWidth = 1 << 22;   // (tiles of longer rows would leave the range of 32-bit offsets)
 int check_ffn(const SvoxGatedFfn* s) {
     if (!s) return fail(SVOX_ERR_NULL_POINTER, "the spec is NULL");
     SVOX_TRY(check_dtype(s->dtype));
     if (s->rows < 0) return fail(SVOX_ERR_BAD_SHAPE, "rows must be >= 0, got %lld", (long long)s->rows);
     if (s->dim < 1 || s->hidden < 1 || s->out < 1)
         return fail(SVOX_ERR_BAD_SHAPE, "dim, hidden and out must be >= 1, got %d, %d, %d", s->dim, s->hidden, s->out);
+    if (s->dim > kMostWidth || s->hidden > kMostWidth || s->out > kMostWidth)
+        return fail(SVOX_ERR_UNSUPPORTED, "dim, hidden and out must be <= %d, got %d, %d, %d", kMostWidth, s->dim, s->hidden, s->out);
     if (s->activation < SVOX_ACTIVATION_SILU || s->activation > SVOX_ACTIVATION_SIGMOID)
         return fail(SVOX_ERR_UNSUPPORTED, "unknown activation %d", s->activation);
     SVOX_TRY(check_matrix("x", s->x, s->rows, s->dim, s->x_stride));

@@ -9,14 +9,15 @@ using T = SVOX_DECODER_TYPE;
 namespace {
 
 constexpr int kPlanes = Form<T>::planes;
+constexpr int64_t kMostLd = TileOf<true, 64, 64, 256>::most_ld;
 constexpr int kKT = kPlanes == 1 ? 64 : 32;
-using HiddenShape = Shape<128, 64, kKT, 2, 2>;
-using OutputShape = Shape<128, 128, kKT, 2, 2>;
-using WeightShape = Shape<128, 128, kKT, 2, 2>;
+using HiddenShape = Shape<128, 64, kKT, 2, 2, 2>;
+using OutputShape = Shape<128, 128, kKT, 2, 2, 2>;
+using WeightShape = Shape<128, 128, kKT, 2, 2, 2>;
 
 // ---- operands: where they are if the tiles can be read from there, else laid out in the workspace
 bool tiles_read(const void* at, int64_t ld, int64_t cols) {
-    return kPlanes == 1 && (uintptr_t)at % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
+    return kPlanes == 1 && (uintptr_t)at % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld <= kMostLd;
 }
 struct Lays {
     LayArgs<T> args{};
@@ -227,7 +228,7 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
                     T* const to = which ? w.job[j].sums_out : w.job[j].out;
                     if (!to) continue;
                     join.job[n] = {which ? w.job[j].sums_part : w.job[j].part, to, which ? w.job[j].m : w.job[j].m * w.job[j].n};
-                    join.blocks[n] = pieces(join.job[n].count, 4 * kJoinThreads);
+                    join.blocks[n] = pieces(join.job[n].count, kJoinNumbers);
                     join_blocks += join.blocks[n++];
                 }
             join.splits = w.splits;

@@ -272,23 +272,29 @@ __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) 
     }
 }
 
-// The gradients of weight and bias from the blocks' sums: 32 columns a block, the blocks' rows over its 8 groups of lanes.
+// The gradients of weight and bias from the blocks' sums: 16 columns a block, the sums over its 64 groups of lanes.
+constexpr int kNormJoinThreads = 1024, kNormJoinColumns = 16;
 template <class T>
-__global__ __launch_bounds__(kNormThreads) void norm_join_kernel(const float* part, int blocks, int dim, T* dweight, T* dbias) {
-    __shared__ float shared[kNormThreads];
-    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+__global__ __launch_bounds__(kNormJoinThreads) void norm_join_kernel(const float* part, int blocks, int dim, T* dweight, T* dbias) {
+    constexpr int groups = kNormJoinThreads / kNormJoinColumns;
+    __shared__ float shared[kNormJoinThreads];
+    const int lane = threadIdx.x % kNormJoinColumns, group = threadIdx.x / kNormJoinColumns;
+    const int64_t c = (int64_t)blockIdx.x * kNormJoinColumns + lane;
     float sum = 0.0f;
     if (c < 2 * (int64_t)dim)
-        for (int b = group; b < blocks; b += kNormThreads / 32) sum += part[(int64_t)b * 2 * dim + c];
+#pragma unroll 4
+        for (int b = group; b < blocks; b += groups) sum += part[(int64_t)b * 2 * dim + c];
     shared[threadIdx.x] = sum;
     __syncthreads();
+    for (int half = groups / 2; half > 0; half /= 2) {
+        if (group < half) shared[threadIdx.x] += shared[threadIdx.x + half * kNormJoinColumns];
+        __syncthreads();
+    }
     if (group != 0 || c >= 2 * (int64_t)dim) return;
-    for (int g = 1; g < kNormThreads / 32; ++g) sum += shared[g * 32 + lane];
     if (c < dim) {
-        if (dweight) dweight[c] = (T)sum;
+        if (dweight) dweight[c] = (T)shared[lane];
     } else if (dbias) {
-        dbias[c - dim] = (T)sum;
+        dbias[c - dim] = (T)shared[lane];
     }
 }
 

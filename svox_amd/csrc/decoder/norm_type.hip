@@ -21,8 +21,6 @@ namespace {
     else if ((pieces) <= 1024) { constexpr int kLanes = 256, kPieces = 4; __VA_ARGS__; }      \
     else { constexpr int kLanes = 0, kPieces = 0; __VA_ARGS__; }
 
-int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
-
 NormArgs<T> args(const SvoxLayerNorm& s) {
     NormArgs<T> p{};
     p.x = (const T*)s.x;
@@ -72,7 +70,8 @@ int launch_norm_backward<T>(const SvoxLayerNorm& s, const float* stats, const vo
             hipLaunchKernelGGL((norm_long_kernel<T, true>), dim3(blocks), dim3(kNormThreads), 0, stream, p);
     });
     if (part)
-        hipLaunchKernelGGL((norm_join_kernel<T>), dim3((unsigned)pieces(2 * (int64_t)s.dim, 32)), dim3(kNormThreads), 0, stream, part,
+        hipLaunchKernelGGL((norm_join_kernel<T>), dim3((unsigned)pieces(2 * (int64_t)s.dim, kNormJoinColumns)),
+                           dim3(kNormJoinThreads), 0, stream, part,
                            blocks, s.dim, (T*)grad_weight, (T*)grad_bias);
     return check_launch("layer_norm_backward");
 }

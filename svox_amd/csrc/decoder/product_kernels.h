@@ -9,12 +9,15 @@
 #pragma once
 #include "tile.h"
 
+#include <utility>
+
 namespace svox_decoder {
 
-// The shape of a block's work: BM x BN numbers of the result, KT of the reduction at a time, WM x WN wavefronts.
-template <int BM_, int BN_, int KT_, int WM_, int WN_>
+// The shape of a block's work: BM x BN numbers of the result, KT of the reduction at a time, WM x WN wavefronts, and how many
+// tiles of the reduction LDS holds (one that is multiplied, the others on their way).
+template <int BM_, int BN_, int KT_, int WM_, int WN_, int stages_>
 struct Shape {
-    static constexpr int BM = BM_, BN = BN_, KT = KT_, WM = WM_, WN = WN_, threads = WM * WN * kWave;
+    static constexpr int BM = BM_, BN = BN_, KT = KT_, WM = WM_, WN = WN_, threads = WM * WN * kWave, stages = stages_;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
 };
 
@@ -26,14 +29,23 @@ struct Product {
     using B = TileOf<along_b, S::BN, S::KT, S::threads>;
     static constexpr int stage = planes * (A::numbers + NB * B::numbers);   // 16-bit numbers
 
-    static __device__ __forceinline__ void load(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds) {
+    static constexpr int loads = planes * (A::loads + NB * B::loads);       // of a lane
+
+    struct Operands {
+        A a;
+        B b[NB];
+        int64_t plane_a, plane_b[NB];
+    };
+    static __device__ __forceinline__ void load(Operands& o, u16* lds) {
 #pragma unroll
         for (int p = 0; p < planes; ++p) {
-            A::load(a, a.at + p * a.plane, m0, k, k_end, lds + p * A::numbers);
+            o.a.load(p * o.plane_a, lds + p * A::numbers);
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-                B::load(b[i], b[i].at + p * b[i].plane, n0, k, k_end, lds + planes * A::numbers + (p * NB + i) * B::numbers);
+            for (int i = 0; i < NB; ++i) o.b[i].load(p * o.plane_b[i], lds + planes * A::numbers + (p * NB + i) * B::numbers);
         }
+        o.a.advance();
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o.b[i].advance();
     }
     // ones: also the sums of the left operand's columns (over the reduction), in `sums`
     template <bool ones>
@@ -66,22 +78,44 @@ struct Product {
                 }
         }
     }
-    // adds the products over [k, k_end) to acc; lds: two stages
+    // Adds the products over [k, k_end) to acc.  LDS holds S::stages tiles; before one is multiplied its loads, and no later
+    // ones, have to have arrived (a lane's loads arrive in their order), and those of the tile that takes the place of the one
+    // before it go out after the barrier that says that every wavefront is done with that.
     template <bool ones>
     static __device__ __forceinline__ void run(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
                                                f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if (k >= k_end) return;
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), wm = wave % S::WM, wn = wave / S::WM;
-        __syncthreads();   // (another product's last stage may still be read)
-        load(a, b, m0, n0, k, k_end, lds);
-        int at = 0;
-        for (; k < k_end; k += S::KT) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();   // this stage is there, the other one is free
-            if (k + S::KT < k_end) load(a, b, m0, n0, k + S::KT, k_end, lds + (at ^ 1) * stage);
-            multiply_stage<ones>(lds + at * stage, wm, wn, acc, sums);
-            at ^= 1;
+        const int tiles = (int)((k_end - k + S::KT - 1) / S::KT);
+        Operands o = operands(a, b, m0, n0, k, std::make_integer_sequence<int, NB>());
+        int loaded = 0;
+        auto load_next = [&] {
+            if (loaded == tiles - 1) {   // (an operand's own end may come a little before k_end, which is a whole number of 8)
+                const int64_t at = k + (int64_t)loaded * S::KT;
+                o.a.last(least(k_end, along_a ? a.cols : a.rows) - at);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o.b[i].last(least(k_end, along_b ? b[i].cols : b[i].rows) - at);
+            }
+            load(o, lds + loaded % S::stages * stage);
+            ++loaded;
+        };
+        __syncthreads();   // (another product's last tile may still be read)
+#pragma unroll
+        for (int i = 0; i < S::stages - 1; ++i)
+            if (i < tiles) load_next();
+        for (int t = 0; t < tiles; ++t) {
+            if (loaded - t - 1 >= S::stages - 2)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::stages - 2) * loads) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (loaded < tiles) load_next();
+            multiply_stage<ones>(lds + t % S::stages * stage, wm, wn, acc, sums);
         }
+    }
+    template <int... i>
+    static __device__ __forceinline__ Operands operands(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k,
+                                                        std::integer_sequence<int, i...>) {
+        return Operands{A(a, m0, k), {B(b[i], n0, k)...}, a.plane, {b[i].plane...}};
     }
 };
 
@@ -151,7 +185,7 @@ __global__ __launch_bounds__(S::threads) void hidden_kernel(HiddenArgs<T> p) {
     using Back = Product<T, S, true, false, 1>;
     constexpr int planes = Form<T>::planes;
     static_assert(Back::stage <= Forward::stage, "room");
-    __shared__ __align__(16) u16 lds[2 * Forward::stage];
+    __shared__ __align__(16) u16 lds[S::stages * Forward::stage];
     int64_t tm, tn;
     tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
@@ -215,7 +249,7 @@ struct OutputArgs {
 template <class T, class S, bool along_b>
 __global__ __launch_bounds__(S::threads) void output_kernel(OutputArgs<T> p) {
     using P = Product<T, S, true, along_b, 1>;
-    __shared__ __align__(16) u16 lds[2 * P::stage];
+    __shared__ __align__(16) u16 lds[S::stages * P::stage];
     int64_t tm, tn;
     tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
@@ -257,7 +291,7 @@ struct WeightArgs {
 template <class T, class S>
 __global__ __launch_bounds__(S::threads) void weight_kernel(WeightArgs<T> p) {
     using P = Product<T, S, false, false, 1>;
-    __shared__ __align__(16) u16 lds[2 * P::stage];
+    __shared__ __align__(16) u16 lds[S::stages * P::stage];
     int64_t block = blockIdx.x;
     int j = 0;
     while (j < 2 && block >= p.job[j].tiles_m * p.job[j].tiles_n) {
@@ -299,7 +333,7 @@ __global__ __launch_bounds__(S::threads) void weight_kernel(WeightArgs<T> p) {
     }
 }
 
-// out = the sum of the parts, in their order
+// out = the sum of the parts, always in the same order: a group of 32 lanes to 128 numbers, the parts over the block's groups.
 template <class T>
 struct JoinArgs {
     struct Job {
@@ -310,17 +344,25 @@ struct JoinArgs {
     int64_t blocks[6];   // of every job
     int splits;
 };
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinNumbers = 32 * 4;
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
+    constexpr int groups = kJoinThreads / 32;
+    __shared__ f32x4 shared[kJoinThreads];
     int64_t block = blockIdx.x;
     int j = 0;
     while (j < 5 && block >= p.blocks[j]) block -= p.blocks[j++];
     const auto job = p.job[j];
-    const int64_t i = (block * kJoinThreads + threadIdx.x) * 4;
-    if (i >= job.count) return;
+    const int64_t i = block * kJoinNumbers + threadIdx.x % 32 * 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.splits; ++s) sum += four_of(job.part + s * job.count, i, job.count);
+    if (i < job.count)
+#pragma unroll 4
+        for (int s = threadIdx.x / 32; s < p.splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count);
+    shared[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 32 || i >= job.count) return;
+#pragma unroll
+    for (int g = 1; g < groups; ++g) sum += shared[g * 32 + threadIdx.x];
     store_four(job.out, sum, i, job.count);
 }
 

@@ -2,8 +2,8 @@
 //
 // An operand is a matrix of 16-bit numbers (Planes: one, or three for float32) whose row length is a whole number of 8.  It
 // is used along its rows (the reduction runs along a row: `along`) or across them (the reduction runs down a column).  Its
-// tiles go to LDS by global_load_lds, 16 bytes a lane, without passing through registers; what lies outside the matrix is
-// read from 16 bytes of zeros, so that no edge needs a branch later.
+// tiles go to LDS by buffer loads, 16 bytes a lane, without passing through registers; what lies outside the matrix arrives as
+// zeros, so that no edge needs a branch later.
 //
 // LDS holds a tile as it lies in memory, but for an order of the 16-byte pieces that depends on the row, chosen so that the
 // eight lanes a clock serves fall on different banks:
@@ -24,47 +24,71 @@ struct Planes {
     int64_t cols;    // readable numbers of a row: a whole number of 8, zeros beyond the matrix
 };
 
-static __device__ __align__(16) const u16 kZeros[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-
 typedef __attribute__((address_space(3))) void Lds;
-typedef const __attribute__((address_space(1))) void Global;
-
-__device__ __forceinline__ void to_lds(const u16* from, u16* lds) {
-    __builtin_amdgcn_global_load_lds((Global*)from, (Lds*)lds, 16, 0, 0);
-}
 
 // One plane's tile of an operand: R rows (along) or columns (across) of the result, KT of the reduction.
+//
+// A lane's pieces lie at offsets from the tile's first number that do not change from tile to tile of the reduction: the loads
+// take them from registers, and the address that moves is scalar.  What lies outside the matrix gets an offset beyond the
+// buffer's range, for which the hardware delivers zeros.
 template <bool along, int R, int KT, int threads>
 struct TileOf {
     static constexpr int numbers = R * KT;
     static constexpr int loads = numbers / 8 / threads;
     static_assert(numbers % (8 * threads) == 0, "whole rounds of 16 bytes a lane");
+    static constexpr unsigned range = 0x80000000u, outside = 0x80000000u;   // bytes
+    static constexpr int64_t most_ld = (int64_t)1 << 22;                    // 256 rows of it stay within the range
 
     static __device__ __forceinline__ int turn_along(int row) { return KT == 64 ? (row & 7) : ((row >> 1) & 3); }
     static __device__ __forceinline__ int turn_across(int k) { return ((k & 3) | ((k >> 1) & 4)) & (R / 16 - 1); }
 
-    // the tile at row (column) r0 and reduction index k0 of `m`, up to k_end
-    static __device__ __forceinline__ void load(const Planes& m, const u16* plane, int64_t r0, int64_t k0, int64_t k_end, u16* lds) {
-        const int t = threadIdx.x, wave = t / kWave;
+    const u16* next;          // plane 0's first number of the next tile to load
+    int64_t step;             // numbers from tile to tile
+    unsigned at[loads];
+
+    // tiles of rows (columns) r0.. from reduction index k0 on
+    __device__ __forceinline__ TileOf(const Planes& m, int64_t r0, int64_t k0) {
+        next = m.at + (along ? r0 * m.ld + k0 : k0 * m.ld + r0);
+        step = along ? KT : KT * m.ld;
+        const int t = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
             const int piece = i * threads + t;
-            const u16* from;
-            bool there;
             if constexpr (along) {
                 const int row = piece / (KT / 8), slot = piece % (KT / 8);
-                const int64_t k = k0 + ((slot ^ turn_along(row)) * 8), r = r0 + row;
-                there = r < m.rows && k < k_end;
-                from = plane + r * m.ld + k;
+                at[i] = r0 + row < m.rows ? (unsigned)((row * m.ld + (slot ^ turn_along(row)) * 8) * 2) : outside;
             } else {
                 const int row = piece / (R / 8), slot = piece % (R / 8);
-                const int64_t k = k0 + row, c = r0 + (((slot >> 1) ^ turn_across(row)) * 2 + (slot & 1)) * 8;
-                there = k < k_end && k < m.rows && c < m.cols;
-                from = plane + k * m.ld + c;
+                const int c = (((slot >> 1) ^ turn_across(row)) * 2 + (slot & 1)) * 8;
+                at[i] = r0 + c < m.cols ? (unsigned)((row * m.ld + c) * 2) : outside;
             }
-            to_lds(there ? from : kZeros, lds + (size_t)(i * threads + wave * kWave) * 8);
         }
     }
+    // before the last tile: `left` indices of the reduction are left of it
+    __device__ __forceinline__ void last(int64_t left) {
+        if (left >= KT) return;
+        const int t = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < loads; ++i) {
+            const int piece = i * threads + t;
+            int k;
+            if constexpr (along) {
+                const int row = piece / (KT / 8), slot = piece % (KT / 8);
+                k = (slot ^ turn_along(row)) * 8;
+            } else {
+                k = piece / (R / 8);
+            }
+            if (k >= left) at[i] = outside;
+        }
+    }
+    __device__ __forceinline__ void load(int64_t plane, u16* lds) const {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc((void*)(next + plane), 0, range, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < loads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (Lds*)(lds + (i * threads + wave * kWave) * 8), 16, at[i], 0, 0, 0);
+    }
+    __device__ __forceinline__ void advance() { next += step; }
 
     // the fragment of rows (columns) r..r+15 and reduction indices 32 step..32 step + 31
     static __device__ __forceinline__ u16x8 fragment(const u16* lds, int r, int step) {
