@@ -1,6 +1,6 @@
 // ffn_type.hip -- the kernels of the gated feed-forward block of one type (SVOX_DECODER_TYPE) and their launches.
 #include "entry.h"
-#include "product_kernels.h"
+#include "few_kernels.h"
 
 namespace svox_decoder {
 
@@ -42,6 +42,43 @@ Planes hidden_numbers(Room& room, const SvoxGatedFfn& s) {
     Planes h{nullptr, wide, s.rows * wide, s.rows, wide};
     h.at = room.take<u16>(kPlanes * s.rows * wide);
     return h;
+}
+
+// ---- few rows
+constexpr int64_t kFewRows = 64;
+template <int MT>
+void launch_few(const FewArgs<T>& p, hipStream_t stream) {
+    const unsigned down = (unsigned)pieces(p.rows, 16 * MT);
+    hipLaunchKernelGGL((few_hidden_kernel<T, MT>), dim3((unsigned)pieces(p.ldh, 16), down), dim3(kFewHiddenWaves * kWave), 0, stream, p);
+    hipLaunchKernelGGL((few_output_kernel<T, MT>), dim3((unsigned)pieces(p.out, 16), down), dim3(kFewOutputWaves * kWave), 0, stream, p);
+}
+int launch_few(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    Room room(workspace);
+    const Planes h = hidden_numbers(room, s);
+    FewArgs<T> p{};
+    p.x = (const T*)s.x;
+    p.w_gate = (const T*)s.w_gate;
+    p.w_up = (const T*)s.w_up;
+    p.w_down = (const T*)s.w_down;
+    p.b_gate = (const T*)s.b_gate;
+    p.b_up = (const T*)s.b_up;
+    p.b_down = (const T*)s.b_down;
+    p.residual = (const T*)s.residual;
+    p.x_ld = s.x_stride;
+    p.residual_ld = s.residual_stride;
+    p.h = const_cast<u16*>(h.at);
+    p.ldh = h.ld;
+    p.plane = h.plane;
+    p.y = (T*)y;
+    p.rows = s.rows;
+    p.dim = s.dim;
+    p.hidden = s.hidden;
+    p.out = s.out;
+    p.activation = s.activation;
+    if (s.rows <= 16) launch_few<1>(p, stream);
+    else if (s.rows <= 32) launch_few<2>(p, stream);
+    else launch_few<4>(p, stream);
+    return check_launch("gated_ffn");
 }
 
 // ---- what a call keeps in its workspace
@@ -138,11 +175,18 @@ void launch_output(OutputArgs<T> p, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
-    return backward ? Backward(s, nullptr, 0, nullptr, true).bytes : Forward(s, nullptr).bytes;
+    if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
+    if (s.rows <= kFewRows) {
+        Room room(nullptr);
+        hidden_numbers(room, s);
+        return room.used;
+    }
+    return Forward(s, nullptr).bytes;
 }
 
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    if (s.rows <= kFewRows) return launch_few(s, y, workspace, stream);
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);

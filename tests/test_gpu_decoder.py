@@ -65,6 +65,17 @@ def test_ffn_sizes(gpu, rows, d, h, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 32, 33, 48, 63, 64])
+@pytest.mark.parametrize("d,h,o", [(31, 33, 17), (32, 32, 16), (100, 257, 3), (256, 1024, 256), (1000, 515, 130)])
+def test_ffn_few_rows(gpu, rows, d, h, o, dtype):
+    t, _ = ffn_inputs(rows, d, h, o, dtype, seed=rows * d)
+    wide = normal(torch.Generator().manual_seed(1), rows, d + 3, dtype=dtype)
+    for x in (t["x"], wide[:, 1:d + 1]):
+        want, _ = gated_ffn({**t, "x": x}, "silu")
+        want.holds(ffn({**t, "x": x}, "silu"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
 @pytest.mark.parametrize("rows,d,h,o", [(9, 40, 72, 24), (300, 48, 96, 49), (520, 264, 160, 264)])
 def test_ffn_activations(gpu, rows, d, h, o, act, dtype):
