@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace svox_decoder {
 
@@ -103,29 +104,34 @@ __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
 }
 // act(g); slope: its derivative too
-template <bool accurate>
-__device__ __forceinline__ float activate(int activation, float g, float* slope) {
+template <bool accurate, int activation>
+__device__ __forceinline__ float activate(float g, float* slope) {
+    if constexpr (activation == kSilu) {
+        const float s = sigmoid<accurate>(g);
+        if (slope) *slope = s * (1.0f + g * (1.0f - s));
+        return g * s;
+    } else if constexpr (activation == kGelu) {
+        const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        if (slope) *slope = below + g * (accurate ? expf(-0.5f * g * g) : __expf(-0.5f * g * g)) * 0.3989422804014327f;
+        return g * below;
+    } else if constexpr (activation == kRelu) {
+        // (NaN stays NaN; the derivative at 0 is 0)
+        if (slope) *slope = g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
+        return g < 0.0f ? 0.0f : g;
+    } else {
+        const float s = sigmoid<accurate>(g);
+        if (slope) *slope = s * (1.0f - s);
+        return s;
+    }
+}
+// f with the activation as a constant, so that a loop over numbers asks once
+template <class F>
+__device__ __forceinline__ void with_activation(int activation, F f) {
     switch (activation) {
-        case kSilu: {
-            const float s = sigmoid<accurate>(g);
-            if (slope) *slope = s * (1.0f + g * (1.0f - s));
-            return g * s;
-        }
-        case kGelu: {
-            const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-            if (slope) *slope = below + g * (accurate ? expf(-0.5f * g * g) : __expf(-0.5f * g * g)) * 0.3989422804014327f;
-            return g * below;
-        }
-        case kRelu: {
-            // (NaN stays NaN; the derivative at 0 is 0)
-            if (slope) *slope = g > 0.0f ? 1.0f : (g != g ? g : 0.0f);
-            return g < 0.0f ? 0.0f : g;
-        }
-        default: {
-            const float s = sigmoid<accurate>(g);
-            if (slope) *slope = s * (1.0f - s);
-            return s;
-        }
+        case kSilu: return f(std::integral_constant<int, kSilu>());
+        case kGelu: return f(std::integral_constant<int, kGelu>());
+        case kRelu: return f(std::integral_constant<int, kRelu>());
+        default: return f(std::integral_constant<int, kSigmoid>());
     }
 }
 

@@ -136,9 +136,11 @@ __global__ __launch_bounds__(kFewHiddenWaves* kWave) void few_hidden_kernel(FewA
     if (wave >= MT || row >= p.rows || col >= p.ldh) return;
     const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
     f32x4 v;
+    with_activation(p.activation, [&](auto activation) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = col + i < p.hidden ? activate<planes == 3>(p.activation, sum[0][i] + bg[i], nullptr) * (sum[1][i] + bu[i]) : 0.0f;
+        for (int i = 0; i < 4; ++i)
+            v[i] = col + i < p.hidden ? activate<planes == 3, decltype(activation)::value>(sum[0][i] + bg[i], nullptr) * (sum[1][i] + bu[i]) : 0.0f;
+    });
     u16x4 part[planes];
     Form<T>::split(v, part);
 #pragma unroll

@@ -1,6 +1,6 @@
 // ffn_type.hip -- the kernels of the gated feed-forward block of one type (SVOX_DECODER_TYPE) and their launches.
 #include "entry.h"
-#include "few_kernels.h"
+#include "narrow_kernels.h"
 
 namespace svox_decoder {
 
@@ -78,6 +78,54 @@ int launch_few(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stre
     if (s.rows <= 16) launch_few<1>(p, stream);
     else if (s.rows <= 32) launch_few<2>(p, stream);
     else launch_few<4>(p, stream);
+    return check_launch("gated_ffn");
+}
+
+// ---- narrow layers
+constexpr int kNarrowMost = kPlanes == 1 ? 128 : 64;   // features, and numbers of the result
+bool narrow(const SvoxGatedFfn& s) { return s.dim <= kNarrowMost && s.out <= kNarrowMost; }
+// KD and KO, the 32s of features and of numbers of the result: 1, 2 or 4
+#define SVOX_NARROW_STEPS(n, K, ...)                                    \
+    if ((n) <= 32) { constexpr int K = 1; __VA_ARGS__; }                \
+    else if ((n) <= 64) { constexpr int K = 2; __VA_ARGS__; }           \
+    else if constexpr (kPlanes == 1) { constexpr int K = 4; __VA_ARGS__; }
+int narrow_steps(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
+int64_t narrow_numbers(const SvoxGatedFfn& s, bool backward) {   // of the chunks, 16-bit
+    const int64_t kd = narrow_steps(s.dim), ko = narrow_steps(s.out);
+    return pieces(s.hidden, 32) * ((4 * kd + 2 * ko + (backward ? 4 * kd : 0)) * kPlanes + 1) * 512;
+}
+NarrowArgs<T> narrow_args(const SvoxGatedFfn& s, const u16* chunks) {
+    NarrowArgs<T> p{};
+    p.x = (const T*)s.x;
+    p.x_ld = s.x_stride;
+    p.chunks = chunks;
+    p.rows = s.rows;
+    p.dim = s.dim;
+    p.hidden = s.hidden;
+    p.out = s.out;
+    p.activation = s.activation;
+    return p;
+}
+template <int KD, int KO, bool backward>
+void launch_narrow_lay(const SvoxGatedFfn& s, u16* to, hipStream_t stream) {
+    using C = Chunk<KD, KO, backward>;
+    NarrowLayArgs<T> p{(const T*)s.w_gate, (const T*)s.w_up, (const T*)s.w_down, (const T*)s.b_gate, (const T*)s.b_up, s.dim, s.hidden, s.out, to};
+    hipLaunchKernelGGL((narrow_lay_kernel<T, KD, KO, backward>), dim3((unsigned)pieces(pieces(s.hidden, 32) * (C::fragments + 1), 4)), dim3(256), 0,
+                       stream, p);
+}
+int launch_narrow(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    Room room(workspace);
+    u16* const chunks = room.take<u16>(narrow_numbers(s, false));
+    NarrowArgs<T> p = narrow_args(s, chunks);
+    p.b_down = (const T*)s.b_down;
+    p.residual = (const T*)s.residual;
+    p.residual_ld = s.residual_stride;
+    p.y = (T*)y;
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
+        constexpr int QT = 2;
+        launch_narrow_lay<KD, KO, false>(s, chunks, stream);
+        hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)), dim3(kNarrowWaves * kWave), 0, stream, p);
+    }));
     return check_launch("gated_ffn");
 }
 
@@ -181,12 +229,18 @@ int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
         hidden_numbers(room, s);
         return room.used;
     }
+    if (narrow(s)) {
+        Room room(nullptr);
+        room.take<u16>(narrow_numbers(s, false));
+        return room.used;
+    }
     return Forward(s, nullptr).bytes;
 }
 
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
     if (s.rows <= kFewRows) return launch_few(s, y, workspace, stream);
+    if (narrow(s)) return launch_narrow(s, y, workspace, stream);
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);

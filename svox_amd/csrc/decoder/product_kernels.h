@@ -198,40 +198,42 @@ __global__ __launch_bounds__(S::threads) void hidden_kernel(HiddenArgs<T> p) {
         Back::template run<false>(p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
     }
     const Place<S> place(m0, n0);
+    with_activation(p.activation, [&](auto activation) {
 #pragma unroll
-    for (int n = 0; n < S::TN; ++n) {
-        const int64_t col = place.col(n);
-        if (col >= p.ldh) continue;
-        const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
+        for (int n = 0; n < S::TN; ++n) {
+            const int64_t col = place.col(n);
+            if (col >= p.ldh) continue;
+            const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
 #pragma unroll
-        for (int m = 0; m < S::TM; ++m) {
-            const int64_t row = place.row(m);
-            if (row >= p.rows) continue;
-            f32x4 h, dg, du;
+            for (int m = 0; m < S::TM; ++m) {
+                const int64_t row = place.row(m);
+                if (row >= p.rows) continue;
+                f32x4 h, dg, du;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float g = acc[0][m][n][i] + bg[i], u = acc[1][m][n][i] + bu[i];
-                float slope;
-                const float a = activate<planes == 3>(p.activation, g, backward ? &slope : nullptr);
-                h[i] = a * u;
+                for (int i = 0; i < 4; ++i) {
+                    const float g = acc[0][m][n][i] + bg[i], u = acc[1][m][n][i] + bu[i];
+                    float slope;
+                    const float a = activate<planes == 3, decltype(activation)::value>(g, backward ? &slope : nullptr);
+                    h[i] = a * u;
+                    if constexpr (backward) {
+                        dg[i] = dh[0][m][n][i] * u * slope;
+                        du[i] = dh[0][m][n][i] * a;
+                    }
+                }
+                u16x4 part[planes];
+                const int64_t at = row * p.ldh + col;
+                auto keep = [&](f32x4 v, u16* to) {
+                    Form<T>::split(v, part);
+                    for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(to + q * p.plane + at) = part[q];
+                };
+                keep(h, p.h);
                 if constexpr (backward) {
-                    dg[i] = dh[0][m][n][i] * u * slope;
-                    du[i] = dh[0][m][n][i] * a;
+                    keep(dg, p.dgate);
+                    keep(du, p.dup);
                 }
             }
-            u16x4 part[planes];
-            const int64_t at = row * p.ldh + col;
-            auto keep = [&](f32x4 v, u16* to) {
-                Form<T>::split(v, part);
-                for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(to + q * p.plane + at) = part[q];
-            };
-            keep(h, p.h);
-            if constexpr (backward) {
-                keep(dg, p.dgate);
-                keep(du, p.dup);
-            }
         }
-    }
+    });
 }
 
 template <class T>

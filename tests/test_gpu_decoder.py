@@ -76,6 +76,16 @@ def test_ffn_few_rows(gpu, rows, d, h, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows", [65, 127, 128, 300, 1111])
+@pytest.mark.parametrize("d,h,o", [(1, 1, 1), (31, 33, 28), (32, 32, 32), (33, 64, 49), (64, 100, 64), (65, 31, 76), (128, 300, 128), (127, 96, 4),
+                                   (28, 160, 120)])
+def test_ffn_narrow_layers(gpu, rows, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=rows + h)
+    wide = normal(torch.Generator().manual_seed(1), rows, d + 5, dtype=dtype)
+    check_ffn({**t, "x": wide[:, 2:d + 2]}, "silu", grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
 @pytest.mark.parametrize("rows,d,h,o", [(9, 40, 72, 24), (300, 48, 96, 49), (520, 264, 160, 264)])
 def test_ffn_activations(gpu, rows, d, h, o, act, dtype):
