@@ -129,6 +129,105 @@ int launch_narrow(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
     return check_launch("gated_ffn");
 }
 
+// the rows of narrow_weight_kernel's splits
+struct NarrowSplit {
+    int64_t down, each;   // blocks over the hidden units
+    int splits;
+};
+template <int KD, int KO>
+constexpr int kNarrowUnits = kPlanes == 1 && KD + KO <= 4 ? 2 : 1;   // tiles of 16 hidden units of a wavefront: as many as its registers hold
+int narrow_units(const SvoxGatedFfn& s) {
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, { return kNarrowUnits<KD, KO>; }));
+    return 1;
+}
+NarrowSplit narrow_split(const SvoxGatedFfn& s) {
+    NarrowSplit n;
+    n.down = pieces(s.hidden, 16 * narrow_units(s) * kNarrowWeightWaves);
+    int64_t splits = pieces(512, n.down);
+    if (splits > pieces(s.rows, 128)) splits = pieces(s.rows, 128);
+    n.each = up_to(pieces(s.rows, splits), 32);
+    n.splits = (int)pieces(s.rows, n.each);
+    return n;
+}
+int64_t gradient_numbers(const SvoxGatedFfn& s) {
+    return 2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + 2 * (int64_t)s.hidden + s.out;
+}
+
+// The parts of the weights' gradients, those of one after those of another, and the launch that adds them up.
+struct Parts {
+    JoinArgs<T> join{};
+    int64_t blocks = 0;
+    int jobs = 0;
+    float* at;
+    Parts(float* part, int splits) : at(part) { join.splits = splits; }
+    float* take(int64_t count, void* out) {
+        float* const part = at;
+        at += join.splits * count;
+        if (out) {
+            join.job[jobs] = {part, (T*)out, count};
+            join.blocks[jobs] = pieces(count, kJoinNumbers);
+            blocks += join.blocks[jobs++];
+        }
+        return part;
+    }
+    void launch(hipStream_t stream) const {
+        if (blocks > 0) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(kJoinThreads), 0, stream, join);
+    }
+};
+
+struct NarrowBackward {
+    u16* chunks;
+    float* part;
+    NarrowSplit split;
+    int64_t bytes;
+    NarrowBackward(const SvoxGatedFfn& s, void* workspace) {
+        Room room(workspace);
+        split = narrow_split(s);
+        chunks = room.take<u16>(narrow_numbers(s, true));
+        part = room.take<float>(split.splits * gradient_numbers(s));
+        bytes = room.used;
+    }
+};
+int launch_narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
+                           hipStream_t stream) {
+    const NarrowBackward b(s, workspace);
+    NarrowArgs<T> p = narrow_args(s, b.chunks);
+    p.dy = (const T*)grad_output;
+    p.dy_ld = grad_stride;
+    p.y = (T*)grads.x;
+    Parts parts(b.part, b.split.splits);
+    NarrowWeightArgs<T> w{};
+    w.x = p.x;
+    w.x_ld = p.x_ld;
+    w.dy = p.dy;
+    w.dy_ld = p.dy_ld;
+    w.chunks = b.chunks;
+    w.gate = parts.take((int64_t)s.hidden * s.dim, grads.w_gate);
+    w.up = parts.take((int64_t)s.hidden * s.dim, grads.w_up);
+    w.down = parts.take((int64_t)s.hidden * s.out, grads.w_down);
+    w.b_gate = parts.take(s.hidden, grads.b_gate);
+    w.b_up = parts.take(s.hidden, grads.b_up);
+    w.b_down = parts.take(s.out, grads.b_down);
+    w.rows = s.rows;
+    w.each = b.split.each;
+    w.dim = s.dim;
+    w.hidden = s.hidden;
+    w.out = s.out;
+    w.activation = s.activation;
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
+        constexpr int QT = 2, HT = kNarrowUnits<KD, KO>;
+        launch_narrow_lay<KD, KO, true>(s, b.chunks, stream);
+        if (grads.x)
+            hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
+                               dim3(kNarrowWaves * kWave), 0, stream, p);
+        if (parts.jobs)
+            hipLaunchKernelGGL((narrow_weight_kernel<T, KD, KO, HT>), dim3((unsigned)b.split.splits, (unsigned)b.split.down),
+                               dim3(kNarrowWeightWaves * kWave), 0, stream, w);
+    }));
+    parts.launch(stream);
+    return check_launch("gated_ffn_backward");
+}
+
 // ---- what a call keeps in its workspace
 struct Forward {
     Lays lays;
@@ -162,10 +261,6 @@ Split weight_split(const SvoxGatedFfn& s) {
     w.splits = (int)pieces(s.rows, w.each);
     return w;
 }
-int64_t gradient_numbers(const SvoxGatedFfn& s) {
-    return 2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + 2 * (int64_t)s.hidden + s.out;
-}
-
 struct Backward {
     Lays lays;
     Planes x, w_gate, w_up, w_down, dy, h, dgate, dup;
@@ -223,6 +318,7 @@ void launch_output(OutputArgs<T> p, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
+    if (backward && narrow(s)) return NarrowBackward(s, nullptr).bytes;
     if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
     if (s.rows <= kFewRows) {
         Room room(nullptr);
@@ -262,6 +358,7 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
 template <>
 int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
                            hipStream_t stream) {
+    if (narrow(s)) return launch_narrow_backward(s, grad_output, grad_stride, grads, workspace, stream);
     Backward b(s, grad_output, grad_stride, workspace, false);
     b.lays.launch(stream);
     HiddenArgs<T> p = hidden_args(s, b.x, b.w_gate, b.w_up, b.h);
@@ -284,15 +381,8 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
     }
     using S = WeightShape;
     WeightArgs<T> w{};
-    JoinArgs<T> join{};
     const int64_t H = s.hidden, D = s.dim, O = s.out;
-    float* part = b.part;
-    auto take = [&](int64_t count) {
-        float* const at = part;
-        if (part) part += b.split.splits * count;
-        return at;
-    };
-    // (a gradient that nobody wants is computed with the others and left in the workspace, or not at all)
+    Parts parts(b.part, b.split.splits);
     void* const outs[3] = {grads.w_gate, grads.w_up, grads.w_down};
     void* const sums[3] = {grads.b_gate, grads.b_up, grads.b_down};
     const Planes left[3] = {b.dgate, b.dup, b.dy}, right[3] = {b.x, b.x, b.h};
@@ -309,8 +399,10 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         job.tiles_n = pieces(job.n, S::BN);
         job.out = (T*)outs[j];
         job.sums_out = (T*)sums[j];
-        job.part = take(job.m * job.n);
-        job.sums_part = take(job.m);
+        if (b.split.splits > 1) {
+            job.part = parts.take(job.m * job.n, outs[j]);
+            job.sums_part = parts.take(job.m, sums[j]);
+        }
         blocks += job.tiles_m * job.tiles_n;
     }
     if (jobs) {
@@ -318,20 +410,7 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         w.each = b.split.each;
         w.splits = b.split.splits;
         hipLaunchKernelGGL((weight_kernel<T, S>), dim3((unsigned)blocks, (unsigned)w.splits), dim3(S::threads), 0, stream, w);
-        if (w.splits > 1) {
-            int64_t join_blocks = 0;
-            int n = 0;
-            for (int j = 0; j < jobs; ++j)
-                for (int which = 0; which < 2; ++which) {
-                    T* const to = which ? w.job[j].sums_out : w.job[j].out;
-                    if (!to) continue;
-                    join.job[n] = {which ? w.job[j].sums_part : w.job[j].part, to, which ? w.job[j].m : w.job[j].m * w.job[j].n};
-                    join.blocks[n] = pieces(join.job[n].count, kJoinNumbers);
-                    join_blocks += join.blocks[n++];
-                }
-            join.splits = w.splits;
-            hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)join_blocks), dim3(kJoinThreads), 0, stream, join);
-        }
+        parts.launch(stream);
     }
     return check_launch("gated_ffn_backward");
 }
