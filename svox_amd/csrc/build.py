@@ -32,6 +32,7 @@ POLICIES = [("SH", 25), ("SG", 25), ("SH", 16), ("SG", 16), ("SH", 9), ("SG", 9)
 
 # the types libsvox_decoder.so has kernels for
 DECODER_TYPES = ["float", "F16", "Bf16"]
+DECODER_ACTIVATIONS = ["kSilu", "kGelu", "kRelu", "kSigmoid"]
 
 
 def library_path():
@@ -52,6 +53,10 @@ def _decoder_units():
     for kernels in ("ffn", "norm"):
         for of in DECODER_TYPES:
             yield f"{kernels}_{of.lower()}", os.path.join("decoder", f"{kernels}_type.hip"), [f"-DSVOX_DECODER_TYPE={of}"]
+    for of in DECODER_TYPES:
+        for activation in DECODER_ACTIVATIONS:
+            yield (f"narrow_{of.lower()}_{activation.lower()}", os.path.join("decoder", "narrow_type.hip"),
+                   [f"-DSVOX_DECODER_TYPE={of}", f"-DSVOX_DECODER_ACTIVATION={activation}"])
     yield "decoder", os.path.join("decoder", "decoder.hip"), []
 
 

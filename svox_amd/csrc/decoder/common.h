@@ -103,16 +103,35 @@ __device__ __forceinline__ float sigmoid(float g) {
     if constexpr (accurate) return 1.0f / (1.0f + expf(-g));
     return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
 }
+// Phi(g), the normal distribution's, and exp(-g^2 / 2).  For results of 16 bits by 7.1.26 of Abramowitz and Stegun, Handbook of
+// Mathematical Functions: erf to 1.5e-7, with the exponential that the derivative needs as well.
+template <bool accurate>
+__device__ __forceinline__ float phi(float g, float& bell) {
+    if constexpr (accurate) {
+        bell = expf(-0.5f * g * g);
+        return 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    } else {
+        bell = __expf(-0.5f * g * g);
+        const float x = __builtin_fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+        float poly = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+        poly = __builtin_fmaf(poly, t, 1.421413741f);
+        poly = __builtin_fmaf(poly, t, -0.284496736f);
+        poly = __builtin_fmaf(poly, t, 0.254829592f);
+        const float beyond = 0.5f * poly * t * bell;   // 1 - Phi(|g|)
+        return g < 0.0f ? beyond : 1.0f - beyond;
+    }
+}
 // act(g); slope: its derivative too
 template <bool accurate, int activation>
 __device__ __forceinline__ float activate(float g, float* slope) {
     if constexpr (activation == kSilu) {
-        const float s = sigmoid<accurate>(g);
-        if (slope) *slope = s * (1.0f + g * (1.0f - s));
-        return g * s;
+        const float s = sigmoid<accurate>(g), a = g * s;
+        if (slope) *slope = __builtin_fmaf(a, 1.0f - s, s);
+        return a;
     } else if constexpr (activation == kGelu) {
-        const float below = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-        if (slope) *slope = below + g * (accurate ? expf(-0.5f * g * g) : __expf(-0.5f * g * g)) * 0.3989422804014327f;
+        float bell;
+        const float below = phi<accurate>(g, bell);
+        if (slope) *slope = __builtin_fmaf(g * 0.3989422804014327f, bell, below);
         return g * below;
     } else if constexpr (activation == kRelu) {
         // (NaN stays NaN; the derivative at 0 is 0)

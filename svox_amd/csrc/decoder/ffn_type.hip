@@ -1,6 +1,5 @@
 // ffn_type.hip -- the kernels of the gated feed-forward block of one type (SVOX_DECODER_TYPE) and their launches.
-#include "entry.h"
-#include "narrow_kernels.h"
+#include "ffn_plan.h"
 
 namespace svox_decoder {
 
@@ -82,150 +81,14 @@ int launch_few(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stre
 }
 
 // ---- narrow layers
-constexpr int kNarrowMost = kPlanes == 1 ? 128 : 64;   // features, and numbers of the result
-bool narrow(const SvoxGatedFfn& s) { return s.dim <= kNarrowMost && s.out <= kNarrowMost; }
-// KD and KO, the 32s of features and of numbers of the result: 1, 2 or 4
-#define SVOX_NARROW_STEPS(n, K, ...)                                    \
-    if ((n) <= 32) { constexpr int K = 1; __VA_ARGS__; }                \
-    else if ((n) <= 64) { constexpr int K = 2; __VA_ARGS__; }           \
-    else if constexpr (kPlanes == 1) { constexpr int K = 4; __VA_ARGS__; }
-int narrow_steps(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
-int64_t narrow_numbers(const SvoxGatedFfn& s, bool backward) {   // of the chunks, 16-bit
-    const int64_t kd = narrow_steps(s.dim), ko = narrow_steps(s.out);
-    return pieces(s.hidden, 32) * ((4 * kd + 2 * ko + (backward ? 4 * kd : 0)) * kPlanes + 1) * 512;
-}
-NarrowArgs<T> narrow_args(const SvoxGatedFfn& s, const u16* chunks) {
-    NarrowArgs<T> p{};
-    p.x = (const T*)s.x;
-    p.x_ld = s.x_stride;
-    p.chunks = chunks;
-    p.rows = s.rows;
-    p.dim = s.dim;
-    p.hidden = s.hidden;
-    p.out = s.out;
-    p.activation = s.activation;
-    return p;
-}
-template <int KD, int KO, bool backward>
-void launch_narrow_lay(const SvoxGatedFfn& s, u16* to, hipStream_t stream) {
-    using C = Chunk<KD, KO, backward>;
-    NarrowLayArgs<T> p{(const T*)s.w_gate, (const T*)s.w_up, (const T*)s.w_down, (const T*)s.b_gate, (const T*)s.b_up, s.dim, s.hidden, s.out, to};
-    hipLaunchKernelGGL((narrow_lay_kernel<T, KD, KO, backward>), dim3((unsigned)pieces(pieces(s.hidden, 32) * (C::fragments + 1), 4)), dim3(256), 0,
-                       stream, p);
-}
-int launch_narrow(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
-    Room room(workspace);
-    u16* const chunks = room.take<u16>(narrow_numbers(s, false));
-    NarrowArgs<T> p = narrow_args(s, chunks);
-    p.b_down = (const T*)s.b_down;
-    p.residual = (const T*)s.residual;
-    p.residual_ld = s.residual_stride;
-    p.y = (T*)y;
-    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
-        constexpr int QT = 2;
-        launch_narrow_lay<KD, KO, false>(s, chunks, stream);
-        hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)), dim3(kNarrowWaves * kWave), 0, stream, p);
-    }));
-    return check_launch("gated_ffn");
-}
-
-// the rows of narrow_weight_kernel's splits
-struct NarrowSplit {
-    int64_t down, each;   // blocks over the hidden units
-    int splits;
-};
-template <int KD, int KO>
-constexpr int kNarrowUnits = kPlanes == 1 && KD + KO <= 4 ? 2 : 1;   // tiles of 16 hidden units of a wavefront: as many as its registers hold
-int narrow_units(const SvoxGatedFfn& s) {
-    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, { return kNarrowUnits<KD, KO>; }));
-    return 1;
-}
-NarrowSplit narrow_split(const SvoxGatedFfn& s) {
-    NarrowSplit n;
-    n.down = pieces(s.hidden, 16 * narrow_units(s) * kNarrowWeightWaves);
-    int64_t splits = pieces(512, n.down);
-    if (splits > pieces(s.rows, 128)) splits = pieces(s.rows, 128);
-    n.each = up_to(pieces(s.rows, splits), 32);
-    n.splits = (int)pieces(s.rows, n.each);
-    return n;
-}
-int64_t gradient_numbers(const SvoxGatedFfn& s) {
-    return 2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + 2 * (int64_t)s.hidden + s.out;
-}
-
-// The parts of the weights' gradients, those of one after those of another, and the launch that adds them up.
-struct Parts {
-    JoinArgs<T> join{};
-    int64_t blocks = 0;
-    int jobs = 0;
-    float* at;
-    Parts(float* part, int splits) : at(part) { join.splits = splits; }
-    float* take(int64_t count, void* out) {
-        float* const part = at;
-        at += join.splits * count;
-        if (out) {
-            join.job[jobs] = {part, (T*)out, count};
-            join.blocks[jobs] = pieces(count, kJoinNumbers);
-            blocks += join.blocks[jobs++];
-        }
-        return part;
+template <class F>
+int by_activation(int activation, F f) {
+    switch (activation) {
+        case kSilu: return f(std::integral_constant<int, kSilu>());
+        case kGelu: return f(std::integral_constant<int, kGelu>());
+        case kRelu: return f(std::integral_constant<int, kRelu>());
+        default: return f(std::integral_constant<int, kSigmoid>());
     }
-    void launch(hipStream_t stream) const {
-        if (blocks > 0) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(kJoinThreads), 0, stream, join);
-    }
-};
-
-struct NarrowBackward {
-    u16* chunks;
-    float* part;
-    NarrowSplit split;
-    int64_t bytes;
-    NarrowBackward(const SvoxGatedFfn& s, void* workspace) {
-        Room room(workspace);
-        split = narrow_split(s);
-        chunks = room.take<u16>(narrow_numbers(s, true));
-        part = room.take<float>(split.splits * gradient_numbers(s));
-        bytes = room.used;
-    }
-};
-int launch_narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
-                           hipStream_t stream) {
-    const NarrowBackward b(s, workspace);
-    NarrowArgs<T> p = narrow_args(s, b.chunks);
-    p.dy = (const T*)grad_output;
-    p.dy_ld = grad_stride;
-    p.y = (T*)grads.x;
-    Parts parts(b.part, b.split.splits);
-    NarrowWeightArgs<T> w{};
-    w.x = p.x;
-    w.x_ld = p.x_ld;
-    w.dy = p.dy;
-    w.dy_ld = p.dy_ld;
-    w.chunks = b.chunks;
-    w.gate = parts.take((int64_t)s.hidden * s.dim, grads.w_gate);
-    w.up = parts.take((int64_t)s.hidden * s.dim, grads.w_up);
-    w.down = parts.take((int64_t)s.hidden * s.out, grads.w_down);
-    w.b_gate = parts.take(s.hidden, grads.b_gate);
-    w.b_up = parts.take(s.hidden, grads.b_up);
-    w.b_down = parts.take(s.out, grads.b_down);
-    w.rows = s.rows;
-    w.each = b.split.each;
-    w.dim = s.dim;
-    w.hidden = s.hidden;
-    w.out = s.out;
-    w.activation = s.activation;
-    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
-        constexpr int QT = 2, HT = kNarrowUnits<KD, KO>;
-        launch_narrow_lay<KD, KO, true>(s, b.chunks, stream);
-        if (grads.x)
-            hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
-                               dim3(kNarrowWaves * kWave), 0, stream, p);
-        if (parts.jobs)
-            hipLaunchKernelGGL((narrow_weight_kernel<T, KD, KO, HT>), dim3((unsigned)b.split.splits, (unsigned)b.split.down),
-                               dim3(kNarrowWeightWaves * kWave), 0, stream, w);
-    }));
-    parts.launch(stream);
-    return check_launch("gated_ffn_backward");
 }
 
 // ---- what a call keeps in its workspace
@@ -318,16 +181,16 @@ void launch_output(OutputArgs<T> p, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
-    if (backward && narrow(s)) return NarrowBackward(s, nullptr).bytes;
+    if (backward && narrow<T>(s)) return NarrowBackward<T>(s, nullptr).bytes;
     if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
     if (s.rows <= kFewRows) {
         Room room(nullptr);
         hidden_numbers(room, s);
         return room.used;
     }
-    if (narrow(s)) {
+    if (narrow<T>(s)) {
         Room room(nullptr);
-        room.take<u16>(narrow_numbers(s, false));
+        room.take<u16>(narrow_numbers<T>(s, false));
         return room.used;
     }
     return Forward(s, nullptr).bytes;
@@ -336,7 +199,7 @@ int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
     if (s.rows <= kFewRows) return launch_few(s, y, workspace, stream);
-    if (narrow(s)) return launch_narrow(s, y, workspace, stream);
+    if (narrow<T>(s)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);
@@ -358,7 +221,10 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
 template <>
 int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
                            hipStream_t stream) {
-    if (narrow(s)) return launch_narrow_backward(s, grad_output, grad_stride, grads, workspace, stream);
+    if (narrow<T>(s))
+        return by_activation(s.activation, [&](auto a) {
+            return Narrow<T, decltype(a)::value>::backward(s, grad_output, grad_stride, grads, workspace, stream);
+        });
     Backward b(s, grad_output, grad_stride, workspace, false);
     b.lays.launch(stream);
     HiddenArgs<T> p = hidden_args(s, b.x, b.w_gate, b.w_up, b.h);
@@ -382,7 +248,7 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
     using S = WeightShape;
     WeightArgs<T> w{};
     const int64_t H = s.hidden, D = s.dim, O = s.out;
-    Parts parts(b.part, b.split.splits);
+    Parts<T> parts(b.part, b.split.splits);
     void* const outs[3] = {grads.w_gate, grads.w_up, grads.w_down};
     void* const sums[3] = {grads.b_gate, grads.b_up, grads.b_down};
     const Planes left[3] = {b.dgate, b.dup, b.dy}, right[3] = {b.x, b.x, b.h};

@@ -122,23 +122,26 @@ struct NarrowArgs {
     int64_t residual_ld;
     T* y;                    // (rows, out); backward: dx (rows, dim)
     int64_t rows, dim, hidden, out;
-    int activation;
 };
 
 constexpr int kNarrowWaves = 4;
 
 // the two tiles of 4 hidden numbers of a lane, as the 8 of a reduction over them
 template <class T>
+__device__ __forceinline__ void turn(const u16x4 (&half)[2][Form<T>::planes], u16x8 (&out)[Form<T>::planes]) {
+#pragma unroll
+    for (int q = 0; q < Form<T>::planes; ++q) out[q] = __builtin_shufflevector(half[0][q], half[1][q], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <class T>
 __device__ __forceinline__ void turn(const f32x4 (&v)[2], u16x8 (&out)[Form<T>::planes]) {
     u16x4 half[2][Form<T>::planes];
     Form<T>::split(v[0], half[0]);
     Form<T>::split(v[1], half[1]);
-#pragma unroll
-    for (int q = 0; q < Form<T>::planes; ++q) out[q] = __builtin_shufflevector(half[0][q], half[1][q], 0, 1, 2, 3, 4, 5, 6, 7);
+    turn<T>(half, out);
 }
 
 // Rows go 16 QT to a wavefront.
-template <class T, int KD, int KO, int QT>
+template <class T, int KD, int KO, int QT, int activation>
 __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<T> p) {
     using C = Chunk<KD, KO, false>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, OT = 2 * KO;
@@ -178,12 +181,10 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<
                     up[q] = multiply<T>(wu, x[q][s], up[q]);
                 }
             }
-            with_activation(p.activation, [&](auto activation) {
 #pragma unroll
-                for (int q = 0; q < QT; ++q)
+            for (int q = 0; q < QT; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[q][t][i] = activate<planes == 3, decltype(activation)::value>(gate[q][i], nullptr) * up[q][i];
-            });
+                for (int i = 0; i < 4; ++i) h[q][t][i] = activate<planes == 3, activation>(gate[q][i], nullptr) * up[q][i];
         }
         u16x8 turned[QT][planes];
 #pragma unroll
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<
 }
 
 // dx: as narrow_kernel, with dh' = Wd' dy' and dx' = Wg' dgate' + Wu' dup' in place of y'.
-template <class T, int KD, int KO, int QT>
+template <class T, int KD, int KO, int QT, int activation>
 __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_backward_kernel(NarrowArgs<T> p) {
     using C = Chunk<KD, KO, true>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, DT = 2 * KD;
@@ -263,17 +264,15 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_backward_kernel(Na
 #pragma unroll
                 for (int q = 0; q < QT; ++q) dh[q] = multiply<T>(wd, dy[q][s], dh[q]);
             }
-            with_activation(p.activation, [&](auto activation) {
 #pragma unroll
-                for (int q = 0; q < QT; ++q)
+            for (int q = 0; q < QT; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float slope;
-                        const float a = activate<planes == 3, decltype(activation)::value>(gate[q][i], &slope);
-                        dg[q][t][i] = dh[q][i] * up[q][i] * slope;
-                        du[q][t][i] = dh[q][i] * a;
-                    }
-            });
+                for (int i = 0; i < 4; ++i) {
+                    float slope;
+                    const float a = activate<planes == 3, activation>(gate[q][i], &slope);
+                    dg[q][t][i] = dh[q][i] * up[q][i] * slope;
+                    du[q][t][i] = dh[q][i] * a;
+                }
         }
         u16x8 turned_g[QT][planes], turned_u[QT][planes];
 #pragma unroll
@@ -362,15 +361,14 @@ struct NarrowWeightArgs {
     float *gate, *up, *down, *b_gate, *b_up, *b_down;   // [splits] of each gradient
     int64_t rows, each;                                 // rows of a split: a whole number of 32
     int64_t dim, hidden, out;
-    int activation;
 };
 
 // The gradients of the weights over a share of the rows: a wavefront has 16 HT hidden units, their weights and their sums in
 // registers, and a block's wavefronts go through the rows together, 32 at a time: gate, up and dh of those rows and units (rows down
 // this time, a lane has 4 rows of a unit), and the products of what comes of them with the columns of x and dy.
-constexpr int kNarrowWeightWaves = 4;
-template <class T, int KD, int KO, int HT>
-__global__ __launch_bounds__(kNarrowWeightWaves* kWave) void narrow_weight_kernel(NarrowWeightArgs<T> p) {
+constexpr int kNarrowWeightWaves = 8;
+template <class T, int KD, int KO, int HT, int activation>
+__global__ __launch_bounds__(kNarrowWeightWaves* kWave, 2) void narrow_weight_kernel(NarrowWeightArgs<T> p) {
     using C = Chunk<KD, KO, true>;
     constexpr int planes = Form<T>::planes, DT = 2 * KD, OT = 2 * KO, threads = kNarrowWeightWaves * kWave;
     using X = RowTile<KD, planes>;
@@ -450,7 +448,7 @@ __global__ __launch_bounds__(kNarrowWeightWaves* kWave) void narrow_weight_kerne
         __syncthreads();
         if (row0 + 32 < end) read(row0 + 32);
         if (!works) continue;
-        f32x4 h[HT][2], dg[HT][2], du[HT][2];
+        u16x4 h[HT][2][planes], dg[HT][2][planes], du[HT][2][planes];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             f32x4 gate[HT], up[HT], dh[HT];
@@ -470,20 +468,23 @@ __global__ __launch_bounds__(kNarrowWeightWaves* kWave) void narrow_weight_kerne
 #pragma unroll
                 for (int t = 0; t < HT; ++t) dh[t] = multiply<T>(a, wd[t][s], dh[t]);
             }
-            with_activation(p.activation, [&](auto activation) {
 #pragma unroll
-                for (int t = 0; t < HT; ++t)
+            for (int t = 0; t < HT; ++t) {
+                f32x4 vh, vg, vu;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float slope;
-                        const float a = activate<planes == 3, decltype(activation)::value>(gate[t][i], &slope);
-                        h[t][q][i] = a * up[t][i];
-                        dg[t][q][i] = dh[t][i] * up[t][i] * slope;
-                        du[t][q][i] = dh[t][i] * a;
-                        bg_sum[t] += dg[t][q][i];
-                        bu_sum[t] += du[t][q][i];
-                    }
-            });
+                for (int i = 0; i < 4; ++i) {
+                    float slope;
+                    const float a = activate<planes == 3, activation>(gate[t][i], &slope);
+                    vh[i] = a * up[t][i];
+                    vg[i] = dh[t][i] * up[t][i] * slope;
+                    vu[i] = dh[t][i] * a;
+                    bg_sum[t] += vg[i];
+                    bu_sum[t] += vu[i];
+                }
+                Form<T>::split(vh, h[t][q]);
+                Form<T>::split(vg, dg[t][q]);
+                Form<T>::split(vu, du[t][q]);
+            }
         }
         u16x8 th[HT][planes], tg[HT][planes], tu[HT][planes];
 #pragma unroll

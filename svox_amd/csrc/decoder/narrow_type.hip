@@ -1,0 +1,97 @@
+// narrow_type.hip -- the kernels of narrow layers of one type (SVOX_DECODER_TYPE) with one activation (SVOX_DECODER_ACTIVATION), and
+// their launches.
+#include "ffn_plan.h"
+
+namespace svox_decoder {
+
+using T = SVOX_DECODER_TYPE;
+constexpr int kActivation = SVOX_DECODER_ACTIVATION;
+
+namespace {
+
+NarrowArgs<T> narrow_args(const SvoxGatedFfn& s, const u16* chunks) {
+    NarrowArgs<T> p{};
+    p.x = (const T*)s.x;
+    p.x_ld = s.x_stride;
+    p.chunks = chunks;
+    p.rows = s.rows;
+    p.dim = s.dim;
+    p.hidden = s.hidden;
+    p.out = s.out;
+    return p;
+}
+template <int KD, int KO, bool backward>
+void launch_narrow_lay(const SvoxGatedFfn& s, u16* to, hipStream_t stream) {
+    using C = Chunk<KD, KO, backward>;
+    NarrowLayArgs<T> p{(const T*)s.w_gate, (const T*)s.w_up, (const T*)s.w_down, (const T*)s.b_gate, (const T*)s.b_up, s.dim, s.hidden, s.out, to};
+    hipLaunchKernelGGL((narrow_lay_kernel<T, KD, KO, backward>), dim3((unsigned)pieces(pieces(s.hidden, 32) * (C::fragments + 1), 4)), dim3(256), 0,
+                       stream, p);
+}
+int narrow_forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    Room room(workspace);
+    u16* const chunks = room.take<u16>(narrow_numbers<T>(s, false));
+    NarrowArgs<T> p = narrow_args(s, chunks);
+    p.b_down = (const T*)s.b_down;
+    p.residual = (const T*)s.residual;
+    p.residual_ld = s.residual_stride;
+    p.y = (T*)y;
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
+        constexpr int QT = 2;
+        launch_narrow_lay<KD, KO, false>(s, chunks, stream);
+        hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)), dim3(kNarrowWaves * kWave), 0, stream, p);
+    }));
+    return check_launch("gated_ffn");
+}
+
+int narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
+                           hipStream_t stream) {
+    const NarrowBackward<T> b(s, workspace);
+    NarrowArgs<T> p = narrow_args(s, b.chunks);
+    p.dy = (const T*)grad_output;
+    p.dy_ld = grad_stride;
+    p.y = (T*)grads.x;
+    Parts<T> parts(b.part, b.split.splits);
+    NarrowWeightArgs<T> w{};
+    w.x = p.x;
+    w.x_ld = p.x_ld;
+    w.dy = p.dy;
+    w.dy_ld = p.dy_ld;
+    w.chunks = b.chunks;
+    w.gate = parts.take((int64_t)s.hidden * s.dim, grads.w_gate);
+    w.up = parts.take((int64_t)s.hidden * s.dim, grads.w_up);
+    w.down = parts.take((int64_t)s.hidden * s.out, grads.w_down);
+    w.b_gate = parts.take(s.hidden, grads.b_gate);
+    w.b_up = parts.take(s.hidden, grads.b_up);
+    w.b_down = parts.take(s.out, grads.b_down);
+    w.rows = s.rows;
+    w.each = b.split.each;
+    w.dim = s.dim;
+    w.hidden = s.hidden;
+    w.out = s.out;
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
+        constexpr int QT = 2, HT = kNarrowUnits<T, KD, KO>;
+        launch_narrow_lay<KD, KO, true>(s, b.chunks, stream);
+        if (grads.x)
+            hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
+                               dim3(kNarrowWaves * kWave), 0, stream, p);
+        if (parts.jobs)
+            hipLaunchKernelGGL((narrow_weight_kernel<T, KD, KO, HT, kActivation>), dim3((unsigned)b.split.splits, (unsigned)b.split.down),
+                               dim3(kNarrowWeightWaves * kWave), 0, stream, w);
+    }));
+    parts.launch(stream);
+    return check_launch("gated_ffn_backward");
+}
+
+}  // namespace
+
+template <>
+int Narrow<T, kActivation>::forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    return narrow_forward(s, y, workspace, stream);
+}
+template <>
+int Narrow<T, kActivation>::backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads,
+                                     void* workspace, hipStream_t stream) {
+    return narrow_backward(s, grad_output, grad_stride, grads, workspace, stream);
+}
+
+}  // namespace svox_decoder
