@@ -113,7 +113,7 @@ constexpr int kFewHiddenWaves = 4, kFewOutputWaves = 8;
 
 // Grid: 16 hidden units a block (the last ones to the end of h's rows), 16 MT rows.
 template <class T, int MT>
-__global__ __launch_bounds__(kFewHiddenWaves* kWave) void few_hidden_kernel(FewArgs<T> p) {
+__global__ __launch_bounds__(kFewHiddenWaves* kWave, 2) void few_hidden_kernel(FewArgs<T> p) {
     constexpr int planes = Form<T>::planes, waves = kFewHiddenWaves;
     __shared__ f32x4 shared[waves * 2 * MT * kWave];
     const int lane = threadIdx.x % kWave, l = lane & 15, wave = threadIdx.x / kWave;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kFewHiddenWaves* kWave) void few_hidden_kernel(FewA
 
 // Grid: 16 numbers of the result a block, 16 MT rows.
 template <class T, int MT>
-__global__ __launch_bounds__(kFewOutputWaves* kWave) void few_output_kernel(FewArgs<T> p) {
+__global__ __launch_bounds__(kFewOutputWaves* kWave, 2) void few_output_kernel(FewArgs<T> p) {
     constexpr int waves = kFewOutputWaves;
     __shared__ f32x4 shared[waves * MT * kWave];
     const int lane = threadIdx.x % kWave, l = lane & 15, wave = threadIdx.x / kWave;

@@ -140,9 +140,17 @@ __device__ __forceinline__ void turn(const f32x4 (&v)[2], u16x8 (&out)[Form<T>::
     turn<T>(half, out);
 }
 
+// The biases of a lane's 4 hidden units, as what their sums begin with: read for each tile anew, straight to where it adds up,
+// since vector instructions are what these kernels run out of and reads of LDS are not.
+__device__ __forceinline__ void biases(const float* bias, int unit, f32x4& gate, f32x4& up) {
+    asm("" : "+v"(unit));   // (or one read would be copied to all tiles)
+    gate = *reinterpret_cast<const f32x4*>(bias + unit);
+    up = *reinterpret_cast<const f32x4*>(bias + 32 + unit);
+}
+
 // Rows go 16 QT to a wavefront.
 template <class T, int KD, int KO, int QT, int activation>
-__global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<T> p) {
+__global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_kernel(NarrowArgs<T> p) {
     using C = Chunk<KD, KO, false>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, OT = 2 * KO;
     __shared__ __align__(16) u16 lds[2][kib * 512];
@@ -166,10 +174,9 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<
         f32x4 h[QT][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const f32x4 bg = *reinterpret_cast<const f32x4*>(bias + t * 16 + g * 4), bu = *reinterpret_cast<const f32x4*>(bias + 32 + t * 16 + g * 4);
             f32x4 gate[QT], up[QT];
 #pragma unroll
-            for (int q = 0; q < QT; ++q) gate[q] = bg, up[q] = bu;
+            for (int q = 0; q < QT; ++q) biases(bias, t * 16 + g * 4, gate[q], up[q]);
 #pragma unroll
             for (int s = 0; s < KD; ++s) {
                 u16x8 wg[planes], wu[planes];
@@ -215,7 +222,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_kernel(NarrowArgs<
 
 // dx: as narrow_kernel, with dh' = Wd' dy' and dx' = Wg' dgate' + Wu' dup' in place of y'.
 template <class T, int KD, int KO, int QT, int activation>
-__global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_backward_kernel(NarrowArgs<T> p) {
+__global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_backward_kernel(NarrowArgs<T> p) {
     using C = Chunk<KD, KO, true>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, DT = 2 * KD;
     __shared__ __align__(16) u16 lds[2][kib * 512];
@@ -242,10 +249,9 @@ __global__ __launch_bounds__(kNarrowWaves* kWave) void narrow_backward_kernel(Na
         f32x4 dg[QT][2], du[QT][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const f32x4 bg = *reinterpret_cast<const f32x4*>(bias + t * 16 + g * 4), bu = *reinterpret_cast<const f32x4*>(bias + 32 + t * 16 + g * 4);
             f32x4 gate[QT], up[QT], dh[QT];
 #pragma unroll
-            for (int q = 0; q < QT; ++q) gate[q] = bg, up[q] = bu, dh[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int q = 0; q < QT; ++q) biases(bias, t * 16 + g * 4, gate[q], up[q]), dh[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < KD; ++s) {
                 u16x8 wg[planes], wu[planes];

@@ -180,7 +180,7 @@ struct HiddenArgs {
 };
 
 template <class T, class S, bool backward>
-__global__ __launch_bounds__(S::threads) void hidden_kernel(HiddenArgs<T> p) {
+__global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) {
     using Forward = Product<T, S, true, true, 2>;
     using Back = Product<T, S, true, false, 1>;
     constexpr int planes = Form<T>::planes;
@@ -249,7 +249,7 @@ struct OutputArgs {
 
 // along_b: b is (cols, reduction), else (reduction, cols)
 template <class T, class S, bool along_b>
-__global__ __launch_bounds__(S::threads) void output_kernel(OutputArgs<T> p) {
+__global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) {
     using P = Product<T, S, true, along_b, 1>;
     __shared__ __align__(16) u16 lds[S::stages * P::stage];
     int64_t tm, tn;
@@ -291,7 +291,7 @@ struct WeightArgs {
 };
 
 template <class T, class S>
-__global__ __launch_bounds__(S::threads) void weight_kernel(WeightArgs<T> p) {
+__global__ __launch_bounds__(S::threads, 2) void weight_kernel(WeightArgs<T> p) {
     using P = Product<T, S, false, false, 1>;
     __shared__ __align__(16) u16 lds[S::stages * P::stage];
     int64_t block = blockIdx.x;
