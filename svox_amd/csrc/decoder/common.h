@@ -94,6 +94,21 @@ __device__ __forceinline__ void store_few(T* at, typename Few<T, N>::vector v) {
     reinterpret_cast<Few<T, N>*>(at)->v = v;
 }
 
+// N numbers from `at` on of which `room` can be read: all of them in one load, or one by one where there is no room.  What a branch
+// leaves is the numbers as they lie in memory; they are converted behind it, so that the load is waited for there and not in the
+// branch.
+template <class T, int N>
+__device__ __forceinline__ typename Few<T, N>::vector load_some(const T* at, int64_t room) {
+    typename Few<T, N>::vector v;
+    if (room >= N) {
+        v = load_few<T, N>(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < room ? at[i] : (T)0.0f;
+    }
+    return v;
+}
+
 // ---- activations
 enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
 

@@ -29,7 +29,7 @@ __device__ __forceinline__ void pieces_of(const T* from, int64_t there, u16x8* o
     if (there >= 8) return pieces_of(from, out);
     u16x4 half[2][Form<T>::planes];
     Form<T>::split(four_of(from, 0, there), half[0]);
-    Form<T>::split(there > 4 ? four_of(from, 4, there) : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, half[1]);
+    Form<T>::split(there > 4 ? four_of(from, 4, there - 4) : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, half[1]);
 #pragma unroll
     for (int p = 0; p < Form<T>::planes; ++p) out[p] = __builtin_shufflevector(half[0][p], half[1][p], 0, 1, 2, 3, 4, 5, 6, 7);
 }
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kFewHiddenWaves* kWave, 2) void few_hidden_kernel(F
     few_join<2, MT, waves>(acc, sum, shared);
     const int64_t row = row0 + wave * 16 + l, col = h0 + lane / 16 * 4;
     if (wave >= MT || row >= p.rows || col >= p.ldh) return;
-    const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
+    const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
     f32x4 v;
     with_activation(p.activation, [&](auto activation) {
 #pragma unroll
@@ -166,8 +166,8 @@ __global__ __launch_bounds__(kFewOutputWaves* kWave, 2) void few_output_kernel(F
     few_join<1, MT, waves>(acc, sum, shared);
     const int64_t row = row0 + wave * 16 + l, col = o0 + lane / 16 * 4;
     if (wave >= MT || row >= p.rows || col >= p.out) return;
-    f32x4 v = sum[0] + four_of(p.b_down, col, p.out);
-    if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, p.out);
+    f32x4 v = sum[0] + four_of(p.b_down, col, p.out - col);
+    if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, p.out - col);
     store_four(p.y + row * p.out, v, col, p.out);
 }
 

@@ -56,17 +56,15 @@ struct NarrowSplit {
     int64_t down, each;   // blocks over the hidden units
     int splits;
 };
-template <class T, int KD, int KO>
-constexpr int kNarrowUnits = Form<T>::planes == 1 && KD + KO <= 2 ? 2 : 1;   // tiles of 16 hidden units of a wavefront: as many as its registers hold
 template <class T>
-int narrow_units(const SvoxGatedFfn& s) {
-    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, { return kNarrowUnits<T, KD, KO>; }));
+int narrow_weight_waves(const SvoxGatedFfn& s) {
+    SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, { return (kNarrowWeightWaves<T, KD, KO>); }));
     return 1;
 }
 template <class T>
 NarrowSplit narrow_split(const SvoxGatedFfn& s) {
     NarrowSplit n;
-    n.down = pieces(s.hidden, 16 * narrow_units<T>(s) * kNarrowWeightWaves);
+    n.down = pieces(s.hidden, 16 * narrow_weight_waves<T>(s));
     int64_t splits = pieces(512, n.down);
     if (splits > pieces(s.rows, 128)) splits = pieces(s.rows, 128);
     n.each = up_to(pieces(s.rows, splits), 32);

@@ -104,15 +104,6 @@ __device__ __forceinline__ void fragment_of(const u16* lds, int f, u16x8 (&out)[
     for (int q = 0; q < planes; ++q) out[q] = *reinterpret_cast<const u16x8*>(lds + (f * planes + q) * 512 + threadIdx.x % kWave * 8);
 }
 
-// Rows in fragments: K * 32 numbers of row `row` (as far as `count` goes; nothing of a row that is not there).
-template <class T, int K>
-__device__ __forceinline__ void row_fragments(const T* m, int64_t ld, int64_t row, int64_t rows, int64_t count, u16x8 (&out)[K][Form<T>::planes]) {
-    const int g = threadIdx.x % kWave / 16;
-    const T* const from = m + least(row, rows - 1) * ld;
-#pragma unroll
-    for (int s = 0; s < K; ++s) pieces_of(from + s * 32 + g * 8, row < rows ? count - (s * 32 + g * 8) : 0, out[s]);
-}
-
 template <class T>
 struct NarrowArgs {
     const T *x, *dy;         // (rows, dim), (rows, out)
@@ -140,6 +131,103 @@ __device__ __forceinline__ void turn(const f32x4 (&v)[2], u16x8 (&out)[Form<T>::
     turn<T>(half, out);
 }
 
+// 8 numbers of a row as they lie in memory, to be laid out when they have arrived.  `there` of them are the row's (all that is read
+// beyond is taken for zeros), `room` can be read.
+template <class T>
+struct Raw {
+    typename Few<T, 8>::vector v;
+    __device__ __forceinline__ void read(const T* at, int64_t there, int64_t room) {
+        if (there > 0)
+            v = load_some<T, 8>(at, room);
+        else
+            v = 0.0f;
+    }
+    // as the matrix cores take them; ragged: rows are not of whole 8 numbers
+    __device__ __forceinline__ void lay(u16x8 (&out)[Form<T>::planes], int64_t there, bool ragged) {
+        if (ragged) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < there ? v[i] : (T)0.0f;
+        }
+        if constexpr (Form<T>::planes == 1) {
+            out[0] = __builtin_bit_cast(u16x8, v);
+        } else {
+            const f32x4 part[2] = {f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}};
+            turn<T>(part, out);
+        }
+    }
+};
+
+// A matrix of rows `ld` apart, and 8 numbers of it from column c of row r on.
+template <class T>
+struct Matrix {
+    const T* at;
+    int64_t ld, rows, cols;
+    __device__ __forceinline__ void read(Raw<T>& raw, int64_t r, int64_t c) const {
+        raw.read(at + r * ld + c, r < rows ? cols - c : 0, (rows - 1 - r) * ld + cols - c);
+    }
+    __device__ __forceinline__ bool ragged() const { return cols % 8 != 0; }
+};
+
+// K * 32 numbers of 16 QT rows on their way; a lane has 8 of each 32 of its rows.
+template <class T, int K, int QT>
+struct RowsRaw {
+    Raw<T> v[QT][K];
+    __device__ __forceinline__ void read(const Matrix<T>& m, int64_t row0) {
+        const int lane = threadIdx.x % kWave;
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int s = 0; s < K; ++s) m.read(v[q][s], row0 + q * 16 + (lane & 15), s * 32 + (lane >> 4) * 8);
+    }
+    __device__ __forceinline__ void lay(const Matrix<T>& m, u16x8 (&out)[QT][K][Form<T>::planes]) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int s = 0; s < K; ++s) v[q][s].lay(out[q][s], m.cols - (s * 32 + threadIdx.x % kWave / 16 * 8), m.ragged());
+    }
+};
+
+// The rows' results: a lane has 4 numbers of each 16 of its rows.
+template <class T, int QT, int tiles>
+__device__ __forceinline__ void store_rows(const f32x4 (&v)[QT][tiles], T* to, int64_t cols, const T* bias, const T* residual, int64_t residual_ld,
+                                           int64_t row0, int64_t rows) {
+    const int lane = threadIdx.x % kWave;
+    // (all that is read, before any of it is used)
+    typename Few<T, 4>::vector r[QT][tiles];
+    if (residual) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+            for (int o = 0; o < tiles; ++o) {
+                const int64_t row = row0 + q * 16 + (lane & 15), col = o * 16 + lane / 16 * 4;
+                if (col < cols && row < rows) r[q][o] = load_some<T, 4>(residual + row * residual_ld + col, (rows - 1 - row) * residual_ld + cols - col);
+            }
+    }
+#pragma unroll
+    for (int o = 0; o < tiles; ++o) {
+        const int64_t col = o * 16 + lane / 16 * 4;
+        if (col >= cols) continue;
+        const f32x4 b = four_of(bias, col, cols - col);
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const int64_t row = row0 + q * 16 + (lane & 15);
+            if (row >= rows) continue;
+            f32x4 sum = v[q][o] + b;
+            if (residual)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += (float)r[q][o][i];
+            store_four(to + row * cols, sum, col, cols);
+        }
+    }
+}
+template <int QT, int tiles>
+__device__ __forceinline__ void clear_rows(f32x4 (&v)[QT][tiles]) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+        for (int i = 0; i < tiles; ++i) v[q][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
 // The biases of a lane's 4 hidden units, as what their sums begin with: read for each tile anew, straight to where it adds up,
 // since vector instructions are what these kernels run out of and reads of LDS are not.
 __device__ __forceinline__ void biases(const float* bias, int unit, f32x4& gate, f32x4& up) {
@@ -154,18 +242,19 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_kernel(NarrowAr
     using C = Chunk<KD, KO, false>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, OT = 2 * KO;
     __shared__ __align__(16) u16 lds[2][kib * 512];
-    const int lane = threadIdx.x % kWave, l = lane & 15, g = lane >> 4, wave = threadIdx.x / kWave;
+    const int g = threadIdx.x % kWave / 16, wave = threadIdx.x / kWave;
     const int64_t row0 = ((int64_t)blockIdx.x * kNarrowWaves + wave) * 16 * QT;
     const int chunks = (int)((p.hidden + 31) / 32);
     chunk_to_lds<kib, kNarrowWaves>(p.chunks, lds[0]);
     u16x8 x[QT][KD][planes];
-#pragma unroll
-    for (int q = 0; q < QT; ++q) row_fragments<T, KD>(p.x, p.x_ld, row0 + q * 16 + l, p.rows, p.dim, x[q]);
+    {
+        const Matrix<T> m{p.x, p.x_ld, p.rows, p.dim};
+        RowsRaw<T, KD, QT> raw;
+        raw.read(m, row0);
+        raw.lay(m, x);
+    }
     f32x4 y[QT][OT];
-#pragma unroll
-    for (int q = 0; q < QT; ++q)
-#pragma unroll
-        for (int o = 0; o < OT; ++o) y[q][o] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    clear_rows(y);
     for (int c = 0; c < chunks; ++c) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (c + 1 < chunks) chunk_to_lds<kib, kNarrowWaves>(p.chunks + (int64_t)(c + 1) * kib * 512, lds[(c + 1) & 1]);
@@ -204,20 +293,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_kernel(NarrowAr
             for (int q = 0; q < QT; ++q) y[q][o] = multiply<T>(wd, turned[q], y[q][o]);
         }
     }
-#pragma unroll
-    for (int o = 0; o < OT; ++o) {
-        const int64_t col = o * 16 + g * 4;
-        if (col >= p.out) continue;
-        const f32x4 bias = four_of(p.b_down, col, p.out);
-#pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            const int64_t row = row0 + q * 16 + l;
-            if (row >= p.rows) continue;
-            f32x4 v = y[q][o] + bias;
-            if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, p.out);
-            store_four(p.y + row * p.out, v, col, p.out);
-        }
-    }
+    store_rows<T>(y, p.y, p.out, p.b_down, p.residual, p.residual_ld, row0, p.rows);
 }
 
 // dx: as narrow_kernel, with dh' = Wd' dy' and dx' = Wg' dgate' + Wu' dup' in place of y'.
@@ -226,21 +302,22 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_backward_kernel
     using C = Chunk<KD, KO, true>;
     constexpr int planes = Form<T>::planes, kib = C::fragments * planes + 1, DT = 2 * KD;
     __shared__ __align__(16) u16 lds[2][kib * 512];
-    const int lane = threadIdx.x % kWave, l = lane & 15, g = lane >> 4, wave = threadIdx.x / kWave;
+    const int g = threadIdx.x % kWave / 16, wave = threadIdx.x / kWave;
     const int64_t row0 = ((int64_t)blockIdx.x * kNarrowWaves + wave) * 16 * QT;
     const int chunks = (int)((p.hidden + 31) / 32);
     chunk_to_lds<kib, kNarrowWaves>(p.chunks, lds[0]);
     u16x8 x[QT][KD][planes], dy[QT][KO][planes];
-#pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        row_fragments<T, KD>(p.x, p.x_ld, row0 + q * 16 + l, p.rows, p.dim, x[q]);
-        row_fragments<T, KO>(p.dy, p.dy_ld, row0 + q * 16 + l, p.rows, p.out, dy[q]);
+    {
+        const Matrix<T> mx{p.x, p.x_ld, p.rows, p.dim}, my{p.dy, p.dy_ld, p.rows, p.out};
+        RowsRaw<T, KD, QT> raw_x;
+        RowsRaw<T, KO, QT> raw_y;
+        raw_x.read(mx, row0);
+        raw_y.read(my, row0);
+        raw_x.lay(mx, x);
+        raw_y.lay(my, dy);
     }
     f32x4 dx[QT][DT];
-#pragma unroll
-    for (int q = 0; q < QT; ++q)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) dx[q][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    clear_rows(dx);
     for (int c = 0; c < chunks; ++c) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (c + 1 < chunks) chunk_to_lds<kib, kNarrowWaves>(p.chunks + (int64_t)(c + 1) * kib * 512, lds[(c + 1) & 1]);
@@ -295,15 +372,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_backward_kernel
             }
         }
     }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-        const int64_t col = d * 16 + g * 4;
-#pragma unroll
-        for (int q = 0; q < QT; ++q) {
-            const int64_t row = row0 + q * 16 + l;
-            if (col < p.dim && row < p.rows) store_four(p.y + row * p.dim, dx[q][d], col, p.dim);
-        }
-    }
+    store_rows<T>(dx, p.y, p.dim, (const T*)nullptr, (const T*)nullptr, 0, row0, p.rows);
 }
 
 // 32 rows of K * 32 numbers in LDS, read along the rows and down the columns.  A row's pieces of 16 numbers lie at their index ^ a
@@ -337,28 +406,6 @@ struct RowTile {
     }
 };
 
-// 8 numbers of a row as they lie in memory, to be laid out when they have arrived
-template <class T>
-struct Raw {
-    T v[8];
-    __device__ __forceinline__ void read(const T* row, int64_t c, int64_t count, bool there) {
-        if (there && c + 8 <= count) {
-            const auto a = load_few<T, 8>(row + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = a[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = there && c + i < count ? row[c + i] : (T)0.0f;
-        }
-    }
-    __device__ __forceinline__ void lay(u16x8 (&out)[Form<T>::planes]) const {
-        f32x4 part[2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) part[i / 4][i % 4] = (float)v[i];
-        turn<T>(part, out);
-    }
-};
-
 template <class T>
 struct NarrowWeightArgs {
     const T *x, *dy;
@@ -369,65 +416,64 @@ struct NarrowWeightArgs {
     int64_t dim, hidden, out;
 };
 
-// The gradients of the weights over a share of the rows: a wavefront has 16 HT hidden units, their weights and their sums in
+// The gradients of the weights over a share of the rows: a wavefront has 16 hidden units, their weights and their sums in
 // registers, and a block's wavefronts go through the rows together, 32 at a time: gate, up and dh of those rows and units (rows down
 // this time, a lane has 4 rows of a unit), and the products of what comes of them with the columns of x and dy.
-constexpr int kNarrowWeightWaves = 8;
-template <class T, int KD, int KO, int HT, int activation>
-__global__ __launch_bounds__(kNarrowWeightWaves* kWave, 2) void narrow_weight_kernel(NarrowWeightArgs<T> p) {
+// Four wavefronts to a block and three to a SIMD where their registers allow it (131 072 rows of 64 -> 256 -> 64 in bfloat16: 64 us
+// with eight and two, 53 with four and three); where they do not, two, and eight to a block where four would have too many of
+// the rows' numbers on their way.
+template <class T, int KD, int KO>
+constexpr int kNarrowWeightWaves = (Form<T>::planes == 1 ? KD + KO > 6 : KD + KO > 2) ? 8 : 4;
+template <class T, int KD, int KO>
+constexpr int kNarrowWeightPerSimd = Form<T>::planes == 1 && KD + KO <= 4 ? 3 : 2;
+template <class T, int KD, int KO, int activation>
+__global__ __launch_bounds__((kNarrowWeightWaves<T, KD, KO> * kWave), (kNarrowWeightPerSimd<T, KD, KO>)) void narrow_weight_kernel(NarrowWeightArgs<T> p) {
     using C = Chunk<KD, KO, true>;
-    constexpr int planes = Form<T>::planes, DT = 2 * KD, OT = 2 * KO, threads = kNarrowWeightWaves * kWave;
+    constexpr int planes = Form<T>::planes, DT = 2 * KD, OT = 2 * KO, waves = kNarrowWeightWaves<T, KD, KO>, threads = waves * kWave;
     using X = RowTile<KD, planes>;
     using Y = RowTile<KO, planes>;
     constexpr int nx = (X::pieces + threads - 1) / threads, ny = (Y::pieces + threads - 1) / threads;
     __shared__ __align__(16) u16 lds[2][X::numbers + Y::numbers];
     const int thread = threadIdx.x, lane = thread % kWave, l = lane & 15, g = lane >> 4, wave = thread / kWave;
-    const int64_t tile0 = ((int64_t)blockIdx.y * kNarrowWeightWaves + wave) * HT, split = blockIdx.x;
+    const int64_t tile = (int64_t)blockIdx.y * waves + wave, split = blockIdx.x;
     const int64_t first = split * p.each, end = least(first + p.each, p.rows);
-    const bool works = tile0 * 16 < p.hidden;
-    u16x8 wg[HT][KD][planes], wu[HT][KD][planes], wd[HT][KO][planes];
-    float bg[HT], bu[HT];
+    const bool works = tile * 16 < p.hidden;
+    u16x8 wg[KD][planes], wu[KD][planes], wd[KO][planes];
+    float bg = 0.0f, bu = 0.0f;
     if (works) {
+        const int half = (int)(tile % 2);
+        const u16* const at = p.chunks + tile / 2 * C::numbers(planes);
 #pragma unroll
-        for (int t = 0; t < HT; ++t) {
-            // (HT 2: the last chunk has both of its tiles, zeros beyond the hidden units)
-            const int64_t tile = tile0 + t;
-            const int half = (int)(tile % 2);
-            const u16* const at = p.chunks + tile / 2 * C::numbers(planes);
+        for (int s = 0; s < KD; ++s) fragment_of<planes>(at, C::gate + half * KD + s, wg[s]), fragment_of<planes>(at, C::up + half * KD + s, wu[s]);
 #pragma unroll
-            for (int s = 0; s < KD; ++s) fragment_of<planes>(at, C::gate + half * KD + s, wg[t][s]), fragment_of<planes>(at, C::up + half * KD + s, wu[t][s]);
-#pragma unroll
-            for (int s = 0; s < KO; ++s) fragment_of<planes>(at, C::down + half * KO + s, wd[t][s]);
-            const float* const bias = reinterpret_cast<const float*>(at + C::fragments * planes * 512);
-            bg[t] = bias[half * 16 + l];
-            bu[t] = bias[32 + half * 16 + l];
-        }
+        for (int s = 0; s < KO; ++s) fragment_of<planes>(at, C::down + half * KO + s, wd[s]);
+        const float* const bias = reinterpret_cast<const float*>(at + C::fragments * planes * 512);
+        bg = bias[half * 16 + l];
+        bu = bias[32 + half * 16 + l];
     }
-    f32x4 gate_sum[HT][DT], up_sum[HT][DT], down_sum[HT][OT];
-    float bg_sum[HT], bu_sum[HT], bd_sum[ny][8];
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 gate_sum[DT], up_sum[DT], down_sum[OT];
+    float bg_sum = 0.0f, bu_sum = 0.0f, bd_sum[ny][8];
 #pragma unroll
-    for (int t = 0; t < HT; ++t) {
-        bg_sum[t] = bu_sum[t] = 0.0f;
+    for (int d = 0; d < DT; ++d) gate_sum[d] = up_sum[d] = zero;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) gate_sum[t][d] = up_sum[t][d] = zero;
-#pragma unroll
-        for (int o = 0; o < OT; ++o) down_sum[t][o] = zero;
-    }
+    for (int o = 0; o < OT; ++o) down_sum[o] = zero;
 #pragma unroll
     for (int i = 0; i < ny; ++i)
         for (int j = 0; j < 8; ++j) bd_sum[i][j] = 0.0f;
     Raw<T> rx[nx], ry[ny];
+    // (the rows of this split: what lies behind them is not theirs)
+    const Matrix<T> mx{p.x, p.x_ld, end, p.dim}, my{p.dy, p.dy_ld, end, p.out};
     auto read = [&](int64_t row0) {
 #pragma unroll
         for (int i = 0; i < nx; ++i) {
             const int piece = i * threads + thread, row = piece / (KD * 4);
-            if (X::pieces % threads == 0 || piece < X::pieces) rx[i].read(p.x + (row0 + row) * p.x_ld, piece % (KD * 4) * 8, p.dim, row0 + row < end);
+            if (X::pieces % threads == 0 || piece < X::pieces) mx.read(rx[i], row0 + row, piece % (KD * 4) * 8);
         }
 #pragma unroll
         for (int i = 0; i < ny; ++i) {
             const int piece = i * threads + thread, row = piece / (KO * 4);
-            if (Y::pieces % threads == 0 || piece < Y::pieces) ry[i].read(p.dy + (row0 + row) * p.dy_ld, piece % (KO * 4) * 8, p.out, row0 + row < end);
+            if (Y::pieces % threads == 0 || piece < Y::pieces) my.read(ry[i], row0 + row, piece % (KO * 4) * 8);
         }
     };
     read(first);
@@ -439,7 +485,7 @@ __global__ __launch_bounds__(kNarrowWeightWaves* kWave, 2) void narrow_weight_ke
             const int piece = i * threads + thread;
             if (X::pieces % threads != 0 && piece >= X::pieces) continue;
             u16x8 laid[planes];
-            rx[i].lay(laid);
+            rx[i].lay(laid, p.dim - piece % (KD * 4) * 8, mx.ragged());
             for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x8*>(X::at(x + q * X::plane, piece / (KD * 4), piece % (KD * 4))) = laid[q];
         }
 #pragma unroll
@@ -447,108 +493,100 @@ __global__ __launch_bounds__(kNarrowWeightWaves* kWave, 2) void narrow_weight_ke
             const int piece = i * threads + thread;
             if (Y::pieces % threads != 0 && piece >= Y::pieces) continue;
             u16x8 laid[planes];
-            ry[i].lay(laid);
+            ry[i].lay(laid, p.out - piece % (KO * 4) * 8, my.ragged());
             for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x8*>(Y::at(dy + q * Y::plane, piece / (KO * 4), piece % (KO * 4))) = laid[q];
             for (int j = 0; j < 8; ++j) bd_sum[i][j] += (float)ry[i].v[j];
         }
         __syncthreads();
         if (row0 + 32 < end) read(row0 + 32);
         if (!works) continue;
-        u16x4 h[HT][2][planes], dg[HT][2][planes], du[HT][2][planes];
+        u16x4 h[2][planes], dg[2][planes], du[2][planes];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            f32x4 gate[HT], up[HT], dh[HT];
-#pragma unroll
-            for (int t = 0; t < HT; ++t) gate[t] = zero + bg[t], up[t] = zero + bu[t], dh[t] = zero;
+            f32x4 gate = zero + bg, up = zero + bu, dh = zero;
 #pragma unroll
             for (int s = 0; s < KD; ++s) {
                 u16x8 a[planes];
                 X::along(x, q, s, a);
-#pragma unroll
-                for (int t = 0; t < HT; ++t) gate[t] = multiply<T>(a, wg[t][s], gate[t]), up[t] = multiply<T>(a, wu[t][s], up[t]);
+                gate = multiply<T>(a, wg[s], gate);
+                up = multiply<T>(a, wu[s], up);
             }
 #pragma unroll
             for (int s = 0; s < KO; ++s) {
                 u16x8 a[planes];
                 Y::along(dy, q, s, a);
-#pragma unroll
-                for (int t = 0; t < HT; ++t) dh[t] = multiply<T>(a, wd[t][s], dh[t]);
+                dh = multiply<T>(a, wd[s], dh);
             }
+            f32x4 vh, vg, vu;
 #pragma unroll
-            for (int t = 0; t < HT; ++t) {
-                f32x4 vh, vg, vu;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float slope;
-                    const float a = activate<planes == 3, activation>(gate[t][i], &slope);
-                    vh[i] = a * up[t][i];
-                    vg[i] = dh[t][i] * up[t][i] * slope;
-                    vu[i] = dh[t][i] * a;
-                    bg_sum[t] += vg[i];
-                    bu_sum[t] += vu[i];
-                }
-                Form<T>::split(vh, h[t][q]);
-                Form<T>::split(vg, dg[t][q]);
-                Form<T>::split(vu, du[t][q]);
+            for (int i = 0; i < 4; ++i) {
+                float slope;
+                const float a = activate<planes == 3, activation>(gate[i], &slope);
+                vh[i] = a * up[i];
+                vg[i] = dh[i] * up[i] * slope;
+                vu[i] = dh[i] * a;
+                bg_sum += vg[i];
+                bu_sum += vu[i];
             }
+            Form<T>::split(vh, h[q]);
+            Form<T>::split(vg, dg[q]);
+            Form<T>::split(vu, du[q]);
         }
-        u16x8 th[HT][planes], tg[HT][planes], tu[HT][planes];
-#pragma unroll
-        for (int t = 0; t < HT; ++t) turn<T>(h[t], th[t]), turn<T>(dg[t], tg[t]), turn<T>(du[t], tu[t]);
+        u16x8 th[planes], tg[planes], tu[planes];
+        turn<T>(h, th);
+        turn<T>(dg, tg);
+        turn<T>(du, tu);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             u16x8 a[planes];
             X::across(x, d, a);
-#pragma unroll
-            for (int t = 0; t < HT; ++t) gate_sum[t][d] = multiply<T>(a, tg[t], gate_sum[t][d]), up_sum[t][d] = multiply<T>(a, tu[t], up_sum[t][d]);
+            gate_sum[d] = multiply<T>(a, tg, gate_sum[d]);
+            up_sum[d] = multiply<T>(a, tu, up_sum[d]);
         }
 #pragma unroll
         for (int o = 0; o < OT; ++o) {
             u16x8 a[planes];
             Y::across(dy, o, a);
-#pragma unroll
-            for (int t = 0; t < HT; ++t) down_sum[t][o] = multiply<T>(th[t], a, down_sum[t][o]);
+            down_sum[o] = multiply<T>(th, a, down_sum[o]);
         }
     }
     if (works) {
+        const int64_t h = tile * 16 + l, h4 = tile * 16 + g * 4;
+        if (h < p.hidden) {   // (a lane has 4 features of a unit)
 #pragma unroll
-        for (int t = 0; t < HT; ++t) {
-            const int64_t h = (tile0 + t) * 16 + l, h4 = (tile0 + t) * 16 + g * 4;
-            if (h < p.hidden) {   // (a lane has 4 features of a unit)
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const int64_t col = d * 16 + g * 4;
-                    if (col >= p.dim) continue;
-                    store_four(p.gate + (split * p.hidden + h) * p.dim, gate_sum[t][d], col, p.dim);
-                    store_four(p.up + (split * p.hidden + h) * p.dim, up_sum[t][d], col, p.dim);
-                }
+            for (int d = 0; d < DT; ++d) {
+                const int64_t col = d * 16 + g * 4;
+                if (col >= p.dim) continue;
+                store_four(p.gate + (split * p.hidden + h) * p.dim, gate_sum[d], col, p.dim);
+                store_four(p.up + (split * p.hidden + h) * p.dim, up_sum[d], col, p.dim);
             }
-#pragma unroll
-            for (int o = 0; o < OT; ++o)   // (4 units of a number of the result)
-                if (o * 16 + l < p.out && h4 < p.hidden) store_four(p.down + (split * p.out + o * 16 + l) * p.hidden, down_sum[t][o], h4, p.hidden);
-            float sg = bg_sum[t], su = bu_sum[t];
-            sg += __shfl_xor(sg, 16, kWave), su += __shfl_xor(su, 16, kWave);
-            sg += __shfl_xor(sg, 32, kWave), su += __shfl_xor(su, 32, kWave);
-            if (g == 0 && h < p.hidden) p.b_gate[split * p.hidden + h] = sg, p.b_up[split * p.hidden + h] = su;
         }
+#pragma unroll
+        for (int o = 0; o < OT; ++o)   // (4 units of a number of the result)
+            if (o * 16 + l < p.out && h4 < p.hidden) store_four(p.down + (split * p.out + o * 16 + l) * p.hidden, down_sum[o], h4, p.hidden);
+        bg_sum += __shfl_xor(bg_sum, 16, kWave), bu_sum += __shfl_xor(bu_sum, 16, kWave);
+        bg_sum += __shfl_xor(bg_sum, 32, kWave), bu_sum += __shfl_xor(bu_sum, 32, kWave);
+        if (g == 0 && h < p.hidden) p.b_gate[split * p.hidden + h] = bg_sum, p.b_up[split * p.hidden + h] = bu_sum;
     }
     if (blockIdx.y != 0) return;
-    // the sums of dy: a thread has 8 columns of a row in 32, its piece's
+    // the sums of dy: a thread has those of its pieces, 8 columns of a row in 32
     float* const sums = reinterpret_cast<float*>(lds);
-    static_assert(sizeof(lds) >= KO * 32 * sizeof(float), "room");
+    static_assert(sizeof(lds) >= 32 * KO * 32 * sizeof(float), "room");
     __syncthreads();
-    for (int c = thread; c < KO * 32; c += threads) sums[c] = 0.0f;
-    __syncthreads();
-    for (int turn_of = 0; turn_of < 32; ++turn_of) {   // (row by row, in one order)
 #pragma unroll
-        for (int i = 0; i < ny; ++i) {
-            const int piece = i * threads + thread;
-            if ((Y::pieces % threads == 0 || piece < Y::pieces) && piece / (KO * 4) == turn_of)
-                for (int j = 0; j < 8; ++j) sums[piece % (KO * 4) * 8 + j] += bd_sum[i][j];
-        }
-        __syncthreads();
+    for (int i = 0; i < ny; ++i) {
+        const int piece = i * threads + thread;
+        if (Y::pieces % threads == 0 || piece < Y::pieces)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sums[piece * 8 + j] = bd_sum[i][j];
     }
-    for (int c = thread; c < p.out; c += threads) p.b_down[split * p.out + c] = sums[c];
+    __syncthreads();
+    for (int c = thread; c < p.out; c += threads) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int row = 0; row < 32; ++row) sum += sums[row * KO * 32 + c];
+        p.b_down[split * p.out + c] = sum;
+    }
 }
 
 }  // namespace svox_decoder

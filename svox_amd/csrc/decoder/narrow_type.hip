@@ -20,6 +20,17 @@ NarrowArgs<T> narrow_args(const SvoxGatedFfn& s, const u16* chunks) {
     p.out = s.out;
     return p;
 }
+// 16 or 32 rows to a wavefront: 32 halve what it reads of LDS, 16 fill the GPU sooner and are all that float32's planes leave room
+// for.  (Rows of 64 -> 256 -> 64, bfloat16, forward and dx: 131 072 rows 27.5, 37.2 us with 16, 25.4, 34.5 with 32; 10 007 rows of
+// 76 -> 203 -> 49, float16: 10.8, 13.1 and 14.1, 17.2.  65 537 rows of 32 -> 128 -> 28, float32, forward: 20.7 and 22.8.)
+template <class F>
+void by_rows(int64_t rows, F launch) {
+    if constexpr (Form<T>::planes == 1) {
+        if (rows >= 98304) return launch(std::integral_constant<int, 2>());
+    }
+    launch(std::integral_constant<int, 1>());
+}
+
 template <int KD, int KO, bool backward>
 void launch_narrow_lay(const SvoxGatedFfn& s, u16* to, hipStream_t stream) {
     using C = Chunk<KD, KO, backward>;
@@ -36,9 +47,13 @@ int narrow_forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t 
     p.residual_ld = s.residual_stride;
     p.y = (T*)y;
     SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
-        constexpr int QT = 2;
         launch_narrow_lay<KD, KO, false>(s, chunks, stream);
-        hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)), dim3(kNarrowWaves * kWave), 0, stream, p);
+        const auto launch = [&](auto rows) {
+            constexpr int QT = decltype(rows)::value;
+            hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
+                               dim3(kNarrowWaves * kWave), 0, stream, p);
+        };
+        by_rows(s.rows, launch);
     }));
     return check_launch("gated_ffn");
 }
@@ -69,14 +84,16 @@ int narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad
     w.hidden = s.hidden;
     w.out = s.out;
     SVOX_NARROW_STEPS(s.dim, KD, SVOX_NARROW_STEPS(s.out, KO, {
-        constexpr int QT = 2, HT = kNarrowUnits<T, KD, KO>;
         launch_narrow_lay<KD, KO, true>(s, b.chunks, stream);
-        if (grads.x)
+        const auto launch = [&](auto rows) {
+            constexpr int QT = decltype(rows)::value;
             hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
                                dim3(kNarrowWaves * kWave), 0, stream, p);
+        };
+        if (grads.x) by_rows(s.rows, launch);
         if (parts.jobs)
-            hipLaunchKernelGGL((narrow_weight_kernel<T, KD, KO, HT, kActivation>), dim3((unsigned)b.split.splits, (unsigned)b.split.down),
-                               dim3(kNarrowWeightWaves * kWave), 0, stream, w);
+            hipLaunchKernelGGL((narrow_weight_kernel<T, KD, KO, kActivation>), dim3((unsigned)b.split.splits, (unsigned)b.split.down),
+                               dim3((kNarrowWeightWaves<T, KD, KO>) * kWave), 0, stream, w);
     }));
     parts.launch(stream);
     return check_launch("gated_ffn_backward");

@@ -39,14 +39,9 @@ __device__ __forceinline__ float sum_over(float v, float* room, int slot) {
 // One piece of a row: V numbers from column c on, zeros beyond the row.
 template <class T, int V>
 __device__ __forceinline__ void read_piece(const T* row, int c, int dim, float* v) {
-    if (c + V <= dim) {
-        const auto f = load_few<T, V>(row + c);
+    const auto f = load_some<T, V>(row + c, dim - c);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)f[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = c + i < dim ? (float)row[c + i] : 0.0f;
-    }
+    for (int i = 0; i < V; ++i) v[i] = (float)f[i];
 }
 template <class T, int V>
 __device__ __forceinline__ void write_piece(T* row, int c, int dim, const float* v) {

@@ -142,17 +142,14 @@ struct Place {
     __device__ int64_t col(int n) const { return n0 + n * 16; }
 };
 
+// numbers n..n+3 of `count`, of which `room` from n on can be read; what is read beyond `count` is of no meaning
 template <class T>
-__device__ __forceinline__ f32x4 four_of(const T* from, int64_t n, int64_t count) {   // zeros beyond `count`
+__device__ __forceinline__ f32x4 four_of(const T* from, int64_t n, int64_t room) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (!from) return v;
-    if (n + 4 <= count) {
-        const auto f = load_few<T, 4>(from + n);
-        for (int i = 0; i < 4; ++i) v[i] = (float)f[i];
-    } else {
-        for (int i = 0; i < 4; ++i)
-            if (n + i < count) v[i] = (float)from[n + i];
-    }
+    const auto f = load_some<T, 4>(from + n, room);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)f[i];
     return v;
 }
 template <class T>
@@ -203,7 +200,7 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
         for (int n = 0; n < S::TN; ++n) {
             const int64_t col = place.col(n);
             if (col >= p.ldh) continue;
-            const f32x4 bg = four_of(p.b_gate, col, p.hidden), bu = four_of(p.b_up, col, p.hidden);
+            const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
 #pragma unroll
             for (int m = 0; m < S::TM; ++m) {
                 const int64_t row = place.row(m);
@@ -263,13 +260,13 @@ __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) 
     for (int n = 0; n < S::TN; ++n) {
         const int64_t col = place.col(n);
         if (col >= p.cols) continue;
-        const f32x4 bias = four_of(p.bias, col, p.cols);
+        const f32x4 bias = four_of(p.bias, col, p.cols - col);
 #pragma unroll
         for (int m = 0; m < S::TM; ++m) {
             const int64_t row = place.row(m);
             if (row >= p.rows) continue;
             f32x4 v = acc[0][m][n] + bias;
-            if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, p.cols);
+            if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, (p.rows - 1 - row) * p.residual_ld + p.cols - col);
             store_four(p.y + row * p.cols, v, col, p.cols);
         }
     }
@@ -359,7 +356,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (i < job.count)
 #pragma unroll 4
-        for (int s = threadIdx.x / 32; s < p.splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count);
+        for (int s = threadIdx.x / 32; s < p.splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count - i);
     shared[threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.x >= 32 || i >= job.count) return;
@@ -394,7 +391,7 @@ __global__ __launch_bounds__(kLayThreads) void lay_kernel(LayArgs<T> p) {
     u16* const to = const_cast<u16*>(job.to.at) + row * job.to.ld + col;
     for (int half = 0; half < 2; ++half) {
         u16x4 part[Form<T>::planes];
-        Form<T>::split(four_of(job.from + row * job.ld, col + half * 4, job.cols), part);
+        Form<T>::split(four_of(job.from + row * job.ld, col + half * 4, job.cols - col - half * 4), part);
         for (int q = 0; q < Form<T>::planes; ++q) *reinterpret_cast<u16x4*>(to + q * job.to.plane + half * 4) = part[q];
     }
 }
