@@ -109,6 +109,20 @@ __device__ __forceinline__ typename Few<T, N>::vector load_some(const T* at, int
     return v;
 }
 
+// 8 numbers as the matrix cores take them
+template <class T>
+__device__ __forceinline__ void planes_of(const typename Few<T, 8>::vector& v, u16x8 (&out)[Form<T>::planes]) {
+    if constexpr (Form<T>::planes == 1) {
+        out[0] = __builtin_bit_cast(u16x8, v);
+    } else {
+        u16x4 half[2][Form<T>::planes];
+        Form<T>::split(f32x4{v[0], v[1], v[2], v[3]}, half[0]);
+        Form<T>::split(f32x4{v[4], v[5], v[6], v[7]}, half[1]);
+#pragma unroll
+        for (int q = 0; q < Form<T>::planes; ++q) out[q] = __builtin_shufflevector(half[0][q], half[1][q], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
 // ---- activations
 enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
 

@@ -10,9 +10,23 @@ namespace {
 constexpr int kPlanes = Form<T>::planes;
 constexpr int64_t kMostLd = TileOf<true, 64, 64, 256>::most_ld;
 constexpr int kKT = kPlanes == 1 ? 64 : 32;
-using HiddenShape = Shape<128, 64, kKT, 2, 2, 2>;
-using OutputShape = Shape<128, 128, kKT, 2, 2, 2>;
-using WeightShape = Shape<128, 128, kKT, 2, 2, 2>;
+// Large tiles, where there are enough of them; small ones with more of the reduction on its way, where a block waits for
+// memory more than it multiplies.
+struct Large {
+    using Hidden = Shape<128, 64, kKT, 2, 4, 2>;
+    using Output = Shape<128, 128, kKT, 2, 4, 2>;
+    using Weight = Output;
+};
+struct Small {
+    using Hidden = Shape<64, 32, kKT, 2, 2, 4>;
+    using Output = Shape<64, 64, kKT, 2, 2, 4>;
+    using Weight = Output;
+};
+constexpr int64_t kLargeTiles = kPlanes == 1 ? 192 : 96;
+template <class S>
+int64_t tiles_of(int64_t m, int64_t n) {
+    return pieces(m, S::BM) * pieces(n, S::BN);
+}
 
 // ---- operands: where they are if the tiles can be read from there, else laid out in the workspace
 bool tiles_read(const void* at, int64_t ld, int64_t cols) {
@@ -28,7 +42,10 @@ struct Lays {
         Planes to{nullptr, wide, rows * wide, rows, wide};
         to.at = room.take<u16>(kPlanes * rows * wide);
         LayJob<T>& job = args.job[count++];
-        job = LayJob<T>{(const T*)at, ld, to, cols, pieces(rows * wide / 8, kLayThreads)};
+        const int lanes = wide >= 1024 ? 256 : wide >= 256 ? 64 : 16;
+        // (16 KiB of numbers or so to a block, and all of its lanes' rows at least)
+        const int64_t each = up_to(pieces(8192, wide), kLayThreads / lanes);
+        job = LayJob<T>{(const T*)at, ld, to, cols, pieces(rows, each), each, lanes};
         blocks += job.blocks;
         return to;
     }
@@ -107,23 +124,29 @@ struct Forward {
     }
 };
 
+// The tiles of the weights' gradients, large or small, and the rows of a split.
 struct Split {
-    int64_t tiles, each;
+    int64_t each;
     int splits;
+    bool large;
 };
+template <class S>
+int64_t weight_tiles(const SvoxGatedFfn& s) {
+    return 2 * tiles_of<S>(s.hidden, s.dim) + tiles_of<S>(s.out, s.hidden);
+}
 Split weight_split(const SvoxGatedFfn& s) {
-    using S = WeightShape;
-    const int64_t across = pieces(s.hidden, S::BM) * pieces(s.dim, S::BN);
     Split w;
-    w.tiles = 2 * across + pieces(s.out, S::BM) * pieces(s.hidden, S::BN);
-    // two blocks a compute unit, of eight stages at least
-    int64_t splits = pieces(512, w.tiles);
-    const int64_t most = pieces(s.rows, 8 * S::KT);
-    if (splits > most) splits = most;
-    w.each = up_to(pieces(s.rows, splits), S::KT);
+    // (rows enough for two blocks a compute unit of eight steps each make up for few tiles)
+    const int64_t large = weight_tiles<Large::Weight>(s), steps = pieces(s.rows, kKT);
+    w.large = large * steps >= 512 * 8;
+    const int64_t tiles = w.large ? large : weight_tiles<Small::Weight>(s);
+    int64_t splits = pieces(512, tiles);
+    if (splits > pieces(steps, 8)) splits = pieces(steps, 8);
+    w.each = up_to(pieces(s.rows, splits), kKT);
     w.splits = (int)pieces(s.rows, w.each);
     return w;
 }
+
 struct Backward {
     Lays lays;
     Planes x, w_gate, w_up, w_down, dy, h, dgate, dup;
@@ -164,17 +187,42 @@ HiddenArgs<T> hidden_args(const SvoxGatedFfn& s, const Planes& x, const Planes& 
     p.dim = s.dim;
     p.hidden = s.hidden;
     p.out = s.out;
-    p.tiles_m = pieces(s.rows, HiddenShape::BM);
-    p.tiles_n = pieces(h.ld, HiddenShape::BN);
     p.activation = s.activation;
     return p;
 }
 
+template <class S, bool backward>
+void launch_hidden_as(HiddenArgs<T> p, hipStream_t stream) {
+    p.tiles_m = pieces(p.rows, S::BM);
+    p.tiles_n = pieces(p.ldh, S::BN);
+    hipLaunchKernelGGL((hidden_kernel<T, S, backward>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(S::threads), 0, stream, p);
+}
+template <bool backward>
+void launch_hidden(const HiddenArgs<T>& p, hipStream_t stream) {
+    if (tiles_of<Large::Hidden>(p.rows, p.ldh) >= kLargeTiles) launch_hidden_as<Large::Hidden, backward>(p, stream);
+    else launch_hidden_as<Small::Hidden, backward>(p, stream);
+}
+template <class S, bool along_b>
+void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
+    p.tiles_m = pieces(p.rows, S::BM);
+    p.tiles_n = pieces(p.cols, S::BN);
+    hipLaunchKernelGGL((output_kernel<T, S, along_b>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(S::threads), 0, stream, p);
+}
 template <bool along_b>
-void launch_output(OutputArgs<T> p, hipStream_t stream) {
-    p.tiles_m = pieces(p.rows, OutputShape::BM);
-    p.tiles_n = pieces(p.cols, OutputShape::BN);
-    hipLaunchKernelGGL((output_kernel<T, OutputShape, along_b>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(OutputShape::threads), 0, stream, p);
+void launch_output(const OutputArgs<T>& p, hipStream_t stream) {
+    if (tiles_of<Large::Output>(p.rows, p.cols) >= kLargeTiles) launch_output_as<Large::Output, along_b>(p, stream);
+    else launch_output_as<Small::Output, along_b>(p, stream);
+}
+
+template <class S>
+void launch_weight_as(WeightArgs<T> w, hipStream_t stream) {
+    int64_t blocks = 0;
+    for (WeightJob<T>& job : w.job) {   // (one that is not there has no columns)
+        job.tiles_m = pieces(job.m, S::BM);
+        job.tiles_n = pieces(job.n, S::BN);
+        blocks += job.tiles_m * job.tiles_n;
+    }
+    hipLaunchKernelGGL((weight_kernel<T, S>), dim3((unsigned)(blocks * w.splits)), dim3(S::threads), 0, stream, w);
 }
 
 }  // namespace
@@ -203,7 +251,7 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);
-    hipLaunchKernelGGL((hidden_kernel<T, HiddenShape, false>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(HiddenShape::threads), 0, stream, p);
+    launch_hidden<false>(p, stream);
     OutputArgs<T> o{};
     o.a[0] = f.h;
     o.b[0] = f.w_down;
@@ -232,7 +280,7 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
     p.w_down = b.w_down;
     p.dgate = const_cast<u16*>(b.dgate.at);
     p.dup = const_cast<u16*>(b.dup.at);
-    hipLaunchKernelGGL((hidden_kernel<T, HiddenShape, true>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(HiddenShape::threads), 0, stream, p);
+    launch_hidden<true>(p, stream);
     if (grads.x) {
         OutputArgs<T> o{};
         o.a[0] = b.dgate;
@@ -245,14 +293,12 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         o.cols = s.dim;
         launch_output<false>(o, stream);
     }
-    using S = WeightShape;
     WeightArgs<T> w{};
     const int64_t H = s.hidden, D = s.dim, O = s.out;
     Parts<T> parts(b.part, b.split.splits);
     void* const outs[3] = {grads.w_gate, grads.w_up, grads.w_down};
     void* const sums[3] = {grads.b_gate, grads.b_up, grads.b_down};
     const Planes left[3] = {b.dgate, b.dup, b.dy}, right[3] = {b.x, b.x, b.h};
-    int64_t blocks = 0;
     int jobs = 0;
     for (int j = 0; j < 3; ++j) {
         if (!outs[j] && !sums[j]) continue;
@@ -261,21 +307,19 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         job.b = right[j];
         job.m = j < 2 ? H : O;
         job.n = j < 2 ? D : H;
-        job.tiles_m = pieces(job.m, S::BM);
-        job.tiles_n = pieces(job.n, S::BN);
         job.out = (T*)outs[j];
         job.sums_out = (T*)sums[j];
         if (b.split.splits > 1) {
             job.part = parts.take(job.m * job.n, outs[j]);
             job.sums_part = parts.take(job.m, sums[j]);
         }
-        blocks += job.tiles_m * job.tiles_n;
     }
     if (jobs) {
         w.rows = s.rows;
         w.each = b.split.each;
         w.splits = b.split.splits;
-        hipLaunchKernelGGL((weight_kernel<T, S>), dim3((unsigned)blocks, (unsigned)w.splits), dim3(S::threads), 0, stream, w);
+        if (b.split.large) launch_weight_as<Large::Weight>(w, stream);
+        else launch_weight_as<Small::Weight>(w, stream);
         parts.launch(stream);
     }
     return check_launch("gated_ffn_backward");

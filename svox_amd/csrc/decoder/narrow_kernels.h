@@ -148,12 +148,7 @@ struct Raw {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < there ? v[i] : (T)0.0f;
         }
-        if constexpr (Form<T>::planes == 1) {
-            out[0] = __builtin_bit_cast(u16x8, v);
-        } else {
-            const f32x4 part[2] = {f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}};
-            turn<T>(part, out);
-        }
+        planes_of<T>(v, out);
     }
 };
 

@@ -47,44 +47,50 @@ struct Product {
 #pragma unroll
         for (int i = 0; i < NB; ++i) o.b[i].advance();
     }
+    // What a wavefront multiplies at a time: its rows and columns over 32 of the reduction.
+    struct Fragments {
+        u16x8 a[S::TM][planes], b[NB][S::TN][planes];
+    };
+    static __device__ __forceinline__ void read(const u16* lds, int step, int wm, int wn, Fragments& f) {
+#pragma unroll
+        for (int m = 0; m < S::TM; ++m)
+#pragma unroll
+            for (int p = 0; p < planes; ++p) f.a[m][p] = A::fragment(lds + p * A::numbers, (wm * S::TM + m) * 16, step);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int n = 0; n < S::TN; ++n)
+#pragma unroll
+                for (int p = 0; p < planes; ++p)
+                    f.b[i][n][p] = B::fragment(lds + planes * A::numbers + (p * NB + i) * B::numbers, (wn * S::TN + n) * 16, step);
+    }
     // ones: also the sums of the left operand's columns (over the reduction), in `sums`
     template <bool ones>
-    static __device__ __forceinline__ void multiply_stage(const u16* lds, int wm, int wn, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
-#pragma unroll
-        for (int step = 0; step < S::KT / 32; ++step) {
-            u16x8 a[S::TM][planes];
+    static __device__ __forceinline__ void multiply_all(const Fragments& f, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
+        if constexpr (ones) {
+            u16x8 one;
+            for (int i = 0; i < 8; ++i) one[i] = Form<T>::one();
 #pragma unroll
             for (int m = 0; m < S::TM; ++m)
 #pragma unroll
-                for (int p = 0; p < planes; ++p) a[m][p] = A::fragment(lds + p * A::numbers, (wm * S::TM + m) * 16, step);
-            if constexpr (ones) {
-                u16x8 one;
-                for (int i = 0; i < 8; ++i) one[i] = Form<T>::one();
-#pragma unroll
-                for (int m = 0; m < S::TM; ++m)
-#pragma unroll
-                    for (int p = planes; p-- > 0;) sums[m] = Form<T>::mma(one, a[m][p], sums[m]);
-            }
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int n = 0; n < S::TN; ++n) {
-                    u16x8 b[planes];
-#pragma unroll
-                    for (int p = 0; p < planes; ++p)
-                        b[p] = B::fragment(lds + planes * A::numbers + (p * NB + i) * B::numbers, (wn * S::TN + n) * 16, step);
-#pragma unroll
-                    for (int m = 0; m < S::TM; ++m) acc[i][m][n] = multiply<T>(b, a[m], acc[i][m][n]);
-                }
+                for (int p = planes; p-- > 0;) sums[m] = Form<T>::mma(one, f.a[m][p], sums[m]);
         }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int n = 0; n < S::TN; ++n)
+#pragma unroll
+                for (int m = 0; m < S::TM; ++m) acc[i][m][n] = multiply<T>(f.b[i][n], f.a[m], acc[i][m][n]);
     }
-    // Adds the products over [k, k_end) to acc.  LDS holds S::stages tiles; before one is multiplied its loads, and no later
-    // ones, have to have arrived (a lane's loads arrive in their order), and those of the tile that takes the place of the one
-    // before it go out after the barrier that says that every wavefront is done with that.
+    // Adds the products over [k, k_end) to acc.  LDS holds S::stages tiles of the reduction, registers the fragments of two steps:
+    // while one is multiplied the next one is read, also from tile to tile.  At the barrier between two tiles every wavefront
+    // has read all of the first, whose place the loads of a later one take, and all lanes' loads of the second have arrived (a
+    // lane's loads arrive in their order, so that waiting for some leaves the later ones on their way).
     template <bool ones>
     static __device__ __forceinline__ void run(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
                                                f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if (k >= k_end) return;
+        constexpr int steps = S::KT / 32;
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), wm = wave % S::WM, wn = wave / S::WM;
         const int tiles = (int)((k_end - k + S::KT - 1) / S::KT);
         Operands o = operands(a, b, m0, n0, k, std::make_integer_sequence<int, NB>());
@@ -99,17 +105,42 @@ struct Product {
             load(o, lds + loaded % S::stages * stage);
             ++loaded;
         };
+        // `later`: whole tiles that may still be on their way
+        auto wait = [&](bool later) {
+            if (later)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::stages - 2) * loads) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
         __syncthreads();   // (another product's last tile may still be read)
 #pragma unroll
         for (int i = 0; i < S::stages - 1; ++i)
             if (i < tiles) load_next();
-        for (int t = 0; t < tiles; ++t) {
-            if (loaded - t - 1 >= S::stages - 2)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::stages - 2) * loads) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (loaded < tiles) load_next();
-            multiply_stage<ones>(lds + t % S::stages * stage, wm, wn, acc, sums);
+        wait(loaded == S::stages - 1);
+        if (loaded < tiles) load_next();
+        Fragments f[2];
+        read(lds, 0, wm, wn, f[0]);
+        auto tile = [&](int t, auto parity) {   // its first step is in f[parity]
+            constexpr int first = decltype(parity)::value;
+#pragma unroll
+            for (int s = 0; s + 1 < steps; ++s) {
+                read(lds + t % S::stages * stage, s + 1, wm, wn, f[(first + s + 1) & 1]);
+                multiply_all<ones>(f[(first + s) & 1], acc, sums);
+            }
+            if (t + 1 < tiles) {
+                wait(loaded - t - 2 >= S::stages - 2);
+                if (loaded < tiles) load_next();
+                read(lds + (t + 1) % S::stages * stage, 0, wm, wn, f[(first + steps) & 1]);
+            }
+            multiply_all<ones>(f[(first + steps - 1) & 1], acc, sums);
+        };
+        if constexpr (steps % 2 == 0) {
+            for (int t = 0; t < tiles; ++t) tile(t, std::integral_constant<int, 0>());
+        } else {
+            for (int t = 0; t < tiles; t += 2) {
+                tile(t, std::integral_constant<int, 0>());
+                if (t + 1 < tiles) tile(t + 1, std::integral_constant<int, 1>());
+            }
         }
     }
     template <int... i>
@@ -184,7 +215,7 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
     static_assert(Back::stage <= Forward::stage, "room");
     __shared__ __align__(16) u16 lds[S::stages * Forward::stage];
     int64_t tm, tn;
-    tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
+    tile_at(position_of_block(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
     f32x4 acc[2][S::TM][S::TN], dh[1][S::TM][S::TN];
     clear(acc);
@@ -250,7 +281,7 @@ __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) 
     using P = Product<T, S, true, along_b, 1>;
     __shared__ __align__(16) u16 lds[S::stages * P::stage];
     int64_t tm, tn;
-    tile_of_block(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
+    tile_at(position_of_block(blockIdx.x, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
     f32x4 acc[1][S::TM][S::TN];
     clear(acc);
@@ -291,14 +322,16 @@ template <class T, class S>
 __global__ __launch_bounds__(S::threads, 2) void weight_kernel(WeightArgs<T> p) {
     using P = Product<T, S, false, false, 1>;
     __shared__ __align__(16) u16 lds[S::stages * P::stage];
-    int64_t block = blockIdx.x;
+    const int64_t position = position_of_block(blockIdx.x, gridDim.x), tiles = gridDim.x / p.splits, split = position / tiles;
+    int64_t t = position % tiles, tm, tn;
     int j = 0;
-    while (j < 2 && block >= p.job[j].tiles_m * p.job[j].tiles_n) {
-        block -= p.job[j].tiles_m * p.job[j].tiles_n;
+    while (j < 2 && t >= p.job[j].tiles_m * p.job[j].tiles_n) {
+        t -= p.job[j].tiles_m * p.job[j].tiles_n;
         ++j;
     }
     const WeightJob<T> job = p.job[j];
-    const int64_t m0 = block / job.tiles_n * S::BM, n0 = block % job.tiles_n * S::BN, split = blockIdx.y;
+    tile_at(t, job.tiles_m, job.tiles_n, tm, tn);
+    const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
     const int64_t k = split * p.each, k_end = k + p.each < p.rows ? k + p.each : p.rows;
     f32x4 acc[1][S::TM][S::TN], sums[S::TM];
     clear(acc);
@@ -365,14 +398,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
     store_four(job.out, sum, i, job.count);
 }
 
-// Matrices laid out for TileOf: rows of whole 8 numbers, zeros beyond the columns, planes for float32.
+// Matrices laid out for TileOf: rows of whole 8 numbers, zeros beyond the columns, planes for float32.  A lane has 8 numbers; a
+// block goes through rows with 256, 64 or 16 lanes to each.
 template <class T>
 struct LayJob {
     const T* from;
     int64_t ld;          // of `from`
     Planes to;
     int64_t cols;        // of `from`
-    int64_t blocks;
+    int64_t blocks, each;   // blocks, and rows of one
+    int lanes;
 };
 template <class T>
 struct LayArgs {
@@ -385,15 +420,22 @@ __global__ __launch_bounds__(kLayThreads) void lay_kernel(LayArgs<T> p) {
     int j = 0;
     while (j < 4 && block >= p.job[j].blocks) block -= p.job[j++].blocks;
     const LayJob<T> job = p.job[j];
-    const int64_t each = job.to.cols / 8, i = block * kLayThreads + threadIdx.x;
-    if (i >= job.to.rows * each) return;
-    const int64_t row = i / each, col = i % each * 8;
-    u16* const to = const_cast<u16*>(job.to.at) + row * job.to.ld + col;
-    for (int half = 0; half < 2; ++half) {
-        u16x4 part[Form<T>::planes];
-        Form<T>::split(four_of(job.from + row * job.ld, col + half * 4, job.cols - col - half * 4), part);
-        for (int q = 0; q < Form<T>::planes; ++q) *reinterpret_cast<u16x4*>(to + q * job.to.plane + half * 4) = part[q];
-    }
+    const int rows = kLayThreads / job.lanes, lane = threadIdx.x % job.lanes;
+    const int64_t first = block * job.each, end = least(first + job.each, job.to.rows);
+#pragma unroll 4
+    for (int64_t row = first + threadIdx.x / job.lanes; row < end; row += rows)
+        for (int64_t col = lane * 8; col < job.to.cols; col += job.lanes * 8) {
+            // (what can be read reaches to the end of the matrix, what is read beyond the row is taken for zeros)
+            auto v = load_some<T, 8>(job.from + row * job.ld + col, (job.to.rows - 1 - row) * job.ld + job.cols - col);
+            if (job.cols % 8 != 0)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = col + i < job.cols ? v[i] : (T)0.0f;
+            u16* const to = const_cast<u16*>(job.to.at) + row * job.to.ld + col;
+            u16x8 out[Form<T>::planes];
+            planes_of<T>(v, out);
+#pragma unroll
+            for (int q = 0; q < Form<T>::planes; ++q) *reinterpret_cast<u16x8*>(to + q * job.to.plane) = out[q];
+        }
 }
 
 }  // namespace svox_decoder

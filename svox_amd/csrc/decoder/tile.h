@@ -34,13 +34,17 @@ typedef __attribute__((address_space(3))) void Lds;
 template <bool along, int R, int KT, int threads>
 struct TileOf {
     static constexpr int numbers = R * KT;
-    static constexpr int loads = numbers / 8 / threads;
-    static_assert(numbers % (8 * threads) == 0, "whole rounds of 16 bytes a lane");
+    static constexpr int pieces = numbers / 8;                                   // of 16 bytes, one a lane and load
+    static constexpr int loads = pieces < threads ? 1 : pieces / threads;
+    static_assert(pieces < threads ? threads % pieces == 0 : pieces % threads == 0, "every wavefront has as many loads");
     static constexpr unsigned range = 0x80000000u, outside = 0x80000000u;   // bytes
     static constexpr int64_t most_ld = (int64_t)1 << 22;                    // 256 rows of it stay within the range
 
     static __device__ __forceinline__ int turn_along(int row) { return KT == 64 ? (row & 7) : ((row >> 1) & 3); }
     static __device__ __forceinline__ int turn_across(int k) { return ((k & 3) | ((k >> 1) & 4)) & (R / 16 - 1); }
+
+    // (where there are more lanes than pieces, several wavefronts load the same ones to the same place)
+    static __device__ __forceinline__ int piece_of(int load, int thread) { return load * threads + (pieces < threads ? thread % pieces : thread); }
 
     const u16* next;          // plane 0's first number of the next tile to load
     int64_t step;             // numbers from tile to tile
@@ -50,10 +54,9 @@ struct TileOf {
     __device__ __forceinline__ TileOf(const Planes& m, int64_t r0, int64_t k0) {
         next = m.at + (along ? r0 * m.ld + k0 : k0 * m.ld + r0);
         step = along ? KT : KT * m.ld;
-        const int t = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
-            const int piece = i * threads + t;
+            const int piece = piece_of(i, threadIdx.x);
             if constexpr (along) {
                 const int row = piece / (KT / 8), slot = piece % (KT / 8);
                 at[i] = r0 + row < m.rows ? (unsigned)((row * m.ld + (slot ^ turn_along(row)) * 8) * 2) : outside;
@@ -67,10 +70,9 @@ struct TileOf {
     // before the last tile: `left` indices of the reduction are left of it
     __device__ __forceinline__ void last(int64_t left) {
         if (left >= KT) return;
-        const int t = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
-            const int piece = i * threads + t;
+            const int piece = piece_of(i, threadIdx.x);
             int k;
             if constexpr (along) {
                 const int row = piece / (KT / 8), slot = piece % (KT / 8);
@@ -82,11 +84,11 @@ struct TileOf {
         }
     }
     __device__ __forceinline__ void load(int64_t plane, u16* lds) const {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+        const int wave_first = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave * kWave);
         const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc((void*)(next + plane), 0, range, 0x00020000);
 #pragma unroll
         for (int i = 0; i < loads; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (Lds*)(lds + (i * threads + wave * kWave) * 8), 16, at[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (Lds*)(lds + piece_of(i, wave_first) * 8), 16, at[i], 0, 0, 0);
     }
     __device__ __forceinline__ void advance() { next += step; }
 
@@ -110,13 +112,16 @@ struct TileOf {
     }
 };
 
-// Which tile of `tiles_m` x `tiles_n` a block works on.  Blocks go round the eight XCDs, each with an L2 of its own: every XCD
-// gets a run of neighbouring tiles, and a run goes through 8 tiles down before the next to the right, so that what its blocks
+// Blocks go round the eight XCDs, each with an L2 of its own: block b of n as the position of its work, so that every XCD gets a run
+// of neighbouring work.
+__device__ __forceinline__ int64_t position_of_block(int64_t b, int64_t n) {
+    const int64_t xcd = b % 8, each = n / 8, left = n % 8;
+    return xcd * each + (xcd < left ? xcd : left) + b / 8;
+}
+// The tile of `tiles_m` x `tiles_n` at position t: `down` tiles down before the next to the right, so that what the blocks of an XCD
 // read at a time is a few rows of tiles and a few columns.
-__device__ __forceinline__ void tile_of_block(int64_t block, int64_t blocks, int64_t tiles_m, int64_t tiles_n, int64_t& m, int64_t& n) {
-    const int64_t xcd = block % 8, each = blocks / 8, left = blocks % 8;
-    const int64_t t = xcd * each + (xcd < left ? xcd : left) + block / 8;
-    constexpr int64_t down = 8;
+__device__ __forceinline__ void tile_at(int64_t t, int64_t tiles_m, int64_t tiles_n, int64_t& m, int64_t& n) {
+    constexpr int64_t down = 4;   // (a step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16: 2 2104, 4 2081, 8 2106, 16 2204 us)
     const int64_t group = t / (down * tiles_n), first = group * down;
     const int64_t high = tiles_m - first < down ? tiles_m - first : down;
     const int64_t within = t - group * down * tiles_n;
