@@ -61,16 +61,28 @@ Planes hidden_numbers(Room& room, const SvoxGatedFfn& s) {
 }
 
 // ---- few rows
-constexpr int64_t kFewRows = 64;
-template <int MT>
-void launch_few(const FewArgs<T>& p, hipStream_t stream) {
-    const unsigned down = (unsigned)pieces(p.rows, 16 * MT);
-    hipLaunchKernelGGL((few_hidden_kernel<T, MT>), dim3((unsigned)pieces(p.ldh, 16), down), dim3(kFewHiddenWaves * kWave), 0, stream, p);
-    hipLaunchKernelGGL((few_output_kernel<T, MT>), dim3((unsigned)pieces(p.out, 16), down), dim3(kFewOutputWaves * kWave), 0, stream, p);
+// Up to 64 rows always; up to 2048 while the products stay small, where the other kernels wait more than they multiply.  (Forward
+// pass of 256 -> 1024 -> 256, bfloat16, 512 rows 18.7 us here and 19.3 on tiles, 1024 rows 24.1 and 18.9; float32, 1024 rows 44 and
+// 53, 2048 rows 68 and 56.  Gradients, 1024 rows 40 and 45, 2048 rows 70 and 60; float32, 103 and 135, 181 and 168.)
+bool few_rows(const SvoxGatedFfn& s, bool backward) {
+    const double most = kPlanes == 1 ? (backward ? 0.9e9 : 0.4e9) : (backward ? 1.5e9 : 1.2e9);
+    return s.rows <= 64 || (s.rows <= 2048 && (double)s.rows * s.hidden * (2.0 * s.dim + s.out) <= most);
 }
-int launch_few(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
-    Room room(workspace);
-    const Planes h = hidden_numbers(room, s);
+template <bool backward>
+void launch_few(const FewArgs<T>& p, bool result, hipStream_t stream) {
+    const auto launch = [&](auto tiles) {
+        constexpr int MT = decltype(tiles)::value;
+        const unsigned down = (unsigned)pieces(p.rows, 16 * MT);
+        hipLaunchKernelGGL((few_hidden_kernel<T, MT, backward>), dim3((unsigned)pieces(p.ldh, 16), down), dim3(kFewHiddenWaves * kWave), 0, stream, p);
+        if (result)
+            hipLaunchKernelGGL((few_output_kernel<T, MT, backward>), dim3((unsigned)pieces(backward ? p.dim : p.out, 16), down),
+                               dim3(kFewOutputWaves * kWave), 0, stream, p);
+    };
+    if (p.rows <= 16) launch(std::integral_constant<int, 1>());
+    else if (p.rows <= 32) launch(std::integral_constant<int, 2>());
+    else launch(std::integral_constant<int, 4>());
+}
+FewArgs<T> few_args(const SvoxGatedFfn& s, const Planes& h) {
     FewArgs<T> p{};
     p.x = (const T*)s.x;
     p.w_gate = (const T*)s.w_gate;
@@ -78,22 +90,25 @@ int launch_few(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stre
     p.w_down = (const T*)s.w_down;
     p.b_gate = (const T*)s.b_gate;
     p.b_up = (const T*)s.b_up;
-    p.b_down = (const T*)s.b_down;
-    p.residual = (const T*)s.residual;
     p.x_ld = s.x_stride;
-    p.residual_ld = s.residual_stride;
     p.h = const_cast<u16*>(h.at);
     p.ldh = h.ld;
     p.plane = h.plane;
-    p.y = (T*)y;
     p.rows = s.rows;
     p.dim = s.dim;
     p.hidden = s.hidden;
     p.out = s.out;
     p.activation = s.activation;
-    if (s.rows <= 16) launch_few<1>(p, stream);
-    else if (s.rows <= 32) launch_few<2>(p, stream);
-    else launch_few<4>(p, stream);
+    return p;
+}
+int launch_few_forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
+    Room room(workspace);
+    FewArgs<T> p = few_args(s, hidden_numbers(room, s));
+    p.b_down = (const T*)s.b_down;
+    p.residual = (const T*)s.residual;
+    p.residual_ld = s.residual_stride;
+    p.y = (T*)y;
+    launch_few<false>(p, true, stream);
     return check_launch("gated_ffn");
 }
 
@@ -153,13 +168,17 @@ struct Backward {
     Split split;
     float* part;
     int64_t bytes;
+    bool few;
     Backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, void* workspace, bool any_grad) {
         Room room(workspace);
         // (grad_output's address is not known when its workspace is asked for: there is room to lay it out)
         x = lays.operand(room, s.x, s.x_stride, s.rows, s.dim);
-        w_gate = lays.operand(room, s.w_gate, s.dim, s.hidden, s.dim);
-        w_up = lays.operand(room, s.w_up, s.dim, s.hidden, s.dim);
-        w_down = lays.operand(room, s.w_down, s.hidden, s.out, s.hidden);
+        few = few_rows(s, true);
+        if (!few) {
+            w_gate = lays.operand(room, s.w_gate, s.dim, s.hidden, s.dim);
+            w_up = lays.operand(room, s.w_up, s.dim, s.hidden, s.dim);
+            w_down = lays.operand(room, s.w_down, s.hidden, s.out, s.hidden);
+        }
         h = hidden_numbers(room, s);
         dgate = hidden_numbers(room, s);
         dup = hidden_numbers(room, s);
@@ -229,9 +248,9 @@ void launch_weight_as(WeightArgs<T> w, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
-    if (backward && narrow<T>(s)) return NarrowBackward<T>(s, nullptr).bytes;
+    if (backward && !few_rows(s, true) && narrow<T>(s)) return NarrowBackward<T>(s, nullptr).bytes;
     if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
-    if (s.rows <= kFewRows) {
+    if (few_rows(s, false)) {
         Room room(nullptr);
         hidden_numbers(room, s);
         return room.used;
@@ -246,7 +265,7 @@ int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
 
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
-    if (s.rows <= kFewRows) return launch_few(s, y, workspace, stream);
+    if (few_rows(s, false)) return launch_few_forward(s, y, workspace, stream);
     if (narrow<T>(s)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
     const Forward f(s, workspace);
     f.lays.launch(stream);
@@ -269,29 +288,39 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
 template <>
 int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
                            hipStream_t stream) {
-    if (narrow<T>(s))
+    if (!few_rows(s, true) && narrow<T>(s))
         return by_activation(s.activation, [&](auto a) {
             return Narrow<T, decltype(a)::value>::backward(s, grad_output, grad_stride, grads, workspace, stream);
         });
     Backward b(s, grad_output, grad_stride, workspace, false);
     b.lays.launch(stream);
-    HiddenArgs<T> p = hidden_args(s, b.x, b.w_gate, b.w_up, b.h);
-    p.dy = b.dy;
-    p.w_down = b.w_down;
-    p.dgate = const_cast<u16*>(b.dgate.at);
-    p.dup = const_cast<u16*>(b.dup.at);
-    launch_hidden<true>(p, stream);
-    if (grads.x) {
-        OutputArgs<T> o{};
-        o.a[0] = b.dgate;
-        o.a[1] = b.dup;
-        o.b[0] = b.w_gate;
-        o.b[1] = b.w_up;
-        o.pairs = 2;
-        o.y = (T*)grads.x;
-        o.rows = s.rows;
-        o.cols = s.dim;
-        launch_output<false>(o, stream);
+    if (b.few) {
+        FewArgs<T> p = few_args(s, b.h);
+        p.dy = (const T*)grad_output;
+        p.dy_ld = grad_stride;
+        p.dgate = const_cast<u16*>(b.dgate.at);
+        p.dup = const_cast<u16*>(b.dup.at);
+        p.y = (T*)grads.x;
+        launch_few<true>(p, grads.x != nullptr, stream);
+    } else {
+        HiddenArgs<T> p = hidden_args(s, b.x, b.w_gate, b.w_up, b.h);
+        p.dy = b.dy;
+        p.w_down = b.w_down;
+        p.dgate = const_cast<u16*>(b.dgate.at);
+        p.dup = const_cast<u16*>(b.dup.at);
+        launch_hidden<true>(p, stream);
+        if (grads.x) {
+            OutputArgs<T> o{};
+            o.a[0] = b.dgate;
+            o.a[1] = b.dup;
+            o.b[0] = b.w_gate;
+            o.b[1] = b.w_up;
+            o.pairs = 2;
+            o.y = (T*)grads.x;
+            o.rows = s.rows;
+            o.cols = s.dim;
+            launch_output<false>(o, stream);
+        }
     }
     WeightArgs<T> w{};
     const int64_t H = s.hidden, D = s.dim, O = s.out;

@@ -76,7 +76,23 @@ def test_ffn_few_rows(gpu, rows, d, h, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
-@pytest.mark.parametrize("rows", [65, 127, 128, 300, 1111])
+@pytest.mark.parametrize("rows,d,h,o", [(1, 33, 31, 17), (7, 100, 257, 3), (16, 32, 32, 32), (33, 31, 130, 65), (64, 256, 96, 40), (65, 64, 72, 24),
+                                        (200, 50, 60, 70), (500, 128, 40, 16)])
+def test_ffn_few_rows_gradients(gpu, rows, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=rows * d)
+    g = torch.Generator().manual_seed(1)
+    check_ffn({**t, "x": normal(g, rows, d + 3, dtype=dtype)[:, 1:d + 1]}, "gelu", normal(g, rows, o + 5, dtype=dtype)[:, 3:o + 3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows,d,h,o", [(2049, 130, 140, 150), (3000, 264, 72, 40), (2100, 24, 40, 200), (2500, 150, 33, 129), (2060, 512, 136, 512)])
+def test_ffn_products_of_whole_matrices(gpu, rows, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=h)
+    check_ffn(t, "silu", grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows", [65, 127, 128, 300, 1111, 2049])
 @pytest.mark.parametrize("d,h,o", [(1, 1, 1), (31, 33, 28), (32, 32, 32), (33, 64, 49), (64, 100, 64), (65, 31, 76), (128, 300, 128), (127, 96, 4),
                                    (28, 160, 120)])
 def test_ffn_narrow_layers(gpu, rows, d, h, o, dtype):
