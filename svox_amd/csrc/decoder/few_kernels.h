@@ -121,6 +121,7 @@ struct FewArgs {
     const T *x, *dy, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down, *residual;
     int64_t x_ld, dy_ld, residual_ld;
     u16 *h, *dgate, *dup;   // planes of (rows, ldh)
+    float *b_gate_part, *b_up_part;   // backward: sums over 16 rows each, or NULL
     int64_t ldh, plane;
     T* y;                   // backward: dx
     int64_t rows, dim, hidden, out;
@@ -159,13 +160,13 @@ __global__ __launch_bounds__(kFewHiddenWaves* kWave, 2) void few_hidden_kernel(F
     }
     few_join<products, MT, waves>(acc, sum, shared);
     const int64_t row = row0 + wave * 16 + l, col = h0 + lane / 16 * 4;
-    if (wave >= MT || row >= p.rows || col >= p.ldh) return;
+    if (wave >= MT || (backward ? row0 + wave * 16 : row) >= p.rows || col >= p.ldh) return;
     const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
     f32x4 h, dg, du;
     with_activation(p.activation, [&](auto activation) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool there = col + i < p.hidden;
+            const bool there = col + i < p.hidden && row < p.rows;
             const float u = sum[1][i] + bu[i];
             float slope;
             const float a = activate<planes == 3, decltype(activation)::value>(sum[0][i] + bg[i], backward ? &slope : nullptr);
@@ -182,10 +183,13 @@ __global__ __launch_bounds__(kFewHiddenWaves* kWave, 2) void few_hidden_kernel(F
 #pragma unroll
         for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(to + q * p.plane + row * p.ldh + col) = part[q];
     };
-    keep(h, p.h);
+    if (row < p.rows) keep(h, p.h);
     if constexpr (backward) {
-        keep(dg, p.dgate);
-        keep(du, p.dup);
+        if (row < p.rows) {
+            keep(dg, p.dgate);
+            keep(du, p.dup);
+        }
+        if (p.b_gate_part || p.b_up_part) keep_bias_sums(dg, du, p.b_gate_part, p.b_up_part, row0 / 16 + wave, col, p.hidden);
     }
 }
 

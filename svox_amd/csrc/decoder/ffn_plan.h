@@ -17,12 +17,13 @@ struct Parts {
     int64_t blocks = 0;
     int jobs = 0;
     float* at;
-    Parts(float* part, int splits) : at(part) { join.splits = splits; }
-    float* take(int64_t count, void* out) {
+    explicit Parts(float* part) : at(part) {}
+    float* take(int64_t count, int64_t splits, void* out) {
         float* const part = at;
-        at += join.splits * count;
+        at += splits * count;
         if (out) {
             join.job[jobs] = {part, (T*)out, count};
+            join.splits[jobs] = (int)splits;
             join.blocks[jobs] = pieces(count, kJoinNumbers);
             blocks += join.blocks[jobs++];
         }

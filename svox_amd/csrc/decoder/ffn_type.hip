@@ -162,12 +162,18 @@ Split weight_split(const SvoxGatedFfn& s) {
     return w;
 }
 
+// The rows of the biases' sums of hidden_kernel.
+bool large_hidden(const SvoxGatedFfn& s) { return tiles_of<Large::Hidden>(s.rows, up_to(s.hidden, 8)) >= kLargeTiles; }
+template <class S>
+int64_t hidden_parts(const SvoxGatedFfn& s) {
+    return pieces(s.rows, S::BM) * S::WM;
+}
 struct Backward {
     Lays lays;
     Planes x, w_gate, w_up, w_down, dy, h, dgate, dup;
     Split split;
     float* part;
-    int64_t bytes;
+    int64_t bytes, bias_parts;
     bool few;
     Backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, void* workspace, bool any_grad) {
         Room room(workspace);
@@ -183,7 +189,9 @@ struct Backward {
         dgate = hidden_numbers(room, s);
         dup = hidden_numbers(room, s);
         split = weight_split(s);
-        part = split.splits > 1 ? room.take<float>(split.splits * gradient_numbers(s)) : nullptr;
+        bias_parts = few ? pieces(s.rows, 16) : large_hidden(s) ? hidden_parts<Large::Hidden>(s) : hidden_parts<Small::Hidden>(s);
+        part = room.take<float>((split.splits > 1 ? split.splits * (2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + s.out) : 0) +
+                                bias_parts * 2 * s.hidden);
         if (any_grad)
             room.take<u16>(kPlanes * s.rows * up_to(s.out, 8));
         else
@@ -294,12 +302,17 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         });
     Backward b(s, grad_output, grad_stride, workspace, false);
     b.lays.launch(stream);
+    Parts<T> parts(b.part);
+    float* const b_gate_part = grads.b_gate ? parts.take(s.hidden, b.bias_parts, grads.b_gate) : nullptr;
+    float* const b_up_part = grads.b_up ? parts.take(s.hidden, b.bias_parts, grads.b_up) : nullptr;
     if (b.few) {
         FewArgs<T> p = few_args(s, b.h);
         p.dy = (const T*)grad_output;
         p.dy_ld = grad_stride;
         p.dgate = const_cast<u16*>(b.dgate.at);
         p.dup = const_cast<u16*>(b.dup.at);
+        p.b_gate_part = b_gate_part;
+        p.b_up_part = b_up_part;
         p.y = (T*)grads.x;
         launch_few<true>(p, grads.x != nullptr, stream);
     } else {
@@ -308,6 +321,8 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         p.w_down = b.w_down;
         p.dgate = const_cast<u16*>(b.dgate.at);
         p.dup = const_cast<u16*>(b.dup.at);
+        p.b_gate_part = b_gate_part;
+        p.b_up_part = b_up_part;
         launch_hidden<true>(p, stream);
         if (grads.x) {
             OutputArgs<T> o{};
@@ -324,9 +339,8 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
     }
     WeightArgs<T> w{};
     const int64_t H = s.hidden, D = s.dim, O = s.out;
-    Parts<T> parts(b.part, b.split.splits);
     void* const outs[3] = {grads.w_gate, grads.w_up, grads.w_down};
-    void* const sums[3] = {grads.b_gate, grads.b_up, grads.b_down};
+    void* const sums[3] = {nullptr, nullptr, grads.b_down};
     const Planes left[3] = {b.dgate, b.dup, b.dy}, right[3] = {b.x, b.x, b.h};
     int jobs = 0;
     for (int j = 0; j < 3; ++j) {
@@ -339,8 +353,8 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         job.out = (T*)outs[j];
         job.sums_out = (T*)sums[j];
         if (b.split.splits > 1) {
-            job.part = parts.take(job.m * job.n, outs[j]);
-            job.sums_part = parts.take(job.m, sums[j]);
+            if (outs[j]) job.part = parts.take(job.m * job.n, b.split.splits, outs[j]);
+            if (sums[j]) job.sums_part = parts.take(job.m, b.split.splits, sums[j]);
         }
     }
     if (jobs) {
@@ -349,8 +363,8 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         w.splits = b.split.splits;
         if (b.split.large) launch_weight_as<Large::Weight>(w, stream);
         else launch_weight_as<Small::Weight>(w, stream);
-        parts.launch(stream);
     }
+    parts.launch(stream);
     return check_launch("gated_ffn_backward");
 }
 

@@ -65,19 +65,19 @@ int narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad
     p.dy = (const T*)grad_output;
     p.dy_ld = grad_stride;
     p.y = (T*)grads.x;
-    Parts<T> parts(b.part, b.split.splits);
+    Parts<T> parts(b.part);
     NarrowWeightArgs<T> w{};
     w.x = p.x;
     w.x_ld = p.x_ld;
     w.dy = p.dy;
     w.dy_ld = p.dy_ld;
     w.chunks = b.chunks;
-    w.gate = parts.take((int64_t)s.hidden * s.dim, grads.w_gate);
-    w.up = parts.take((int64_t)s.hidden * s.dim, grads.w_up);
-    w.down = parts.take((int64_t)s.hidden * s.out, grads.w_down);
-    w.b_gate = parts.take(s.hidden, grads.b_gate);
-    w.b_up = parts.take(s.hidden, grads.b_up);
-    w.b_down = parts.take(s.out, grads.b_down);
+    w.gate = parts.take((int64_t)s.hidden * s.dim, b.split.splits, grads.w_gate);
+    w.up = parts.take((int64_t)s.hidden * s.dim, b.split.splits, grads.w_up);
+    w.down = parts.take((int64_t)s.hidden * s.out, b.split.splits, grads.w_down);
+    w.b_gate = parts.take(s.hidden, b.split.splits, grads.b_gate);
+    w.b_up = parts.take(s.hidden, b.split.splits, grads.b_up);
+    w.b_down = parts.take(s.out, b.split.splits, grads.b_down);
     w.rows = s.rows;
     w.each = b.split.each;
     w.dim = s.dim;

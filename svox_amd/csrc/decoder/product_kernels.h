@@ -201,11 +201,26 @@ struct HiddenArgs {
     Planes dy, w_down;           // backward: (rows, out), (out, hidden)
     const T *b_gate, *b_up;      // or NULL
     u16 *h, *dgate, *dup;        // planes of (rows, ldh)
+    float *b_gate_part, *b_up_part;   // backward: sums over rows of dgate and dup, (tiles_m WM, hidden), or NULL
     int64_t ldh, plane;
     int64_t rows, dim, hidden, out;
     int64_t tiles_m, tiles_n;
     int activation;
 };
+
+// The sums over 16 lanes (16 rows) of the biases' gradients, before they are rounded, at `row` of the parts.
+__device__ __forceinline__ void keep_bias_sums(f32x4 gate, f32x4 up, float* gate_part, float* up_part, int64_t row, int64_t col, int64_t hidden) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            gate[i] += __shfl_xor(gate[i], d, kWave);
+            up[i] += __shfl_xor(up[i], d, kWave);
+        }
+    if ((threadIdx.x & 15) != 0) return;
+    if (gate_part) store_four(gate_part + row * hidden, gate, col, hidden);
+    if (up_part) store_four(up_part + row * hidden, up, col, hidden);
+}
 
 template <class T, class S, bool backward>
 __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) {
@@ -232,6 +247,7 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
             const int64_t col = place.col(n);
             if (col >= p.ldh) continue;
             const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
+            f32x4 gate_sum = {0.0f, 0.0f, 0.0f, 0.0f}, up_sum = gate_sum;
 #pragma unroll
             for (int m = 0; m < S::TM; ++m) {
                 const int64_t row = place.row(m);
@@ -258,8 +274,13 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
                 if constexpr (backward) {
                     keep(dg, p.dgate);
                     keep(du, p.dup);
+                    gate_sum += dg;
+                    up_sum += du;
                 }
             }
+            if constexpr (backward)
+                if (p.b_gate_part || p.b_up_part)
+                    keep_bias_sums(gate_sum, up_sum, p.b_gate_part, p.b_up_part, tm * S::WM + threadIdx.x / kWave % S::WM, col, p.hidden);
         }
     });
 }
@@ -374,9 +395,9 @@ struct JoinArgs {
         int64_t count;
     } job[6];
     int64_t blocks[6];   // of every job
-    int splits;
+    int splits[6];
 };
-constexpr int kJoinThreads = 256, kJoinNumbers = 32 * 4;
+constexpr int kJoinThreads = 1024, kJoinNumbers = 32 * 4;
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
     constexpr int groups = kJoinThreads / 32;
@@ -385,11 +406,12 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
     int j = 0;
     while (j < 5 && block >= p.blocks[j]) block -= p.blocks[j++];
     const auto job = p.job[j];
+    const int splits = p.splits[j];
     const int64_t i = block * kJoinNumbers + threadIdx.x % 32 * 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (i < job.count)
 #pragma unroll 4
-        for (int s = threadIdx.x / 32; s < p.splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count - i);
+        for (int s = threadIdx.x / 32; s < splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count - i);
     shared[threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.x >= 32 || i >= job.count) return;
