@@ -3,11 +3,15 @@
 // A call on a few rows lasts as long as the host needs to make it, so the whole of it is here, the backward pass too.
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
-#include <optional>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
@@ -15,9 +19,8 @@
 
 namespace py = pybind11;
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
-using Maybe = std::optional<Tensor>;
 
 namespace {
 
@@ -83,7 +86,7 @@ int32_t size32(int64_t n, const char* name) {
 // x as rows of its last dimension: as it is where the rows lie one stride apart, else a copy
 struct Rows {
     Tensor x;
-    int64_t rows, stride;
+    int64_t rows = 0, stride = 0;
 };
 Rows rows_of(const Tensor& x) {
     const int64_t d = x.size(-1), rows = d ? x.numel() / d : 0;
@@ -103,40 +106,41 @@ Rows rows_of(const Tensor& x) {
     return Rows{x.contiguous(), rows, d};
 }
 
+// ---- what a call takes and makes
 struct On {
     c10::DeviceGuard guard;
     void* stream;
     explicit On(const Tensor& x)
         : guard(x.device()), stream((void*)c10::hip::getCurrentHIPStream(x.device().index()).stream()) {}
 };
-Tensor fresh_like(const Tensor& x) { return at::empty(x.sizes(), x.options().requires_grad(false)); }
-Tensor bytes_on(const Tensor& x, int64_t bytes) {
-    return bytes > 0 ? at::empty({bytes}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
-}
+Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor& on) { return at::detail::empty_cuda(shape, type, on.device(), std::nullopt); }
+Tensor make_like(const Tensor& x) { return make(x.sizes(), x.scalar_type(), x); }
+Tensor bytes_on(const Tensor& x, int64_t bytes) { return bytes > 0 ? make({bytes}, at::kByte, x) : Tensor(); }
 void* at_or_null(const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; }
 
-// Whether a call has to make an autograd node.  (A tangent of forward mode does not show in requires_grad: the node refuses it, where
-// the operator called by itself would drop it.)
-bool wants_node(std::initializer_list<const Tensor*> inputs) {
-    const bool grad = at::GradMode::is_enabled();
-    for (const Tensor* x : inputs)
-        if (x->defined() && ((grad && x->requires_grad()) || x->_fw_grad(0).defined())) return true;
-    return false;
+// Whether a call has to make an autograd node.  A tangent of forward mode has no node to go to.
+template <size_t n>
+bool wants_node(const Tensor* const (&inputs)[n], const char* name) {
+    bool wants = false;
+    for (const Tensor* x : inputs) {
+        if (!x->defined()) continue;
+        wants = wants || x->requires_grad();
+        if (x->_fw_grad(0).defined()) fail(std::string("svox.") + name + " has no derivatives in forward mode");
+    }
+    return wants && at::GradMode::is_enabled();
 }
-// A node has an edge for each tensor it was given: wanted(ctx, i) says whether the gradient of argument i is asked for.
-void keep_edges(AutogradContext* ctx, std::initializer_list<const Tensor*> inputs) {
-    int64_t given = 0, i = 0;
-    for (const Tensor* x : inputs) given |= (int64_t)x->defined() << i++;
-    ctx->saved_data["given"] = given;
-}
-bool wanted(AutogradContext* ctx, int argument) {
-    const int64_t given = ctx->saved_data["given"].toInt();
-    if (!(given >> argument & 1)) return false;
-    return ctx->needs_input_grad((size_t)__builtin_popcountll(given & ((1ll << argument) - 1)));
-}
-Maybe given(const Tensor& x) { return x.defined() ? Maybe(x) : Maybe(); }
 void once(const char* name) {
     if (at::GradMode::is_enabled()) fail(std::string("svox.") + name + ": its gradient cannot be differentiated again (create_graph)");
+}
+// A node of the given inputs' graph, to which `y` is then tied.
+template <class N, class... Inputs>
+std::shared_ptr<N> node_of(const Inputs&... inputs) {
+    std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return node;
+}
+void make_contiguous(Tensor& x) {
+    if (x.defined() && !x.is_contiguous()) x = x.contiguous();
 }
 
 // ---- layer norm
@@ -155,65 +159,75 @@ SvoxLayerNorm norm_spec(const Rows& x, const Tensor& weight, const Tensor& bias,
 Tensor norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, Tensor* stats) {
     const On on(x);
     const Rows rows = rows_of(x);
-    Tensor y = fresh_like(x);
-    if (stats) *stats = at::empty({rows.rows, 2}, x.options().dtype(at::kFloat).requires_grad(false));
+    Tensor y = make_like(x);
+    if (stats) *stats = make({rows.rows, 2}, at::kFloat, x);
     const SvoxLayerNorm s = norm_spec(rows, weight, bias, eps);
     status(lib.svox_layer_norm(&s, y.data_ptr(), stats ? (float*)stats->data_ptr() : nullptr, on.stream), "layer_norm");
     return y;
 }
 
-struct NormNode : torch::autograd::Function<NormNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& weight_, const Maybe& bias_, double eps) {
-        const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
-        Tensor stats;
-        Tensor y = norm_forward(x, weight, bias, eps, &stats);
-        ctx->save_for_backward({x, weight, stats});
-        keep_edges(ctx, {&x, &weight, &bias});
-        ctx->saved_data["eps"] = eps;
-        return y;
+struct NormNode : torch::autograd::Node {
+    SavedVariable x_, weight_, stats_;
+    double eps = 0.0;
+
+    std::string name() const override { return "SvoxLayerNormBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        weight_.reset_data();
+        stats_.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        variable_list out(4);
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(3);
         if (!grads[0].defined()) return out;
         once("layer_norm");
-        const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
+        const Tensor x = x_.unpack(), weight = weight_.unpack(), stats = stats_.unpack();
         const On on(x);
         check_like(grads[0], x, "grad_output");
         const Rows rows = rows_of(x), dy = rows_of(grads[0]);
-        const SvoxLayerNorm s = norm_spec(rows, weight, Tensor(), ctx->saved_data["eps"].toDouble());
-        Tensor dw, db;
-        if (wanted(ctx, 0)) out[0] = fresh_like(x);
-        if (wanted(ctx, 1)) out[1] = dw = at::empty({s.dim}, x.options().requires_grad(false));
-        if (wanted(ctx, 2)) out[2] = db = at::empty({s.dim}, x.options().requires_grad(false));
-        const int64_t bytes = status(lib.svox_layer_norm_workspace_bytes(&s, dw.defined() || db.defined()), "layer_norm");
+        const SvoxLayerNorm s = norm_spec(rows, weight, Tensor(), eps);
+        if (task_should_compute_output(0)) out[0] = make_like(x);
+        if (task_should_compute_output(1)) out[1] = make({s.dim}, x.scalar_type(), x);
+        if (task_should_compute_output(2)) out[2] = make({s.dim}, x.scalar_type(), x);
+        const int64_t bytes = status(lib.svox_layer_norm_workspace_bytes(&s, out[1].defined() || out[2].defined()), "layer_norm");
         const Tensor space = bytes_on(x, bytes);
-        status(lib.svox_layer_norm_backward(&s, (const float*)stats.data_ptr(), dy.x.data_ptr(), dy.stride, at_or_null(out[0]), at_or_null(dw),
-                                            at_or_null(db), at_or_null(space), bytes, on.stream),
+        status(lib.svox_layer_norm_backward(&s, (const float*)stats.data_ptr(), dy.x.data_ptr(), dy.stride, at_or_null(out[0]), at_or_null(out[1]),
+                                            at_or_null(out[2]), at_or_null(space), bytes, on.stream),
                "layer_norm_backward");
         return out;
     }
 };
 
-Tensor layer_norm(const Tensor& x, const Maybe& weight_, const Maybe& bias_, double eps) {
-    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+Tensor layer_norm(const Tensor& x, Tensor weight, Tensor bias, double eps) {
     check_like(x, x, "x");
     dtype_code(x, "x");
     if (x.dim() < 1) fail("x must have at least one dimension");
     const int64_t d = size32(x.size(-1), "the size of x's rows");
     if (weight.defined()) check_like(weight, x, "weight"), check_shape(weight, {d}, "weight");
     if (bias.defined()) check_like(bias, x, "bias"), check_shape(bias, {d}, "bias");
-    const py::gil_scoped_release unlocked;
-    const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
-    if (wants_node({&x, &w, &b})) return NormNode::apply(x, given(w), given(b), eps);
-    return norm_forward(x, w, b, eps, nullptr);
+    make_contiguous(weight);
+    make_contiguous(bias);
+    if (!wants_node({&x, &weight, &bias}, "layer_norm")) return norm_forward(x, weight, bias, eps, nullptr);
+    const auto node = node_of<NormNode>(x, weight, bias);
+    Tensor stats, y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView guard;
+        y = norm_forward(x, weight, bias, eps, &stats);
+    }
+    node->x_ = SavedVariable(x, false);
+    node->weight_ = SavedVariable(weight, false);
+    node->stats_ = SavedVariable(stats, false);
+    node->eps = eps;
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 // ---- the gated feed-forward block
 struct Ffn {
     Tensor x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual;
 };
-SvoxGatedFfn ffn_spec(const Ffn& f, const Rows& x, int64_t activation) {
+SvoxGatedFfn ffn_spec(const Ffn& f, const Rows& x, int32_t activation) {
     SvoxGatedFfn s{};
     s.x = x.x.data_ptr();
     s.w_gate = f.w_gate.data_ptr();
@@ -228,15 +242,15 @@ SvoxGatedFfn ffn_spec(const Ffn& f, const Rows& x, int64_t activation) {
     s.hidden = (int32_t)f.w_gate.size(0);
     s.out = (int32_t)f.w_down.size(0);
     s.dtype = dtype_code(f.x, "x");
-    s.activation = (int32_t)activation;
+    s.activation = activation;
     return s;
 }
-std::vector<int64_t> out_shape(const Ffn& f) {
-    std::vector<int64_t> shape = f.x.sizes().vec();
+c10::SmallVector<int64_t, 6> out_shape(const Ffn& f) {
+    c10::SmallVector<int64_t, 6> shape(f.x.sizes().begin(), f.x.sizes().end());
     shape.back() = f.w_down.size(0);
     return shape;
 }
-Tensor ffn_forward(const Ffn& f, int64_t activation) {
+Tensor ffn_forward(const Ffn& f, int32_t activation) {
     const On on(f.x);
     const Rows x = rows_of(f.x);
     SvoxGatedFfn s = ffn_spec(f, x, activation);
@@ -246,40 +260,38 @@ Tensor ffn_forward(const Ffn& f, int64_t activation) {
         s.residual = residual.x.data_ptr();
         s.residual_stride = residual.stride;
     }
-    Tensor y = at::empty(out_shape(f), f.x.options().requires_grad(false));
+    Tensor y = make(out_shape(f), f.x.scalar_type(), f.x);
     const int64_t bytes = status(lib.svox_gated_ffn_workspace_bytes(&s, 0), "gated_ffn");
     const Tensor space = bytes_on(f.x, bytes);
     status(lib.svox_gated_ffn(&s, y.data_ptr(), at_or_null(space), bytes, on.stream), "gated_ffn");
     return y;
 }
 
-struct FfnNode : torch::autograd::Function<FfnNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down, const Maybe& b_gate,
-                          const Maybe& b_up, const Maybe& b_down, const Maybe& residual, int64_t activation) {
-        const Tensor none;
-        const Ffn f{x, w_gate, w_up, w_down, b_gate.value_or(none), b_up.value_or(none), b_down.value_or(none), residual.value_or(none)};
-        Tensor y = ffn_forward(f, activation);
-        ctx->save_for_backward({x, w_gate, w_up, w_down, f.b_gate, f.b_up});
-        keep_edges(ctx, {&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up, &f.b_down, &f.residual});
-        ctx->saved_data["activation"] = activation;
-        return y;
+struct FfnNode : torch::autograd::Node {
+    SavedVariable saved_[6];   // x, w_gate, w_up, w_down, b_gate, b_up
+    int32_t activation = 0;
+
+    std::string name() const override { return "SvoxGatedFfnBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable& v : saved_) v.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        variable_list out(9);
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(8);
         if (!grads[0].defined()) return out;
         once("gated_ffn");
-        const variable_list saved = ctx->get_saved_variables();
-        const Ffn f{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], Tensor(), Tensor()};
+        const Ffn f{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), saved_[5].unpack(), Tensor(), Tensor()};
         const On on(f.x);
         check_like(grads[0], f.x, "grad_output");
-        if (wanted(ctx, 7)) out[7] = grads[0];
+        if (task_should_compute_output(7)) out[7] = grads[0];
         const Rows x = rows_of(f.x), dy = rows_of(grads[0]);
-        const SvoxGatedFfn s = ffn_spec(f, x, ctx->saved_data["activation"].toInt());
-        const Tensor shaped[7] = {f.x, f.w_gate, f.w_up, f.w_down, f.b_gate, f.b_up, Tensor()};
+        const SvoxGatedFfn s = ffn_spec(f, x, activation);
+        const Tensor* const shaped[6] = {&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up};
         bool any = false;
         for (int i = 0; i < 7; ++i)
-            if (wanted(ctx, i)) {
-                out[i] = i == 6 ? at::empty({s.out}, f.x.options().requires_grad(false)) : fresh_like(shaped[i]);
+            if (task_should_compute_output(i)) {
+                out[i] = i == 6 ? make({s.out}, f.x.scalar_type(), f.x) : make_like(*shaped[i]);
                 any = true;
             }
         if (!any) return out;
@@ -292,38 +304,94 @@ struct FfnNode : torch::autograd::Function<FfnNode> {
     }
 };
 
-Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Tensor& w_down, const Maybe& b_gate, const Maybe& b_up,
-                 const Maybe& b_down, const Maybe& residual, int64_t activation) {
-    Ffn f{x, w_gate, w_up, w_down, b_gate.value_or(Tensor()), b_up.value_or(Tensor()), b_down.value_or(Tensor()), residual.value_or(Tensor())};
+Tensor gated_ffn(Ffn& f, int64_t activation) {
+    const Tensor& x = f.x;
     check_like(x, x, "x");
     dtype_code(x, "x");
     if (x.dim() < 1) fail("x must have at least one dimension");
-    check_like(w_gate, x, "w_gate");
-    check_like(w_up, x, "w_up");
-    check_like(w_down, x, "w_down");
-    if (w_gate.dim() != 2 || w_down.dim() != 2) fail("w_gate, w_up and w_down must be 2-D");
-    const int64_t d = size32(x.size(-1), "the size of x's rows"), h = size32(w_gate.size(0), "the number of hidden units"),
-                  o = size32(w_down.size(0), "the size of the result's rows");
-    check_shape(w_gate, {h, d}, "w_gate");
-    check_shape(w_up, {h, d}, "w_up");
-    check_shape(w_down, {o, h}, "w_down");
+    check_like(f.w_gate, x, "w_gate");
+    check_like(f.w_up, x, "w_up");
+    check_like(f.w_down, x, "w_down");
+    if (f.w_gate.dim() != 2 || f.w_down.dim() != 2) fail("w_gate, w_up and w_down must be 2-D");
+    const int64_t d = size32(x.size(-1), "the size of x's rows"), h = size32(f.w_gate.size(0), "the number of hidden units"),
+                  o = size32(f.w_down.size(0), "the size of the result's rows");
+    check_shape(f.w_gate, {h, d}, "w_gate");
+    check_shape(f.w_up, {h, d}, "w_up");
+    check_shape(f.w_down, {o, h}, "w_down");
     if (f.b_gate.defined()) check_like(f.b_gate, x, "b_gate"), check_shape(f.b_gate, {h}, "b_gate");
     if (f.b_up.defined()) check_like(f.b_up, x, "b_up"), check_shape(f.b_up, {h}, "b_up");
     if (f.b_down.defined()) check_like(f.b_down, x, "b_down"), check_shape(f.b_down, {o}, "b_down");
     if (f.residual.defined()) check_like(f.residual, x, "residual"), check_shape(f.residual, out_shape(f), "residual");
     if (activation < SVOX_ACTIVATION_SILU || activation > SVOX_ACTIVATION_SIGMOID) fail("unknown activation " + std::to_string(activation));
-    const py::gil_scoped_release unlocked;
-    for (Tensor* t : {&f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up, &f.b_down})
-        if (t->defined()) *t = t->contiguous();
-    if (wants_node({&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up, &f.b_down, &f.residual}))
-        return FfnNode::apply(f.x, f.w_gate, f.w_up, f.w_down, given(f.b_gate), given(f.b_up), given(f.b_down), given(f.residual), activation);
-    return ffn_forward(f, activation);
+    for (Tensor* t : {&f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up, &f.b_down}) make_contiguous(*t);
+    if (!wants_node({&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up, &f.b_down, &f.residual}, "gated_ffn"))
+        return ffn_forward(f, (int32_t)activation);
+    const auto node = node_of<FfnNode>(f.x, f.w_gate, f.w_up, f.w_down, f.b_gate, f.b_up, f.b_down, f.residual);
+    Tensor y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView guard;
+        y = ffn_forward(f, (int32_t)activation);
+    }
+    const Tensor* const saved[6] = {&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up};
+    for (int i = 0; i < 6; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
+    node->activation = (int32_t)activation;
+    torch::autograd::set_history(y, node);
+    return y;
 }
+
+// ---- called from Python with positional arguments
+struct WrongType {
+    const char* name;
+};
+const Tensor& tensor(PyObject* x, const char* name) {
+    if (!THPVariable_Check(x)) throw WrongType{name};
+    return THPVariable_Unpack(x);
+}
+Tensor tensor_or_none(PyObject* x, const char* name) { return x == Py_None ? Tensor() : tensor(x, name); }
+
+template <class F>
+PyObject* call(Py_ssize_t given, Py_ssize_t wanted, F f) {
+    if (given != wanted) {
+        PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", wanted, given);
+        return nullptr;
+    }
+    try {
+        return THPVariable_Wrap(f());
+    } catch (const WrongType& e) {
+        PyErr_Format(PyExc_TypeError, "%s must be a tensor", e.name);
+    } catch (py::error_already_set& e) {
+        e.restore();
+    } catch (...) {
+        torch::translate_exception_to_python(std::current_exception());
+    }
+    return nullptr;
+}
+PyObject* layer_norm_py(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return call(given, 4, [&] {
+        const Tensor &x = tensor(args[0], "x"), weight = tensor_or_none(args[1], "weight"), bias = tensor_or_none(args[2], "bias");
+        const double eps = PyFloat_AsDouble(args[3]);
+        if (eps == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+        const py::gil_scoped_release unlocked;
+        return layer_norm(x, weight, bias, eps);
+    });
+}
+PyObject* gated_ffn_py(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return call(given, 9, [&] {
+        Ffn f{tensor(args[0], "x"), tensor(args[1], "w_gate"), tensor(args[2], "w_up"), tensor(args[3], "w_down"), tensor_or_none(args[4], "b_gate"),
+              tensor_or_none(args[5], "b_up"), tensor_or_none(args[6], "b_down"), tensor_or_none(args[7], "residual")};
+        const int64_t activation = PyLong_AsLongLong(args[8]);
+        if (activation == -1 && PyErr_Occurred()) throw py::error_already_set();
+        const py::gil_scoped_release unlocked;
+        return gated_ffn(f, activation);
+    });
+}
+PyMethodDef kCalls[] = {{"layer_norm", (PyCFunction)(void (*)())layer_norm_py, METH_FASTCALL, nullptr},
+                        {"gated_ffn", (PyCFunction)(void (*)())gated_ffn_py, METH_FASTCALL, nullptr},
+                        {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("init", &init);
-    m.def("layer_norm", &layer_norm);
-    m.def("gated_ffn", &gated_ffn);
+    PyModule_AddFunctions(m.ptr(), kCalls);
 }

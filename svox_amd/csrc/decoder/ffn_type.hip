@@ -12,9 +12,12 @@ constexpr int64_t kMostLd = TileOf<true, 64, 64, 256>::most_ld;
 constexpr int kKT = kPlanes == 1 ? 64 : 32;
 // Large tiles, where there are enough of them; small ones with more of the reduction on its way, where a block waits for
 // memory more than it multiplies.
+// (The step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16 takes 2021 us with eight wavefronts to a block, 2090 with four; that of
+// 8192 rows of 256 -> 1024 -> 256 in float32, whose planes make tiles three times as large, 537 us with tiles of 128 x 128 and one
+// block to a compute unit, 500 with half as large ones and two.)
 struct Large {
-    using Hidden = Shape<128, 64, kKT, 2, 4, 2>;
-    using Output = Shape<128, 128, kKT, 2, 4, 2>;
+    using Hidden = std::conditional_t<kPlanes == 1, Shape<128, 64, kKT, 2, 4, 2>, Shape<64, 64, kKT, 2, 2, 2>>;
+    using Output = std::conditional_t<kPlanes == 1, Shape<128, 128, kKT, 2, 4, 2>, Shape<64, 128, kKT, 2, 2, 2>>;
     using Weight = Output;
 };
 struct Small {
@@ -22,7 +25,7 @@ struct Small {
     using Output = Shape<64, 64, kKT, 2, 2, 4>;
     using Weight = Output;
 };
-constexpr int64_t kLargeTiles = kPlanes == 1 ? 192 : 96;
+constexpr int64_t kLargeTiles = 192;
 template <class S>
 int64_t tiles_of(int64_t m, int64_t n) {
     return pieces(m, S::BM) * pieces(n, S::BN);

@@ -26,7 +26,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     Mean, variance and the sums of the gradients are held in 32 bits and do not depend on the order in which the GPU works.
     """
-    return _calls().layer_norm(x, weight, bias, eps)
+    return (_native or _calls()).layer_norm(x, weight, bias, eps)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, residual=None, activation="silu"):
@@ -46,4 +46,4 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, resi
     code = _D.ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"unknown activation {activation!r}: one of {', '.join(_D.ACTIVATIONS)}")
-    return _calls().gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, code)
+    return (_native or _calls()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, code)
