@@ -2,7 +2,7 @@
 
 Use it where `import svox` was used:  `import svox_amd as svox`.
 """
-from .decoder import gated_ffn, layer_norm
+from .decoder import LeafDecoder, gated_ffn, layer_norm
 from .formats import DataFormat, LocalIndex, NDCConfig, Rays
 from .renderer import VolumeRenderer
 from .tree import N3Tree
@@ -10,4 +10,4 @@ from .view import N3TreeView
 
 __version__ = "0.1.0"
 __all__ = ["N3Tree", "N3TreeView", "VolumeRenderer", "NDCConfig", "Rays", "LocalIndex", "DataFormat",
-           "layer_norm", "gated_ffn"]
+           "LeafDecoder", "layer_norm", "gated_ffn"]

@@ -1,10 +1,16 @@
-"""The operators of a leaf decoder, a small network that turns the features kept in the leaves of a tree into records a
-renderer reads: layer norm and the gated feed-forward block, each a few HIP kernels with its gradient.  The reference has no
-such operators.
+"""A leaf decoder: a small network that turns the features kept in the leaves of a tree into records a renderer reads.
+
+A tree may hold any numbers (`N3Tree(data_format=None, data_dim=D)`); what the renderer reads are records of basis
+coefficients and density.  `LeafDecoder` makes the one from the other with two operators, `layer_norm` and `gated_ffn`, each a
+few HIP kernels with its gradient; the gradient of the records that a rendering leaves goes back through it to the network's
+weights and to the features.  The reference has no such operators.
 """
+import torch
+from torch import nn
+
 from .csrc import decoder as _D
 
-__all__ = ["layer_norm", "gated_ffn"]
+__all__ = ["layer_norm", "gated_ffn", "LeafDecoder"]
 
 _native = None
 
@@ -47,3 +53,89 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, resi
     if code is None:
         raise ValueError(f"unknown activation {activation!r}: one of {', '.join(_D.ACTIVATIONS)}")
     return (_native or _calls()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, code)
+
+
+class _Norm(nn.Module):
+    def __init__(self, dim, eps, **kw):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim, **kw))
+        self.bias = nn.Parameter(torch.zeros(dim, **kw))
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class _Ffn(nn.Module):
+    def __init__(self, dim, hidden, out, activation, **kw):
+        super().__init__()
+        self.activation = activation
+        self.w_gate = nn.Parameter(torch.randn(hidden, dim, **kw) * dim ** -0.5)
+        self.w_up = nn.Parameter(torch.randn(hidden, dim, **kw) * dim ** -0.5)
+        self.w_down = nn.Parameter(torch.randn(out, hidden, **kw) * hidden ** -0.5)
+        self.b_gate = nn.Parameter(torch.zeros(hidden, **kw))
+        self.b_up = nn.Parameter(torch.zeros(hidden, **kw))
+        self.b_down = nn.Parameter(torch.zeros(out, **kw))
+
+    def forward(self, x, residual=None):
+        return gated_ffn(x, self.w_gate, self.w_up, self.w_down, self.b_gate, self.b_up, self.b_down, residual=residual,
+                         activation=self.activation)
+
+
+class LeafDecoder(nn.Module):
+    """Features of a leaf to its record: `depth` blocks x + ffn(norm(x)) over the features, then ffn(norm(x)) to the record.
+
+    A decoder that is trained through a renderer, with the features of every leaf:
+
+        features = svox.N3Tree(data_format=None, data_dim=16, init_refine=4, device="cuda:0")
+        tree = svox.N3Tree(data_format="SH4", init_refine=4, device="cuda:0")
+        decoder = svox.LeafDecoder(16, tree.data_dim, hidden=64).cuda()
+        renderer = svox.VolumeRenderer(tree)
+        for rays, target in batches:
+            loss = decoder.backward_through(features, tree, lambda: ((renderer(rays) - target) ** 2).mean())
+            optimizer.step()
+
+    :param features: numbers of a leaf's features
+    :param record: numbers of a record (`tree.data_dim`)
+    :param hidden: hidden units of every block (default: four for each feature)
+    """
+
+    def __init__(self, features, record, hidden=None, depth=1, activation="silu", eps=1e-5, device=None, dtype=torch.float32):
+        super().__init__()
+        if activation not in _D.ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(_D.ACTIVATIONS)}")
+        kw = dict(device=device, dtype=dtype)
+        hidden = 4 * features if hidden is None else hidden
+        self.norms = nn.ModuleList(_Norm(features, eps, **kw) for _ in range(depth + 1))
+        self.ffns = nn.ModuleList([_Ffn(features, hidden, features, activation, **kw) for _ in range(depth)]
+                                  + [_Ffn(features, hidden, record, activation, **kw)])
+
+    def forward(self, x):
+        """(..., features) to (..., record), in the type of the weights."""
+        x = x.to(self.norms[0].weight.dtype)
+        for norm, ffn in zip(self.norms[:-1], self.ffns[:-1]):
+            x = ffn(norm(x), residual=x)
+        return self.ffns[-1](self.norms[-1](x))
+
+    def decode_tree(self, features, tree):
+        """Writes the records of the features in the tree `features` into `tree`, a tree of the same structure, and returns
+        them, (cells, record), for a backward pass.  Every cell is decoded, also those that have children and are not read."""
+        if features.child.shape != tree.child.shape or features.data.shape[:4] != tree.data.shape[:4]:
+            raise ValueError("features and tree must have the same structure")
+        records = self(features.data.reshape(-1, features.data_dim))
+        if records.shape[1] != tree.data_dim:
+            raise ValueError(f"the decoder makes records of {records.shape[1]} numbers, the tree's have {tree.data_dim}")
+        with torch.no_grad():
+            tree.data.copy_(records.view_as(tree.data))
+        return records
+
+    def backward_through(self, features, tree, loss):
+        """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
+        adds the gradients of what it returns to those of the decoder's weights and of `features.data`.  Returns the loss."""
+        records = self.decode_tree(features, tree)
+        tree.data.grad = None
+        value = loss()
+        value.backward()
+        records.backward(tree.data.grad.view_as(records).to(records.dtype))
+        tree.data.grad = None
+        return value.detach()

@@ -88,6 +88,21 @@ def test_there_is_no_cpu_path():
         svox.layer_norm(None)
 
 
+def test_leaf_decoder_is_a_module_like_others(tmp_path):
+    decoder = svox.LeafDecoder(12, 28, hidden=40, depth=2, activation="gelu")
+    assert [tuple(p.shape) for p in decoder.ffns[2].parameters()] == [(40, 12), (40, 12), (28, 40), (40,), (40,), (28,)]
+    assert len(decoder.norms) == len(decoder.ffns) == 3 and all(p.requires_grad for p in decoder.parameters())
+    torch.save(decoder.state_dict(), tmp_path / "decoder.pt")
+    other = svox.LeafDecoder(12, 28, hidden=40, depth=2)
+    other.load_state_dict(torch.load(tmp_path / "decoder.pt", weights_only=True))
+    assert all(torch.equal(a, b) for a, b in zip(decoder.parameters(), other.parameters()))
+    assert svox.LeafDecoder(16, 4).ffns[0].w_gate.shape == (64, 16)
+    with pytest.raises(ValueError, match="unknown activation"):
+        svox.LeafDecoder(12, 4, activation="tanh")
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        decoder(torch.zeros(5, 12))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_the_bounds_hold_for_torch_and_see_a_mistake(dtype):
     """torch's own float32 result, rounded once, lies within the reference's bounds; one with numbers of a column out of place does not."""
