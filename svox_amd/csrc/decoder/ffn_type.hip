@@ -46,8 +46,8 @@ struct Lays {
         to.at = room.take<u16>(kPlanes * rows * wide);
         LayJob<T>& job = args.job[count++];
         const int lanes = wide >= 1024 ? 256 : wide >= 256 ? 64 : 16;
-        // (16 KiB of numbers or so to a block, and all of its lanes' rows at least)
-        const int64_t each = up_to(pieces(8192, wide), kLayThreads / lanes);
+        // (some 4096 numbers to a block, and all of its lanes' rows at least)
+        const int64_t each = up_to(pieces(4096, wide), kLayThreads / lanes);
         job = LayJob<T>{(const T*)at, ld, to, cols, pieces(rows, each), each, lanes};
         blocks += job.blocks;
         return to;
