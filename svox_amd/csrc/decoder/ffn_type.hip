@@ -285,7 +285,6 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
     OutputArgs<T> o{};
     o.a[0] = f.h;
     o.b[0] = f.w_down;
-    o.pairs = 1;
     o.bias = (const T*)s.b_down;
     o.residual = (const T*)s.residual;
     o.residual_ld = s.residual_stride;
@@ -333,7 +332,6 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
             o.a[1] = b.dup;
             o.b[0] = b.w_gate;
             o.b[1] = b.w_up;
-            o.pairs = 2;
             o.y = (T*)grads.x;
             o.rows = s.rows;
             o.cols = s.dim;

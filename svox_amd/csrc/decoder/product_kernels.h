@@ -47,15 +47,22 @@ struct Product {
 #pragma unroll
         for (int i = 0; i < NB; ++i) o.b[i].advance();
     }
-    // What a wavefront multiplies at a time: its rows and columns over 32 of the reduction.
-    struct Fragments {
-        u16x8 a[S::TM][planes], b[NB][S::TN][planes];
+    // What a wavefront multiplies at a time: `part` of its rows and all of its columns over 32 of the reduction.
+    static constexpr int parts = S::TM > 4 ? 2 : 1, PM = S::TM / parts;
+    static_assert(PM * parts == S::TM, "equal parts");
+    struct Rows {
+        u16x8 a[PM][planes];
     };
-    static __device__ __forceinline__ void read(const u16* lds, int step, int wm, int wn, Fragments& f) {
+    struct Columns {
+        u16x8 b[NB][S::TN][planes];
+    };
+    static __device__ __forceinline__ void read(const u16* lds, int step, int part, int wm, Rows& f) {
 #pragma unroll
-        for (int m = 0; m < S::TM; ++m)
+        for (int m = 0; m < PM; ++m)
 #pragma unroll
-            for (int p = 0; p < planes; ++p) f.a[m][p] = A::fragment(lds + p * A::numbers, (wm * S::TM + m) * 16, step);
+            for (int p = 0; p < planes; ++p) f.a[m][p] = A::fragment(lds + p * A::numbers, (wm * S::TM + part * PM + m) * 16, step);
+    }
+    static __device__ __forceinline__ void read(const u16* lds, int step, int wn, Columns& f) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -66,21 +73,22 @@ struct Product {
     }
     // ones: also the sums of the left operand's columns (over the reduction), in `sums`
     template <bool ones>
-    static __device__ __forceinline__ void multiply_all(const Fragments& f, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
+    static __device__ __forceinline__ void multiply_all(const Rows& rows, const Columns& columns, int part, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if constexpr (ones) {
             u16x8 one;
             for (int i = 0; i < 8; ++i) one[i] = Form<T>::one();
 #pragma unroll
-            for (int m = 0; m < S::TM; ++m)
+            for (int m = 0; m < PM; ++m)
 #pragma unroll
-                for (int p = planes; p-- > 0;) sums[m] = Form<T>::mma(one, f.a[m][p], sums[m]);
+                for (int p = planes; p-- > 0;) sums[part * PM + m] = Form<T>::mma(one, rows.a[m][p], sums[part * PM + m]);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int n = 0; n < S::TN; ++n)
 #pragma unroll
-                for (int m = 0; m < S::TM; ++m) acc[i][m][n] = multiply<T>(f.b[i][n], f.a[m], acc[i][m][n]);
+                for (int m = 0; m < PM; ++m)
+                    acc[i][part * PM + m][n] = multiply<T>(columns.b[i][n], rows.a[m], acc[i][part * PM + m][n]);
     }
     // Adds the products over [k, k_end) to acc.  LDS holds S::stages tiles of the reduction, registers the fragments of two steps:
     // while one is multiplied the next one is read, also from tile to tile.  At the barrier between two tiles every wavefront
@@ -118,21 +126,32 @@ struct Product {
             if (i < tiles) load_next();
         wait(loaded == S::stages - 1);
         if (loaded < tiles) load_next();
-        Fragments f[2];
-        read(lds, 0, wm, wn, f[0]);
-        auto tile = [&](int t, auto parity) {   // its first step is in f[parity]
+        Rows rows[2];
+        Columns columns[2];
+        read(lds, 0, 0, wm, rows[0]);
+        read(lds, 0, wn, columns[0]);
+        constexpr int units = steps * parts;
+        auto tile = [&](int t, auto parity) {   // its first fragments are in rows[parity], columns[parity]
             constexpr int first = decltype(parity)::value;
+            static_assert(parts == 1 || first == 0, "");
+            const u16 *at = lds + t % S::stages * stage;
 #pragma unroll
-            for (int s = 0; s + 1 < steps; ++s) {
-                read(lds + t % S::stages * stage, s + 1, wm, wn, f[(first + s + 1) & 1]);
-                multiply_all<ones>(f[(first + s) & 1], acc, sums);
+            for (int u = 0; u < units; ++u) {
+                const int next = (u + 1) % units;
+                if (u + 1 == units) {
+                    if (t + 1 < tiles) {
+                        wait(loaded - t - 2 >= S::stages - 2);
+                        if (loaded < tiles) load_next();
+                        at = lds + (t + 1) % S::stages * stage;
+                        read(at, 0, 0, wm, rows[(first + units) & 1]);
+                        read(at, 0, wn, columns[(first + steps) & 1]);
+                    }
+                } else {
+                    read(at, next / parts, next % parts, wm, rows[(first + u + 1) & 1]);
+                    if (next % parts == 0) read(at, next / parts, wn, columns[(first + next / parts) & 1]);
+                }
+                multiply_all<ones>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
             }
-            if (t + 1 < tiles) {
-                wait(loaded - t - 2 >= S::stages - 2);
-                if (loaded < tiles) load_next();
-                read(lds + (t + 1) % S::stages * stage, 0, wm, wn, f[(first + steps) & 1]);
-            }
-            multiply_all<ones>(f[(first + steps - 1) & 1], acc, sums);
         };
         if constexpr (steps % 2 == 0) {
             for (int t = 0; t < tiles; ++t) tile(t, std::integral_constant<int, 0>());
@@ -287,8 +306,7 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
 
 template <class T>
 struct OutputArgs {
-    Planes a[2], b[2];     // y = sum over `pairs` of a[i] times b[i]
-    int pairs;
+    Planes a[2], b[2];     // y = a[0] b[0] + a[1] b[1]; one product where b is used along its rows
     const T *bias, *residual;
     int64_t residual_ld;
     T* y;                  // (rows, cols), dense
@@ -306,7 +324,8 @@ __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) 
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
     f32x4 acc[1][S::TM][S::TN];
     clear(acc);
-    for (int i = 0; i < p.pairs; ++i) P::template run<false>(p.a[i], &p.b[i], m0, n0, 0, p.a[i].cols, lds, acc, nullptr);
+    P::template run<false>(p.a[0], &p.b[0], m0, n0, 0, p.a[0].cols, lds, acc, nullptr);
+    if constexpr (!along_b) P::template run<false>(p.a[1], &p.b[1], m0, n0, 0, p.a[1].cols, lds, acc, nullptr);
     const Place<S> place(m0, n0);
 #pragma unroll
     for (int n = 0; n < S::TN; ++n) {
