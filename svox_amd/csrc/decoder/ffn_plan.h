@@ -22,9 +22,9 @@ struct Parts {
         float* const part = at;
         at += splits * count;
         if (out) {
-            join.job[jobs] = {part, (T*)out, count};
-            join.splits[jobs] = (int)splits;
-            join.blocks[jobs] = pieces(count, kJoinNumbers);
+            const int groups = join_groups(splits);
+            join.job[jobs] = {part, (T*)out, count, (int)splits, groups};
+            join.blocks[jobs] = pieces(count, kJoinThreads / groups * 4);
             blocks += join.blocks[jobs++];
         }
         return part;

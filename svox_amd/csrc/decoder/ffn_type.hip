@@ -10,12 +10,16 @@ namespace {
 constexpr int kPlanes = Form<T>::planes;
 constexpr int64_t kMostLd = TileOf<true, 64, 64, 256>::most_ld;
 constexpr int kKT = kPlanes == 1 ? 64 : 32;
-// Large tiles, where there are enough of them; small ones with more of the reduction on its way, where a block waits for
-// memory more than it multiplies.
-// (The step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16 takes 2021 us with eight wavefronts to a block, 2090 with four; that of
-// 8192 rows of 256 -> 1024 -> 256 in float32, whose planes make tiles three times as large, 537 us with tiles of 128 x 128 and one
-// block to a compute unit, 500 with half as large ones and two.)
-struct Large {
+// Medium tiles, two blocks of them to a compute unit, where there are enough; small ones with more of the reduction on its way, where
+// a block waits for memory more than it multiplies; and for 16 bits large ones, of which each block has a compute unit's LDS for
+// itself, where these fill the compute units as well: a tile of 256 x 256 takes half as many bytes from the L2 for a product as one
+// of 128 x 128 does, and two thirds as many from LDS.
+// (The step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16 takes 1553 us with large tiles, 1799 with medium ones; its hidden
+// numbers 281 and 315, result 125 and 145, their gradients 499 and 575, x's 241 and 295, the weights' 447 and 500.  Medium tiles
+// take it 2021 us with eight wavefronts to a block, 2090 with four.  The step of 8192 rows of 256 -> 1024 -> 256 in float32, whose planes
+// make tiles three times as large, 537 us with tiles of 128 x 128 and one block to a compute unit, 500 with half as large ones and
+// two.)
+struct Medium {
     using Hidden = std::conditional_t<kPlanes == 1, Shape<128, 64, kKT, 2, 4, 2>, Shape<64, 64, kKT, 2, 2, 2>>;
     using Output = std::conditional_t<kPlanes == 1, Shape<128, 128, kKT, 2, 4, 2>, Shape<64, 128, kKT, 2, 2, 2>>;
     using Weight = Output;
@@ -25,10 +29,35 @@ struct Small {
     using Output = Shape<64, 64, kKT, 2, 2, 4>;
     using Weight = Output;
 };
-constexpr int64_t kLargeTiles = 192;
+struct Large {
+    using Hidden = std::conditional_t<kPlanes == 1, Shape<256, 128, kKT, 2, 4, 2>, Medium::Hidden>;
+    using Output = std::conditional_t<kPlanes == 1, Shape<256, 256, kKT, 2, 4, 2>, Medium::Output>;
+    using Weight = Output;
+};
+constexpr int64_t kMediumTiles = 192, kUnits = 256;
+constexpr double kMediumSlower = 1.15;
 template <class S>
 int64_t tiles_of(int64_t m, int64_t n) {
     return pieces(m, S::BM) * pieces(n, S::BN);
+}
+enum Size { kSmall, kMedium, kLarge };
+// the time that `tiles` take, `at_once` of them to a compute unit and the reduction in `splits`: in rounds of the compute units, by
+// the numbers of a tile
+template <class S>
+double time_of(int64_t tiles, int at_once, int64_t splits) {
+    return (double)(pieces(tiles * splits, at_once * kUnits) * at_once * S::BM * S::BN) / (double)splits;
+}
+bool large_pays(double medium, double large) { return kPlanes == 1 && large <= kMediumSlower * medium; }
+template <class M, class L>
+Size size_of(int64_t m, int64_t n) {
+    const int64_t medium = tiles_of<M>(m, n);
+    return medium < kMediumTiles ? kSmall : large_pays(time_of<M>(medium, 2, 1), time_of<L>(tiles_of<L>(m, n), 1, 1)) ? kLarge : kMedium;
+}
+template <class F>
+void by_size(Size size, F f) {
+    if (size == kSmall) f(Small());
+    else if (size == kMedium) f(Medium());
+    else f(Large());
 }
 
 // ---- operands: where they are if the tiles can be read from there, else laid out in the workspace
@@ -142,11 +171,11 @@ struct Forward {
     }
 };
 
-// The tiles of the weights' gradients, large or small, and the rows of a split.
+// The tiles of the weights' gradients, and the rows of a split.
 struct Split {
     int64_t each;
     int splits;
-    bool large;
+    Size size;
 };
 template <class S>
 int64_t weight_tiles(const SvoxGatedFfn& s) {
@@ -154,11 +183,14 @@ int64_t weight_tiles(const SvoxGatedFfn& s) {
 }
 Split weight_split(const SvoxGatedFfn& s) {
     Split w;
+    const int64_t small = weight_tiles<Small::Weight>(s), medium = weight_tiles<Medium::Weight>(s), large = weight_tiles<Large::Weight>(s);
+    const int64_t steps = pieces(s.rows, kKT);
+    const int64_t large_splits = large < kUnits ? kUnits / large : 1, medium_splits = pieces(2 * kUnits, medium);
     // (rows enough for two blocks a compute unit of eight steps each make up for few tiles)
-    const int64_t large = weight_tiles<Large::Weight>(s), steps = pieces(s.rows, kKT);
-    w.large = large * steps >= 512 * 8;
-    const int64_t tiles = w.large ? large : weight_tiles<Small::Weight>(s);
-    int64_t splits = pieces(512, tiles);
+    w.size = kMedium;
+    if (medium * steps < 2 * kUnits * 8) w.size = kSmall;
+    else if (large_pays(time_of<Medium::Weight>(medium, 2, medium_splits), time_of<Large::Weight>(large, 1, large_splits))) w.size = kLarge;
+    int64_t splits = w.size == kLarge ? large_splits : w.size == kMedium ? medium_splits : pieces(2 * kUnits, small);
     if (splits > pieces(steps, 8)) splits = pieces(steps, 8);
     w.each = up_to(pieces(s.rows, splits), kKT);
     w.splits = (int)pieces(s.rows, w.each);
@@ -166,10 +198,14 @@ Split weight_split(const SvoxGatedFfn& s) {
 }
 
 // The rows of the biases' sums of hidden_kernel.
-bool large_hidden(const SvoxGatedFfn& s) { return tiles_of<Large::Hidden>(s.rows, up_to(s.hidden, 8)) >= kLargeTiles; }
-template <class S>
+Size hidden_size(int64_t rows, int64_t ldh) { return size_of<Medium::Hidden, Large::Hidden>(rows, ldh); }
 int64_t hidden_parts(const SvoxGatedFfn& s) {
-    return pieces(s.rows, S::BM) * S::WM;
+    int64_t parts = 0;
+    by_size(hidden_size(s.rows, up_to(s.hidden, 8)), [&](auto shapes) {
+        using S = typename decltype(shapes)::Hidden;
+        parts = pieces(s.rows, S::BM) * S::WM;
+    });
+    return parts;
 }
 struct Backward {
     Lays lays;
@@ -192,7 +228,7 @@ struct Backward {
         dgate = hidden_numbers(room, s);
         dup = hidden_numbers(room, s);
         split = weight_split(s);
-        bias_parts = few ? pieces(s.rows, 16) : large_hidden(s) ? hidden_parts<Large::Hidden>(s) : hidden_parts<Small::Hidden>(s);
+        bias_parts = few ? pieces(s.rows, 16) : hidden_parts(s);
         part = room.take<float>((split.splits > 1 ? split.splits * (2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + s.out) : 0) +
                                 bias_parts * 2 * s.hidden);
         if (any_grad)
@@ -229,8 +265,7 @@ void launch_hidden_as(HiddenArgs<T> p, hipStream_t stream) {
 }
 template <bool backward>
 void launch_hidden(const HiddenArgs<T>& p, hipStream_t stream) {
-    if (tiles_of<Large::Hidden>(p.rows, p.ldh) >= kLargeTiles) launch_hidden_as<Large::Hidden, backward>(p, stream);
-    else launch_hidden_as<Small::Hidden, backward>(p, stream);
+    by_size(hidden_size(p.rows, p.ldh), [&](auto shapes) { launch_hidden_as<typename decltype(shapes)::Hidden, backward>(p, stream); });
 }
 template <class S, bool along_b>
 void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
@@ -240,8 +275,8 @@ void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
 }
 template <bool along_b>
 void launch_output(const OutputArgs<T>& p, hipStream_t stream) {
-    if (tiles_of<Large::Output>(p.rows, p.cols) >= kLargeTiles) launch_output_as<Large::Output, along_b>(p, stream);
-    else launch_output_as<Small::Output, along_b>(p, stream);
+    by_size(size_of<Medium::Output, Large::Output>(p.rows, p.cols),
+            [&](auto shapes) { launch_output_as<typename decltype(shapes)::Output, along_b>(p, stream); });
 }
 
 template <class S>
@@ -362,8 +397,7 @@ int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64
         w.rows = s.rows;
         w.each = b.split.each;
         w.splits = b.split.splits;
-        if (b.split.large) launch_weight_as<Large::Weight>(w, stream);
-        else launch_weight_as<Small::Weight>(w, stream);
+        by_size(b.split.size, [&](auto shapes) { launch_weight_as<typename decltype(shapes)::Weight>(w, stream); });
     }
     parts.launch(stream);
     return check_launch("gated_ffn_backward");

@@ -90,23 +90,26 @@ struct Product {
                 for (int m = 0; m < PM; ++m)
                     acc[i][part * PM + m][n] = multiply<T>(columns.b[i][n], rows.a[m], acc[i][part * PM + m][n]);
     }
-    // Adds the products over [k, k_end) to acc.  LDS holds S::stages tiles of the reduction, registers the fragments of two steps:
+    // Adds the products over [k, k_end) of a and b to acc, with two `pairs` also those of a[1] and b[1], which are as large.  LDS holds S::stages tiles of the reduction, registers the fragments of two steps:
     // while one is multiplied the next one is read, also from tile to tile.  At the barrier between two tiles every wavefront
     // has read all of the first, whose place the loads of a later one take, and all lanes' loads of the second have arrived (a
     // lane's loads arrive in their order, so that waiting for some leaves the later ones on their way).
-    template <bool ones>
-    static __device__ __forceinline__ void run(const Planes& a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
+    template <bool ones, int pairs = 1>
+    static __device__ __forceinline__ void run(const Planes* a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
                                                f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if (k >= k_end) return;
         constexpr int steps = S::KT / 32;
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), wm = wave % S::WM, wn = wave / S::WM;
-        const int tiles = (int)((k_end - k + S::KT - 1) / S::KT);
-        Operands o = operands(a, b, m0, n0, k, std::make_integer_sequence<int, NB>());
+        static_assert(pairs == 1 || NB == 1, "");
+        const int each = (int)((k_end - k + S::KT - 1) / S::KT), tiles = pairs * each;
+        Operands o = operands(a[0], b, m0, n0, k, std::make_integer_sequence<int, NB>());
         int loaded = 0;
         auto load_next = [&] {
-            if (loaded == tiles - 1) {   // (an operand's own end may come a little before k_end, which is a whole number of 8)
-                const int64_t at = k + (int64_t)loaded * S::KT;
-                o.a.last(least(k_end, along_a ? a.cols : a.rows) - at);
+            if (pairs == 2 && loaded == each) o = operands(a[1], b + 1, m0, n0, k, std::make_integer_sequence<int, NB>());
+            const int of_pair = pairs == 2 && loaded >= each ? loaded - each : loaded;
+            if (of_pair == each - 1) {   // (an operand's own end may come a little before k_end, which is a whole number of 8)
+                const int64_t at = k + (int64_t)of_pair * S::KT;
+                o.a.last(least(k_end, along_a ? a[0].cols : a[0].rows) - at);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) o.b[i].last(least(k_end, along_b ? b[i].cols : b[i].rows) - at);
             }
@@ -214,6 +217,68 @@ __device__ __forceinline__ void store_four(T* to, f32x4 v, int64_t n, int64_t co
     }
 }
 
+// Results go to memory through LDS, whole rows of a block's tile at a time.  From a lane's own four numbers a store writes 16 pieces of
+// 32 bytes, each to a row of its own, and that is slow: the hidden numbers' gradients of 16 384 rows of 1024 -> 4096, in bfloat16 on
+// tiles of 256 x 128, take 775 us so and 497 through LDS (387 with nothing stored).  `of` tiles of rows of each wavefront have
+// room at a time; pieces of 16 bytes lie in an order that depends on the row, as the operands' tiles do.
+constexpr int fitting(int tiles, int bytes, int room) {
+    int of = tiles;
+    while (tiles % of != 0 || of * bytes > room) --of;
+    return of;
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <class S, class N, int of>
+struct Staged {
+    static constexpr int per = 16 / (int)sizeof(N), pieces = S::BN / per, rows = S::WM * of * 16, numbers = rows * S::BN;
+    static constexpr int turn = pieces < 8 ? pieces - 1 : 7;
+    static __device__ __forceinline__ int at(int row, int col) { return row * S::BN + ((col / per) ^ (row & turn)) * per + col % per; }
+    // where a lane's four numbers of tile (m, n) lie
+    static __device__ __forceinline__ int at_tile(int m, int n) {
+        const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+        return at((wave % S::WM * of + m % of) * 16 + (lane & 15), (wave / S::WM * S::TN + n) * 16 + (lane >> 4) * 4);
+    }
+    // f(where it lies, its row, its first column) of every piece, `m` the first of the tiles
+    template <class F>
+    static __device__ __forceinline__ void each(int64_t m0, int64_t n0, int m, F f) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < rows * pieces; i += S::threads) {
+            const int row = i / pieces, col = i % pieces * per;
+            f(at(row, col), m0 + (row / (of * 16) * S::TM + m) * 16 + row % (of * 16), n0 + col);
+        }
+    }
+};
+// A tile of results, rounded to N, to rows of `cols` numbers
+template <class S, int room, class N, class V>
+__device__ __forceinline__ void store_tile(u16* lds, N* to, int64_t m0, int64_t n0, int64_t rows, int64_t cols, V value) {
+    constexpr int of = fitting(S::TM, S::WM * 16 * S::BN * (int)sizeof(N), room * 2);
+    using Tile = Staged<S, N, of>;
+    N* const staged = reinterpret_cast<N*>(lds);
+    typedef typename Few<N, 4>::vector four;
+    typedef typename Few<N, Tile::per>::vector piece;
+#pragma unroll
+    for (int m = 0; m < S::TM; m += of) {
+        lds_barrier();
+#pragma unroll
+        for (int n = 0; n < S::TN; ++n)
+#pragma unroll
+            for (int i = 0; i < of; ++i)
+                *reinterpret_cast<four*>(staged + Tile::at_tile(m + i, n)) = __builtin_convertvector(value(m + i, n), four);
+        lds_barrier();
+        Tile::each(m0, n0, m, [&](int at, int64_t row, int64_t col) {
+            if (row >= rows) return;
+            const piece v = *reinterpret_cast<const piece*>(staged + at);
+            N* const out = to + row * cols + col;
+            if (col + Tile::per <= cols) {
+                store_few<N, Tile::per>(out, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < Tile::per; ++i)
+                    if (col + i < cols) out[i] = v[i];
+            }
+        });
+    }
+}
+
 template <class T>
 struct HiddenArgs {
     Planes x, w_gate, w_up;      // (rows, dim), (hidden, dim) twice
@@ -254,53 +319,74 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
     f32x4 acc[2][S::TM][S::TN], dh[1][S::TM][S::TN];
     clear(acc);
     const Planes w[2] = {p.w_gate, p.w_up};
-    Forward::template run<false>(p.x, w, m0, n0, 0, p.x.cols, lds, acc, nullptr);
+    Forward::template run<false>(&p.x, w, m0, n0, 0, p.x.cols, lds, acc, nullptr);
     if constexpr (backward) {
         clear(dh);
-        Back::template run<false>(p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
+        Back::template run<false>(&p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
     }
     const Place<S> place(m0, n0);
+    constexpr int results = backward ? 3 : 1;
+    constexpr int of = fitting(S::TM, results * planes * S::WM * 16 * S::BN * 2, S::stages * Forward::stage * 2);
+    using Tile = Staged<S, u16, of>;
     with_activation(p.activation, [&](auto activation) {
+        f32x4 gate_sum[S::TN], up_sum[S::TN];
 #pragma unroll
-        for (int n = 0; n < S::TN; ++n) {
-            const int64_t col = place.col(n);
-            if (col >= p.ldh) continue;
-            const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
-            f32x4 gate_sum = {0.0f, 0.0f, 0.0f, 0.0f}, up_sum = gate_sum;
+        for (int m = 0; m < S::TM; m += of) {
+            lds_barrier();
 #pragma unroll
-            for (int m = 0; m < S::TM; ++m) {
-                const int64_t row = place.row(m);
-                if (row >= p.rows) continue;
-                f32x4 h, dg, du;
+            for (int n = 0; n < S::TN; ++n) {
+                if (m == 0) gate_sum[n] = up_sum[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                const int64_t col = place.col(n);
+                if (col >= p.ldh) continue;
+                const f32x4 bg = four_of(p.b_gate, col, p.hidden - col), bu = four_of(p.b_up, col, p.hidden - col);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float g = acc[0][m][n][i] + bg[i], u = acc[1][m][n][i] + bu[i];
-                    float slope;
-                    const float a = activate<planes == 3, decltype(activation)::value>(g, backward ? &slope : nullptr);
-                    h[i] = a * u;
-                    if constexpr (backward) {
-                        dg[i] = dh[0][m][n][i] * u * slope;
-                        du[i] = dh[0][m][n][i] * a;
+                for (int j = 0; j < of; ++j) {
+                    f32x4 result[3];   // h, dgate, dup
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float g = acc[0][m + j][n][i] + bg[i], u = acc[1][m + j][n][i] + bu[i];
+                        float slope;
+                        const float a = activate<planes == 3, decltype(activation)::value>(g, backward ? &slope : nullptr);
+                        result[0][i] = a * u;
+                        if constexpr (backward) {
+                            result[1][i] = dh[0][m + j][n][i] * u * slope;
+                            result[2][i] = dh[0][m + j][n][i] * a;
+                        }
                     }
-                }
-                u16x4 part[planes];
-                const int64_t at = row * p.ldh + col;
-                auto keep = [&](f32x4 v, u16* to) {
-                    Form<T>::split(v, part);
-                    for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(to + q * p.plane + at) = part[q];
-                };
-                keep(h, p.h);
-                if constexpr (backward) {
-                    keep(dg, p.dgate);
-                    keep(du, p.dup);
-                    gate_sum += dg;
-                    up_sum += du;
+                    const int at = Tile::at_tile(m + j, n);
+#pragma unroll
+                    for (int r = 0; r < results; ++r) {
+                        u16x4 part[planes];
+                        Form<T>::split(result[r], part);
+#pragma unroll
+                        for (int q = 0; q < planes; ++q) *reinterpret_cast<u16x4*>(lds + (r * planes + q) * Tile::numbers + at) = part[q];
+                    }
+                    if constexpr (backward)
+                        if (place.row(m + j) < p.rows) {
+                            gate_sum[n] += result[1];
+                            up_sum[n] += result[2];
+                        }
                 }
             }
-            if constexpr (backward)
-                if (p.b_gate_part || p.b_up_part)
-                    keep_bias_sums(gate_sum, up_sum, p.b_gate_part, p.b_up_part, tm * S::WM + threadIdx.x / kWave % S::WM, col, p.hidden);
+            lds_barrier();
+            Tile::each(m0, n0, m, [&](int at, int64_t row, int64_t col) {
+                if (row >= p.rows || col >= p.ldh) return;
+                u16* const to[3] = {p.h, p.dgate, p.dup};
+#pragma unroll
+                for (int r = 0; r < results; ++r)
+#pragma unroll
+                    for (int q = 0; q < planes; ++q)
+                        *reinterpret_cast<u16x8*>(to[r] + q * p.plane + row * p.ldh + col) =
+                            *reinterpret_cast<const u16x8*>(lds + (r * planes + q) * Tile::numbers + at);
+            });
         }
+        if constexpr (backward)
+            if (p.b_gate_part || p.b_up_part)
+#pragma unroll
+                for (int n = 0; n < S::TN; ++n)
+                    if (place.col(n) < p.ldh)
+                        keep_bias_sums(gate_sum[n], up_sum[n], p.b_gate_part, p.b_up_part, tm * S::WM + threadIdx.x / kWave % S::WM, place.col(n),
+                                       p.hidden);
     });
 }
 
@@ -324,8 +410,7 @@ __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) 
     const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
     f32x4 acc[1][S::TM][S::TN];
     clear(acc);
-    P::template run<false>(p.a[0], &p.b[0], m0, n0, 0, p.a[0].cols, lds, acc, nullptr);
-    if constexpr (!along_b) P::template run<false>(p.a[1], &p.b[1], m0, n0, 0, p.a[1].cols, lds, acc, nullptr);
+    P::template run<false, along_b ? 1 : 2>(p.a, p.b, m0, n0, 0, p.a[0].cols, lds, acc, nullptr);
     const Place<S> place(m0, n0);
 #pragma unroll
     for (int n = 0; n < S::TN; ++n) {
@@ -336,11 +421,11 @@ __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) 
         for (int m = 0; m < S::TM; ++m) {
             const int64_t row = place.row(m);
             if (row >= p.rows) continue;
-            f32x4 v = acc[0][m][n] + bias;
-            if (p.residual) v += four_of(p.residual + row * p.residual_ld, col, (p.rows - 1 - row) * p.residual_ld + p.cols - col);
-            store_four(p.y + row * p.cols, v, col, p.cols);
+            acc[0][m][n] += bias;
+            if (p.residual) acc[0][m][n] += four_of(p.residual + row * p.residual_ld, col, (p.rows - 1 - row) * p.residual_ld + p.cols - col);
         }
     }
+    store_tile<S, S::stages * P::stage>(lds, p.y, m0, n0, p.rows, p.cols, [&](int m, int n) { return acc[0][m][n]; });
 }
 
 // One weight's gradient: a' b over the rows, (m, n), and the sums of a's columns.
@@ -378,65 +463,68 @@ __global__ __launch_bounds__(S::threads, 2) void weight_kernel(WeightArgs<T> p) 
     for (int m = 0; m < S::TM; ++m) sums[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const bool with_sums = job.sums_out && n0 == 0;
     if (with_sums)
-        P::template run<true>(job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
+        P::template run<true>(&job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
     else
-        P::template run<false>(job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
+        P::template run<false>(&job.a, &job.b, m0, n0, k, k_end, lds, acc, sums);
     const Place<S> place(m0, n0);
+    if (with_sums && place.n0 == 0)   // (every column of the product with ones is the sum)
 #pragma unroll
-    for (int m = 0; m < S::TM; ++m) {
-        const int64_t row = place.row(m);
-        if (row >= job.m) continue;
-#pragma unroll
-        for (int n = 0; n < S::TN; ++n) {
-            const int64_t col = place.col(n);
-            if (col >= job.n) continue;
-            if (!job.out) continue;
-            if (p.splits > 1)
-                store_four(job.part + (split * job.m + row) * job.n, acc[0][m][n], col, job.n);
-            else
-                store_four(job.out + row * job.n, acc[0][m][n], col, job.n);
-        }
-        if (with_sums && place.n0 == 0) {   // (every column of the product with ones is the sum)
+        for (int m = 0; m < S::TM; ++m) {
+            const int64_t row = place.row(m);
+            if (row >= job.m) continue;
             if (p.splits > 1)
                 job.sums_part[split * job.m + row] = sums[m][0];
             else
                 job.sums_out[row] = (T)sums[m][0];
         }
-    }
+    if (!job.out) return;
+    const auto value = [&](int m, int n) { return acc[0][m][n]; };
+    if (p.splits > 1)
+        store_tile<S, S::stages * P::stage>(lds, job.part + split * job.m * job.n, m0, n0, job.m, job.n, value);
+    else
+        store_tile<S, S::stages * P::stage>(lds, job.out, m0, n0, job.m, job.n, value);
 }
 
-// out = the sum of the parts, always in the same order: a group of 32 lanes to 128 numbers, the parts over the block's groups.
+// out = the sum of the parts, always in the same order: a block's lanes in 1 to 32 groups, four numbers to a lane, the parts over the
+// groups.  Bound by the bytes of the parts.
 template <class T>
 struct JoinArgs {
     struct Job {
         const float* part;
         T* out;
         int64_t count;
+        int splits, groups;
     } job[6];
     int64_t blocks[6];   // of every job
-    int splits[6];
 };
-constexpr int kJoinThreads = 1024, kJoinNumbers = 32 * 4;
+constexpr int kJoinThreads = 1024;
+// (Up to four parts to a lane.  Three weights of 2048 x 768 and two parts: 13 us so, 117 with 32 groups whatever the parts are.)
+inline int join_groups(int64_t splits) {
+    int groups = 1;
+    while (groups < 32 && groups * 4 < splits) groups *= 2;
+    return groups;
+}
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(JoinArgs<T> p) {
-    constexpr int groups = kJoinThreads / 32;
     __shared__ f32x4 shared[kJoinThreads];
     int64_t block = blockIdx.x;
     int j = 0;
     while (j < 5 && block >= p.blocks[j]) block -= p.blocks[j++];
     const auto job = p.job[j];
-    const int splits = p.splits[j];
-    const int64_t i = block * kJoinNumbers + threadIdx.x % 32 * 4;
+    const int lanes = kJoinThreads / job.groups, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    const int64_t i = (block * lanes + lane) * 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (i < job.count)
 #pragma unroll 4
-        for (int s = threadIdx.x / 32; s < splits; s += groups) sum += four_of(job.part + s * job.count, i, job.count - i);
-    shared[threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.x >= 32 || i >= job.count) return;
-#pragma unroll
-    for (int g = 1; g < groups; ++g) sum += shared[g * 32 + threadIdx.x];
-    store_four(job.out, sum, i, job.count);
+        for (int s = group; s < job.splits; s += job.groups) sum += four_of(job.part + s * job.count, i, job.count - i);
+    if (job.groups > 1) {
+        shared[threadIdx.x] = sum;
+        __syncthreads();
+        if (group == 0)
+#pragma unroll 4
+            for (int g = 1; g < job.groups; ++g) sum += shared[g * lanes + lane];
+    }
+    if (group == 0 && i < job.count) store_four(job.out, sum, i, job.count);
 }
 
 // Matrices laid out for TileOf: rows of whole 8 numbers, zeros beyond the columns, planes for float32.  A lane has 8 numbers; a
