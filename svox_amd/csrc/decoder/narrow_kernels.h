@@ -510,7 +510,10 @@ __global__ __launch_bounds__((kNarrowWeightWaves<T, KD, KO> * kWave), (kNarrowWe
             for (int s = 0; s < KO; ++s) {
                 u16x8 a[planes];
                 Y::along(dy, q, s, a);
-                dh = multiply<T>(a, wd[s], dh);
+                if (planes == 3 && q == 1)   // (half of the rows turned around: what the biases' gradients are sums of)
+                    dh = multiply_turned<T>(a, wd[s], dh);
+                else
+                    dh = multiply<T>(a, wd[s], dh);
             }
             f32x4 vh, vg, vu;
 #pragma unroll

@@ -72,7 +72,7 @@ struct Product {
                     f.b[i][n][p] = B::fragment(lds + planes * A::numbers + (p * NB + i) * B::numbers, (wn * S::TN + n) * 16, step);
     }
     // ones: also the sums of the left operand's columns (over the reduction), in `sums`
-    template <bool ones>
+    template <bool ones, bool turned>
     static __device__ __forceinline__ void multiply_all(const Rows& rows, const Columns& columns, int part, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if constexpr (ones) {
             u16x8 one;
@@ -87,14 +87,20 @@ struct Product {
 #pragma unroll
             for (int n = 0; n < S::TN; ++n)
 #pragma unroll
-                for (int m = 0; m < PM; ++m)
-                    acc[i][part * PM + m][n] = multiply<T>(columns.b[i][n], rows.a[m], acc[i][part * PM + m][n]);
+                for (int m = 0; m < PM; ++m) {
+                    f32x4& c = acc[i][part * PM + m][n];
+                    if constexpr (turned)
+                        c = multiply_turned<T>(columns.b[i][n], rows.a[m], c);
+                    else
+                        c = multiply<T>(columns.b[i][n], rows.a[m], c);
+                }
     }
     // Adds the products over [k, k_end) of a and b to acc, with two `pairs` also those of a[1] and b[1], which are as large.  LDS holds S::stages tiles of the reduction, registers the fragments of two steps:
     // while one is multiplied the next one is read, also from tile to tile.  At the barrier between two tiles every wavefront
     // has read all of the first, whose place the loads of a later one take, and all lanes' loads of the second have arrived (a
     // lane's loads arrive in their order, so that waiting for some leaves the later ones on their way).
-    template <bool ones, int pairs = 1>
+    // turning: every other 32 of the reduction by multiply_turned, for float32 numbers that are summed up afterwards
+    template <bool ones, int pairs = 1, bool turning = false>
     static __device__ __forceinline__ void run(const Planes* a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
                                                f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if (k >= k_end) return;
@@ -153,7 +159,10 @@ struct Product {
                     read(at, next / parts, next % parts, wm, rows[(first + u + 1) & 1]);
                     if (next % parts == 0) read(at, next / parts, wn, columns[(first + next / parts) & 1]);
                 }
-                multiply_all<ones>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
+                if (turning && ((first + u / parts) & 1))
+                    multiply_all<ones, turning>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
+                else
+                    multiply_all<ones, false>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
             }
         };
         if constexpr (steps % 2 == 0) {
@@ -322,7 +331,7 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
     Forward::template run<false>(&p.x, w, m0, n0, 0, p.x.cols, lds, acc, nullptr);
     if constexpr (backward) {
         clear(dh);
-        Back::template run<false>(&p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
+        Back::template run<false, 1, planes == 3>(&p.dy, &p.w_down, m0, n0, 0, p.dy.cols, lds, dh, nullptr);
     }
     const Place<S> place(m0, n0);
     constexpr int results = backward ? 3 : 1;

@@ -214,6 +214,29 @@ def test_no_rows(gpu):
 
 
 # ---- layer norm
+# enough of tiles of 256 x 256 and 256 x 128 for every product and every gradient, whole numbers of nothing; laid out and in place
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=name_of)
+@pytest.mark.parametrize("rows,d,h,o", [(32700, 266, 500, 510), (32600, 520, 504, 264)])
+def test_ffn_on_large_tiles(gpu, rows, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=rows)
+    check_ffn(t, "silu", grad)
+
+
+# Sums over many rows of what the matrix cores computed: a gradient of the hidden numbers is off by some 2^-24 of itself, up or down, and
+# so is a sum of them that mostly cancel (their signs are as random); 2^-21 holds it apart from numbers that are all rounded one way,
+# whose errors add up while the numbers cancel (rows^0.5 times 2^-24 at worst).
+@pytest.mark.parametrize("rows,d,h,o", [(65536, 32, 64, 32), (65536, 64, 130, 64), (40000, 239, 127, 239), (20000, 130, 300, 500)])
+def test_sums_over_many_rows_do_not_drift(gpu, rows, d, h, o):
+    t, grad = ffn_inputs(rows, d, h, o, torch.float32, seed=h, residual=False)
+    _, grads = ffn_step(t, "relu", grad)
+    x, wg, wu, wd = (t[n].double() for n in ("x", "w_gate", "w_up", "w_down"))
+    dh = grad.double() @ wd
+    gate, up = x @ wg.t() + t["b_gate"].double(), x @ wu.t() + t["b_up"].double()
+    for n, want in (("b_gate", (dh * up * (gate > 0)).sum(dim=0)), ("b_up", (dh * gate.clamp(min=0)).sum(dim=0))):
+        off = (grads[n].double() - want).norm() / want.norm()
+        assert off < 2.0 ** -21, (n, float(off))
+
+
 def norm_step(x, weight, bias, grad, eps=1e-5):
     leaves = {n: v.detach().requires_grad_() for n, v in (("x", x), ("weight", weight), ("bias", bias)) if v is not None}
     y = svox.layer_norm(leaves["x"], leaves.get("weight"), leaves.get("bias"), eps)
