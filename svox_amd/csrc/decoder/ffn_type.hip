@@ -294,14 +294,14 @@ void launch_weight_as(WeightArgs<T> w, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
-    if (backward && !few_rows(s, true) && narrow<T>(s)) return NarrowBackward<T>(s, nullptr).bytes;
+    if (backward && !few_rows(s, true) && narrow<T>(s, true)) return NarrowBackward<T>(s, nullptr).bytes;
     if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
     if (few_rows(s, false)) {
         Room room(nullptr);
         hidden_numbers(room, s);
         return room.used;
     }
-    if (narrow<T>(s)) {
+    if (narrow<T>(s, false)) {
         Room room(nullptr);
         room.take<u16>(narrow_numbers<T>(s, false));
         return room.used;
@@ -312,7 +312,7 @@ int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
     if (few_rows(s, false)) return launch_few_forward(s, y, workspace, stream);
-    if (narrow<T>(s)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
+    if (narrow<T>(s, false)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);
@@ -333,7 +333,7 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
 template <>
 int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
                            hipStream_t stream) {
-    if (!few_rows(s, true) && narrow<T>(s))
+    if (!few_rows(s, true) && narrow<T>(s, true))
         return by_activation(s.activation, [&](auto a) {
             return Narrow<T, decltype(a)::value>::backward(s, grad_output, grad_stride, grads, workspace, stream);
         });

@@ -222,6 +222,57 @@ def test_ffn_on_large_tiles(gpu, rows, d, h, o, dtype):
     check_ffn(t, "silu", grad)
 
 
+# Narrow layers of many rows, whose hidden numbers stay in registers.
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows,act", [(12290, "silu"), (16385, "gelu"), (12289, "relu"), (12303, "sigmoid")])
+@pytest.mark.parametrize("d,h,o", [(1, 1, 1), (31, 33, 28), (32, 32, 32), (33, 64, 49), (64, 100, 64), (65, 31, 76), (128, 300, 128), (127, 96, 4),
+                                   (28, 160, 120)])
+def test_ffn_narrow_layers_of_many_rows(gpu, rows, act, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=rows + h, bias=act != "gelu", residual=act != "relu")
+    wide = normal(torch.Generator().manual_seed(1), rows, d + 5, dtype=dtype)
+    check_ffn({**t, "x": wide[:, 2:d + 2]}, act, grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_ffn_layouts_of_many_rows(gpu, dtype):
+    g = torch.Generator().manual_seed(1)
+    rows = 8200
+    t, grad = ffn_inputs(rows, 24, 40, 24, dtype, seed=2)
+    wide = normal(g, 2 * rows, 37, dtype=dtype)
+    check_ffn({**t, "x": wide[::2, 1:25], "residual": wide[1::2, 13:37]}, "silu", wide[1::2, 2:26])
+    check_ffn({**t, "x": normal(g, 24, rows, dtype=dtype).t()}, "silu", grad)
+    check_ffn({**t, "x": wide[:1, :24].expand(rows, 24)}, "silu", grad.new_ones(1, 1).expand(rows, 24))
+    check_ffn({**t, "w_gate": t["w_gate"].t().contiguous().t(), "b_up": wide[0, ::2][:1].expand(40)}, "silu", grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows,d,h,o", [(8300, 40, 72, 24), (12300, 128, 40, 128), (32700, 264, 260, 264)])
+def test_ffn_infinities_and_nan_among_many_rows(gpu, rows, d, h, o, dtype):
+    t, grad = ffn_inputs(rows, d, h, o, dtype, seed=4)
+    clean_y, clean = ffn_step(t, "silu", grad)
+    keep = torch.arange(rows, device="cuda:0") != 5001
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x, dy = t["x"].clone(), grad.clone()
+        x[5001, 0] = bad
+        y, grads = ffn_step({**t, "x": x}, "silu", grad)
+        assert torch.equal(y[keep], clean_y[keep]) and torch.equal(grads["x"][keep], clean["x"][keep])
+        assert not torch.isfinite(y[5001]).any()
+        dy[5001, 0] = bad
+        y, grads = ffn_step(t, "silu", dy)
+        assert torch.equal(y, clean_y) and torch.equal(grads["x"][keep], clean["x"][keep]) and not torch.isfinite(grads["x"][5001]).any()
+
+
+@pytest.mark.parametrize("rows,d,h,o", [(8300, 40, 72, 24), (32700, 264, 260, 264)])
+def test_ffn_only_what_is_asked_for_of_many_rows(gpu, rows, d, h, o):
+    t, grad = ffn_inputs(rows, d, h, o, torch.bfloat16, seed=9)
+    _, all_grads = ffn_step(t, "silu", grad)
+    for names in (["x"], ["w_gate"], ["w_up", "b_up"], ["w_down"], ["b_gate"], ["b_down"], ["b_up", "x"], ["residual"]):
+        leaves = {n: v.detach().requires_grad_(n in names) for n, v in t.items()}
+        got = torch.autograd.grad(ffn(leaves, "silu"), [leaves[n] for n in names], grad)
+        for n, g in zip(names, got):
+            assert torch.equal(g, all_grads[n]), n
+
+
 # Sums over many rows of what the matrix cores computed: a gradient of the hidden numbers is off by some 2^-24 of itself, up or down, and
 # so is a sum of them that mostly cancel (their signs are as random); 2^-21 holds it apart from numbers that are all rounded one way,
 # whose errors add up while the numbers cancel (rows^0.5 times 2^-24 at worst).
