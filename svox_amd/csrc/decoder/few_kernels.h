@@ -130,6 +130,8 @@ struct FewArgs {
 
 constexpr int kFewHiddenWaves = 4, kFewOutputWaves = 8;
 
+// Measured: one row of 512 -> 2048 -> 512 in bfloat16 8.1 us for this kernel and the next (6.3 MB, 0.8 TB/s), 37 rows of 256 -> 1024 -> 256
+// in float16 10.2 us: two launches, one after the other's end, and two trips to memory each.
 // Grid: 16 hidden units a block (the last ones to the end of h's rows), 16 MT rows.
 template <class T, int MT, bool backward>
 __global__ __launch_bounds__(kFewHiddenWaves* kWave, 2) void few_hidden_kernel(FewArgs<T> p) {

@@ -131,7 +131,7 @@ __device__ __forceinline__ int64_t position_of_block(int64_t b, int64_t n) {
 // The tile of `tiles_m` x `tiles_n` at position t: `down` tiles down before the next to the right, so that what the blocks of an XCD
 // read at a time is a few rows of tiles and a few columns.
 __device__ __forceinline__ void tile_at(int64_t t, int64_t tiles_m, int64_t tiles_n, int64_t& m, int64_t& n) {
-    constexpr int64_t down = 4;   // (a step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16: 2 2104, 4 2081, 8 2106, 16 2204 us)
+    constexpr int64_t down = 4;   // (a step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16: 2 1580, 4 1556, 8 1557, 16 1591 us)
     const int64_t group = t / (down * tiles_n), first = group * down;
     const int64_t high = tiles_m - first < down ? tiles_m - first : down;
     const int64_t within = t - group * down * tiles_n;
