@@ -34,13 +34,22 @@ struct Large {
     using Output = std::conditional_t<kPlanes == 1, Shape<256, 256, kKT, 2, 4, 2>, Medium::Output>;
     using Weight = Output;
 };
+// Tiles of float32 that get a compute unit each: 64 of the reduction at a time, for twice as many wavefronts.  (Medium tiles, deep ones
+// and small ones, y and x's gradient: 8192 rows of 256 -> 1024 -> 256, 256 tiles, 43 and 75, 34 and 62, 52 and 102 us; 9000 rows, 282
+// tiles, 52 and 78, 55 and 104, 72 and 144; 4096 rows, 128 tiles, 36 and 65, 28 and 53, 28 and 54.  Hidden numbers and their gradients
+// of 2300 rows of 256 -> 440, 252 tiles, 16 and 24, 13 and 20, 20 and 30.)
+struct Deep {
+    using Hidden = std::conditional_t<kPlanes == 1, Medium::Hidden, Shape<64, 64, 64, 2, 4, 2>>;
+    using Output = std::conditional_t<kPlanes == 1, Medium::Output, Shape<64, 128, 64, 2, 4, 2>>;
+    using Weight = Medium::Weight;
+};
 constexpr int64_t kMediumTiles = 192, kUnits = 256;
 constexpr double kMediumSlower = 1.15;
 template <class S>
 int64_t tiles_of(int64_t m, int64_t n) {
     return pieces(m, S::BM) * pieces(n, S::BN);
 }
-enum Size { kSmall, kMedium, kLarge };
+enum Size { kSmall, kDeep, kMedium, kLarge };
 // the time that `tiles` take, `at_once` of them to a compute unit and the reduction in `splits`: in rounds of the compute units, by
 // the numbers of a tile
 template <class S>
@@ -51,11 +60,13 @@ bool large_pays(double medium, double large) { return kPlanes == 1 && large <= k
 template <class M, class L>
 Size size_of(int64_t m, int64_t n) {
     const int64_t medium = tiles_of<M>(m, n);
+    if (kPlanes == 3 && medium <= kUnits) return medium <= kUnits / 2 ? kSmall : kDeep;
     return medium < kMediumTiles ? kSmall : large_pays(time_of<M>(medium, 2, 1), time_of<L>(tiles_of<L>(m, n), 1, 1)) ? kLarge : kMedium;
 }
 template <class F>
 void by_size(Size size, F f) {
     if (size == kSmall) f(Small());
+    else if (size == kDeep) f(Deep());
     else if (size == kMedium) f(Medium());
     else f(Large());
 }

@@ -48,7 +48,7 @@ struct Product {
         for (int i = 0; i < NB; ++i) o.b[i].advance();
     }
     // What a wavefront multiplies at a time: `part` of its rows and all of its columns over 32 of the reduction.
-    static constexpr int parts = S::TM > 4 ? 2 : 1, PM = S::TM / parts;
+    static constexpr int parts = S::TM * planes > 6 ? 2 : 1, PM = S::TM / parts;
     static_assert(PM * parts == S::TM, "equal parts");
     struct Rows {
         u16x8 a[PM][planes];
@@ -141,9 +141,8 @@ struct Product {
         read(lds, 0, 0, wm, rows[0]);
         read(lds, 0, wn, columns[0]);
         constexpr int units = steps * parts;
-        auto tile = [&](int t, auto parity) {   // its first fragments are in rows[parity], columns[parity]
-            constexpr int first = decltype(parity)::value;
-            static_assert(parts == 1 || first == 0, "");
+        auto tile = [&](int t, auto odd) {   // its first fragments are in rows[odd * units mod 2], columns[odd * steps mod 2]
+            constexpr int row = decltype(odd)::value * units, column = decltype(odd)::value * steps;
             const u16 *at = lds + t % S::stages * stage;
 #pragma unroll
             for (int u = 0; u < units; ++u) {
@@ -153,17 +152,19 @@ struct Product {
                         wait(loaded - t - 2 >= S::stages - 2);
                         if (loaded < tiles) load_next();
                         at = lds + (t + 1) % S::stages * stage;
-                        read(at, 0, 0, wm, rows[(first + units) & 1]);
-                        read(at, 0, wn, columns[(first + steps) & 1]);
+                        read(at, 0, 0, wm, rows[(row + units) & 1]);
+                        read(at, 0, wn, columns[(column + steps) & 1]);
                     }
                 } else {
-                    read(at, next / parts, next % parts, wm, rows[(first + u + 1) & 1]);
-                    if (next % parts == 0) read(at, next / parts, wn, columns[(first + next / parts) & 1]);
+                    read(at, next / parts, next % parts, wm, rows[(row + u + 1) & 1]);
+                    if (next % parts == 0) read(at, next / parts, wn, columns[(column + next / parts) & 1]);
                 }
-                if (turning && ((first + u / parts) & 1))
-                    multiply_all<ones, turning>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
+                const Rows& r = rows[(row + u) & 1];
+                const Columns& c = columns[(column + u / parts) & 1];
+                if (turning && ((column + u / parts) & 1))
+                    multiply_all<ones, turning>(r, c, u % parts, acc, sums);
                 else
-                    multiply_all<ones, false>(rows[(first + u) & 1], columns[(first + u / parts) & 1], u % parts, acc, sums);
+                    multiply_all<ones, false>(r, c, u % parts, acc, sums);
             }
         };
         if constexpr (steps % 2 == 0) {
@@ -414,7 +415,7 @@ struct OutputArgs {
 };
 
 // along_b: b is (cols, reduction), else (reduction, cols).  Measured, as above: bfloat16 124 us, 1112 TFLOP/s, and 244 us, 1126 TFLOP/s (x's
-// gradient); float32 44 and 71 us, 97 and 121 TFLOP/s.
+// gradient); float32 34 and 60 us, 126 and 145 TFLOP/s.
 template <class T, class S, bool along_b>
 __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) {
     using P = Product<T, S, true, along_b, 1>;

@@ -222,6 +222,13 @@ def test_ffn_on_large_tiles(gpu, rows, d, h, o, dtype):
     check_ffn(t, "silu", grad)
 
 
+# float32 tiles that fill the card once, 64 of the reduction at a time
+@pytest.mark.parametrize("rows,d,h,o", [(5000, 250, 130, 250), (2300, 200, 440, 520), (2570, 65, 500, 400)])
+def test_ffn_on_deep_tiles(gpu, rows, d, h, o):
+    t, grad = ffn_inputs(rows, d, h, o, torch.float32, seed=rows)
+    check_ffn(t, "gelu", grad)
+
+
 # Narrow layers of many rows, whose hidden numbers stay in registers.
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
 @pytest.mark.parametrize("rows,act", [(12290, "silu"), (16385, "gelu"), (12289, "relu"), (12303, "sigmoid")])
