@@ -318,7 +318,7 @@ __device__ __forceinline__ void keep_bias_sums(f32x4 gate, f32x4 up, float* gate
 }
 
 // Measured, 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16: forward 281 us, 979 TFLOP/s, of which storing 134 MB is some 50 us that nothing
-// else covers; gradients 494 us, 835 TFLOP/s, with 403 MB to store (a library's product of 4096^3 1403).  8192 rows of 256 -> 1024 ->
+// else covers; gradients 482 us, 855 TFLOP/s, with 403 MB to store (a library's product of 4096^3 1403).  8192 rows of 256 -> 1024 ->
 // 256 in float32: 74 and 123 us, 116 and 105 TFLOP/s of float32, six times that of the matrix cores'.
 template <class T, class S, bool backward>
 __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) {
@@ -340,7 +340,9 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
     }
     const Place<S> place(m0, n0);
     constexpr int results = backward ? 3 : 1;
-    constexpr int of = fitting(S::TM, results * planes * S::WM * 16 * S::BN * 2, S::stages * Forward::stage * 2);
+    // (half of LDS at a time where that is enough: the gradients of large tiles 482 us so, 495 with all of it, which is stored later)
+    constexpr int row_tile = results * planes * S::WM * 16 * S::BN * 2, room = S::stages * Forward::stage * 2;
+    constexpr int of = fitting(S::TM, row_tile, row_tile * 2 <= room ? room / 2 : room);
     using Tile = Staged<S, u16, of>;
     with_activation(p.activation, [&](auto activation) {
         f32x4 gate_sum[S::TN], up_sum[S::TN];

@@ -30,7 +30,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes of every lane to LDS, where a wavefront's lie one lane's after another.  Written out because the compiler, where it knows of
 // such a load, lets every transposing read of LDS wait for all of them, the next tiles' too (a step of 16 384 rows of 1024 -> 4096 ->
 // 1024 in bfloat16: 1845 us so, 2011 from the builtin).  No register is loaded.  Who reads waits for vmcnt and a barrier first.
-// (The address of the buffer may come from a vector instruction just before: five wait states.)
+// (The address of the buffer may come from a vector instruction just before: five wait states.  Where the compiler cannot tell that it
+// is the same for all lanes the build fails; to make it so by readfirstlane costs the weights' kernel registers it does not have.)
 __device__ __forceinline__ void load_to_lds(u32x4 buffer, unsigned at, u16* lds) {
     const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(Lds*)lds);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(buffer) : "m0", "memory");
