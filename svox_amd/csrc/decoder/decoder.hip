@@ -110,7 +110,7 @@ __global__ void zero_kernel(u16* at, int64_t count) {
 int zero(void* at, int64_t count, int dtype, hipStream_t stream) {
     if (!at) return SVOX_OK;
     count *= dtype == SVOX_DECODER_F32 ? 2 : 1;
-    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)pieces(count, 256)), dim3(256), 0, stream, (u16*)at, count);
+    hipLaunchKernelGGL(zero_kernel, grid_of(pieces(count, 256), 256), dim3(256), 0, stream, (u16*)at, count);
     return check_launch("zero");
 }
 

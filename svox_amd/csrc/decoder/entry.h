@@ -9,6 +9,11 @@ namespace svox_decoder {
 __attribute__((format(printf, 2, 3))) int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+// `blocks` blocks of a launch.  The runtime counts a launch's threads along each axis in 32 bits and runs what is left of a larger number,
+// without an error (of the 16 777 218 blocks of 256 that 2^30 + 77 rows came to it ran two): such a launch gets no blocks here, which is
+// an error that check_launch sees.
+inline dim3 grid_of(int64_t blocks, int threads) { return dim3(blocks < ((int64_t)1 << 32) / threads ? (unsigned)blocks : 0); }
+
 // A caller's workspace, given out in pieces of whole 256 bytes; with no address, only counted.
 struct Room {
     char* at;

@@ -30,7 +30,7 @@ struct Parts {
         return part;
     }
     void launch(hipStream_t stream) const {
-        if (blocks > 0) hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(kJoinThreads), 0, stream, join);
+        if (blocks > 0) hipLaunchKernelGGL((join_kernel<T>), grid_of(blocks, kJoinThreads), dim3(kJoinThreads), 0, stream, join);
     }
 };
 

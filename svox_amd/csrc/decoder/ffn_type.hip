@@ -93,7 +93,7 @@ struct Lays {
         return to;
     }
     void launch(hipStream_t stream) const {
-        if (blocks > 0) hipLaunchKernelGGL((lay_kernel<T>), dim3((unsigned)blocks), dim3(kLayThreads), 0, stream, args);
+        if (blocks > 0) hipLaunchKernelGGL((lay_kernel<T>), grid_of(blocks, kLayThreads), dim3(kLayThreads), 0, stream, args);
     }
 };
 Planes hidden_numbers(Room& room, const SvoxGatedFfn& s) {
@@ -272,7 +272,7 @@ template <class S, bool backward>
 void launch_hidden_as(HiddenArgs<T> p, hipStream_t stream) {
     p.tiles_m = pieces(p.rows, S::BM);
     p.tiles_n = pieces(p.ldh, S::BN);
-    hipLaunchKernelGGL((hidden_kernel<T, S, backward>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(S::threads), 0, stream, p);
+    hipLaunchKernelGGL((hidden_kernel<T, S, backward>), grid_of(p.tiles_m * p.tiles_n, S::threads), dim3(S::threads), 0, stream, p);
 }
 template <bool backward>
 void launch_hidden(const HiddenArgs<T>& p, hipStream_t stream) {
@@ -282,7 +282,7 @@ template <class S, bool along_b>
 void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
     p.tiles_m = pieces(p.rows, S::BM);
     p.tiles_n = pieces(p.cols, S::BN);
-    hipLaunchKernelGGL((output_kernel<T, S, along_b>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(S::threads), 0, stream, p);
+    hipLaunchKernelGGL((output_kernel<T, S, along_b>), grid_of(p.tiles_m * p.tiles_n, S::threads), dim3(S::threads), 0, stream, p);
 }
 template <bool along_b>
 void launch_output(const OutputArgs<T>& p, hipStream_t stream) {
@@ -298,7 +298,7 @@ void launch_weight_as(WeightArgs<T> w, hipStream_t stream) {
         job.tiles_n = pieces(job.n, S::BN);
         blocks += job.tiles_m * job.tiles_n;
     }
-    hipLaunchKernelGGL((weight_kernel<T, S>), dim3((unsigned)(blocks * w.splits)), dim3(S::threads), 0, stream, w);
+    hipLaunchKernelGGL((weight_kernel<T, S>), grid_of(blocks * w.splits, S::threads), dim3(S::threads), 0, stream, w);
 }
 
 }  // namespace

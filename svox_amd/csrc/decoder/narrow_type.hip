@@ -31,12 +31,26 @@ void by_rows(int64_t rows, F launch) {
     launch(std::integral_constant<int, 1>());
 }
 
+// `launch` for all rows, 2^28 of them at a time: four lanes to a row or two, and a launch has less than 2^32.  cols: numbers of a row of y
+template <class F>
+void in_launches(NarrowArgs<T> p, int64_t cols, F launch) {
+    constexpr int64_t most = (int64_t)1 << 28;
+    for (int64_t left = p.rows; left > 0; left -= most) {
+        p.rows = least(left, most);
+        launch(p);
+        p.x += p.rows * p.x_ld;
+        p.y += p.rows * cols;
+        if (p.dy) p.dy += p.rows * p.dy_ld;
+        if (p.residual) p.residual += p.rows * p.residual_ld;
+    }
+}
+
 template <int KD, int KO, bool backward>
 void launch_narrow_lay(const SvoxGatedFfn& s, u16* to, hipStream_t stream) {
     using C = Chunk<KD, KO, backward>;
     NarrowLayArgs<T> p{(const T*)s.w_gate, (const T*)s.w_up, (const T*)s.w_down, (const T*)s.b_gate, (const T*)s.b_up, s.dim, s.hidden, s.out, to};
-    hipLaunchKernelGGL((narrow_lay_kernel<T, KD, KO, backward>), dim3((unsigned)pieces(pieces(s.hidden, 32) * (C::fragments + 1), 4)), dim3(256), 0,
-                       stream, p);
+    hipLaunchKernelGGL((narrow_lay_kernel<T, KD, KO, backward>), grid_of(pieces(pieces(s.hidden, 32) * (C::fragments + 1), 4), 256), dim3(256), 0, stream,
+                       p);
 }
 int narrow_forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
     Room room(workspace);
@@ -50,8 +64,10 @@ int narrow_forward(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t 
         launch_narrow_lay<KD, KO, false>(s, chunks, stream);
         const auto launch = [&](auto rows) {
             constexpr int QT = decltype(rows)::value;
-            hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
-                               dim3(kNarrowWaves * kWave), 0, stream, p);
+            in_launches(p, s.out, [&](const NarrowArgs<T>& some) {
+                hipLaunchKernelGGL((narrow_kernel<T, KD, KO, QT, kActivation>), grid_of(pieces(some.rows, 16 * QT * kNarrowWaves), kNarrowWaves * kWave),
+                                   dim3(kNarrowWaves * kWave), 0, stream, some);
+            });
         };
         by_rows(s.rows, launch);
     }));
@@ -87,8 +103,10 @@ int narrow_backward(const SvoxGatedFfn& s, const void* grad_output, int64_t grad
         launch_narrow_lay<KD, KO, true>(s, b.chunks, stream);
         const auto launch = [&](auto rows) {
             constexpr int QT = decltype(rows)::value;
-            hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT, kActivation>), dim3((unsigned)pieces(s.rows, 16 * QT * kNarrowWaves)),
-                               dim3(kNarrowWaves * kWave), 0, stream, p);
+            in_launches(p, s.dim, [&](const NarrowArgs<T>& some) {
+                hipLaunchKernelGGL((narrow_backward_kernel<T, KD, KO, QT, kActivation>),
+                                   grid_of(pieces(some.rows, 16 * QT * kNarrowWaves), kNarrowWaves * kWave), dim3(kNarrowWaves * kWave), 0, stream, some);
+            });
         };
         if (grads.x) by_rows(s.rows, launch);
         if (parts.jobs)

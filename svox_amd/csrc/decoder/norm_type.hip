@@ -70,9 +70,8 @@ int launch_norm_backward<T>(const SvoxLayerNorm& s, const float* stats, const vo
             hipLaunchKernelGGL((norm_long_kernel<T, true>), dim3(blocks), dim3(kNormThreads), 0, stream, p);
     });
     if (part)
-        hipLaunchKernelGGL((norm_join_kernel<T>), dim3((unsigned)pieces(2 * (int64_t)s.dim, kNormJoinColumns)),
-                           dim3(kNormJoinThreads), 0, stream, part,
-                           blocks, s.dim, (T*)grad_weight, (T*)grad_bias);
+        hipLaunchKernelGGL((norm_join_kernel<T>), grid_of(pieces(2 * (int64_t)s.dim, kNormJoinColumns), kNormJoinThreads),
+                           dim3(kNormJoinThreads), 0, stream, part, blocks, s.dim, (T*)grad_weight, (T*)grad_bias);
     return check_launch("layer_norm_backward");
 }
 

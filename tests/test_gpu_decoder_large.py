@@ -1,0 +1,31 @@
+"""The leaf decoder's operators at the largest sizes they take: beyond what a launch counts in 32 bits."""
+import pytest
+import torch
+
+import svox_amd as svox
+from decoder_reference import gated_ffn
+
+pytestmark = pytest.mark.gpu
+
+
+# Four lanes to a row in float32: 2^30 rows are as many threads as a launch cannot have.
+@pytest.mark.parametrize("dtype,rows", [(torch.float32, (1 << 30) + 77), (torch.bfloat16, (1 << 31) + 77)], ids=["float32", "bfloat16"])
+def test_narrow_layers_of_more_rows_than_a_launch_has_lanes_for(gpu, dtype, rows):
+    g = torch.Generator("cuda:0").manual_seed(1)
+    x = torch.empty(rows, 1, dtype=dtype, device=gpu).normal_(generator=g)
+    residual = torch.empty(rows, 1, dtype=dtype, device=gpu).normal_(generator=g)
+    t = {n: torch.full((1, 1), v, dtype=dtype, device=gpu) for n, v in (("w_gate", 0.5), ("w_up", -1.5), ("w_down", 0.75))}
+    pick = torch.cat([torch.arange(at, at + 300, device=gpu) for at in (0, 64, (1 << 28) - 150, rows // 2, (1 << 30) - 300, rows - 300)])
+    x.requires_grad_()
+    y = svox.gated_ffn(x, **t, residual=residual)
+    (gx,) = torch.autograd.grad(y, [x], residual)
+    want, wanted = gated_ffn({"x": x.detach()[pick], "residual": residual[pick], **t}, "silu", residual[pick])
+    want.holds(y[pick], "y")
+    wanted["x"].holds(gx[pick], "gradient of x")
+    # every number: the result is that of the same rows in a call of their own
+    for part in range(0, rows - 77, 1 << 27):
+        rows_of = slice(part, part + (1 << 27) if part + (1 << 27) < rows - 77 else rows)
+        again = x.detach()[rows_of].requires_grad_()
+        z = svox.gated_ffn(again, **t, residual=residual[rows_of])
+        assert torch.equal(z, y[rows_of]), part
+        assert torch.equal(torch.autograd.grad(z, [again], residual[rows_of])[0], gx[rows_of]), part
