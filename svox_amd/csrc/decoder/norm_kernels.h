@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) 
     }
 }
 
-// The gradients of weight and bias from the blocks' sums: 16 columns a block, the sums over its 64 groups of lanes.
+// The gradients of weight and bias from the blocks' sums: 16 columns a block at a time, the sums over its 64 groups of lanes.
 // (1024 columns 5 us, 48 columns 4 us: a launch and its first loads.)
 constexpr int kNormJoinThreads = 1024, kNormJoinColumns = 16;
 template <class T>
@@ -278,22 +278,27 @@ __global__ __launch_bounds__(kNormJoinThreads) void norm_join_kernel(const float
     constexpr int groups = kNormJoinThreads / kNormJoinColumns;
     __shared__ float shared[kNormJoinThreads];
     const int lane = threadIdx.x % kNormJoinColumns, group = threadIdx.x / kNormJoinColumns;
-    const int64_t c = (int64_t)blockIdx.x * kNormJoinColumns + lane;
-    float sum = 0.0f;
-    if (c < 2 * (int64_t)dim)
+    const int64_t columns = 2 * (int64_t)dim;
+    for (int64_t first = (int64_t)blockIdx.x * kNormJoinColumns; first < columns; first += (int64_t)gridDim.x * kNormJoinColumns) {
+        const int64_t c = first + lane;
+        float sum = 0.0f;
+        if (c < columns)
 #pragma unroll 4
-        for (int b = group; b < blocks; b += groups) sum += part[(int64_t)b * 2 * dim + c];
-    shared[threadIdx.x] = sum;
-    __syncthreads();
-    for (int half = groups / 2; half > 0; half /= 2) {
-        if (group < half) shared[threadIdx.x] += shared[threadIdx.x + half * kNormJoinColumns];
+            for (int b = group; b < blocks; b += groups) sum += part[b * columns + c];
+        shared[threadIdx.x] = sum;
         __syncthreads();
-    }
-    if (group != 0 || c >= 2 * (int64_t)dim) return;
-    if (c < dim) {
-        if (dweight) dweight[c] = (T)shared[lane];
-    } else if (dbias) {
-        dbias[c - dim] = (T)shared[lane];
+        for (int half = groups / 2; half > 0; half /= 2) {
+            if (group < half) shared[threadIdx.x] += shared[threadIdx.x + half * kNormJoinColumns];
+            __syncthreads();
+        }
+        if (group == 0 && c < columns) {
+            if (c < dim) {
+                if (dweight) dweight[c] = (T)shared[lane];
+            } else if (dbias) {
+                dbias[c - dim] = (T)shared[lane];
+            }
+        }
+        __syncthreads();
     }
 }
 

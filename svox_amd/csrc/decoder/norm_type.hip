@@ -70,7 +70,7 @@ int launch_norm_backward<T>(const SvoxLayerNorm& s, const float* stats, const vo
             hipLaunchKernelGGL((norm_long_kernel<T, true>), dim3(blocks), dim3(kNormThreads), 0, stream, p);
     });
     if (part)
-        hipLaunchKernelGGL((norm_join_kernel<T>), grid_of(pieces(2 * (int64_t)s.dim, kNormJoinColumns), kNormJoinThreads),
+        hipLaunchKernelGGL((norm_join_kernel<T>), grid_of(least(pieces(2 * (int64_t)s.dim, kNormJoinColumns), 1 << 16), kNormJoinThreads),
                            dim3(kNormJoinThreads), 0, stream, part, blocks, s.dim, (T*)grad_weight, (T*)grad_bias);
     return check_launch("layer_norm_backward");
 }

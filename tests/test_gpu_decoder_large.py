@@ -29,3 +29,18 @@ def test_narrow_layers_of_more_rows_than_a_launch_has_lanes_for(gpu, dtype, rows
         z = svox.gated_ffn(again, **t, residual=residual[rows_of])
         assert torch.equal(z, y[rows_of]), part
         assert torch.equal(torch.autograd.grad(z, [again], residual[rows_of])[0], gx[rows_of]), part
+
+
+# Sixteen columns of the parameters' gradients to a block of 1024 lanes: 2^25 columns of both are as many as a launch cannot have.
+def test_norm_gradients_of_more_columns_than_a_launch_has_lanes_for(gpu):
+    dim = (1 << 25) + 9
+    g = torch.Generator("cuda:0").manual_seed(2)
+    x, grad = (torch.empty(2, dim, dtype=torch.bfloat16, device=gpu).normal_(generator=g) for _ in range(2))
+    x.requires_grad_()
+    w, b = torch.ones(dim, dtype=torch.bfloat16, device=gpu).requires_grad_(), torch.zeros(dim, dtype=torch.bfloat16, device=gpu).requires_grad_()
+    dw, db = torch.autograd.grad(svox.layer_norm(x, w, b), [w, b], grad)
+    assert torch.equal(db, (grad[0].float() + grad[1].float()).bfloat16())     # (two numbers have one sum)
+    n = torch.nn.functional.layer_norm(x.detach().double(), (dim,))
+    off = (dw.double() - (grad.double() * n).sum(dim=0)).abs()
+    # a rounding to 8 bits of the sum, and n's own error: the mean and the deviation are sums of 2^17 numbers a lane
+    assert bool((off <= 2.0 ** -8 * dw.double().abs() + 2.0 ** -7 * (grad.double() * n).abs().sum(dim=0) + 2.0 ** -7 * grad.double().abs().sum(dim=0)).all())
