@@ -37,14 +37,14 @@ __device__ __forceinline__ float sum_over(float v, float* room, int slot) {
 }
 
 // One piece of a row: V numbers from column c on, zeros beyond the row.
-template <class T, int V>
-__device__ __forceinline__ void read_piece(const T* row, int c, int dim, float* v) {
+template <class T, int V, class Column>
+__device__ __forceinline__ void read_piece(const T* row, Column c, int dim, float* v) {
     const auto f = load_some<T, V>(row + c, dim - c);
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = (float)f[i];
 }
-template <class T, int V>
-__device__ __forceinline__ void write_piece(T* row, int c, int dim, const float* v) {
+template <class T, int V, class Column>
+__device__ __forceinline__ void write_piece(T* row, Column c, int dim, const float* v) {
     if (c + V <= dim) {
         typename Few<T, V>::vector f;
 #pragma unroll
@@ -191,7 +191,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormArgs<T>
         }
 }
 
-// Rows longer than the registers of a block: a block to a row, which it reads again for every sum (from a cache).
+// Rows longer than the registers of a block: a block to a row, which it reads again for every sum (from a cache).  Columns are counted in 64
+// bits: the last step of a row of nearly 2^31 numbers goes beyond them.
 template <class T, bool backward>
 __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) {
     constexpr int V = kNormPiece<T>, stride = kNormThreads * V;
@@ -204,18 +205,18 @@ __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) 
         T* const y = p.y + row * p.dim;
         if constexpr (!backward) {
             float sum = 0.0f, squares = 0.0f;
-            for (int c = threadIdx.x * V; c < p.dim; c += stride) {
+            for (int64_t c = threadIdx.x * V; c < p.dim; c += stride) {
                 read_piece<T, V>(x, c, p.dim, v);
                 for (int i = 0; i < V; ++i) sum += v[i];
             }
             const float mean = sum_over<kNormThreads>(sum, room, 0) / dim;
-            for (int c = threadIdx.x * V; c < p.dim; c += stride) {
+            for (int64_t c = threadIdx.x * V; c < p.dim; c += stride) {
                 read_piece<T, V>(x, c, p.dim, v);
                 for (int i = 0; i < V; ++i)
                     if (c + i < p.dim) squares += (v[i] - mean) * (v[i] - mean);
             }
             const float rstd = 1.0f / sqrtf(sum_over<kNormThreads>(squares, room, 1) / dim + p.eps);
-            for (int c = threadIdx.x * V; c < p.dim; c += stride) {
+            for (int64_t c = threadIdx.x * V; c < p.dim; c += stride) {
                 read_piece<T, V>(x, c, p.dim, v);
                 for (int i = 0; i < V; ++i) w[i] = 1.0f, d[i] = 0.0f;
                 if (p.weight) read_piece<T, V>(p.weight, c, p.dim, w);
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) 
             const float mean = p.stats[row * 2], rstd = p.stats[row * 2 + 1];
             float sum = 0.0f, dot = 0.0f;
             const bool first = row == blockIdx.x;
-            for (int c = threadIdx.x * V; c < p.dim; c += stride) {
+            for (int64_t c = threadIdx.x * V; c < p.dim; c += stride) {
                 read_piece<T, V>(x, c, p.dim, v);
                 read_piece<T, V>(dy, c, p.dim, d);
                 for (int i = 0; i < V; ++i) w[i] = 1.0f;
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_long_kernel(NormArgs<T> p) 
             sum = sum_over<kNormThreads>(sum, room, 0) / dim;
             dot = sum_over<kNormThreads>(dot, room, 1) / dim;
             if (!p.y) continue;
-            for (int c = threadIdx.x * V; c < p.dim; c += stride) {
+            for (int64_t c = threadIdx.x * V; c < p.dim; c += stride) {
                 read_piece<T, V>(x, c, p.dim, v);
                 read_piece<T, V>(dy, c, p.dim, d);
                 for (int i = 0; i < V; ++i) w[i] = 1.0f;

@@ -44,3 +44,41 @@ def test_norm_gradients_of_more_columns_than_a_launch_has_lanes_for(gpu):
     off = (dw.double() - (grad.double() * n).sum(dim=0)).abs()
     # a rounding to 8 bits of the sum, and n's own error: the mean and the deviation are sums of 2^17 numbers a lane
     assert bool((off <= 2.0 ** -8 * dw.double().abs() + 2.0 ** -7 * (grad.double() * n).abs().sum(dim=0) + 2.0 ** -7 * grad.double().abs().sum(dim=0)).all())
+
+
+# The longest row there is, whose last step goes beyond what 32 bits count.  Numbers here and there in a row of zeros, whose sums are exact.
+def test_norm_of_the_longest_row(gpu):
+    dim = (1 << 31) - 1
+    at = torch.tensor([0, 9, 1 << 30, dim - 2050, dim - 8, dim - 7, dim - 2, dim - 1])
+    values, slopes = torch.tensor([512.0, -1024, 256, 768, -512, 1024, 640, -384]), torch.tensor([1.0, -2, 0.5, 3, 1, -1, 2, 4])
+    weights, shifts = torch.tensor([1.0, 2, 3, 0.5, 1, 2, 1, 3]), torch.tensor([0.0, 1, -1, 2, 0.5, 0, -2, 1])
+
+    def row(numbers, others=0.0):
+        v = torch.full((dim,), others, dtype=torch.bfloat16, device=gpu)
+        v[at.to(gpu)] = numbers.bfloat16().to(gpu)
+        return v
+
+    x, w, b, grad = row(values).requires_grad_(), row(weights, 1.0).requires_grad_(), row(shifts, 0.25).requires_grad_(), row(slopes)
+    y = svox.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], grad)
+    values, slopes, weights, shifts = (v.double() for v in (values, slopes, weights, shifts))
+    mean = values.sum() / dim
+    rstd = 1 / ((((values - mean) ** 2).sum() + (dim - len(at)) * mean ** 2) / dim + 1e-5).sqrt()
+    n, dn = (values - mean) * rstd, slopes * weights
+    others = -mean * rstd    # n where x is zero
+    m1, m2 = dn.sum() / dim, (dn * n).sum() / dim
+    want = {"y": (y, n * weights + shifts, others + 0.25), "x": (dx, rstd * (dn - m1 - n * m2), rstd * (-m1 - others * m2)),
+            "weight": (dw, slopes * n, 0.0), "bias": (db, slopes, 0.0)}
+    for name, (got, there, elsewhere) in want.items():
+        got = got.detach()
+        near = got[at.to(gpu)].double().cpu()
+        # (8 bits, and sums of some ten numbers in 32)
+        assert bool(((near - there).abs() <= 2.0 ** -8 * there.abs() + 1e-5).all()), (name, near, there)
+        got[at.to(gpu)] = 0
+        rest = torch.tensor(float(elsewhere)).bfloat16().to(gpu)
+        for part in range(0, dim, 1 << 28):
+            some = got[part:part + (1 << 28)]
+            off = some != rest
+            off[at[(at >= part) & (at < part + (1 << 28))].to(gpu) - part] = False
+            # (the last of a number's 8 bits may differ)
+            assert not bool(off.any()) or bool(((some[off].double() - float(elsewhere)).abs() <= 2.0 ** -8 * abs(float(elsewhere)) + 1e-12).all()), (name, part)
