@@ -104,13 +104,12 @@ int64_t norm_space(const SvoxLayerNorm& s, bool affine) {
 
 // a gradient summed over no rows
 __global__ void zero_kernel(u16* at, int64_t count) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) at[i] = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) at[i] = 0;
 }
 int zero(void* at, int64_t count, int dtype, hipStream_t stream) {
     if (!at) return SVOX_OK;
     count *= dtype == SVOX_DECODER_F32 ? 2 : 1;
-    hipLaunchKernelGGL(zero_kernel, grid_of(pieces(count, 256), 256), dim3(256), 0, stream, (u16*)at, count);
+    hipLaunchKernelGGL(zero_kernel, grid_of(least(pieces(count, 256), 1 << 16), 256), dim3(256), 0, stream, (u16*)at, count);
     return check_launch("zero");
 }
 

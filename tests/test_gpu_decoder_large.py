@@ -1,9 +1,12 @@
 """The leaf decoder's operators at the largest sizes they take: beyond what a launch counts in 32 bits."""
+import ctypes
+
 import pytest
 import torch
 
 import svox_amd as svox
 from decoder_reference import gated_ffn
+from svox_amd.csrc import decoder as D
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +85,15 @@ def test_norm_of_the_longest_row(gpu):
             off[at[(at >= part) & (at < part + (1 << 28))].to(gpu) - part] = False
             # (the last of a number's 8 bits may differ)
             assert not bool(off.any()) or bool(((some[off].double() - float(elsewhere)).abs() <= 2.0 ** -8 * abs(float(elsewhere)) + 1e-12).all()), (name, part)
+
+
+# The gradient of a weight of more than 2^32 numbers over no rows: zeros, and nothing beyond them.
+def test_no_rows_and_a_weight_of_more_numbers_than_a_launch_has_lanes(gpu):
+    hidden, dim, margin = 1 << 22, 1025, 1000
+    w = torch.ones(hidden * dim + margin, dtype=torch.bfloat16, device=gpu)
+    spec = D.GatedFfnC(x=16, w_gate=16, w_up=16, w_down=16, rows=0, x_stride=dim, dim=dim, hidden=hidden, out=1, dtype=D.BF16)
+    grads = D.GatedFfnGradsC(w_gate=w.data_ptr())
+    lib = D.load_library()
+    assert lib.svox_gated_ffn_backward(ctypes.byref(spec), None, 1, ctypes.byref(grads), None, 0, None) == 0, lib.svox_decoder_last_error()
+    torch.cuda.synchronize()
+    assert not bool(w[:-margin].any()) and bool((w[-margin:] == 1).all())
