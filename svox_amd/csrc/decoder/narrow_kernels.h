@@ -231,6 +231,18 @@ __device__ __forceinline__ void biases(const float* bias, int unit, f32x4& gate,
     up = *reinterpret_cast<const f32x4*>(bias + 32 + unit);
 }
 
+// Zeros for the hidden units from `left` on that pad the last chunk (a row of infinities has made NaN of them).
+template <int QT>
+__device__ __forceinline__ void clear_padding(f32x4 (&v)[QT][2], int64_t left) {
+    const int unit = threadIdx.x % kWave / 16 * 4;
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[q][t][i] = t * 16 + unit + i < left ? v[q][t][i] : 0.0f;
+}
+
 // Bound by vector instructions: a hidden number costs an exponential and a reciprocal, 16 cycles of a SIMD each for 64 lanes, and some
 // ten others of 4.  Measured, bfloat16, silu: 262 144 rows of 64 -> 256 -> 49 in 39.6 us, 67 million hidden numbers, 600 TFLOP/s of
 // products (59 MB, for which a copy takes 12 us); 65 537 rows of 32 -> 128 -> 28 in float32 21 us.
@@ -280,6 +292,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_kernel(NarrowAr
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[q][t][i] = activate<planes == 3, activation>(gate[q][i], nullptr) * up[q][i];
         }
+        if (p.hidden - c * 32 < 32) clear_padding(h, p.hidden - c * 32);
         u16x8 turned[QT][planes];
 #pragma unroll
         for (int q = 0; q < QT; ++q) turn<T>(h[q], turned[q]);
@@ -356,6 +369,7 @@ __global__ __launch_bounds__(kNarrowWaves* kWave, 2) void narrow_backward_kernel
                     du[q][t][i] = dh[q][i] * a;
                 }
         }
+        if (p.hidden - c * 32 < 32) clear_padding(dg, p.hidden - c * 32), clear_padding(du, p.hidden - c * 32);
         u16x8 turned_g[QT][planes], turned_u[QT][planes];
 #pragma unroll
         for (int q = 0; q < QT; ++q) turn<T>(dg[q], turned_g[q]), turn<T>(du[q], turned_u[q]);
