@@ -388,17 +388,21 @@ __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) 
             Tile::each(m0, n0, m, [&](int at, int64_t row, int64_t col) {
                 if (row >= p.rows || col >= p.ldh) return;
                 u16* const to[3] = {p.h, p.dgate, p.dup};
-                const bool ends = col + 8 > p.hidden;   // (zeros from there on: a row of infinities has made NaN of those that pad it)
+                auto keep = [&](auto ends) {
 #pragma unroll
-                for (int r = 0; r < results; ++r)
+                    for (int r = 0; r < results; ++r)
 #pragma unroll
-                    for (int q = 0; q < planes; ++q) {
-                        u16x8 v = *reinterpret_cast<const u16x8*>(lds + (r * planes + q) * Tile::numbers + at);
-                        if (ends)
+                        for (int q = 0; q < planes; ++q) {
+                            u16x8 v = *reinterpret_cast<const u16x8*>(lds + (r * planes + q) * Tile::numbers + at);
+                            if constexpr (decltype(ends)::value)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] = col + i < p.hidden ? v[i] : (u16)0;
-                        *reinterpret_cast<u16x8*>(to[r] + q * p.plane + row * p.ldh + col) = v;
-                    }
+                                for (int i = 0; i < 8; ++i) v[i] = col + i < p.hidden ? v[i] : (u16)0;
+                            *reinterpret_cast<u16x8*>(to[r] + q * p.plane + row * p.ldh + col) = v;
+                        }
+                };
+                // (zeros beyond the last hidden unit: a row of infinities has made NaN of those that pad it)
+                if (col + 8 > p.hidden) keep(std::true_type());
+                else keep(std::false_type());
             });
         }
         if constexpr (backward)
