@@ -71,16 +71,25 @@ struct Product {
                 for (int p = 0; p < planes; ++p)
                     f.b[i][n][p] = B::fragment(lds + planes * A::numbers + (p * NB + i) * B::numbers, (wn * S::TN + n) * 16, step);
     }
-    // ones: also the sums of the left operand's columns (over the reduction), in `sums`
-    template <bool ones, bool turned>
+    // ones: also the sums of the left operand's columns (over the reduction), in `sums`; those of float32 as the products are, this unit's
+    // by themselves and added to the others in 32 bits, and every other time with minus ones.  odd: of the steps of the reduction; turning:
+    // see run
+    template <bool ones, bool odd, bool turning>
     static __device__ __forceinline__ void multiply_all(const Rows& rows, const Columns& columns, int part, f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
         if constexpr (ones) {
             u16x8 one;
-            for (int i = 0; i < 8; ++i) one[i] = Form<T>::one();
+            for (int i = 0; i < 8; ++i) one[i] = Form<T>::one() ^ (planes == 3 && odd ? 0x8000 : 0);
 #pragma unroll
-            for (int m = 0; m < PM; ++m)
+            for (int m = 0; m < PM; ++m) {
+                f32x4& all = sums[part * PM + m];
+                f32x4 sum = planes == 3 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : all;
 #pragma unroll
-                for (int p = planes; p-- > 0;) sums[part * PM + m] = Form<T>::mma(one, rows.a[m][p], sums[part * PM + m]);
+                for (int p = planes; p-- > 0;) sum = Form<T>::mma(one, rows.a[m][p], sum);
+                if constexpr (planes == 3)
+                    all = odd ? all - sum : all + sum;
+                else
+                    all = sum;
+            }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
@@ -89,7 +98,7 @@ struct Product {
 #pragma unroll
                 for (int m = 0; m < PM; ++m) {
                     f32x4& c = acc[i][part * PM + m][n];
-                    if constexpr (turned)
+                    if (turning && ((part * PM + m) & 1) == odd)
                         c = multiply_turned<T>(columns.b[i][n], rows.a[m], c);
                     else
                         c = multiply<T>(columns.b[i][n], rows.a[m], c);
@@ -100,7 +109,8 @@ struct Product {
     // one is multiplied the next one is read, also from tile to tile.  At the barrier between two tiles every wavefront has read
     // all of the first, whose place the loads of a later one take, and all lanes' loads of the second have arrived (a lane's
     // loads arrive in their order, so that waiting for some leaves the later ones on their way).
-    // turning: every other 32 of the reduction by multiply_turned, for float32 numbers that are summed up afterwards
+    // turning: every other 32 of the reduction by multiply_turned, for float32 numbers that are summed up over the rows afterwards; of two
+    // neighbouring tiles of rows it is not the same ones, so that a reduction of one step has turned rows too
     template <bool ones, int pairs = 1, bool turning = false>
     static __device__ __forceinline__ void run(const Planes* a, const Planes* b, int64_t m0, int64_t n0, int64_t k, int64_t k_end, u16* lds,
                                                f32x4 (&acc)[NB][S::TM][S::TN], f32x4* sums) {
@@ -161,10 +171,10 @@ struct Product {
                 }
                 const Rows& r = rows[(row + u) & 1];
                 const Columns& c = columns[(column + u / parts) & 1];
-                if (turning && ((column + u / parts) & 1))
-                    multiply_all<ones, turning>(r, c, u % parts, acc, sums);
+                if ((column + u / parts) & 1)
+                    multiply_all<ones, true, turning>(r, c, u % parts, acc, sums);
                 else
-                    multiply_all<ones, false>(r, c, u % parts, acc, sums);
+                    multiply_all<ones, false, turning>(r, c, u % parts, acc, sums);
             }
         };
         if constexpr (steps % 2 == 0) {
