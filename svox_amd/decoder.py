@@ -82,6 +82,12 @@ class _Ffn(nn.Module):
                          activation=self.activation)
 
 
+def _cells(data, tree):
+    """The cells of the tree's nodes in `data`, without its spare capacity."""
+    nodes = tree._structure().nodes
+    return data if nodes == data.shape[0] else data[:nodes]
+
+
 class LeafDecoder(nn.Module):
     """Features of a leaf to its record: `depth` blocks x + ffn(norm(x)) over the features, then ffn(norm(x)) to the record.
 
@@ -118,15 +124,17 @@ class LeafDecoder(nn.Module):
         return self.ffns[-1](self.norms[-1](x))
 
     def decode_tree(self, features, tree):
-        """Writes the records of the features in the tree `features` into `tree`, a tree of the same structure, and returns
-        them, (cells, record), for a backward pass.  Every cell is decoded, also those that have children and are not read."""
-        if features.child.shape != tree.child.shape or features.data.shape[:4] != tree.data.shape[:4]:
+        """Writes the records of the features in the tree `features` into `tree`, a tree of the same structure (the same nodes, the
+        same cells divided; their spare capacity may differ), and returns them, (cells, record), for a backward pass.  Every cell of
+        a node is decoded, also those that have children and are not read."""
+        if not features._divided_like(tree):
             raise ValueError("features and tree must have the same structure")
-        records = self(features.data.reshape(-1, features.data_dim))
+        source = _cells(features.data, features)
+        records = self(source.reshape(-1, features.data_dim))
         if records.shape[1] != tree.data_dim:
             raise ValueError(f"the decoder makes records of {records.shape[1]} numbers, the tree's have {tree.data_dim}")
         with torch.no_grad():
-            tree.data.copy_(records.view_as(tree.data))
+            _cells(tree.data, tree).copy_(records.view(*source.shape[:-1], -1))
         return records
 
     def backward_through(self, features, tree, loss):
@@ -136,6 +144,6 @@ class LeafDecoder(nn.Module):
         tree.data.grad = None
         value = loss()
         value.backward()
-        records.backward(tree.data.grad.view_as(records).to(records.dtype))
+        records.backward(_cells(tree.data.grad, tree).reshape(records.shape).to(records.dtype))
         tree.data.grad = None
         return value.detach()

@@ -77,6 +77,11 @@ def _no_fallback(what):
         "the reference's PyTorch fallback is not included")
 
 
+class _Structure:
+    def __init__(self, nodes):
+        self.nodes = nodes
+
+
 class N3Tree(nn.Module):
     """PyTorch N^3-tree with HIP acceleration on MI355X.
 
@@ -682,6 +687,25 @@ class N3Tree(nn.Module):
             else:
                 self._leaf_marks = None      # the tree has changed since: the marks are void
         return spec
+
+    def _structure(self):
+        """How the cells are divided now, as an object: the same one until a method of the tree or a torch operation on `child`
+        changes that.  Two trees that are found to be divided alike share theirs (`_divided_like`)."""
+        key = (self._ver, self.child._version, self.child.data_ptr())
+        if self.__dict__.get("_structure_key") != key:
+            self._structure_now, self._structure_key = _Structure(self.n_internal), key
+        return self._structure_now
+
+    def _divided_like(self, other):
+        """Whether both trees have the same nodes and every cell has the same child, whatever capacity they keep beside."""
+        mine, theirs = self._structure(), other._structure()
+        if mine is theirs:
+            return True
+        n = mine.nodes
+        if n != theirs.nodes or self.child.shape[1:] != other.child.shape[1:] or not torch.equal(self.child[:n], other.child[:n].to(self.child.device)):
+            return False
+        other._structure_now = mine
+        return True
 
     # ------------------------------------------------------------------ marks of the empty leaves
     def mark_empty_leaves(self, sigma_thresh=0.0, density_softplus=False):
