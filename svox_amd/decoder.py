@@ -139,11 +139,16 @@ class LeafDecoder(nn.Module):
 
     def backward_through(self, features, tree, loss):
         """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
-        adds the gradients of what it returns to those of the decoder's weights and of `features.data`.  Returns the loss."""
+        adds the gradients of what it returns to those of the decoder's weights and of `features.data`, and to those of whatever else
+        it was made of.  Returns the loss.  (`tree.data` has to require its gradient, which is that of the records.)"""
+        if not tree.data.requires_grad:
+            raise ValueError("tree.data does not require a gradient: that of the records has to come through it")
         records = self.decode_tree(features, tree)
         tree.data.grad = None
         value = loss()
         value.backward()
-        records.backward(_cells(tree.data.grad, tree).reshape(records.shape).to(records.dtype))
+        grad = tree.data.grad
+        if grad is not None and records.requires_grad:    # (None: the loss does not depend on the records)
+            records.backward(_cells(grad, tree).reshape(records.shape).to(records.dtype))
         tree.data.grad = None
         return value.detach()

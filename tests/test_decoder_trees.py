@@ -74,3 +74,49 @@ def test_other_branching_factors_are_refused():
     features, tree, decoder = pair()
     assert not taken(decoder, features, svox.N3Tree(N=3, data_format="SH1"))
     assert not taken(decoder, svox.N3Tree(N=3, data_format=None, data_dim=12), svox.N3Tree(data_format="SH1"))
+
+
+class Plain(svox.LeafDecoder):
+    """A decoder whose network is one product, of torch's own."""
+
+    def forward(self, x):
+        return x @ self.ffns[0].w_gate.t()
+
+
+def plain():
+    features, tree, _ = pair()
+    torch.manual_seed(0)
+    features.data.data.normal_()
+    return features, tree, Plain(12, tree.data_dim, hidden=tree.data_dim)
+
+
+def test_a_loss_without_the_records():
+    features, tree, decoder = plain()
+    other = torch.ones(3, requires_grad=True)
+    assert decoder.backward_through(features, tree, lambda: (other ** 2).sum()) == 3
+    assert torch.equal(other.grad, torch.full((3,), 2.0)) and features.data.grad is None and decoder.ffns[0].w_gate.grad is None
+
+
+def test_a_tree_that_requires_no_gradient_is_refused_before_anything_is_done():
+    features, tree, decoder = plain()
+    tree.data.requires_grad_(False)
+    other = torch.ones(3, requires_grad=True)
+    with pytest.raises(ValueError, match="does not require a gradient"):
+        decoder.backward_through(features, tree, lambda: (other ** 2).sum() + tree.data.sum())
+    assert other.grad is None and not bool(tree.data.any())
+
+
+def test_gradients_add_up_and_nothing_trained_is_no_error():
+    features, tree, decoder = plain()
+    loss = lambda: (tree.data ** 2).sum()  # noqa: E731
+    decoder.backward_through(features, tree, loss)
+    once = decoder.ffns[0].w_gate.grad.clone(), features.data.grad.clone()
+    x, w = features.data.detach().reshape(-1, 12), decoder.ffns[0].w_gate.detach()
+    records = x @ w.t()
+    torch.testing.assert_close(once[0], 2 * records.t() @ x)
+    torch.testing.assert_close(once[1].reshape(-1, 12), 2 * records @ w)
+    decoder.backward_through(features, tree, loss)
+    torch.testing.assert_close(decoder.ffns[0].w_gate.grad, 2 * once[0])
+    decoder.requires_grad_(False)
+    features.data.requires_grad_(False)
+    assert decoder.backward_through(features, tree, loss) == loss().detach()
