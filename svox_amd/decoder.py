@@ -97,7 +97,9 @@ class LeafDecoder(nn.Module):
         tree = svox.N3Tree(data_format="SH4", init_refine=4, device="cuda:0")
         decoder = svox.LeafDecoder(16, tree.data_dim, hidden=64).cuda()
         renderer = svox.VolumeRenderer(tree)
+        optimizer = torch.optim.Adam([features.data, *decoder.parameters()], lr=1e-2)
         for rays, target in batches:
+            optimizer.zero_grad()
             loss = decoder.backward_through(features, tree, lambda: ((renderer(rays) - target) ** 2).mean())
             optimizer.step()
 
@@ -140,15 +142,18 @@ class LeafDecoder(nn.Module):
     def backward_through(self, features, tree, loss):
         """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
         adds the gradients of what it returns to those of the decoder's weights and of `features.data`, and to those of whatever else
-        it was made of.  Returns the loss.  (`tree.data` has to require its gradient, which is that of the records.)"""
+        it was made of.  Returns the loss.  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
+        holds stays as it is.)"""
         if not tree.data.requires_grad:
             raise ValueError("tree.data does not require a gradient: that of the records has to come through it")
         records = self.decode_tree(features, tree)
-        tree.data.grad = None
-        value = loss()
-        value.backward()
-        grad = tree.data.grad
+        kept, tree.data.grad = tree.data.grad, None
+        try:
+            value = loss()
+            value.backward()
+            grad = tree.data.grad
+        finally:
+            tree.data.grad = kept
         if grad is not None and records.requires_grad:    # (None: the loss does not depend on the records)
             records.backward(_cells(grad, tree).reshape(records.shape).to(records.dtype))
-        tree.data.grad = None
         return value.detach()

@@ -120,3 +120,25 @@ def test_gradients_add_up_and_nothing_trained_is_no_error():
     decoder.requires_grad_(False)
     features.data.requires_grad_(False)
     assert decoder.backward_through(features, tree, loss) == loss().detach()
+
+
+def test_the_gradient_a_tree_holds_stays():
+    features, tree, decoder = plain()
+    held = torch.randn_like(tree.data)
+    tree.data.grad = held.clone()
+    decoder.backward_through(features, tree, lambda: (tree.data ** 2).sum())
+    want = decoder.ffns[0].w_gate.grad.clone()
+    assert torch.equal(tree.data.grad, held)
+    decoder.zero_grad()
+    tree.data.grad = None
+    decoder.backward_through(features, tree, lambda: (tree.data ** 2).sum())
+    assert tree.data.grad is None and torch.equal(decoder.ffns[0].w_gate.grad, want)
+
+    def fails():
+        (tree.data ** 2).sum().backward()
+        raise KeyError("no rays")
+
+    tree.data.grad = held.clone()
+    with pytest.raises(KeyError):
+        decoder.backward_through(features, tree, fails)
+    assert torch.equal(tree.data.grad, held)
