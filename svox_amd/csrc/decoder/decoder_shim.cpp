@@ -5,11 +5,13 @@
 
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <mutex>
 #include <stdexcept>
@@ -118,6 +120,11 @@ Tensor make_like(const Tensor& x) { return make(x.sizes(), x.scalar_type(), x); 
 Tensor bytes_on(const Tensor& x, int64_t bytes) { return bytes > 0 ? make({bytes}, at::kByte, x) : Tensor(); }
 void* at_or_null(const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; }
 
+// (A tracer does not see these calls: it would take their results for constants.)
+void no_tracing(const char* name) {
+    using namespace c10::impl;
+    if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY)) fail(std::string("svox.") + name + " cannot be traced");
+}
 // Whether a call has to make an autograd node.  A tangent of forward mode has no node to go to.
 template <size_t n>
 bool wants_node(const Tensor* const (&inputs)[n], const char* name) {
@@ -200,6 +207,7 @@ struct NormNode : torch::autograd::Node {
 };
 
 Tensor layer_norm(const Tensor& x, Tensor weight, Tensor bias, double eps) {
+    no_tracing("layer_norm");
     check_like(x, x, "x");
     dtype_code(x, "x");
     if (x.dim() < 1) fail("x must have at least one dimension");
@@ -306,6 +314,7 @@ struct FfnNode : torch::autograd::Node {
 
 Tensor gated_ffn(Ffn& f, int64_t activation) {
     const Tensor& x = f.x;
+    no_tracing("gated_ffn");
     check_like(x, x, "x");
     dtype_code(x, "x");
     if (x.dim() < 1) fail("x must have at least one dimension");
