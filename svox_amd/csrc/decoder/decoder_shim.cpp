@@ -136,8 +136,9 @@ bool wants_node(const Tensor* const (&inputs)[n], const char* name) {
     }
     return wants && at::GradMode::is_enabled();
 }
-void once(const char* name) {
+void once(const char* name, const Tensor& grad_output) {
     if (at::GradMode::is_enabled()) fail(std::string("svox.") + name + ": its gradient cannot be differentiated again (create_graph)");
+    if (grad_output._fw_grad(0).defined()) fail(std::string("svox.") + name + ": its gradient has no derivatives in forward mode");
 }
 // A node of the given inputs' graph, to which `y` is then tied.
 template <class N, class... Inputs>
@@ -188,7 +189,7 @@ struct NormNode : torch::autograd::Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        once("layer_norm");
+        once("layer_norm", grads[0]);
         const Tensor x = x_.unpack(), weight = weight_.unpack(), stats = stats_.unpack();
         const On on(x);
         check_like(grads[0], x, "grad_output");
@@ -288,7 +289,7 @@ struct FfnNode : torch::autograd::Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(8);
         if (!grads[0].defined()) return out;
-        once("gated_ffn");
+        once("gated_ffn", grads[0]);
         const Ffn f{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), saved_[5].unpack(), Tensor(), Tensor()};
         const On on(f.x);
         check_like(grads[0], f.x, "grad_output");

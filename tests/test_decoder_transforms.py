@@ -1,6 +1,7 @@
 """What the leaf decoder's operators refuse rather than get wrong: ways of torch to take a function apart (up to the device check)."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import svox_amd as svox
@@ -17,3 +18,17 @@ def test_tracing_is_refused(gradients):
                 make_fx(call)(x)
         with pytest.raises(RuntimeError, match="CUDA tensor"):
             svox.layer_norm(x)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused(gpu):
+    x, w = torch.randn(3, 8, device=gpu), torch.randn(8, 8, device=gpu)
+    for call in (lambda x: svox.layer_norm(x), lambda x: svox.gated_ffn(x, w, w, w)):
+        for leaf in (x, x.clone().requires_grad_()):
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+                call(forward_ad.make_dual(leaf, torch.ones_like(x)))
+        leaf = x.clone().requires_grad_()
+        y = call(leaf)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(x), x))
+        torch.autograd.grad(call(leaf), leaf, torch.ones_like(x))
