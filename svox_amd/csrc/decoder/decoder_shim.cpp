@@ -91,6 +91,7 @@ struct Rows {
     int64_t rows = 0, stride = 0;
 };
 Rows rows_of(const Tensor& x) {
+    if (x.is_neg()) return rows_of(x.resolve_neg());   // (what memory holds is turned around)
     const int64_t d = x.size(-1), rows = d ? x.numel() / d : 0;
     if (x.is_contiguous()) return Rows{x, rows, d};
     if (rows > 0 && (x.stride(-1) == 1 || d == 1)) {
@@ -148,7 +149,9 @@ std::shared_ptr<N> node_of(const Inputs&... inputs) {
     return node;
 }
 void make_contiguous(Tensor& x) {
-    if (x.defined() && !x.is_contiguous()) x = x.contiguous();
+    if (!x.defined()) return;
+    if (x.is_neg()) x = x.resolve_neg();
+    if (!x.is_contiguous()) x = x.contiguous();
 }
 
 // ---- layer norm

@@ -32,3 +32,27 @@ def test_tangents_are_refused(gpu):
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(x), x))
         torch.autograd.grad(call(leaf), leaf, torch.ones_like(x))
+
+
+@pytest.mark.gpu
+def test_tensors_that_are_turned_around_where_they_are_read(gpu):
+    """Views whose numbers are the negatives of what lies in memory (the imaginary part of a conjugate), as every argument and as a gradient."""
+    g = torch.Generator().manual_seed(0)
+    t = [torch.randn(*shape, generator=g).to(gpu) for shape in ((5, 8), (12, 8), (12, 8), (8, 12), (12,), (12,), (8,), (5, 8))]
+    grad = torch.randn(5, 8, generator=g).to(gpu)
+
+    def step(call, tensors, grad):
+        leaves = [v.detach().requires_grad_() for v in tensors]
+        y = call(*leaves)
+        return [y, *torch.autograd.grad(y, leaves, grad)]
+
+    turned = lambda v: torch._neg_view(-v)  # noqa: E731
+    for call, tensors in ((svox.gated_ffn, t), (svox.layer_norm, (t[0], t[6], t[1][0]))):
+        want = step(call, tensors, grad)
+        for i in range(len(tensors) + 1):
+            some = [turned(v) if j == i else v for j, v in enumerate(tensors)]
+            got = step(call, some, turned(grad) if i == len(tensors) else grad)
+            assert all(torch.equal(a, b) for a, b in zip(want, got)), i
+            assert torch.equal(call(*some), want[0])
+    assert torch.complex(t[0], -t[0]).conj().imag.is_neg()
+    assert torch.equal(svox.layer_norm(torch.complex(t[0], -t[0]).conj().imag), svox.layer_norm(t[0]))
