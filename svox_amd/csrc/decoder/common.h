@@ -13,6 +13,8 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "rules.h"
+
 namespace svox_decoder {
 
 typedef unsigned short u16;
@@ -28,8 +30,6 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 typedef __bf16 Bf16;
 typedef _Float16 F16;
-
-constexpr int kWave = 64;
 
 // ---- a type's planes
 template <class T>
@@ -207,7 +207,5 @@ __device__ __forceinline__ void with_activation(int activation, F f) {
 }
 
 __host__ __device__ inline int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
-inline int64_t up_to(int64_t n, int64_t whole) { return (n + whole - 1) / whole * whole; }
-inline int64_t pieces(int64_t n, int64_t size) { return (n + size - 1) / size; }
 
 }  // namespace svox_decoder

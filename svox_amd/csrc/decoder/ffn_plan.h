@@ -35,26 +35,11 @@ struct Parts {
 };
 
 // ---- narrow layers
-template <class T>
-constexpr int kNarrowMost = Form<T>::planes == 1 ? 128 : 64;   // features, and numbers of the result
-// Where rows enough fill the compute units with blocks that go through all hidden numbers; with fewer the products of whole matrices have
-// more blocks.  (Forward pass in bfloat16 of 64 -> 2048 -> 64, 4500 rows 45.7 us here and 32.6 there, 14 000 rows 46.9 and 54.5; of
-// 112 -> 1024 -> 128, 8000 rows 36.4 and 26.1, 20 000 rows 41.4 and 49.8; of 32 -> 1000 -> 28, 4500 rows 25.0 and 23.3, 14 000
-// rows 25.5 and 33.0; in float32, 4500 rows 47.9 and 54.9; of 64 -> 2048 -> 64, 4500 rows 122 and 89, 14 000 rows 124 and 168.
-// Gradients in bfloat16 of 64 -> 2048 -> 64, 3000 rows 74 and 66, 8000 rows 87 and 118; of 112 -> 1024 -> 128, 8000 rows 94 and 72,
-// 20 000 rows 150 and 131; of 32 -> 1000 -> 28, 3000 rows 37 and 47; in float32 of 64 -> 2048 -> 64, 3000 rows 235 and 178, 8000
-// rows 282 and 303.)
-template <class T>
-bool narrow(const SvoxGatedFfn& s, bool backward) {
-    const int64_t wide = (int64_t)s.dim + s.out, most = backward ? 48 * wide : Form<T>::planes == 1 ? 8192 : 64 * wide;
-    return s.dim <= kNarrowMost<T> && s.out <= kNarrowMost<T> && s.rows >= most;
-}
 // KD and KO, the 32s of features and of numbers of the result: 1, 2 or 4
 #define SVOX_NARROW_STEPS(n, K, ...)                                    \
     if ((n) <= 32) { constexpr int K = 1; __VA_ARGS__; }                \
     else if ((n) <= 64) { constexpr int K = 2; __VA_ARGS__; }           \
     else if constexpr (Form<T>::planes == 1) { constexpr int K = 4; __VA_ARGS__; }
-inline int narrow_steps(int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 template <class T>
 int64_t narrow_numbers(const SvoxGatedFfn& s, bool backward) {   // of the chunks, 16-bit
     const int64_t kd = narrow_steps(s.dim), ko = narrow_steps(s.out);

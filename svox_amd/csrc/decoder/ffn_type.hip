@@ -9,60 +9,11 @@ namespace {
 
 constexpr int kPlanes = Form<T>::planes;
 constexpr int64_t kMostLd = TileOf<true, 64, 64, 256>::most_ld;
-constexpr int kKT = kPlanes == 1 ? 64 : 32;
-// Medium tiles, two blocks of them to a compute unit, where there are enough; small ones with more of the reduction on its way, where
-// a block waits for memory more than it multiplies; and for 16 bits large ones, of which each block has a compute unit's LDS for
-// itself, where these fill the compute units as well: a tile of 256 x 256 takes half as many bytes from the L2 for a product as one
-// of 128 x 128 does, and two thirds as many from LDS.
-// (The step of 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16 takes 1553 us with large tiles, 1799 with medium ones; its hidden
-// numbers 281 and 315, result 125 and 145, their gradients 499 and 575, x's 241 and 295, the weights' 447 and 500.  Medium tiles
-// take it 2021 us with eight wavefronts to a block, 2090 with four.  The step of 8192 rows of 256 -> 1024 -> 256 in float32, whose planes
-// make tiles three times as large, 537 us with tiles of 128 x 128 and one block to a compute unit, 500 with half as large ones and
-// two.)
-struct Medium {
-    using Hidden = std::conditional_t<kPlanes == 1, Shape<128, 64, kKT, 2, 4, 2>, Shape<64, 64, kKT, 2, 2, 2>>;
-    using Output = std::conditional_t<kPlanes == 1, Shape<128, 128, kKT, 2, 4, 2>, Shape<64, 128, kKT, 2, 2, 2>>;
-    using Weight = Output;
-};
-struct Small {
-    using Hidden = Shape<64, 32, kKT, 2, 2, 4>;
-    using Output = Shape<64, 64, kKT, 2, 2, 4>;
-    using Weight = Output;
-};
-struct Large {
-    using Hidden = std::conditional_t<kPlanes == 1, Shape<256, 128, kKT, 2, 4, 2>, Medium::Hidden>;
-    using Output = std::conditional_t<kPlanes == 1, Shape<256, 256, kKT, 2, 4, 2>, Medium::Output>;
-    using Weight = Output;
-};
-// Tiles of float32 that get a compute unit each: 64 of the reduction at a time, for twice as many wavefronts.  (Medium tiles, deep ones
-// and small ones, y and x's gradient: 8192 rows of 256 -> 1024 -> 256, 256 tiles, 43 and 75, 34 and 62, 52 and 102 us; 9000 rows, 282
-// tiles, 52 and 78, 55 and 104, 72 and 144; 4096 rows, 128 tiles, 36 and 65, 28 and 53, 28 and 54.  Hidden numbers and their gradients
-// of 2300 rows of 256 -> 440, 252 tiles, 16 and 24, 13 and 20, 20 and 30.)
-struct Deep {
-    using Hidden = std::conditional_t<kPlanes == 1, Medium::Hidden, Shape<64, 64, 64, 2, 4, 2>>;
-    using Output = std::conditional_t<kPlanes == 1, Medium::Output, Shape<64, 128, 64, 2, 4, 2>>;
-    using Weight = Medium::Weight;
-};
-constexpr int64_t kMediumTiles = 192, kUnits = 256;
-constexpr double kMediumSlower = 1.15;
-template <class S>
-int64_t tiles_of(int64_t m, int64_t n) {
-    return pieces(m, S::BM) * pieces(n, S::BN);
-}
-enum Size { kSmall, kDeep, kMedium, kLarge };
-// the time that `tiles` take, `at_once` of them to a compute unit and the reduction in `splits`: in rounds of the compute units, by
-// the numbers of a tile
-template <class S>
-double time_of(int64_t tiles, int at_once, int64_t splits) {
-    return (double)(pieces(tiles * splits, at_once * kUnits) * at_once * S::BM * S::BN) / (double)splits;
-}
-bool large_pays(double medium, double large) { return kPlanes == 1 && large <= kMediumSlower * medium; }
-template <class M, class L>
-Size size_of(int64_t m, int64_t n) {
-    const int64_t medium = tiles_of<M>(m, n);
-    if (kPlanes == 3 && medium <= kUnits) return medium <= kUnits / 2 ? kSmall : kDeep;
-    return medium < kMediumTiles ? kSmall : large_pays(time_of<M>(medium, 2, 1), time_of<L>(tiles_of<L>(m, n), 1, 1)) ? kLarge : kMedium;
-}
+using R = Rules<kPlanes>;
+using Small = R::Small;
+using Deep = R::Deep;
+using Medium = R::Medium;
+using Large = R::Large;
 template <class F>
 void by_size(Size size, F f) {
     if (size == kSmall) f(Small());
@@ -104,13 +55,6 @@ Planes hidden_numbers(Room& room, const SvoxGatedFfn& s) {
 }
 
 // ---- few rows
-// Up to 64 rows always; up to 2048 while the products stay small, where the other kernels wait more than they multiply.  (Forward
-// pass of 256 -> 1024 -> 256, bfloat16, 512 rows 18.7 us here and 19.3 on tiles, 1024 rows 24.1 and 18.9; float32, 1024 rows 44 and
-// 53, 2048 rows 68 and 56.  Gradients, 1024 rows 40 and 45, 2048 rows 70 and 60; float32, 103 and 135, 181 and 168.)
-bool few_rows(const SvoxGatedFfn& s, bool backward) {
-    const double most = kPlanes == 1 ? (backward ? 0.9e9 : 0.4e9) : (backward ? 1.5e9 : 1.2e9);
-    return s.rows <= 64 || (s.rows <= 2048 && (double)s.rows * s.hidden * (2.0 * s.dim + s.out) <= most);
-}
 template <bool backward>
 void launch_few(const FewArgs<T>& p, bool result, hipStream_t stream) {
     const auto launch = [&](auto tiles) {
@@ -182,37 +126,10 @@ struct Forward {
     }
 };
 
-// The tiles of the weights' gradients, and the rows of a split.
-struct Split {
-    int64_t each;
-    int splits;
-    Size size;
-};
-template <class S>
-int64_t weight_tiles(const SvoxGatedFfn& s) {
-    return 2 * tiles_of<S>(s.hidden, s.dim) + tiles_of<S>(s.out, s.hidden);
-}
-Split weight_split(const SvoxGatedFfn& s) {
-    Split w;
-    const int64_t small = weight_tiles<Small::Weight>(s), medium = weight_tiles<Medium::Weight>(s), large = weight_tiles<Large::Weight>(s);
-    const int64_t steps = pieces(s.rows, kKT);
-    const int64_t large_splits = large < kUnits ? kUnits / large : 1, medium_splits = pieces(2 * kUnits, medium);
-    // (rows enough for two blocks a compute unit of eight steps each make up for few tiles)
-    w.size = kMedium;
-    if (medium * steps < 2 * kUnits * 8) w.size = kSmall;
-    else if (large_pays(time_of<Medium::Weight>(medium, 2, medium_splits), time_of<Large::Weight>(large, 1, large_splits))) w.size = kLarge;
-    int64_t splits = w.size == kLarge ? large_splits : w.size == kMedium ? medium_splits : pieces(2 * kUnits, small);
-    if (splits > pieces(steps, 8)) splits = pieces(steps, 8);
-    w.each = up_to(pieces(s.rows, splits), kKT);
-    w.splits = (int)pieces(s.rows, w.each);
-    return w;
-}
-
 // The rows of the biases' sums of hidden_kernel.
-Size hidden_size(int64_t rows, int64_t ldh) { return size_of<Medium::Hidden, Large::Hidden>(rows, ldh); }
 int64_t hidden_parts(const SvoxGatedFfn& s) {
     int64_t parts = 0;
-    by_size(hidden_size(s.rows, up_to(s.hidden, 8)), [&](auto shapes) {
+    by_size(R::hidden_size(s.rows, up_to(s.hidden, 8)), [&](auto shapes) {
         using S = typename decltype(shapes)::Hidden;
         parts = pieces(s.rows, S::BM) * S::WM;
     });
@@ -221,7 +138,7 @@ int64_t hidden_parts(const SvoxGatedFfn& s) {
 struct Backward {
     Lays lays;
     Planes x, w_gate, w_up, w_down, dy, h, dgate, dup;
-    Split split;
+    R::Split split;
     float* part;
     int64_t bytes, bias_parts;
     bool few;
@@ -229,7 +146,7 @@ struct Backward {
         Room room(workspace);
         // (grad_output's address is not known when its workspace is asked for: there is room to lay it out)
         x = lays.operand(room, s.x, s.x_stride, s.rows, s.dim);
-        few = few_rows(s, true);
+        few = R::few_rows(s, true);
         if (!few) {
             w_gate = lays.operand(room, s.w_gate, s.dim, s.hidden, s.dim);
             w_up = lays.operand(room, s.w_up, s.dim, s.hidden, s.dim);
@@ -238,7 +155,7 @@ struct Backward {
         h = hidden_numbers(room, s);
         dgate = hidden_numbers(room, s);
         dup = hidden_numbers(room, s);
-        split = weight_split(s);
+        split = R::weight_split(s);
         bias_parts = few ? pieces(s.rows, 16) : hidden_parts(s);
         part = room.take<float>((split.splits > 1 ? split.splits * (2 * (int64_t)s.hidden * s.dim + (int64_t)s.hidden * s.out + s.out) : 0) +
                                 bias_parts * 2 * s.hidden);
@@ -276,7 +193,7 @@ void launch_hidden_as(HiddenArgs<T> p, hipStream_t stream) {
 }
 template <bool backward>
 void launch_hidden(const HiddenArgs<T>& p, hipStream_t stream) {
-    by_size(hidden_size(p.rows, p.ldh), [&](auto shapes) { launch_hidden_as<typename decltype(shapes)::Hidden, backward>(p, stream); });
+    by_size(R::hidden_size(p.rows, p.ldh), [&](auto shapes) { launch_hidden_as<typename decltype(shapes)::Hidden, backward>(p, stream); });
 }
 template <class S, bool along_b>
 void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
@@ -286,7 +203,7 @@ void launch_output_as(OutputArgs<T> p, hipStream_t stream) {
 }
 template <bool along_b>
 void launch_output(const OutputArgs<T>& p, hipStream_t stream) {
-    by_size(size_of<Medium::Output, Large::Output>(p.rows, p.cols),
+    by_size(R::output_size(p.rows, p.cols),
             [&](auto shapes) { launch_output_as<typename decltype(shapes)::Output, along_b>(p, stream); });
 }
 
@@ -305,14 +222,14 @@ void launch_weight_as(WeightArgs<T> w, hipStream_t stream) {
 
 template <>
 int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
-    if (backward && !few_rows(s, true) && narrow<T>(s, true)) return NarrowBackward<T>(s, nullptr).bytes;
+    if (backward && !R::few_rows(s, true) && R::narrow(s, true)) return NarrowBackward<T>(s, nullptr).bytes;
     if (backward) return Backward(s, nullptr, 0, nullptr, true).bytes;
-    if (few_rows(s, false)) {
+    if (R::few_rows(s, false)) {
         Room room(nullptr);
         hidden_numbers(room, s);
         return room.used;
     }
-    if (narrow<T>(s, false)) {
+    if (R::narrow(s, false)) {
         Room room(nullptr);
         room.take<u16>(narrow_numbers<T>(s, false));
         return room.used;
@@ -322,8 +239,8 @@ int64_t ffn_workspace<T>(const SvoxGatedFfn& s, bool backward) {
 
 template <>
 int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t stream) {
-    if (few_rows(s, false)) return launch_few_forward(s, y, workspace, stream);
-    if (narrow<T>(s, false)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
+    if (R::few_rows(s, false)) return launch_few_forward(s, y, workspace, stream);
+    if (R::narrow(s, false)) return by_activation(s.activation, [&](auto a) { return Narrow<T, decltype(a)::value>::forward(s, y, workspace, stream); });
     const Forward f(s, workspace);
     f.lays.launch(stream);
     const HiddenArgs<T> p = hidden_args(s, f.x, f.w_gate, f.w_up, f.h);
@@ -344,7 +261,7 @@ int launch_ffn<T>(const SvoxGatedFfn& s, void* y, void* workspace, hipStream_t s
 template <>
 int launch_ffn_backward<T>(const SvoxGatedFfn& s, const void* grad_output, int64_t grad_stride, const SvoxGatedFfnGrads& grads, void* workspace,
                            hipStream_t stream) {
-    if (!few_rows(s, true) && narrow<T>(s, true))
+    if (!R::few_rows(s, true) && R::narrow(s, true))
         return by_activation(s.activation, [&](auto a) {
             return Narrow<T, decltype(a)::value>::backward(s, grad_output, grad_stride, grads, workspace, stream);
         });

@@ -20,13 +20,10 @@ NarrowArgs<T> narrow_args(const SvoxGatedFfn& s, const u16* chunks) {
     p.out = s.out;
     return p;
 }
-// 16 or 32 rows to a wavefront: 32 halve what it reads of LDS, 16 fill the GPU sooner and are all that float32's planes leave room
-// for.  (Rows of 64 -> 256 -> 64, bfloat16, forward and dx: 131 072 rows 27.5, 37.2 us with 16, 25.4, 34.5 with 32; 10 007 rows of
-// 76 -> 203 -> 49, float16: 10.8, 13.1 and 14.1, 17.2.  65 537 rows of 32 -> 128 -> 28, float32, forward: 20.7 and 22.8.)
 template <class F>
 void by_rows(int64_t rows, F launch) {
     if constexpr (Form<T>::planes == 1) {
-        if (rows >= 98304) return launch(std::integral_constant<int, 2>());
+        if (Rules<1>::narrow_tiles(rows) == 2) return launch(std::integral_constant<int, 2>());
     }
     launch(std::integral_constant<int, 1>());
 }

@@ -13,14 +13,6 @@
 
 namespace svox_decoder {
 
-// The shape of a block's work: BM x BN numbers of the result, KT of the reduction at a time, WM x WN wavefronts, and how many
-// tiles of the reduction LDS holds (one that is multiplied, the others on their way).
-template <int BM_, int BN_, int KT_, int WM_, int WN_, int stages_>
-struct Shape {
-    static constexpr int BM = BM_, BN = BN_, KT = KT_, WM = WM_, WN = WN_, threads = WM * WN * kWave, stages = stages_;
-    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-};
-
 // NB products of one left operand with NB right ones, a block's tile of each.
 template <class T, class S, bool along_a, bool along_b, int NB>
 struct Product {
