@@ -8,8 +8,9 @@ import pytest
 import torch
 
 import decoder_rules
-from decoder_reference import gated_ffn
-from test_gpu_decoder import DTYPES, ffn, ffn_inputs, ffn_step, name_of, normal
+import svox_amd as svox
+from decoder_reference import gated_ffn, layer_norm
+from test_gpu_decoder import DTYPES, ffn, ffn_inputs, ffn_step, name_of, norm_step, normal
 
 ACTIVATIONS = ["silu", "gelu", "relu", "sigmoid"]
 
@@ -48,6 +49,13 @@ def test_gradients_of_some_rows_among_many(gpu, rows, d, h, o, dtype):
         wanted[n].holds(found, f"gradient of {n}")
 
 
+def balanced(rows, g):
+    """As many 1 as -1 in any order, and a 0 where the rows are odd."""
+    signs = torch.zeros(rows)
+    signs[:rows // 2], signs[rows // 2:rows // 2 * 2] = 1, -1
+    return signs[torch.randperm(rows, generator=g)]
+
+
 def alike(rows, d, h, o, dtype, device="cuda:0"):
     """Rows that are all the same, and weights of which dh comes out exactly, whatever the order of its terms: sums of -1, -1/2, 1/2 and 1."""
     g = torch.Generator().manual_seed(rows + h)
@@ -68,11 +76,7 @@ def test_rows_alike_but_for_their_sign_add_up_to_nothing(gpu, rows, d, h, o, dty
     x = t["x"].repeat(rows, 1)
     for seed in range(3):
         g = torch.Generator().manual_seed(seed)
-        signs = torch.ones(rows)
-        signs[torch.randperm(rows, generator=g)[:rows // 2]] = -1
-        if rows % 2:
-            signs[int(torch.randint(rows, (1,), generator=g)) if seed else -1] = 0
-            signs[:] = balanced(signs)
+        signs = balanced(rows, g)
         y, grads = ffn_step({**t, "x": x}, "silu", signs.to(gpu).to(dtype)[:, None] * u)
         assert bool((y == y[:1]).all())
         for sign in (-1, 0, 1):
@@ -85,13 +89,47 @@ def test_rows_alike_but_for_their_sign_add_up_to_nothing(gpu, rows, d, h, o, dty
             assert (share <= 2.0 ** -20).all(), (n, float(share.max()))
 
 
-def balanced(signs):
-    """As many +1 as -1 where one row is 0, by turning one around if that takes it."""
-    extra = int(signs.sum())
-    at = torch.nonzero(signs == (1 if extra > 0 else -1)).flatten()[:abs(extra) // 2]
-    signs[at] *= -1
-    assert int(signs.sum()) == 0
-    return signs
+# Rows on every number of lanes, and more of them than the blocks go through at once.
+NORMS = [(140003, 3), (70001, 30), (40003, 60), (40003, 100), (20011, 250), (9001, 500), (9001, 1000), (9001, 2000), (2500, 4000), (2500, 8000), (2500, 9000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows,dim", NORMS)
+def test_norm_gradients_of_some_rows_among_many(gpu, rows, dim, dtype):
+    g = torch.Generator("cuda:0").manual_seed(dim)
+    x, grad = (torch.randn(rows, dim + 1, generator=g, device=gpu).to(dtype)[:, 1:] for _ in range(2))
+    w, b = (torch.randn(dim, generator=g, device=gpu).to(dtype) for _ in range(2))
+    pick = torch.tensor(some_rows(rows, seed=dim), device=gpu)
+    others = torch.ones(rows, dtype=torch.bool, device=gpu)
+    others[pick] = False
+    grad[others] = 0
+    y, grads = norm_step(x, w, b, grad)
+    want, wanted = layer_norm(x[pick], w, b, grad=grad[pick])
+    want.holds(y[pick], "y")
+    assert not bool(grads["x"][others].any())
+    wanted["x"].holds(grads["x"][pick], "gradient of x")
+    for n in ("weight", "bias"):
+        wanted[n].holds(grads[n], f"gradient of {n}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("rows,dim", NORMS)
+def test_norm_rows_alike_but_for_their_sign_add_up_to_nothing(gpu, rows, dim, dtype):
+    g = torch.Generator().manual_seed(dim)
+    x, w, b, u = (normal(g, *shape, dtype=dtype) for shape in ((1, dim), (dim,), (dim,), (1, dim)))
+    _, one = layer_norm(x, w, b, grad=u)
+    for seed in range(3):
+        signs = balanced(rows, g).to(gpu).to(dtype)
+        y, grads = norm_step(x.repeat(rows, 1), w, b, signs[:, None] * u)
+        assert bool((y == y[:1]).all())
+        for sign in (-1, 0, 1):
+            rows_of = grads["x"][signs == sign]
+            assert bool((rows_of == rows_of[:1]).all()), sign
+        for n in ("weight", "bias"):
+            # (as above: sums in 32 bits of rows / 256 terms and more to a lane)
+            assert (np.abs(grads[n].double().cpu().numpy()) <= 0.25 * np.abs(one[n].v) + 2.0 ** -20).all(), n
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
