@@ -58,8 +58,9 @@ int svox_layer_norm_backward(const SvoxLayerNorm* spec, const float* stats, cons
 int64_t svox_layer_norm_workspace_bytes(const SvoxLayerNorm* spec, int32_t affine);
 
 /* y = (act(x w_gate' + b_gate) * (x w_up' + b_up)) w_down' + b_down + residual
- * The products of float16 and bfloat16 take the hidden numbers, and their gradients, rounded to that type; those of float32
- * hold 24 bits throughout.  An infinite number in a float32 row makes that row of y NaN. */
+ * The products of float16 and bfloat16 take the hidden numbers, and their gradients, rounded to that type: in float16 those beyond 65504
+ * become infinite and those below 2^-25 zero.  The products of float32 hold 24 bits throughout; an infinite number, or a finite one from
+ * 3.396e38 on, makes NaN of the sums it is part of. */
 typedef struct SvoxGatedFfn {
     const void* x;          /* (rows, dim), rows x_stride numbers apart */
     const void* w_gate;     /* (hidden, dim) */

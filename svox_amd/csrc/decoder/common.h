@@ -6,7 +6,8 @@
 // and a product of two of them as the six products of planes whose weights are at least 2^-16 of the whole,
 //     hi*hi' + hi*mid' + mid*hi' + hi*lo' + lo*hi' + mid*mid';
 // what is left out is below 2^-24 of the product, as much as a 32-bit multiplication rounds away.  Six bfloat16 products cost
-// 6/16 of what the 32-bit matrix instructions cost.  (Infinite inputs give NaN: inf - inf in the second plane.)
+// 6/16 of what the 32-bit matrix instructions cost.  (Infinite inputs, and finite ones from 3.396e38 on, of which the first plane is
+// infinite, give NaN: inf - inf in the second plane.)
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -71,9 +72,11 @@ struct Form<float> {
 // The matrix cores round a sum a little downwards whatever its sign.  float32 shows it: the planes' six products are therefore added
 // up by themselves and c is added in 32 bits, rounded to nearest; and where results are summed up over many rows afterwards, as the
 // gradients of the hidden numbers are for the biases', every other time the product of an operand turned around is taken away
-// (multiply_turned), so that the sums do not drift.  (A step of 43 345 rows of 239 -> 127 -> 239, relu, against 64 bits: gradients of
-// x, the weights and b_up 3.9e-7, 6.5e-7 and 15e-7 off with all products added to c, 1.3e-7, 3.6e-7 and 20e-7 with the planes' by
-// themselves, b_up's 2.7e-7 with both.)
+// (multiply_turned), by steps of the reduction and by tiles of rows, so that the sums do not drift; b_down's sums, products with ones, are
+// taken with minus ones every other time.  (A step of 43 345 rows of 239 -> 127 -> 239, relu, against 64 bits: gradients of x, the weights
+// and b_up 3.9e-7, 6.5e-7 and 15e-7 off with all products added to c; 1.3e-7, 3.1e-7 and 2.0e-7 so, b_down's 1.4e-7.  131 072 rows of
+// 80 -> 33 -> 20: b_gate, b_up and b_down 7.9e-7, 19e-7 and 2.9e-7 off where only the steps alternate and the ones do not, 2.7e-7, 2.6e-7 and
+// 1.1e-7 so.)
 template <class T>
 __device__ __forceinline__ f32x4 product(const u16x8 (&a)[Form<T>::planes], const u16x8 (&b)[Form<T>::planes]) {
     f32x4 p = Form<T>::mma(a[1], b[1], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
@@ -156,7 +159,8 @@ __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
 }
 // Phi(g), the normal distribution's, and exp(-g^2 / 2).  For results of 16 bits by 7.1.26 of Abramowitz and Stegun, Handbook of
-// Mathematical Functions: erf to 1.5e-7, with the exponential that the derivative needs as well.
+// Mathematical Functions: erf to 1.5e-7, with the exponential that the derivative needs as well.  (That is an absolute error: g Phi(g) is
+// off by 2.1e-7 at most, but by 2^-11 of itself at g = -4, 2^-8 at -6.2 and more beyond, where it is below 2e-9.)
 template <bool accurate>
 __device__ __forceinline__ float phi(float g, float& bell) {
     if constexpr (accurate) {

@@ -436,7 +436,9 @@ struct NarrowWeightArgs {
 // numbers' gradients that narrow_backward_kernel stored would be 201 MB written and read, 80 us.
 // Four wavefronts to a block and three to a SIMD where their registers allow it (131 072 rows of 64 -> 256 -> 64 in bfloat16: 64 us
 // with eight and two, 53 with four and three); where they do not, two, and eight to a block where four would have too many of
-// the rows' numbers on their way.
+// the rows' numbers on their way.  In float32 the planes of the weights and the sums do not fit two wavefronts' registers where features or
+// numbers of the result are more than 32: 20 to 32 bytes of a lane wait in memory, 120 to 176 where both are.  (A step of 131 072 rows
+// of 64 -> 256 -> 64: 505 us.)
 template <class T, int KD, int KO>
 constexpr int kNarrowWeightWaves = (Form<T>::planes == 1 ? KD + KO > 6 : KD + KO > 2) ? 8 : 4;
 template <class T, int KD, int KO>

@@ -320,8 +320,9 @@ __device__ __forceinline__ void keep_bias_sums(f32x4 gate, f32x4 up, float* gate
 }
 
 // Measured, 16 384 rows of 1024 -> 4096 -> 1024 in bfloat16: forward 281 us, 979 TFLOP/s, of which storing 134 MB is some 50 us that nothing
-// else covers; gradients 482 us, 855 TFLOP/s, with 403 MB to store (a library's product of 4096^3 1403).  8192 rows of 256 -> 1024 ->
-// 256 in float32: 74 and 123 us, 116 and 105 TFLOP/s of float32, six times that of the matrix cores'.
+// else covers; gradients 481 us, 857 TFLOP/s, with 403 MB to store (a library's product of 4096^3 1403), and five registers of a lane that
+// wait in memory, once a tile.  8192 rows of 256 -> 1024 -> 256 in float32: 78 and 132 us, 110 and 98 TFLOP/s of float32, six times that of
+// the matrix cores'.
 template <class T, class S, bool backward>
 __global__ __launch_bounds__(S::threads, 2) void hidden_kernel(HiddenArgs<T> p) {
     using Forward = Product<T, S, true, true, 2>;
@@ -428,7 +429,7 @@ struct OutputArgs {
 };
 
 // along_b: b is (cols, reduction), else (reduction, cols).  Measured, as above: bfloat16 124 us, 1112 TFLOP/s, and 244 us, 1126 TFLOP/s (x's
-// gradient); float32 34 and 60 us, 126 and 145 TFLOP/s.
+// gradient); float32 35 and 61 us, 121 and 141 TFLOP/s.
 template <class T, class S, bool along_b>
 __global__ __launch_bounds__(S::threads, 2) void output_kernel(OutputArgs<T> p) {
     using P = Product<T, S, true, along_b, 1>;
@@ -472,7 +473,7 @@ struct WeightArgs {
 };
 
 // Measured, as above: bfloat16 441 us, 935 TFLOP/s, on 192 tiles and as many of 256 compute units (four splits would fill them, and
-// leave 201 MB of parts to write and read); float32 101 us, 128 TFLOP/s.
+// leave 201 MB of parts to write and read); float32 105 us, 122 TFLOP/s.
 template <class T, class S>
 __global__ __launch_bounds__(S::threads, 2) void weight_kernel(WeightArgs<T> p) {
     using P = Product<T, S, false, false, 1>;

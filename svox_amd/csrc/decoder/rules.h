@@ -45,14 +45,16 @@ struct Rules {
     // rows 25.5 and 33.0; in float32, 4500 rows 47.9 and 54.9; of 64 -> 2048 -> 64, 4500 rows 122 and 89, 14 000 rows 124 and 168.
     // Gradients in bfloat16 of 64 -> 2048 -> 64, 3000 rows 74 and 66, 8000 rows 87 and 118; of 112 -> 1024 -> 128, 8000 rows 94 and 72,
     // 20 000 rows 150 and 131; of 32 -> 1000 -> 28, 3000 rows 37 and 47; in float32 of 64 -> 2048 -> 64, 3000 rows 235 and 178, 8000
-    // rows 282 and 303.)
+    // rows 282 and 303.)  The rule does not ask for the hidden units, of which the rows it was measured on have 1000 and more, and is wrong
+    // where the figures say so: gradients of 112 -> 1024 -> 128 from 11 520 rows to 20 000 and more.
     static bool narrow(const SvoxGatedFfn& s, bool backward) {
         const int64_t wide = (int64_t)s.dim + s.out, most = backward ? 48 * wide : planes == 1 ? 8192 : 64 * wide;
         return s.dim <= kNarrowMost && s.out <= kNarrowMost && s.rows >= most;
     }
     // 16 or 32 rows to a wavefront: 32 halve what it reads of LDS, 16 fill the GPU sooner and are all that float32's planes leave room
     // for.  (Rows of 64 -> 256 -> 64, bfloat16, forward and dx: 131 072 rows 27.5, 37.2 us with 16, 25.4, 34.5 with 32; 10 007 rows of
-    // 76 -> 203 -> 49, float16: 10.8, 13.1 and 14.1, 17.2.  65 537 rows of 32 -> 128 -> 28, float32, forward: 20.7 and 22.8.)
+    // 76 -> 203 -> 49, float16: 10.8, 13.1 and 14.1, 17.2.  65 537 rows of 32 -> 128 -> 28, float32, forward: 20.7 and 22.8.)  Where
+    // between the two the line is best was not measured: 98 304 rows fill the compute units three times with blocks of 128.
     static int narrow_tiles(int64_t rows) { return planes == 1 && rows >= 98304 ? 2 : 1; }
 
     // ---- products of whole matrices

@@ -46,8 +46,10 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, resi
     :return: (..., K), differentiable once with respect to every tensor
 
     All tensors have x's type.  Products are summed in 32 bits; float16 and bfloat16 round the hidden numbers (and, in the
-    backward pass, their gradients) to that type between the two products, float32 keeps 24 bits throughout.  Training keeps x
-    alone: the backward pass computes the hidden numbers again.
+    backward pass, their gradients) to that type between the two products, as the matrix cores take them: the result is off by 1.4
+    times what one rounding of it is, and in float16 a hidden number or a gradient beyond 65504 becomes infinite and one below 2^-25
+    zero (scale the loss).  float32 keeps 24 bits throughout; there numbers from 3.396e38 on make NaN, as infinite ones do.
+    Training keeps x alone: the backward pass computes the hidden numbers again.
     """
     code = _D.ACTIVATIONS.get(activation)
     if code is None:
@@ -142,7 +144,8 @@ class LeafDecoder(nn.Module):
     def backward_through(self, features, tree, loss):
         """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
         adds the gradients of what it returns to those of the decoder's weights and of `features.data`, and to those of whatever else
-        it was made of.  Returns the loss.  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
+        it was made of.  Returns the loss.  The records' gradient takes the decoder's type: in float16 what is below 2^-25 becomes zero,
+        so scale the loss there.  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
         holds stays as it is.)"""
         if not tree.data.requires_grad:
             raise ValueError("tree.data does not require a gradient: that of the records has to come through it")
