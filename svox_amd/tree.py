@@ -691,8 +691,9 @@ class N3Tree(nn.Module):
     def _structure(self):
         """How the cells are divided now, as an object: the same one until a method of the tree or a torch operation on `child`
         changes that.  Two trees that are found to be divided alike share theirs (`_divided_like`)."""
-        key = (self._ver, self.child._version, self.child.data_ptr())
-        if self.__dict__.get("_structure_key") != key:
+        # (a table made in inference mode does not say when it is written to)
+        key = None if self.child.is_inference() else (self._ver, self.child._version, self.child.data_ptr())
+        if key is None or self.__dict__.get("_structure_key") != key:
             self._structure_now, self._structure_key = _Structure(self.n_internal), key
         return self._structure_now
 

@@ -142,3 +142,11 @@ def test_the_gradient_a_tree_holds_stays():
     with pytest.raises(KeyError):
         decoder.backward_through(features, tree, fails)
     assert torch.equal(tree.data.grad, held)
+
+
+def test_trees_made_in_inference_mode():
+    with torch.inference_mode():
+        features, tree, decoder = pair(init_reserve=5)
+        assert taken(decoder, features, tree) and taken(decoder, features, tree)
+        features.child[1, 0, 0, 0] = 1
+        assert not taken(decoder, features, tree)
