@@ -147,8 +147,8 @@ class LeafDecoder(nn.Module):
         it was made of.  Returns the loss.  The records' gradient takes the decoder's type: in float16 what is below 2^-25 becomes zero,
         so scale the loss there.  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
         holds stays as it is.)"""
-        if not tree.data.requires_grad:
-            raise ValueError("tree.data does not require a gradient: that of the records has to come through it")
+        if not (tree.data.requires_grad and tree.data.is_leaf):
+            raise ValueError("tree.data does not require a gradient, or is computed from something else: that of the records has to come through it")
         records = self.decode_tree(features, tree)
         kept, tree.data.grad = tree.data.grad, None
         try:

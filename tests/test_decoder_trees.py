@@ -106,6 +106,13 @@ def test_a_tree_that_requires_no_gradient_is_refused_before_anything_is_done():
     assert other.grad is None and not bool(tree.data.any())
 
 
+def test_records_that_are_computed_from_something_else_are_refused():
+    features, tree, decoder = plain()
+    torch.nn.utils.parametrize.register_parametrization(tree, "data", torch.nn.Softplus())
+    with pytest.raises(ValueError, match="computed from something else"):
+        decoder.backward_through(features, tree, lambda: (tree.data ** 2).sum())
+
+
 def test_gradients_add_up_and_nothing_trained_is_no_error():
     features, tree, decoder = plain()
     loss = lambda: (tree.data ** 2).sum()  # noqa: E731
