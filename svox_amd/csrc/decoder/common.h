@@ -7,7 +7,7 @@
 //     hi*hi' + hi*mid' + mid*hi' + hi*lo' + lo*hi' + mid*mid';
 // what is left out is below 2^-24 of the product, as much as a 32-bit multiplication rounds away.  Six bfloat16 products cost
 // 6/16 of what the 32-bit matrix instructions cost.  (Infinite inputs, and finite ones from 3.396e38 on, of which the first plane is
-// infinite, give NaN: inf - inf in the second plane.)
+// infinite, give NaN: inf - inf in the second plane.  Numbers below 2^-109 lose bits, where bfloat16's numbers run out for the third plane.)
 #pragma once
 #include <hip/hip_runtime.h>
 
