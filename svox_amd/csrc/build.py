@@ -1,7 +1,8 @@
 """Build libsvox_hip.so for gfx950 with hipcc, in-tree (next to the sources): one object for the entry points and one
 per policy of the march kernels, compiled side by side and linked; and, beside them, the host extension _host_shim.so
 (host_shim.cpp: plain C++ against torch's headers, no device code).  The operators of a leaf decoder are a library of their
-own, libsvox_decoder.so, with a host extension of its own, _decoder_shim.so (decoder/)."""
+own, libsvox_decoder.so, with a host extension of its own, _decoder_shim.so (decoder/); those of networks over cells are libsvox_network.so
+and _network_shim.so (network/)."""
 import os
 import shutil
 import subprocess
@@ -15,6 +16,8 @@ LIB_NAME = "libsvox_hip.so"
 SHIM_NAME = "_host_shim.so"
 DECODER_LIB_NAME = "libsvox_decoder.so"
 DECODER_SHIM_NAME = "_decoder_shim.so"
+NETWORK_LIB_NAME = "libsvox_network.so"
+NETWORK_SHIM_NAME = "_network_shim.so"
 
 # -ffp-contract=off: the kernels spell their fused multiply-adds out; the compiler adds none.
 # -munsafe-fp-atomics: floating-point atomicAdd becomes the hardware global_atomic_add.
@@ -60,6 +63,14 @@ def _decoder_units():
     yield "decoder", os.path.join("decoder", "decoder.hip"), []
 
 
+def _network_units():
+    """... and of libsvox_network.so."""
+    for of in DECODER_TYPES:
+        yield f"rotate_{of.lower()}", os.path.join("network", "rotate_type.hip"), [f"-DSVOX_DECODER_TYPE={of}"]
+    yield "clip", os.path.join("network", "clip.hip"), []
+    yield "network", os.path.join("network", "network.hip"), []
+
+
 def _run(cmd):
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     log = "\n".join(l for l in proc.stdout.splitlines() if "packed-fp32-ops" not in l)
@@ -81,13 +92,15 @@ def _shim_command(out, name=SHIM_NAME, source="host_shim.cpp"):
 
 
 def build_library(verbose=True):
-    """Compile the sources into svox_amd/csrc/: libsvox_hip.so, _host_shim.so, libsvox_decoder.so and _decoder_shim.so.
-    Raises on failure.  Returns the first one's path."""
+    """Compile the sources into svox_amd/csrc/: libsvox_hip.so, _host_shim.so, libsvox_decoder.so, _decoder_shim.so, libsvox_network.so and
+    _network_shim.so.  Raises on failure.  Returns the first one's path."""
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     out = library_path()
-    decoder = os.path.join(HERE, DECODER_LIB_NAME)
     shims = [(os.path.join(HERE, SHIM_NAME), SHIM_NAME, "host_shim.cpp"),
-             (os.path.join(HERE, DECODER_SHIM_NAME), DECODER_SHIM_NAME, os.path.join("decoder", "decoder_shim.cpp"))]
+             (os.path.join(HERE, DECODER_SHIM_NAME), DECODER_SHIM_NAME, os.path.join("decoder", "decoder_shim.cpp")),
+             (os.path.join(HERE, NETWORK_SHIM_NAME), NETWORK_SHIM_NAME, os.path.join("network", "network_shim.cpp"))]
+    libraries = [(out, list(_units())), (os.path.join(HERE, DECODER_LIB_NAME), list(_decoder_units())),
+                 (os.path.join(HERE, NETWORK_LIB_NAME), list(_network_units()))]
     with tempfile.TemporaryDirectory(prefix="svox_build_") as scratch:
         def compile_unit(unit):
             name, source, extra = unit
@@ -99,17 +112,15 @@ def build_library(verbose=True):
         workers = int(os.environ.get("MAX_JOBS", 0)) or min(8, os.cpu_count() or 1)
         with ThreadPoolExecutor(max_workers=workers) as pool:
             host = [pool.submit(_run, _shim_command(path + ".tmp", name, source)) for path, name, source in shims]
-            units, decoder_units = list(_units()), list(_decoder_units())
-            made = list(pool.map(compile_unit, units + decoder_units))
+            made = [list(m) for m in [pool.map(compile_unit, units) for _, units in libraries]]
             logs = [h.result() for h in host]
-        for log in logs + [log for _, log in made]:
+        for log in logs + [log for library in made for _, log in library]:
             if verbose and log.strip():
                 print(log)
-        objects = [obj for obj, _ in made]
         link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o"]
-        _run(link + [out + ".tmp"] + objects[:len(units)])
-        _run(link + [decoder + ".tmp"] + objects[len(units):])
-    for path in [out, decoder] + [path for path, _, _ in shims]:
+        for (path, _), objects in zip(libraries, made):
+            _run(link + [path + ".tmp"] + [obj for obj, _ in objects])
+    for path in [path for path, _ in libraries] + [path for path, _, _ in shims]:
         os.replace(path + ".tmp", path)
     return out
 

@@ -1,0 +1,147 @@
+"""The C ABI of the operators of networks over cells, their refusals that need no GPU, and the bounds their GPU tests compare with."""
+import ctypes
+import math
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+import svox_amd as svox
+from network_reference import clip_norm, rotate_heads
+from svox_amd.csrc import network as N
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "svox_network.h")
+STRUCTS = {"SvoxClipTensor": N.ClipTensorC, "SvoxRotateHeads": N.RotateHeadsC}
+
+
+def test_header_library_and_mirror_agree():
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    declared = sorted(set(re.findall(r"\b(svox_[a-z_]+)\s*\(", text)))
+    assert sorted(N.SIGNATURES) == declared
+    out = subprocess.run(["nm", "-D", "--defined-only", N.LIB_PATH], stdout=subprocess.PIPE, text=True, check=True).stdout
+    assert sorted(line.split()[-1] for line in out.splitlines() if " T " in line) == declared
+
+
+def test_struct_layouts_match_the_c_compiler(tmp_path):
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {"]
+    for name, mirror in STRUCTS.items():
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f.rstrip("_")}));' for f, _ in mirror._fields_]
+    (tmp_path / "layout.c").write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-o", str(tmp_path / "layout"), str(tmp_path / "layout.c")], check=True)
+    got = dict(line.split() for line in subprocess.run([str(tmp_path / "layout")], stdout=subprocess.PIPE, text=True, check=True).stdout.splitlines())
+    for name, mirror in STRUCTS.items():
+        assert int(got[name]) == ctypes.sizeof(mirror), name
+        for f, _ in mirror._fields_:
+            assert int(got[f"{name}.{f}"]) == getattr(mirror, f).offset, f"{name}.{f}"
+
+
+def with_fields(spec, kw):
+    for k, v in kw.items():
+        setattr(spec, k, v)
+    return ctypes.byref(spec)
+
+
+def test_argument_errors_of_clip_norm_come_before_anything_touches_a_device():
+    lib = N.load_library()
+
+    def table(**kw):
+        t = N.ClipTensorC(from_=16, to=16, count=5, dtype=0)
+        return with_fields(t, kw)
+
+    assert lib.svox_clip_norm(table(), 1, 1.0, None, 16, 64, None) == -1
+    assert lib.svox_clip_norm(None, 1, 1.0, 16, 16, 64, None) == -1
+    for kw, rc in [({"count": -1}, -2), ({"dtype": 3}, -3), ({"dtype": -1}, -3), ({"from_": None}, -1), ({"to": None}, -1), ({"count": 1 << 60}, -2)]:
+        assert lib.svox_clip_norm(table(**kw), 1, 1.0, 16, 16, 64, None) == rc, kw
+        assert lib.svox_network_last_error()
+    for most in (-1.0, math.nan):
+        assert lib.svox_clip_norm(table(), 1, most, 16, 16, 64, None) == -2
+    assert lib.svox_clip_norm(table(), -1, 1.0, 16, 16, 64, None) == -2
+    least = lib.svox_clip_norm_workspace_bytes(table(), 1)
+    assert least == 8 and lib.svox_clip_norm_workspace_bytes(table(count=0, from_=None), 1) == 0 and lib.svox_clip_norm_workspace_bytes(None, 0) == 0
+    assert lib.svox_clip_norm(table(), 1, 1.0, 16, 16, least - 1, None) == -2
+    assert lib.svox_clip_norm(table(), 1, 1.0, 16, 8, least, None) == -2
+    assert lib.svox_clip_norm(table(), 1, 1.0, 16, None, least, None) == -1
+
+
+def test_argument_errors_of_rotate_heads_come_before_anything_touches_a_device():
+    lib = N.load_library()
+
+    def spec(**kw):
+        return with_fields(N.RotateHeadsC(q=16, k=16, positions=16, frequencies=16, rows=4, q_stride=32, q_head=8, k_stride=16, k_head=8, heads=4, kv_heads=2,
+                                          dim=8, rotated=6, axes=3, eps=1e-6), kw)
+
+    grad = (ctypes.c_int64 * 4)(32, 8, 16, 8)
+    assert lib.svox_rotate_heads(None, 16, 16, None) == -1
+    for kw, rc in [({"dtype": 3}, -3), ({"rows": -1}, -2), ({"heads": 0}, -2), ({"kv_heads": 0}, -2), ({"heads": 1 << 21}, -2), ({"dim": 0}, -2),
+                   ({"dim": 257}, -4), ({"rotated": 5}, -2), ({"rotated": 10}, -2), ({"rotated": -2}, -2), ({"axes": 0}, -2), ({"axes": 5}, -2),
+                   ({"position_type": 4}, -3), ({"q": None}, -1), ({"k": None}, -1), ({"positions": None}, -1), ({"frequencies": None}, -1),
+                   ({"q_stride": -1}, -2), ({"k_head": -8}, -2), ({"rows": 1 << 45}, -2), ({"q_stride": 1 << 45}, -2)]:
+        assert lib.svox_rotate_heads(spec(**kw), 16, 16, None) == rc, kw
+        assert lib.svox_rotate_heads_backward(spec(**kw), 16, 16, grad, 16, 16, 16, 16, 16, 1 << 20, None) == rc, kw
+    assert lib.svox_rotate_heads(spec(), None, 16, None) == -1
+    assert lib.svox_rotate_heads(spec(rows=0, q=None, k=None, positions=None), None, None, None) == 0
+    least = lib.svox_rotate_heads_workspace_bytes(spec(), 1)
+    assert least > 0 and lib.svox_rotate_heads_workspace_bytes(spec(), 0) == 0
+    assert lib.svox_rotate_heads_backward(spec(), 16, 16, None, 16, 16, 16, 16, 16, least, None) == -1
+    assert lib.svox_rotate_heads_backward(spec(), None, 16, grad, 16, 16, 16, 16, 16, least, None) == -1
+    assert lib.svox_rotate_heads_backward(spec(), 16, 16, grad, 16, 16, 16, 16, 16, least - 1, None) == -2
+    assert lib.svox_rotate_heads_backward(spec(), 16, 16, grad, None, None, None, None, None, 0, None) == 0
+
+
+CALLS = {"rotate_heads": lambda x: svox.rotate_heads(x, x, torch.zeros(3), torch.zeros(4))[0], "clip_norm": lambda x: svox.clip_norm([x], 1.0)[0]}
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_there_is_no_cpu_path_and_no_tracing(name):
+    call, x = CALLS[name], torch.ones(3, 2, 8)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        call(x)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(x)
+
+
+def test_gradients_that_are_not_there():
+    p = torch.zeros(3, requires_grad=True)
+    assert svox.clip_grad_norm([p], 1.0) == 0 and svox.clip_grad_norm(p, 1.0) == 0 and svox.clip_grad_norm([], 1.0) == 0
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        svox.clip_grad_norm(p, 1.0)
+
+
+def sees_a_mistake(near, got):
+    """The bound holds for `got`, and not where its numbers are out of place."""
+    near.holds(got)
+    off = got.detach().clone().reshape(-1)
+    off[0] += max(1.0, float(off.abs().max()))
+    with pytest.raises(AssertionError):
+        near.holds(off.reshape(got.shape))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_the_bounds_hold_for_torch_and_see_a_mistake(dtype, interleaved):
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(30, 3, 24, generator=g).to(dtype), (1 + 0.2 * torch.randn(24, generator=g)).to(dtype)
+    grad, p, f = torch.randn(30, 3, 24, generator=g).to(dtype), torch.rand(30, 2, generator=g) * 9, torch.rand(2, 10, generator=g)
+    xx, ww = x.float().requires_grad_(), w.float().requires_grad_()
+    n = xx * torch.rsqrt((xx * xx).mean(-1, keepdim=True) + 1e-6) * ww
+    angle = (p.double() @ f.double())[:, None]
+    c, s = angle.cos().float(), angle.sin().float()
+    a, b = (n[..., :20:2], n[..., 1:20:2]) if interleaved else (n[..., :10], n[..., 10:20])
+    turned = [a * c - b * s, b * c + a * s]
+    y = torch.cat([torch.stack(turned, -1).flatten(-2) if interleaved else torch.cat(turned, -1), n[..., 20:]], -1)
+    dx, dw = torch.autograd.grad(y, (xx, ww), grad.float())
+    want, wanted = rotate_heads(x, p, f, w, interleaved=interleaved, grad=grad)
+    sees_a_mistake(want, y.to(dtype))
+    sees_a_mistake(wanted["x"], dx.to(dtype))
+    sees_a_mistake(wanted["weight"], dw.to(dtype))
+    norm = torch.linalg.vector_norm(x.double()).float()
+    near, (scaled,) = clip_norm([x], 2.0)
+    sees_a_mistake(near, norm)
+    sees_a_mistake(scaled, (x.float() * (2.0 / norm)).to(dtype))
