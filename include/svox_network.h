@@ -75,6 +75,41 @@ int svox_rotate_heads_backward(const SvoxRotateHeads* spec, const void* grad_q, 
 /* The least workspace of svox_rotate_heads_backward: 0 where no weight's gradient is asked for (`weights` 0). */
 int64_t svox_rotate_heads_workspace_bytes(const SvoxRotateHeads* spec, int32_t weights);
 
+/* Attention within packed sequences: sequence s holds queries offsets[s] .. offsets[s + 1] - 1 and keys key_offsets[s] ..
+ * key_offsets[s + 1] - 1; a query sees the keys of its own sequence, all of them, or where `causal` those up to its own place counted from
+ * the sequences' ends (query i of a sees keys up to i + b - a of b).  Query head h goes with kv head h / (heads / kv_heads).
+ *   out = sum over keys of softmax(scale q . k) v;  0 where a query sees no key or belongs to no sequence
+ * What the offsets hold is read on the GPU and not checked: places outside of 0 .. queries (keys) count as the nearest inside, and what
+ * sequences that are not in order give is unspecified, but nothing outside of the arrays is read or written. */
+typedef struct SvoxAttention {
+    const void *q, *k, *v;       /* (queries, heads, dim), (keys, kv_heads, dim) twice; a head's numbers lie side by side */
+    const void* offsets;         /* (sequences + 1) int32, or int64 where wide_offsets; NULL: one sequence of all */
+    const void* key_offsets;     /* the same of the keys; NULL: as offsets */
+    int64_t queries, keys;       /* >= 0; queries * heads / kv_heads and keys < 2^31 - 2^10 */
+    int64_t sequences;           /* >= 1 (1 without offsets) */
+    int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;   /* from row to row and from head to head */
+    int32_t heads, kv_heads;     /* heads a multiple of kv_heads */
+    int32_t dim;                 /* 1 .. 128 */
+    int32_t dtype, wide_offsets, causal;
+    float scale;                 /* > 0 */
+} SvoxAttention;
+
+/* out (queries, heads, dim); lse (queries * heads floats) or NULL: what svox_attention_backward needs of the scores' sums. */
+int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+typedef struct SvoxAttentionGrads {
+    const void* out;                      /* what svox_attention left */
+    const float* lse;
+    const void* grad;                     /* of out, (queries, heads, dim) */
+    int64_t grad_stride, grad_head;       /* from row to row and from head to head */
+    void *q, *k, *v;                      /* where the gradients go, dense; NULL where one is not wanted */
+} SvoxAttentionGrads;
+
+int svox_attention_backward(const SvoxAttention* spec, const SvoxAttentionGrads* grads, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The least workspace of svox_attention (backward 0) or svox_attention_backward (1), or a negative SvoxStatus. */
+int64_t svox_attention_workspace_bytes(const SvoxAttention* spec, int32_t backward);
+
 #ifdef __cplusplus
 }
 #endif

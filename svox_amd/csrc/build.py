@@ -35,6 +35,7 @@ POLICIES = [("SH", 25), ("SG", 25), ("SH", 16), ("SG", 16), ("SH", 9), ("SG", 9)
 
 # the types libsvox_decoder.so has kernels for
 DECODER_TYPES = ["float", "F16", "Bf16"]
+ATTENTION_WIDTHS = [128, 64, 32]
 DECODER_ACTIVATIONS = ["kSilu", "kGelu", "kRelu", "kSigmoid"]
 
 
@@ -65,6 +66,10 @@ def _decoder_units():
 
 def _network_units():
     """... and of libsvox_network.so."""
+    for width in ATTENTION_WIDTHS:
+        for of in DECODER_TYPES:
+            yield (f"attention_{of.lower()}_{width}", os.path.join("network", "attention_type.hip"),
+                   [f"-DSVOX_DECODER_TYPE={of}", f"-DSVOX_ATTEND_WIDTH={width}"])
     for of in DECODER_TYPES:
         yield f"rotate_{of.lower()}", os.path.join("network", "rotate_type.hip"), [f"-DSVOX_DECODER_TYPE={of}"]
     yield "clip", os.path.join("network", "clip.hip"), []

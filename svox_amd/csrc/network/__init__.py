@@ -25,6 +25,18 @@ class RotateHeadsC(ctypes.Structure):
                 ("position_type", c_int32), ("eps", c_float)]
 
 
+class AttentionC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("offsets", c_void_p), ("key_offsets", c_void_p), ("queries", c_int64),
+                ("keys", c_int64), ("sequences", c_int64), ("q_stride", c_int64), ("q_head", c_int64), ("k_stride", c_int64), ("k_head", c_int64),
+                ("v_stride", c_int64), ("v_head", c_int64), ("heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32), ("dtype", c_int32),
+                ("wide_offsets", c_int32), ("causal", c_int32), ("scale", c_float)]
+
+
+class AttentionGradsC(ctypes.Structure):
+    _fields_ = [("out", c_void_p), ("lse", c_void_p), ("grad", c_void_p), ("grad_stride", c_int64), ("grad_head", c_int64), ("q", c_void_p),
+                ("k", c_void_p), ("v", c_void_p)]
+
+
 P = ctypes.POINTER
 
 # name -> (restype, argtypes); the entry points of include/svox_network.h
@@ -37,6 +49,9 @@ SIGNATURES = {
     "svox_rotate_heads_backward": (
         ctypes.c_int, [P(RotateHeadsC), c_void_p, c_void_p, P(c_int64), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "svox_rotate_heads_workspace_bytes": (c_int64, [P(RotateHeadsC), c_int32]),
+    "svox_attention": (ctypes.c_int, [P(AttentionC), c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "svox_attention_backward": (ctypes.c_int, [P(AttentionC), P(AttentionGradsC), c_void_p, c_int64, c_void_p]),
+    "svox_attention_workspace_bytes": (c_int64, [P(AttentionC), c_int32]),
 }
 
 _lib = None

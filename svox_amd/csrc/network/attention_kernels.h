@@ -1,0 +1,616 @@
+// attention_kernels.h -- attention within packed sequences, and its gradients.
+//
+//   s_ij = scale q_i . k_j,  o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - m_i) / l_i,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i)
+//   delta_i = do_i . o_i,  dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i),  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//
+// over the keys j that query i sees.  Heads that share keys are taken together: a "row" is a query's token and one of the `group` heads of
+// a head of keys, rows of a token side by side, so that a tile of keys is read once for all of them and the gradients of keys are sums
+// over rows in registers.  A block takes a tile of rows and goes through the union of the keys that they see, which is one piece as
+// sequences are packed in order: short sequences share a tile, and no launch depends on their lengths, which only the GPU knows.
+//
+// The backward pass computes scores twice, once for dq and once for dk and dv: seven products where one pass with atomic sums of dq
+// would do with five, but sums in a fixed order, the same call the same bits.
+//
+// Scores and their exponentials, sums, maxima and results are in 32 bits.  p and ds are rounded to 16-bit operands where the type has 16 bits.
+#pragma once
+#include "attention_tile.h"
+
+namespace svox_network {
+
+template <class T>
+struct AttendArgs {
+    const T *q, *k, *v, *out, *grad;   // out (tokens, heads, dim) dense
+    T* y;                              // forward: the result
+    T *dq, *dk, *dv;                   // dense
+    float *lse, *delta;                // [kv head][row]: log2 of the sum of exponentials, and its sum of do o
+    float* part;                       // where the work of a tile is split: [kv head][split][row][DP] (keys and values: two of them)
+    f32x2* stats;                      // [kv head][split][row]: maximum (of base 2) and sum
+    int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, grad_stride, grad_head;
+    Sequences seq;
+    int rows, keys;                    // of a kv head
+    int group, kv_heads, dim;
+    int tiles, splits;
+    int runs;                          // blocks of an XCD take tiles side by side, else heads go round the XCDs and the last tiles come first
+    float scale;
+};
+
+constexpr float kLog2E = 1.4426950408889634f;
+
+// The work of a block: a tile, a kv head, a part of the tile's other axis.
+struct Place {
+    int tile, head, split;
+};
+template <class T>
+__device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
+    const unsigned id = blockIdx.x, unit = id / p.splits;
+    Place at;
+    at.split = id - unit * p.splits;
+    if (p.runs) {
+        const unsigned n = (unsigned)p.tiles * p.kv_heads, xcd = unit % 8, each = n / 8, left = n % 8;
+        const unsigned position = xcd * each + min(xcd, left) + unit / 8;
+        at.head = position / p.tiles;
+        at.tile = position - at.head * p.tiles;
+    } else {
+        at.tile = unit / p.kv_heads;
+        at.head = unit - at.tile * p.kv_heads;
+        if (p.seq.causal) at.tile = p.tiles - 1 - at.tile;
+    }
+    return at;
+}
+// the tiles of `size` of a span that a split goes through: the first one's begin, and where the last one ends
+__device__ __forceinline__ Span part_of(const Spans& all, int size, int split, int splits) {
+    if (all.low >= all.high) return {0, 0};
+    if (splits == 1) return {all.low, all.high};
+    const int tiles = (all.high - all.low + size - 1) / size, each = (tiles + splits - 1) / splits;
+    const int64_t low = all.low + (int64_t)split * each * size, high = low + (int64_t)each * size;
+    return {(int)(low < all.high ? low : all.high), (int)(high < all.high ? high : all.high)};
+}
+
+template <int N>
+__device__ __forceinline__ void clip(Span (&see)[N], const Span& part) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) see[n].high = min(see[n].high, part.high);
+}
+
+// rows r of `x`, (tokens, heads, dim) with strides
+template <class T>
+__device__ __forceinline__ const T* row_at(const T* x, int r, int group, int head, int64_t stride, int64_t head_stride) {
+    const unsigned token = group == 1 ? (unsigned)r : (unsigned)r / (unsigned)group;
+    return x + (int64_t)token * stride + ((int64_t)head * group + (r - (int)token * group)) * head_stride;
+}
+
+// What the rows of a wavefront's lanes (row `first` + lane % 32 of each of N) see.  Rows that are not there see everything, so that
+// they never make a mask necessary.
+template <int N>
+__device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int first, int count, int group, int low_row, int high_row, Span (&see)[N]) {
+    // the sequences of the block's first and last row
+    const Offsets& mine = keys ? s.q : s.k;
+    const int a = last_not_beyond(mine, keys ? low_row / group : low_row), b = last_not_beyond(mine, keys ? high_row / group : high_row);
+    Spans all{INT32_MAX, INT32_MIN, INT32_MIN, INT32_MAX};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int r = first + 32 * n + (int)threadIdx.x % 32;
+        const bool there = r < count;
+        Span v{0, 0};
+        if (there) {
+            if (keys) {
+                v = s.keys_of(r / group, a, b);
+            } else {                                   // (of rows)
+                v = s.queries_of(r, a, b);
+                v.low *= group, v.high *= group;
+            }
+        }
+        const bool some = v.low < v.high;
+        all.low = min(all.low, some ? v.low : INT32_MAX), all.high = max(all.high, some ? v.high : INT32_MIN);
+        if (!there) v = {INT32_MIN, INT32_MAX};
+        all.all_low = max(all.all_low, v.low), all.all_high = min(all.all_high, v.high);
+        see[n] = v;
+    }
+    all.low = least_of_wave(all.low), all.high = most_of_wave(-1 > all.high ? -1 : all.high);
+    all.all_low = most_of_wave(all.all_low < -1 ? -1 : all.all_low), all.all_high = least_of_wave(all.all_high);
+    return all;
+}
+
+// ---- forward.  Four wavefronts, of which `across` share rows and take a part of every tile's keys each.
+template <class T, int DP, int N, int across>
+struct ForwardShape {
+    static constexpr int down = 4 / across, rows = down * 32 * N;
+    static constexpr int keys = across == 4 ? 128 : (sizeof(T) == 4 && DP == 128 ? 32 : 64), mine = keys / across, blocks = mine / 32;
+    static constexpr int stages = across == 4 ? 1 : 2;   // tiles in LDS
+    static constexpr int tile = keys * DP;
+};
+
+template <class T, int DP, int N, int across, bool whole>
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_kernel(AttendArgs<T> p) {
+    using S = ForwardShape<T, DP, N, across>;
+    using F = Frag<T>;
+    using Eight = typename F::Eight;
+    constexpr int DB = DP / 32, KB = S::blocks;
+    constexpr int join_numbers = across > 1 ? 4 * 32 * (DP + 2) : 0;   // floats
+    constexpr int tile_bytes = 2 * S::stages * S::tile * (int)sizeof(T), join_bytes = join_numbers * 4;
+    __shared__ __attribute__((aligned(16))) char lds[tile_bytes > join_bytes ? tile_bytes : join_bytes];
+    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
+    const Place place = place_of_block(p);
+    const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32 * N;
+
+    Span see[N];
+    const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + S::rows, p.rows) - 1, see);
+    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
+    const Spans block = spans_of_block(spans, room);
+    const Span part = part_of(block, S::keys, place.split, p.splits);
+    clip(see, part);
+
+    Eight q[N][DP / 16];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        load_row<T, DP, whole>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
+
+    const float to2 = p.scale * kLog2E;
+    f32x16 acc[N][DB];
+    float m[N], l[N];
+    T* const tiles = reinterpret_cast<T*>(lds);
+    const T* const k = p.k + place.head * p.k_head;
+    const T* const v = p.v + place.head * p.v_head;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        m[n] = -__builtin_inff(), l[n] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[n][db] = f32x16{};
+    }
+    Stage<T, DP, S::keys, whole> ks, vs;
+    const auto load = [&](int k0) {
+        const int last = part.high - 1 - k0;
+        ks.load([&](int row) { return k + (k0 + (int64_t)row) * p.k_stride; }, last, p.dim);
+        vs.load([&](int row) { return v + (k0 + (int64_t)row) * p.v_stride; }, last, p.dim);
+    };
+    const auto store = [&](int stage, int k0) {
+        ks.store(tiles + stage * 2 * S::tile);
+        vs.store(tiles + (stage * 2 + 1) * S::tile);
+        if (block.masks(k0, S::keys) && vs.odd()) odd[stage] = k0;
+    };
+    __syncthreads();
+    if (part.low < part.high) {
+        load(part.low);
+        store(0, part.low);
+        __syncthreads();
+    }
+    int stage = 0;
+    for (int k0 = part.low; k0 < part.high; k0 += S::keys) {
+        const bool more = k0 + S::keys < part.high;
+        if (more) load(k0 + S::keys);
+        const T* const kt = tiles + stage * 2 * S::tile;
+        const T* const vt = kt + S::tile;
+        const int kw = k0 + wave % across * S::mine;   // this wavefront's keys
+        if (kw < spans.high && kw + S::mine > spans.low && kw < part.high) {
+            f32x16 s[KB][N];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[b][n] = f32x16{};
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    const Eight a = Tile<T, DP>::along(kt, wave % across * S::mine + 32 * b, t);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) s[b][n] = F::mma(a, q[n][t], s[b][n]);
+                }
+            }
+            const bool mask = kw < spans.all_low || kw + S::mine > spans.all_high || kw + S::mine > part.high;
+            if (mask) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int low = see[n].low, high = see[n].high;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = kw + 32 * b + row_of(r) + 4 * h;
+                            s[b][n][r] = key >= low && key < high ? s[b][n][r] : -__builtin_inff();
+                        }
+                }
+            }
+            Eight e[KB][2][N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float most = m[n];
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][n][r]);
+                most = fmaxf(most, other_half(most));
+                const float from = most == -__builtin_inff() ? 0.0f : most * to2;   // (nothing seen yet: exponentials of -inf are 0)
+                if (__any(most != m[n])) {
+                    const float less = __builtin_amdgcn_exp2f(__builtin_fmaf(m[n], to2, -from));
+                    l[n] *= less;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[n][db] *= less;
+                    m[n] = most;
+                }
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    float x[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][r], to2, -from));
+                        l[n] += x[r];
+                    }
+                    e[b][0][n] = F::pack(x);
+                    e[b][1][n] = F::pack(x + 8);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int at = wave % across * S::mine + 32 * b + 16 * c;
+                    if (mask && odd[stage] == k0) accumulate_odd<T, DP, true>(acc, vt, at, e[b][c], see, k0 + at);
+                    else accumulate<T, DP, N>(acc, vt, at, e[b][c]);
+                }
+        }
+        if constexpr (S::stages == 2) {
+            if (more) store(stage ^ 1, k0 + S::keys);
+            stage ^= 1;
+            __syncthreads();
+        } else {
+            __syncthreads();
+            if (more) store(0, k0 + S::keys);
+            __syncthreads();
+        }
+    }
+
+#pragma unroll
+    for (int n = 0; n < N; ++n) l[n] += other_half(l[n]);
+    if constexpr (across > 1) {
+        // the wavefronts' sums, joined by the first: every lane finds its own numbers of the others
+        static_assert(across == 4 && N == 1, "all wavefronts share rows");
+        float* const shared = reinterpret_cast<float*>(lds);
+        const int lane = (int)threadIdx.x % kWave;
+        constexpr int each = DB * 16 * kWave;   // numbers of a wavefront, then its maxima and sums
+        static_assert(4 * (each + 64) <= join_numbers, "room");
+        float* const own = shared + wave * (each + 64);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) own[(db * 16 + r) * kWave + lane] = acc[0][db][r];
+        if (lane < 32) own[each + lane] = m[0], own[each + 32 + lane] = l[0];
+        __syncthreads();
+        if (wave != 0) return;
+        float most = m[0];
+        for (int w = 1; w < 4; ++w) most = fmaxf(most, shared[w * (each + 64) + each + lane % 32]);
+        const float from = most == -__builtin_inff() ? 0.0f : most;
+        l[0] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
+        for (int w = 0; w < 4; ++w) {
+            const float* const other = shared + w * (each + 64);
+            if (other[each + lane % 32] == -__builtin_inff() && other[each + 32 + lane % 32] == 0.0f) continue;
+            const float less = __builtin_amdgcn_exp2f((other[each + lane % 32] - from) * to2);
+            l[0] = __builtin_fmaf(other[each + 32 + lane % 32], less, l[0]);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[0][db][r] = __builtin_fmaf(other[(db * 16 + r) * kWave + lane], less, acc[0][db][r]);
+        }
+        m[0] = most;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int r = mine + 32 * n + (int)threadIdx.x % 32;
+        if (r >= p.rows) continue;
+        // (what a row that sees keys has, though all of its scores are -inf, is not what one that sees none has)
+        const bool some = max(see[n].low, part.low) < see[n].high;
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
+            if (h == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
+            if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f);
+        } else {
+            const unsigned token = (unsigned)r / (unsigned)p.group;
+            store_row<T, DB>(p.y + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[n],
+                             some ? 1.0f / l[n] : 0.0f);
+            if (p.lse && h == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : __builtin_inff();
+        }
+    }
+}
+
+// The splits' sums of a row, one joined row a block at a time: 32 lanes read a row's numbers, DP / 4 of them used, eight splits at once.
+template <class T, int DP>
+__global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs<T> p) {
+    constexpr int lanes = DP / 4, groups = kAttendThreads / lanes;
+    __shared__ f32x4 room[kAttendThreads];
+    __shared__ float sums[kAttendThreads];
+    const int lane = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
+    for (int64_t i = blockIdx.x; i < (int64_t)p.kv_heads * p.rows; i += gridDim.x) {
+        const int head = (int)(i / p.rows), r = (int)(i - (int64_t)head * p.rows);
+        const int64_t first = (int64_t)head * p.splits * p.rows + r;
+        float most = -__builtin_inff();
+        for (int s = (int)threadIdx.x % kWave; s < p.splits; s += kWave) most = fmaxf(most, p.stats[first + (int64_t)s * p.rows][0]);
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d, kWave));
+        f32x4 sum = {};
+        float l = 0.0f;
+        for (int s = group; s < p.splits; s += groups) {
+            const int64_t at = first + (int64_t)s * p.rows;
+            const f32x2 stat = p.stats[at];
+            if (stat[0] == -__builtin_inff()) continue;   // (nothing seen, nothing stored)
+            const float less = __builtin_amdgcn_exp2f(stat[0] - most);
+            l = __builtin_fmaf(stat[1], less, l);
+            sum += *reinterpret_cast<const f32x4*>(p.part + at * DP + 4 * lane) * less;
+        }
+        __syncthreads();
+        room[threadIdx.x] = sum;
+        if (lane == 0) sums[group] = l;
+        __syncthreads();
+        if (group != 0) continue;
+        l = 0.0f;
+        for (int g = 0; g < groups; ++g) l += sums[g];
+        for (int g = 1; g < groups; ++g) sum += room[g * lanes + lane];
+        const bool some = most != -__builtin_inff();
+        const float factor = some ? 1.0f / l : 0.0f;
+        const int token = r / p.group;
+        T* const to = p.y + (((int64_t)token * p.kv_heads + head) * p.group + (r - token * p.group)) * p.dim;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * lane + j < p.dim) to[4 * lane + j] = (T)(sum[j] * factor);
+        if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : __builtin_inff();
+    }
+}
+
+// delta: a row's sum of do o, by sixteen lanes
+template <class T>
+__global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs<T> p) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int lane = (int)threadIdx.x % 16;
+    const int64_t all = (int64_t)p.rows * p.kv_heads;
+    // (in memory's order: token, kv head, head of the group)
+    for (int64_t first = (int64_t)blockIdx.x * 16; first < all; first += (int64_t)gridDim.x * 16) {
+        const int64_t i = first + threadIdx.x / 16;
+        if (i >= all) continue;
+        const int64_t heads = (int64_t)p.kv_heads * p.group, token = i / heads;
+        const int head = (int)(i - token * heads);
+        const T* const o = p.out + i * p.dim;
+        const T* const g = p.grad + token * p.grad_stride + head * p.grad_head;
+        float sum = 0.0f;
+        for (int c = lane * V; c < p.dim; c += 16 * V) {
+            const auto a = load_some<T, V>(o + c, p.dim - c), b = load_some<T, V>(g + c, p.dim - c);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum = __builtin_fmaf((float)a[j], (float)b[j], sum);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) sum += __shfl_xor(sum, d, kWave);
+        if (lane == 0) p.delta[(int64_t)(head / p.group) * p.rows + token * p.group + head % p.group] = sum;
+    }
+}
+
+// ---- dq: rows as forward, through the keys they see
+template <class T, int DP, bool whole>
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_query_grad_kernel(AttendArgs<T> p) {
+    using F = Frag<T>;
+    using Eight = typename F::Eight;
+    constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
+    __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
+    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
+    const Place place = place_of_block(p);
+    const int r0 = place.tile * rows, mine = r0 + wave * 32, row = min(mine + (int)threadIdx.x % 32, p.rows - 1);
+
+    Span see[1];
+    const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + rows, p.rows) - 1, see);
+    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
+    const Spans block = spans_of_block(spans, room);
+    const Span part = part_of(block, keys, place.split, p.splits);
+    clip(see, part);
+
+    Eight q[DP / 16], g[DP / 16];
+    load_row<T, DP, whole>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
+    load_row<T, DP, whole>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
+    const float lse = p.lse[(int64_t)place.head * p.rows + row], delta = p.delta[(int64_t)place.head * p.rows + row];
+    const float to2 = p.scale * kLog2E;
+    const T* const k = p.k + place.head * p.k_head;
+    const T* const v = p.v + place.head * p.v_head;
+    f32x16 acc[1][DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
+    Stage<T, DP, keys, whole> ks, vs;
+    const auto load = [&](int k0) {
+        const int last = part.high - 1 - k0;
+        ks.load([&](int row) { return k + (k0 + (int64_t)row) * p.k_stride; }, last, p.dim);
+        vs.load([&](int row) { return v + (k0 + (int64_t)row) * p.v_stride; }, last, p.dim);
+    };
+    const auto store = [&](int stage, int k0) {
+        ks.store(tiles + stage * 2 * tile);
+        vs.store(tiles + (stage * 2 + 1) * tile);
+        if (block.masks(k0, keys) && ks.odd()) odd[stage] = k0;
+    };
+    __syncthreads();
+    if (part.low < part.high) {
+        load(part.low);
+        store(0, part.low);
+        __syncthreads();
+    }
+    int stage = 0;
+    for (int k0 = part.low; k0 < part.high; k0 += keys) {
+        const bool more = k0 + keys < part.high;
+        if (more) load(k0 + keys);
+        const T* const kt = tiles + stage * 2 * tile;
+        const T* const vt = kt + tile;
+        if (k0 < spans.high && k0 + keys > spans.low) {
+            const bool mask = k0 < spans.all_low || k0 + keys > spans.all_high || k0 + keys > part.high;
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    s = F::mma(Tile<T, DP>::along(kt, 32 * b, t), q[t], s);
+                    dp = F::mma(Tile<T, DP>::along(vt, 32 * b, t), g[t], dp);
+                }
+                float ds[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to2, -lse)) * (dp[r] - delta);
+                if (mask) {
+                    const int low = see[0].low, high = see[0].high;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = k0 + 32 * b + row_of(r) + 4 * h;
+                        ds[r] = key >= low && key < high ? ds[r] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Eight e[1] = {F::pack(ds + 8 * c)};
+                    if (mask && odd[stage] == k0) accumulate_odd<T, DP, false>(acc, kt, 32 * b + 16 * c, e, see, k0 + 32 * b + 16 * c);
+                    else accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
+                }
+            }
+        }
+        if (more) store(stage ^ 1, k0 + keys);
+        stage ^= 1;
+        __syncthreads();
+    }
+    const int r = mine + (int)threadIdx.x % 32;
+    if (r >= p.rows) return;
+    if (p.splits > 1) {
+        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f);
+    } else {
+        const unsigned token = (unsigned)r / (unsigned)p.group;
+        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale);
+    }
+}
+
+// ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them
+template <class T, int DP, bool whole>
+__global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
+    using F = Frag<T>;
+    using Eight = typename F::Eight;
+    constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
+    __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
+    __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
+    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
+    const Place place = place_of_block(p);
+    const int j0 = place.tile * keys, mine = j0 + wave * 32, key = min(mine + (int)threadIdx.x % 32, p.keys - 1);
+
+    Span see[1];
+    const Spans spans = spans_of<1>(p.seq, false, mine, p.keys, p.group, j0, min(j0 + keys, p.keys) - 1, see);
+    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
+    const Spans block = spans_of_block(spans, room);
+    const Span part = part_of(block, rows, place.split, p.splits);
+    clip(see, part);
+
+    Eight k[DP / 16], v[DP / 16];
+    load_row<T, DP, whole>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
+    load_row<T, DP, whole>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
+    const float to2 = p.scale * kLog2E;
+    const float* const lse = p.lse + (int64_t)place.head * p.rows;
+    const float* const delta = p.delta + (int64_t)place.head * p.rows;
+    f32x16 dk[1][DB], dv[1][DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[0][db] = dv[0][db] = f32x16{};
+    Stage<T, DP, rows, whole> qs, gs;
+    float stat = 0.0f;
+    const auto load = [&](int i0) {
+        const int last = part.high - 1 - i0;
+        qs.load([&](int row) { return row_at(p.q, i0 + row, p.group, place.head, p.q_stride, p.q_head); }, last, p.dim);
+        gs.load([&](int row) { return row_at(p.grad, i0 + row, p.group, place.head, p.grad_stride, p.grad_head); }, last, p.dim);
+        if ((int)threadIdx.x < 2 * rows) {
+            const int row = (int)threadIdx.x % rows, at = i0 + (row < last ? row : last);
+            stat = (int)threadIdx.x < rows ? lse[at] : delta[at];
+        }
+    };
+    const auto store = [&](int stage, int i0) {
+        qs.store(tiles + stage * 2 * tile);
+        gs.store(tiles + (stage * 2 + 1) * tile);
+        if (block.masks(i0, rows) && (qs.odd() || gs.odd())) odd[stage] = i0;
+        if ((int)threadIdx.x < 2 * rows) shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
+    };
+    __syncthreads();
+    if (part.low < part.high) {
+        load(part.low);
+        store(0, part.low);
+        __syncthreads();
+    }
+    int stage = 0;
+    for (int i0 = part.low; i0 < part.high; i0 += rows) {
+        const bool more = i0 + rows < part.high;
+        if (more) load(i0 + rows);
+        const T* const qt = tiles + stage * 2 * tile;
+        const T* const gt = qt + tile;
+        if (i0 < spans.high && i0 + rows > spans.low) {
+            const bool mask = i0 < spans.all_low || i0 + rows > spans.all_high || i0 + rows > part.high;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) {
+                    s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
+                    dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
+                }
+                float e[16], ds[16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 from = *reinterpret_cast<const f32x4*>(&shared[stage][0][32 * b + 8 * i + 4 * h]);
+                    const f32x4 less = *reinterpret_cast<const f32x4*>(&shared[stage][1][32 * b + 8 * i + 4 * h]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        e[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], to2, -from[j]));
+                        ds[4 * i + j] = e[4 * i + j] * (dp[4 * i + j] - less[j]);
+                    }
+                }
+                if (mask) {
+                    const int low = see[0].low, high = see[0].high;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = i0 + 32 * b + row_of(r) + 4 * h;
+                        const bool seen = row >= low && row < high;
+                        e[r] = seen ? e[r] : 0.0f, ds[r] = seen ? ds[r] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int at = 32 * b + 16 * c;
+                    const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
+                    if (mask && odd[stage] == i0) {
+                        accumulate_odd<T, DP, true>(dv, gt, at, pe, see, i0 + at);
+                        accumulate_odd<T, DP, false>(dk, qt, at, pd, see, i0 + at);
+                    } else {
+                        accumulate<T, DP, 1>(dv, gt, at, pe);
+                        accumulate<T, DP, 1>(dk, qt, at, pd);
+                    }
+                }
+            }
+        }
+        if (more) store(stage ^ 1, i0 + rows);
+        stage ^= 1;
+        __syncthreads();
+    }
+    const int j = mine + (int)threadIdx.x % 32;
+    if (j >= p.keys) return;
+    if (p.splits > 1) {
+        float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
+        store_row<float, DB>(at, DP, dk[0], 1.0f);
+        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], 1.0f);
+    } else {
+        const int64_t at = ((int64_t)j * p.kv_heads + place.head) * p.dim;
+        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale);
+        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], 1.0f);
+    }
+}
+
+// The splits' sums of a gradient: [kv head][split][row][DP] to (tokens, kv heads, group, dim)
+template <class T, int DP>
+__global__ __launch_bounds__(kAttendThreads) void attend_sum_kernel(const float* part, int64_t rows, int kv_heads, int group, int dim, int splits, float factor,
+                                                                    T* to) {
+    constexpr int lanes = DP / 4;
+    const int lane = (int)threadIdx.x % lanes;
+    const int64_t all = rows * kv_heads, step = (int64_t)gridDim.x * (kAttendThreads / lanes);
+    for (int64_t i = (int64_t)blockIdx.x * (kAttendThreads / lanes) + threadIdx.x / lanes; i < all; i += step) {
+        const int64_t head = i / rows, r = i - head * rows, token = r / group;
+        f32x4 sum = {};
+        for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4*>(part + ((head * splits + s) * rows + r) * DP + 4 * lane);
+        T* const at = to + ((token * kv_heads + head) * group + (r - token * group)) * dim;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * lane + j < dim) at[4 * lane + j] = (T)(sum[j] * factor);
+    }
+}
+
+}  // namespace svox_network

@@ -1,0 +1,338 @@
+// attention_tile.h -- what the attention kernels are made of: products of 32 x 32 on the matrix cores, tiles of rows in LDS and the two
+// ways to read them, and which keys a query sees.
+//
+// All kernels compute scores the way round that leaves a lane with one query (or one key: backward, for keys and values) and 16 of the
+// others, in the order in which the matrix cores hand results out: number r of a lane is row (r mod 4) + 8 (r / 4) + 4 half, half = lane / 32.
+// As the order of a reduction is free as long as both operands have the same, those 16 numbers go into the next product as they lie in
+// the registers, eight to a fragment, and only the other operand is read in that order: no score passes through LDS.
+#pragma once
+#include "../decoder/common.h"
+
+namespace svox_network {
+
+using namespace svox_decoder;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4 LdsFour;
+
+constexpr int kAttendThreads = 256;
+
+// A fragment is 16 of the reduction, eight of them in each half of a wavefront.  float32 goes through the matrix cores as it is, two of the
+// reduction at a time.
+template <class T>
+struct Frag {
+    typedef u16x8 Eight;
+    typedef typename Few<T, 8>::vector Numbers;
+    static __device__ __forceinline__ f32x16 mma(Eight a, Eight b, f32x16 c) {
+        if constexpr (std::is_same_v<T, Bf16>)
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Eight pack(const float* v) {
+        return __builtin_bit_cast(Eight, __builtin_convertvector((f32x8){v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, Numbers));
+    }
+};
+template <>
+struct Frag<float> {
+    typedef f32x8 Eight;
+    typedef f32x8 Numbers;
+    static __device__ __forceinline__ f32x16 mma(Eight a, Eight b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Eight pack(const float* v) { return (Eight){v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}; }
+};
+
+// row of a result's number r, and of a fragment's number e that holds results
+__device__ __forceinline__ constexpr int row_of(int r) { return (r & 3) + 8 * (r >> 2); }
+
+__device__ __forceinline__ int half_of() { return (int)threadIdx.x / 32 % 2; }
+
+// A tile of rows of DP numbers in LDS.  The 16-byte pieces of a row lie in an order that depends on the row, so that both the eight
+// lanes that read eight rows at a time and the sixteen that read four rows across find them in different banks.
+template <class T, int DP>
+struct Tile {
+    static constexpr int V = 16 / (int)sizeof(T), pieces = DP / V;   // numbers of a piece, pieces of a row
+    static constexpr int ring = pieces < 8 ? pieces : 8;              // pieces that change places
+    static __device__ __forceinline__ int turn(int row) {
+        if constexpr (pieces == 4) return (row & 2) | (row >> 2 & 1);
+        else return (row & 3) << 1 | (row >> 2 & 1);
+    }
+    // (what is the same for all lanes stands by itself: it goes into the instructions' own offsets)
+    static __device__ __forceinline__ int at(int row, int piece) { return row * DP + piece / ring * ring * V + ((piece % ring) ^ turn(row)) * V; }
+
+    // numbers 16 t + 8 half .. of row r0 + lane % 32; r0 a whole number of 8
+    static __device__ __forceinline__ typename Frag<T>::Eight along(const T* lds, int r0, int t) {
+        const int row = (int)threadIdx.x % 32, h = half_of(), turned = turn(row);
+        const T* const from = lds + row * DP;
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const u16x8*>(from + r0 * DP + 2 * t / ring * ring * V + ((2 * t % ring) ^ (h ^ turned)) * V);
+        } else {
+            const int even = 4 * t % ring, beyond = r0 * DP + 4 * t / ring * ring * V;
+            const f32x4 a = *reinterpret_cast<const f32x4*>(from + beyond + (even ^ (2 * h ^ turned)) * V);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(from + beyond + ((even + 1) ^ (2 * h ^ turned)) * V);
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // number 32 db + lane % 32 of rows r0 + row_of(0 .. 7) + 4 half; r0 a whole number of 16
+    static __device__ __forceinline__ typename Frag<T>::Eight across(const T* lds, int r0, int db) {
+        const int lane = (int)threadIdx.x % kWave, h = half_of();
+        if constexpr (sizeof(T) == 2) {
+            const int l = lane & 15, row = 4 * h + (l >> 2), piece = (lane >> 3 & 2) + (l >> 1 & 1);   // of the first 32 columns
+            const T* const from = lds + row * DP + (l & 1) * 4 + ((4 * db % ring) ^ (piece ^ turn(row))) * V;
+            u16x8 both;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(from + (r0 + 8 * half) * DP + 4 * db / ring * ring * V));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) both[half * 4 + i] = (u16)four[i];
+            }
+            return both;
+        } else {
+            const int c = lane % 32;
+            typename Frag<T>::Eight v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int row = row_of(e) + 4 * h;   // (the eight pieces of a row's 32 columns)
+                v[e] = lds[(r0 + row) * DP + 32 * db + ((c / 4) ^ turn(row)) * 4 + c % 4];
+            }
+            return v;
+        }
+    }
+};
+
+// `rows` rows of memory on their way to a tile, through registers: the next tile's loads are in flight while this one is multiplied.
+// Rows from `last` on repeat it (whoever reads them knows that they are not there), numbers beyond a row are zeros.
+template <class T, int DP, int rows, bool whole>
+struct Stage {
+    using Shape = Tile<T, DP>;
+    static constexpr int each = rows * Shape::pieces / kAttendThreads;
+    static_assert(rows * Shape::pieces % kAttendThreads == 0, "as many pieces for every thread");
+    typename Few<T, Shape::V>::vector v[each];
+
+    template <class Row>
+    __device__ __forceinline__ void load(Row row_at, int last, int dim) {
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+            const int piece = i * kAttendThreads + (int)threadIdx.x, row = piece / Shape::pieces, column = piece % Shape::pieces * Shape::V;
+            const T* const from = row_at(row < last ? row : last) + column;
+            if constexpr (whole) v[i] = load_few<T, Shape::V>(from);
+            else v[i] = load_some<T, Shape::V>(from, dim - column);
+        }
+    }
+    // whether one of this thread's numbers is infinite or NaN
+    __device__ __forceinline__ bool odd() const {
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+            typedef unsigned Words __attribute__((ext_vector_type(4)));
+            // (an exponent of ones becomes a carry into the sign's place)
+            constexpr unsigned low = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu, sign = ~low;
+            constexpr unsigned one = sizeof(T) == 4 ? 0x00800000u : std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u;
+            const Words w = (__builtin_bit_cast(Words, v[i]) & low) + one;
+            found = found || ((w[0] | w[1] | w[2] | w[3]) & sign) != 0;
+        }
+        return found;
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+            const int piece = i * kAttendThreads + (int)threadIdx.x;
+            *reinterpret_cast<typename Few<T, Shape::V>::vector*>(lds + Shape::at(piece / Shape::pieces, piece % Shape::pieces)) = v[i];
+        }
+    }
+};
+
+// Fragments of a row in memory, as an operand that stays in registers: numbers 16 t + 8 half .. of `row`.
+template <class T, int DP, bool whole>
+__device__ __forceinline__ void load_row(const T* row, int dim, typename Frag<T>::Eight (&out)[DP / 16]) {
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+        const int at = 16 * t + 8 * half_of();
+        if constexpr (whole) out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_few<T, 8>(row + at));
+        else out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_some<T, 8>(row + at, dim - at));
+    }
+}
+
+// ---- packed sequences
+// Where they begin and end, n + 1 places, as they come from the caller's memory: whatever stands there is brought within 0 .. total.
+struct Offsets {
+    const void* at;   // or NULL: one sequence, 0 .. total
+    int wide, n;
+    int total;
+    __device__ __forceinline__ int operator()(int i) const {
+        if (!at) return i == 0 ? 0 : total;
+        const int64_t v = wide ? ((const int64_t*)at)[i] : (int64_t)((const int32_t*)at)[i];
+        return v < 0 ? 0 : v > total ? total : (int)v;
+    }
+};
+// The last i with offsets(i) <= t, or -1: by the whole wavefront, 64 places at a time.  (At most n whatever the places hold.)
+__device__ __forceinline__ int last_not_beyond(const Offsets& o, int t) {
+    if (!o.at) return t < o.total ? 0 : 1;
+    const int lane = (int)threadIdx.x % kWave;
+    int low = 0, size = o.n + 1;
+    while (true) {
+        const int step = (size + kWave - 1) / kWave, at = lane * step;
+        const int found = __popcll(__ballot(at < size && o(low + at) <= t));
+        if (found == 0) return low == 0 ? -1 : low;
+        low += (found - 1) * step;
+        if (step == 1) return low;
+        size = min(step, size - (found - 1) * step);
+    }
+}
+// the sequence of t, which lies among low .. high
+__device__ __forceinline__ int sequence_of(const Offsets& o, int t, int low, int high) {
+    while (low < high) {
+        const int middle = (low + high + 1) / 2;
+        if (o(middle) <= t) low = middle;
+        else high = middle - 1;
+    }
+    return low;
+}
+
+struct Span {
+    int low, high;   // none: low == high
+};
+struct Sequences {
+    Offsets q, k;
+    int causal;
+    // of keys that query t sees, t's sequence among first .. last
+    __device__ __forceinline__ Span keys_of(int t, int first, int last) const {
+        const int s = sequence_of(q, t, max(first, 0), last);
+        if (s >= q.n) return {0, 0};
+        const int q0 = q(s), q1 = q(s + 1), k0 = k(s), k1 = max(k0, k(s + 1));
+        if (t < q0 || t >= q1) return {0, 0};
+        if (!causal) return {k0, k1};
+        const int64_t seen = (int64_t)(t - q0) + (k1 - k0) - (q1 - q0) + 1;
+        return {k0, k0 + (int)(seen < 0 ? 0 : seen > k1 - k0 ? k1 - k0 : seen)};
+    }
+    // of queries that see key t
+    __device__ __forceinline__ Span queries_of(int t, int first, int last) const {
+        const int s = sequence_of(k, t, max(first, 0), last);
+        if (s >= k.n) return {0, 0};
+        const int q0 = q(s), q1 = max(q0, q(s + 1)), k0 = k(s), k1 = k(s + 1);
+        if (t < k0 || t >= k1) return {0, 0};
+        if (!causal) return {q0, q1};
+        const int64_t hidden = (int64_t)(t - k0) - ((k1 - k0) - (q1 - q0));
+        return {q0 + (int)(hidden < 0 ? 0 : hidden > q1 - q0 ? q1 - q0 : hidden), q1};
+    }
+};
+
+// What the lanes of a wavefront see: the span of all, and the one that every lane sees whole.
+struct Spans {
+    int low, high;            // of all; none: low >= high
+    int all_low, all_high;
+    // whether some lane does not see all of the `n` from `first` on
+    __device__ __forceinline__ bool masks(int first, int n) const { return first < all_low || first + n > all_high; }
+};
+__device__ __forceinline__ int least_of_wave(int v) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) v = min(v, __shfl_xor(v, d, kWave));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int most_of_wave(int v) { return -least_of_wave(-v); }
+
+// of every wavefront's spans the block's
+__device__ __forceinline__ Spans spans_of_block(const Spans& s, int* room) {
+    const int wave = (int)threadIdx.x / kWave;
+    if (threadIdx.x % kWave == 0) room[4 * wave] = s.low, room[4 * wave + 1] = s.high, room[4 * wave + 2] = s.all_low, room[4 * wave + 3] = s.all_high;
+    __syncthreads();
+    Spans b{room[0], room[1], room[2], room[3]};
+#pragma unroll
+    for (int w = 1; w < kAttendThreads / kWave; ++w) {
+        b.low = min(b.low, room[4 * w]), b.high = max(b.high, room[4 * w + 1]);
+        b.all_low = max(b.all_low, room[4 * w + 2]), b.all_high = min(b.all_high, room[4 * w + 3]);
+    }
+    return {__builtin_amdgcn_readfirstlane(b.low), __builtin_amdgcn_readfirstlane(b.high), __builtin_amdgcn_readfirstlane(b.all_low),
+            __builtin_amdgcn_readfirstlane(b.all_high)};
+}
+
+template <class T>
+__device__ __forceinline__ float number_of(typename Frag<T>::Eight a, int e) {
+    if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(T, (u16)a[e]);
+    else return a[e];
+}
+template <class T, class F>
+__device__ __forceinline__ typename Frag<T>::Eight ones_where(F f) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f(e) ? 1.0f : 0.0f;
+    return Frag<T>::pack(v);
+}
+
+// acc += across rows r0 .. r0 + 15 of a tile times `b`
+template <class T, int DP, int N>
+__device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* lds, int r0, const typename Frag<T>::Eight (&b)[N]) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+        const auto a = Tile<T, DP>::across(lds, r0, db);
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n][db] = Frag<T>::mma(a, b[n], acc[n][db]);
+    }
+}
+
+// The same of a tile that holds infinite numbers or NaN, in rows that not every lane sees.  A score that is masked is 0 in b, and 0 times
+// what its row holds is 0, unless that is infinite or NaN.  Such numbers are therefore taken out of the product, and what the lanes that do
+// see them get of them is found by products of ones: NaN of NaN, of infinite ones themselves if `infinite` (b's numbers are not negative),
+// else NaN as well.  (`first`: the tile's row r0 in the numbers that the spans count)
+template <class T, int DP, bool infinite, int N>
+__device__ __forceinline__ void accumulate_odd(f32x16 (&acc)[N][DP / 32], const T* lds, int r0, const typename Frag<T>::Eight (&b)[N], const Span (&see)[N],
+                                               int first) {
+    using Eight = typename Frag<T>::Eight;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const Eight seen = ones_where<T>([&](int e) {
+            const int row = first + row_of(e) + 4 * half_of();
+            return row >= see[n].low && row < see[n].high;
+        });
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            const Eight a = Tile<T, DP>::across(lds, r0, db);
+            Eight finite = a;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(__builtin_fabsf(number_of<T>(a, e)) < __builtin_inff())) finite[e] = 0;
+            acc[n][db] = Frag<T>::mma(finite, b[n], acc[n][db]);
+#pragma unroll
+            for (int kind = 0; kind < (infinite ? 3 : 1); ++kind) {
+                const float inf = kind == 1 ? __builtin_inff() : -__builtin_inff();
+                const Eight ones = ones_where<T>([&](int e) {
+                    const float v = number_of<T>(a, e);
+                    return kind == 0 ? (infinite ? v != v : !(__builtin_fabsf(v) < __builtin_inff())) : v == inf;
+                });
+                const f32x16 count = Frag<T>::mma(ones, seen, f32x16{});
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (count[r] > 0.0f) acc[n][db][r] += kind == 0 ? __builtin_nanf("") : inf;
+                __builtin_amdgcn_sched_barrier(0);   // (one count at a time: this path is not to cost the others registers)
+            }
+        }
+    }
+}
+
+// the other half's number
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
+
+// A row of a result, a lane's 16 numbers of every 32: to memory as `V`, times `factor`.
+template <class V, int DB>
+__device__ __forceinline__ void store_row(V* row, int dim, const f32x16 (&acc)[DB], float factor) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = db * 32 + 8 * i + 4 * half_of();
+            const f32x4 v = {acc[db][4 * i] * factor, acc[db][4 * i + 1] * factor, acc[db][4 * i + 2] * factor, acc[db][4 * i + 3] * factor};
+            if (at + 4 <= dim) {
+                store_few<V, 4>(row + at, __builtin_convertvector(v, typename Few<V, 4>::vector));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < dim) row[at + j] = (V)v[j];
+            }
+        }
+}
+
+}  // namespace svox_network

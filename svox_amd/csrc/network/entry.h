@@ -23,4 +23,10 @@ int launch_rotate_backward(const SvoxRotateHeads& s, const void* grad_q, const v
 template <class T>
 int rotate_backward_blocks(const SvoxRotateHeads& s);   // each with a row of partial sums
 
+// (defined for every type and width in attention_type.hip)
+template <class T, int width>
+int launch_attention(const SvoxAttention& s, void* out, float* lse, void* workspace, hipStream_t stream);
+template <class T, int width>
+int launch_attention_backward(const SvoxAttention& s, const SvoxAttentionGrads& grads, void* workspace, hipStream_t stream);
+
 }  // namespace svox_network

@@ -5,6 +5,7 @@
 #include <cstdio>
 
 #include "../decoder/common.h"
+#include "attention_rules.h"
 #include "entry.h"
 #include "rotate_kernels.h"
 
@@ -107,6 +108,36 @@ int64_t rotate_space(const SvoxRotateHeads& s, bool weights) {
     return blocks * 2 * s.dim * (int64_t)sizeof(float);
 }
 
+int check_attention(const SvoxAttention* s) {
+    if (!s) return fail(SVOX_ERR_NULL_POINTER, "the spec is NULL");
+    SVOX_TRY(check_dtype(s->dtype));
+    if (s->queries < 0 || s->keys < 0) return fail(SVOX_ERR_BAD_SHAPE, "queries and keys must be >= 0, got %lld and %lld", (long long)s->queries, (long long)s->keys);
+    if (s->heads < 1 || s->kv_heads < 1 || s->heads > kMostHeads || s->heads % s->kv_heads)
+        return fail(SVOX_ERR_BAD_SHAPE, "heads must be a multiple of kv_heads and between 1 and %d, got %d and %d", kMostHeads, s->heads, s->kv_heads);
+    if (s->dim < 1) return fail(SVOX_ERR_BAD_SHAPE, "dim must be >= 1, got %d", s->dim);
+    if (s->dim > 128) return fail(SVOX_ERR_UNSUPPORTED, "dim must be <= 128, got %d", s->dim);
+    if (!(s->scale > 0.0f) || std::isinf(s->scale)) return fail(SVOX_ERR_BAD_SHAPE, "scale must be > 0 and finite, got %g", (double)s->scale);
+    if (s->sequences < 1 || s->sequences > INT32_MAX - 1024) return fail(SVOX_ERR_BAD_SHAPE, "sequences must be between 1 and 2^31 - 2^10, got %lld", (long long)s->sequences);
+    if (!s->offsets && (s->key_offsets || s->sequences != 1)) return fail(SVOX_ERR_NULL_POINTER, "offsets is NULL");
+    if (s->offsets && !s->key_offsets && s->queries != s->keys)
+        return fail(SVOX_ERR_BAD_SHAPE, "without key_offsets there must be as many keys as queries, got %lld and %lld", (long long)s->keys, (long long)s->queries);
+    // (rows of a kv head are counted in 32 bits, and a launch has fewer than 2^24 blocks of 32 of them and more)
+    const int64_t most = INT32_MAX - 1024, rows = s->heads / s->kv_heads;
+    if (s->keys > most || s->queries > most / rows) return fail(SVOX_ERR_UNSUPPORTED, "queries * heads / kv_heads and keys must be < 2^31 - 2^10");
+    if ((svox_decoder::pieces(s->queries * rows, 128) + 1) * s->kv_heads >= 1 << 24 || (svox_decoder::pieces(s->keys, 128) + 1) * s->kv_heads >= 1 << 24)
+        return fail(SVOX_ERR_UNSUPPORTED, "queries * heads and keys * kv_heads must be < 2^31");
+    SVOX_TRY(check_heads("q", s->q, s->queries, s->heads, s->q_stride, s->q_head));
+    SVOX_TRY(check_heads("k", s->k, s->keys, s->kv_heads, s->k_stride, s->k_head));
+    return check_heads("v", s->v, s->keys, s->kv_heads, s->v_stride, s->v_head);
+}
+// the kernels of a call's type and width
+#define SVOX_BY_TYPE_AND_WIDTH(s, ...)                              \
+    SVOX_BY_TYPE((s).dtype, switch (attend_width((s).dim)) {        \
+        case 32: { constexpr int width = 32; __VA_ARGS__; }         \
+        case 64: { constexpr int width = 64; __VA_ARGS__; }         \
+        default: { constexpr int width = 128; __VA_ARGS__; }        \
+    })
+
 // a gradient summed over no rows
 __global__ void zero_kernel(uint16_t* at, int64_t count) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) at[i] = 0;
@@ -170,4 +201,27 @@ SVOX_API int svox_rotate_heads_backward(const SvoxRotateHeads* spec, const void*
     SVOX_TRY(check_space(workspace, workspace_bytes, rotate_space(*spec, weights)));
     SVOX_BY_TYPE(spec->dtype, return launch_rotate_backward<T>(*spec, grad_q, grad_k, grad, out_q, out_k, out_q_weight, out_k_weight,
                                                                weights ? (float*)workspace : nullptr, (hipStream_t)stream));
+}
+
+SVOX_API int64_t svox_attention_workspace_bytes(const SvoxAttention* spec, int32_t backward) {
+    SVOX_TRY(check_attention(spec));
+    return attention_space(*spec, backward != 0);
+}
+
+SVOX_API int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    SVOX_TRY(check_attention(spec));
+    if (spec->queries == 0) return SVOX_OK;
+    if (!out) return fail(SVOX_ERR_NULL_POINTER, "out is NULL");
+    SVOX_TRY(check_space(workspace, workspace_bytes, attention_space(*spec, false)));
+    SVOX_BY_TYPE_AND_WIDTH(*spec, return (launch_attention<T, width>(*spec, out, lse, workspace, (hipStream_t)stream)));
+}
+
+SVOX_API int svox_attention_backward(const SvoxAttention* spec, const SvoxAttentionGrads* grads, void* workspace, int64_t workspace_bytes, void* stream) {
+    SVOX_TRY(check_attention(spec));
+    if (!grads) return fail(SVOX_ERR_NULL_POINTER, "grads is NULL");
+    if (!grads->q && !grads->k && !grads->v) return SVOX_OK;
+    SVOX_TRY(check_heads("grad", grads->grad, spec->queries, spec->heads, grads->grad_stride, grads->grad_head));
+    if (spec->queries > 0 && (!grads->out || !grads->lse)) return fail(SVOX_ERR_NULL_POINTER, "out or lse is NULL");
+    SVOX_TRY(check_space(workspace, workspace_bytes, attention_space(*spec, true)));
+    SVOX_BY_TYPE_AND_WIDTH(*spec, return (launch_attention_backward<T, width>(*spec, *grads, workspace, (hipStream_t)stream)));
 }

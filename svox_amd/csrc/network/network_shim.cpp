@@ -11,7 +11,8 @@ namespace {
 
 #define SVOX_CALLS(X)                                                                           \
     X(svox_network_last_error) X(svox_clip_norm) X(svox_clip_norm_workspace_bytes)              \
-    X(svox_rotate_heads) X(svox_rotate_heads_backward) X(svox_rotate_heads_workspace_bytes)
+    X(svox_rotate_heads) X(svox_rotate_heads_backward) X(svox_rotate_heads_workspace_bytes)     \
+    X(svox_attention) X(svox_attention_backward) X(svox_attention_workspace_bytes)
 SVOX_LIBRARY
 
 int64_t status(int64_t rc, const char* name) {
@@ -267,11 +268,148 @@ std::pair<Tensor, Tensor> rotate_heads(Heads h) {
     return y;
 }
 
+// ---- attention
+constexpr double kDefaultScale = -HUGE_VAL;   // 1 / sqrt(numbers of a head)
+struct Attend {
+    Tensor q, k, v, offsets, key_offsets;
+    bool causal = false;
+    double scale = 0.0;
+};
+SvoxAttention attention_spec(const Attend& a) {
+    SvoxAttention s{};
+    s.q = a.q.data_ptr(), s.k = a.k.data_ptr(), s.v = a.v.data_ptr();
+    s.offsets = at_or_null(a.offsets);
+    s.key_offsets = at_or_null(a.key_offsets);
+    s.queries = a.q.size(0);
+    s.keys = a.k.size(0);
+    s.sequences = a.offsets.defined() ? a.offsets.numel() - 1 : 1;
+    s.q_stride = a.q.stride(0), s.q_head = a.q.stride(1);
+    s.k_stride = a.k.stride(0), s.k_head = a.k.stride(1);
+    s.v_stride = a.v.stride(0), s.v_head = a.v.stride(1);
+    s.heads = (int32_t)a.q.size(1);
+    s.kv_heads = (int32_t)a.k.size(1);
+    s.dim = (int32_t)a.q.size(2);
+    s.dtype = dtype_code(a.q, "q");
+    s.wide_offsets = a.offsets.defined() && a.offsets.scalar_type() == at::kLong;
+    s.causal = a.causal;
+    s.scale = (float)a.scale;
+    return s;
+}
+Attend dense_heads(Attend a) {
+    a.q = heads_of(a.q), a.k = heads_of(a.k), a.v = heads_of(a.v);
+    return a;
+}
+Tensor attention_forward(const Attend& a, Tensor* lse) {
+    const On on(a.q);
+    Tensor y = make_like(a.q);
+    if (lse) *lse = make({a.q.size(0) * a.q.size(1)}, at::kFloat, a.q);
+    const SvoxAttention s = attention_spec(a);
+    const int64_t bytes = status(lib.svox_attention_workspace_bytes(&s, 0), "attention");
+    const Tensor space = bytes_on(a.q, bytes);
+    status(lib.svox_attention(&s, y.data_ptr(), lse ? (float*)lse->data_ptr() : nullptr, at_or_null(space), bytes, on.stream), "attention");
+    return y;
+}
+
+struct AttendNode : torch::autograd::Node {
+    SavedVariable saved_[5], out_, lse_;   // q, k, v and the offsets
+    bool causal = false;
+    double scale = 0.0;
+
+    std::string name() const override { return "SvoxAttentionBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable& v : saved_) v.reset_data();
+        out_.reset_data();
+        lse_.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        once("attention", grads[0]);
+        Attend a{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), causal, scale};
+        const Tensor y = out_.unpack(shared_from_this()), lse = lse_.unpack();
+        const On on(a.q);
+        check_like(grads[0], a.q, "grad_output", "q");
+        a = dense_heads(a);
+        const Tensor dy = heads_of(grads[0]);
+        const SvoxAttention s = attention_spec(a);
+        const Tensor* const like[3] = {&a.q, &a.k, &a.v};
+        for (int i = 0; i < 3; ++i)
+            if (task_should_compute_output(i)) out[i] = make_like(*like[i]);
+        SvoxAttentionGrads g{};
+        g.out = y.data_ptr();
+        g.lse = (const float*)lse.data_ptr();
+        g.grad = dy.data_ptr();
+        g.grad_stride = dy.stride(0), g.grad_head = dy.stride(1);
+        g.q = at_or_null(out[0]), g.k = at_or_null(out[1]), g.v = at_or_null(out[2]);
+        const int64_t bytes = status(lib.svox_attention_workspace_bytes(&s, 1), "attention");
+        const Tensor space = bytes_on(a.q, bytes);
+        status(lib.svox_attention_backward(&s, &g, at_or_null(space), bytes, on.stream), "attention_backward");
+        return out;
+    }
+};
+
+void check_offsets(const Tensor& x, const Tensor& q, const char* name) {
+    if (!x.is_cuda() || x.device() != q.device() || x.layout() != at::kStrided) fail(std::string(name) + " must be a dense tensor on the device of q (" + q.device().str() + ")");
+    if (x.scalar_type() != at::kInt && x.scalar_type() != at::kLong) fail(std::string(name) + " must be an int32 or int64 tensor, got " + dtype_text(x.scalar_type()));
+    if (x.dim() != 1 || x.numel() < 2) fail(std::string(name) + " must have shape (sequences + 1,), got " + shape_text(x.sizes()));
+}
+
+Tensor attention(Attend a) {
+    no_tracing("attention");
+    const Tensor &q = a.q, &k = a.k, &v = a.v;
+    check_like(q, q, "q", "q");
+    dtype_code(q, "q");
+    check_like(k, q, "k", "q");
+    check_like(v, q, "v", "q");
+    check_3d(q, "q");
+    check_3d(k, "k");
+    check_shape(v, k.sizes(), "v");
+    if (k.size(2) != q.size(2)) fail("q and k must have the same numbers of a head, got " + shape_text(q.sizes()) + " and " + shape_text(k.sizes()));
+    const int64_t h = size32(q.size(1), "the number of heads"), g = size32(k.size(1), "the number of k's heads");
+    size32(q.size(2), "the numbers of a head");
+    if (h % g) fail("the number of heads must be a multiple of that of k's, got " + std::to_string(h) + " and " + std::to_string(g));
+    if (a.offsets.defined()) check_offsets(a.offsets, q, "offsets");
+    if (a.key_offsets.defined()) {
+        if (!a.offsets.defined()) fail("key_offsets need offsets");
+        check_offsets(a.key_offsets, q, "key_offsets");
+        if (a.key_offsets.numel() != a.offsets.numel() || a.key_offsets.scalar_type() != a.offsets.scalar_type())
+            fail("offsets and key_offsets must have the same shape and type, got " + shape_text(a.offsets.sizes()) + " " + dtype_text(a.offsets.scalar_type()) + " and " +
+                 shape_text(a.key_offsets.sizes()) + " " + dtype_text(a.key_offsets.scalar_type()));
+    } else if (a.offsets.defined() && q.size(0) != k.size(0)) {
+        fail("without key_offsets there must be as many keys as queries, got " + std::to_string(k.size(0)) + " and " + std::to_string(q.size(0)));
+    }
+    if (a.scale == kDefaultScale) a.scale = 1.0 / std::sqrt((double)q.size(2));
+    if (!(a.scale > 0.0) || std::isinf(a.scale)) fail("scale must be > 0 and finite, got " + std::to_string(a.scale));
+    make_contiguous(a.offsets);
+    make_contiguous(a.key_offsets);
+    if (!wants_node({&q, &k, &v}, "attention")) return attention_forward(dense_heads(a), nullptr);
+    const auto node = node_of<AttendNode>(q, k, v);
+    Tensor lse, y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView guard;
+        y = attention_forward(dense_heads(a), &lse);
+    }
+    const Tensor* const saved[5] = {&q, &k, &v, &a.offsets, &a.key_offsets};
+    for (int i = 0; i < 5; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
+    node->lse_ = SavedVariable(lse, false);
+    node->causal = a.causal;
+    node->scale = a.scale;
+    torch::autograd::set_history(y, node);
+    node->out_ = SavedVariable(y, true);
+    return y;
+}
+
 // ---- called from Python with positional arguments
 double number(PyObject* x) {
     const double v = PyFloat_AsDouble(x);
     if (v == -1.0 && PyErr_Occurred()) throw py::error_already_set();
     return v;
+}
+double scale_of(PyObject* x) {
+    const double v = number(x);
+    return v == kDefaultScale ? HUGE_VAL : v;   // (refused alike)
 }
 bool truth(PyObject* x) {
     const int v = PyObject_IsTrue(x);
@@ -329,7 +467,16 @@ PyObject* rotate_heads_py(PyObject*, PyObject* const* args, Py_ssize_t given) {
         return pair_of(THPVariable_Wrap(y.first), THPVariable_Wrap(y.second));
     });
 }
-PyMethodDef kCalls[] = {{"clip_norm", (PyCFunction)(void (*)())clip_norm_py, METH_FASTCALL, nullptr},
+PyObject* attention_py(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return call(given, 7, [&] {
+        const Attend a{tensor(args[0], "q"), tensor(args[1], "k"), tensor(args[2], "v"), tensor_or_none(args[3], "offsets"), tensor_or_none(args[4], "key_offsets"),
+                       truth(args[5]), args[6] == Py_None ? kDefaultScale : scale_of(args[6])};
+        const py::gil_scoped_release unlocked;
+        return attention(a);
+    });
+}
+PyMethodDef kCalls[] = {{"attention", (PyCFunction)(void (*)())attention_py, METH_FASTCALL, nullptr},
+                        {"clip_norm", (PyCFunction)(void (*)())clip_norm_py, METH_FASTCALL, nullptr},
                         {"clip_in_place", (PyCFunction)(void (*)())clip_in_place_py, METH_FASTCALL, nullptr},
                         {"rotate_heads", (PyCFunction)(void (*)())rotate_heads_py, METH_FASTCALL, nullptr},
                         {nullptr, nullptr, 0, nullptr}};

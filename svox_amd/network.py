@@ -1,11 +1,11 @@
-"""Operators of networks over the cells of a tree, beside those of the leaf decoder: heads of queries and keys rotated by their cells'
-positions, and the norm of many gradients together with its clipping.  Each is a few HIP kernels.  The reference has no such operators.
+"""Operators of networks over the cells of a tree, beside those of the leaf decoder: attention within packed sequences of cells, heads of
+queries and keys rotated by their cells' positions, and the norm of many gradients together with its clipping.  Each is a few HIP kernels.  The reference has no such operators.
 """
 import torch
 
 from .csrc import network as _N
 
-__all__ = ["rotate_heads", "clip_norm", "clip_grad_norm"]
+__all__ = ["attention", "rotate_heads", "clip_norm", "clip_grad_norm"]
 
 _native = None
 
@@ -15,6 +15,24 @@ def _calls():
     if _native is None:
         _native = _N.native()
     return _native
+
+
+def attention(q, k, v, offsets=None, key_offsets=None, causal=False, scale=None):
+    """softmax(scale q . k) v for every query, over the keys of its own sequence.
+
+    :param q: (T, H, D) float32, float16 or bfloat16, on a GPU, D up to 128; rows and heads may lie any distance apart
+    :param k, v: (S, G, D) of q's type; H a multiple of G, heads h of q go with head h // (H / G) of k and v
+    :param offsets: (sequences + 1,) int32 or int64 on the GPU: sequence s holds rows offsets[s] to offsets[s + 1] - 1 of q; None: one of all
+    :param key_offsets: the same of k and v; None: they are packed as q is
+    :param causal: a query sees the keys up to its own place, counted from the ends of its sequence's queries and keys
+    :param scale: > 0; None: 1 / sqrt(D)
+    :return: (T, H, D), differentiable once with respect to q, k and v; 0 for rows that see no key or belong to no sequence
+
+    Scores, their exponentials and all sums are held in 32 bits; 16-bit types round exponentials and the gradients of scores once, as operands of
+    the next product.  The same call gives the same bits.  Rows that a query does not see have no influence on it, whatever they hold.  The
+    offsets are read on the GPU: nothing waits for it.
+    """
+    return (_native or _calls()).attention(q, k, v, offsets, key_offsets, causal, scale)
 
 
 def rotate_heads(q, k, positions, frequencies, q_weight=None, k_weight=None, interleaved=False, eps=1e-6):

@@ -10,11 +10,12 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import svox_amd as svox
-from network_reference import clip_norm, rotate_heads
+from network_reference import attention, clip_norm, rotate_heads
 from svox_amd.csrc import network as N
 
 HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "svox_network.h")
-STRUCTS = {"SvoxClipTensor": N.ClipTensorC, "SvoxRotateHeads": N.RotateHeadsC}
+STRUCTS = {"SvoxClipTensor": N.ClipTensorC, "SvoxRotateHeads": N.RotateHeadsC, "SvoxAttention": N.AttentionC,
+           "SvoxAttentionGrads": N.AttentionGradsC}
 
 
 def test_header_library_and_mirror_agree():
@@ -92,7 +93,44 @@ def test_argument_errors_of_rotate_heads_come_before_anything_touches_a_device()
     assert lib.svox_rotate_heads_backward(spec(), 16, 16, grad, None, None, None, None, None, 0, None) == 0
 
 
-CALLS = {"rotate_heads": lambda x: svox.rotate_heads(x, x, torch.zeros(3), torch.zeros(4))[0], "clip_norm": lambda x: svox.clip_norm([x], 1.0)[0]}
+def test_argument_errors_of_attention_come_before_anything_touches_a_device():
+    lib = N.load_library()
+
+    def spec(**kw):
+        return with_fields(N.AttentionC(q=16, k=16, v=16, queries=5, keys=7, sequences=1, q_stride=32, q_head=8, k_stride=16, k_head=8, v_stride=16, v_head=8,
+                                        heads=4, kv_heads=2, dim=8, scale=0.5), kw)
+
+    def grads(**kw):
+        return with_fields(N.AttentionGradsC(out=16, lse=16, grad=16, grad_stride=32, grad_head=8, q=16, k=16, v=16), kw)
+
+    assert lib.svox_attention(None, 16, None, 16, 1 << 20, None) == -1
+    for kw, rc in [({"dtype": 3}, -3), ({"queries": -1}, -2), ({"keys": -1}, -2), ({"heads": 0}, -2), ({"kv_heads": 0}, -2), ({"heads": 5}, -2), ({"dim": 0}, -2),
+                   ({"dim": 129}, -4), ({"scale": 0.0}, -2), ({"scale": -1.0}, -2), ({"scale": math.nan}, -2), ({"scale": math.inf}, -2), ({"sequences": 0}, -2),
+                   ({"sequences": 2}, -1), ({"key_offsets": 16}, -1), ({"offsets": 16}, -2), ({"q": None}, -1), ({"k": None}, -1), ({"v": None}, -1),
+                   ({"queries": 1 << 30, "offsets": 16, "key_offsets": 16}, -4), ({"keys": 1 << 31}, -4), ({"heads": 1 << 20, "queries": 1 << 11}, -4),
+                   ({"q_stride": -1}, -2), ({"v_head": -8}, -2), ({"k_stride": 1 << 45}, -2)]:
+        assert lib.svox_attention(spec(**kw), 16, None, 16, 1 << 40, None) == rc, kw
+        assert lib.svox_attention_backward(spec(**kw), grads(), 16, 1 << 40, None) == rc, kw
+        assert lib.svox_network_last_error()
+    assert lib.svox_attention(spec(), None, None, 16, 1 << 20, None) == -1
+    assert lib.svox_attention(spec(queries=0, q=None), None, None, None, 0, None) == 0
+    long = spec(keys=100000)
+    least = lib.svox_attention_workspace_bytes(long, 0)
+    assert least > 0 and lib.svox_attention_workspace_bytes(spec(), 0) == 0
+    assert lib.svox_attention(long, 16, None, None, least, None) == -1
+    assert lib.svox_attention(long, 16, None, 16, least - 1, None) == -2
+    assert lib.svox_attention(long, 16, None, 8, least, None) == -2
+    least = lib.svox_attention_workspace_bytes(spec(), 1)
+    assert least > 0
+    assert lib.svox_attention_backward(spec(), None, 16, least, None) == -1
+    for kw, rc in [({"grad": None}, -1), ({"out": None}, -1), ({"lse": None}, -1), ({"grad_stride": -1}, -2)]:
+        assert lib.svox_attention_backward(spec(), grads(**kw), 16, least, None) == rc, kw
+    assert lib.svox_attention_backward(spec(), grads(), 16, least - 1, None) == -2
+    assert lib.svox_attention_backward(spec(), grads(q=None, k=None, v=None), None, 0, None) == 0
+
+
+CALLS = {"rotate_heads": lambda x: svox.rotate_heads(x, x, torch.zeros(3), torch.zeros(4))[0], "clip_norm": lambda x: svox.clip_norm([x], 1.0)[0],
+         "attention": lambda x: svox.attention(x, x, x)}
 
 
 @pytest.mark.parametrize("name", list(CALLS))
@@ -104,6 +142,14 @@ def test_there_is_no_cpu_path_and_no_tracing(name):
         torch.jit.trace(call, (x,), check_trace=False)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(call)(x)
+
+
+def test_what_is_no_tensor():
+    x = torch.zeros(3, 2, 8)
+    for call in (lambda: svox.attention(None, x, x), lambda: svox.attention(x, x, x, [0, 3]), lambda: svox.rotate_heads(x, x, [0, 1, 2], x), lambda: svox.clip_norm([1.0], 1.0),
+                 lambda: svox.attention(x, x, x, scale="1")):
+        with pytest.raises(TypeError):
+            call()
 
 
 def test_gradients_that_are_not_there():
@@ -145,3 +191,24 @@ def test_the_bounds_hold_for_torch_and_see_a_mistake(dtype, interleaved):
     near, (scaled,) = clip_norm([x], 2.0)
     sees_a_mistake(near, norm)
     sees_a_mistake(scaled, (x.float() * (2.0 / norm)).to(dtype))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_the_bounds_of_attention_hold_for_torch_and_see_a_mistake(dtype, causal):
+    g = torch.Generator().manual_seed(1)
+    q, k, v, grad = (torch.randn(*s, generator=g).to(dtype) for s in ((20, 4, 24), (30, 2, 24), (30, 2, 24), (20, 4, 24)))
+    want, wanted = attention(q, k, v, [0, 12, 20], [0, 9, 30], causal=causal, grad=grad)
+    f = [x.float().requires_grad_() for x in (q, k, v)]
+    parts = []
+    for q0, q1, k0, k1 in ((0, 12, 0, 9), (12, 20, 9, 30)):
+        qq, kk, vv = (x.transpose(0, 1) for x in (f[0][q0:q1], f[1][k0:k1].repeat_interleave(2, 1), f[2][k0:k1].repeat_interleave(2, 1)))
+        s = qq @ kk.transpose(1, 2) * 24 ** -0.5
+        hidden = (torch.arange(k1 - k0) - torch.arange(q1 - q0)[:, None] > (k1 - k0) - (q1 - q0)) & causal
+        empty = hidden.all(1, keepdim=True)
+        p = torch.softmax(s.masked_fill(hidden & ~empty, float("-inf")), -1).masked_fill(empty, 0.0)
+        parts.append((p @ vv).transpose(0, 1))
+    y = torch.cat(parts)
+    sees_a_mistake(want, y.to(dtype))
+    for name, got in zip("qkv", torch.autograd.grad(y, f, grad.float())):
+        sees_a_mistake(wanted[name], got.to(dtype))
