@@ -2,13 +2,16 @@
 
 A tree may hold any numbers (`N3Tree(data_format=None, data_dim=D)`); what the renderer reads are records of basis
 coefficients and density.  `LeafDecoder` makes the one from the other with two operators, `layer_norm` and `gated_ffn`, each a
-few HIP kernels with its gradient; the gradient of the records that a rendering leaves goes back through it to the network's
+few HIP kernels with its gradient, and, where cells are to see their neighbours, with those of `svox_amd.network`; the gradient of the records that a rendering leaves goes back through it to the network's
 weights and to the features.  The reference has no such operators.
 """
+import math
+
 import torch
 from torch import nn
 
 from .csrc import decoder as _D
+from .network import attention, clip_grad_norm, rotate_heads
 
 __all__ = ["layer_norm", "gated_ffn", "LeafDecoder"]
 
@@ -84,6 +87,31 @@ class _Ffn(nn.Module):
                          activation=self.activation)
 
 
+class _Attend(nn.Module):
+    def __init__(self, features, heads, kv_heads, eps, **kw):
+        super().__init__()
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, features // heads
+        self.norm = _Norm(features, eps, **kw)
+        self.w_qkv = nn.Parameter(torch.randn((heads + 2 * kv_heads) * self.dim, features, **kw) * features ** -0.5)
+        self.w_out = nn.Parameter(torch.randn(features, features, **kw) * features ** -0.5)
+        self.q_weight = nn.Parameter(torch.ones(self.dim, **kw))
+        self.k_weight = nn.Parameter(torch.ones(self.dim, **kw))
+
+    def forward(self, x, positions, frequencies, offsets):
+        wide, narrow = self.heads * self.dim, self.kv_heads * self.dim
+        q, k, v = nn.functional.linear(self.norm(x), self.w_qkv).split([wide, narrow, narrow], dim=1)
+        heads = lambda t: t.unflatten(1, (-1, self.dim))  # noqa: E731
+        q, k = rotate_heads(heads(q), heads(k), positions, frequencies, self.q_weight, self.k_weight)
+        return torch.addmm(x, attention(q, k, heads(v), offsets).flatten(1), self.w_out.t())
+
+
+def _cell_centres(tree):
+    """(cells, 3) float32, the centres of all cells of the tree's nodes in tree coordinates."""
+    at = tree._unpack_index(torch.arange(tree._structure().nodes * tree.N ** 3, device=tree.data.device))
+    depth = tree.parent_depth[:, 1].to(at.device)[at[:, 0]]
+    return tree._calc_corners(at).float() + 0.5 * float(tree.N) ** -(depth + 1.0)[:, None]
+
+
 def _cells(data, tree):
     """The cells of the tree's nodes in `data`, without its spare capacity."""
     nodes = tree._structure().nodes
@@ -91,7 +119,8 @@ def _cells(data, tree):
 
 
 class LeafDecoder(nn.Module):
-    """Features of a leaf to its record: `depth` blocks x + ffn(norm(x)) over the features, then ffn(norm(x)) to the record.
+    """Features of a leaf to its record: `depth` blocks x + ffn(norm(x)) over the features, then ffn(norm(x)) to the record.  With `heads`, each
+    block begins with x + attention among the cells of a window, of queries and keys that are rotated by the cells' centres.
 
     A decoder that is trained through a renderer, with the features of every leaf:
 
@@ -108,9 +137,13 @@ class LeafDecoder(nn.Module):
     :param features: numbers of a leaf's features
     :param record: numbers of a record (`tree.data_dim`)
     :param hidden: hidden units of every block (default: four for each feature)
+    :param heads: heads of the attention in every block; 0: cells are decoded by themselves
+    :param kv_heads: heads of its keys and values (default: as many)
+    :param window: cells of a window: consecutive ones, which lie near one another in space, as a node's children follow one another
     """
 
-    def __init__(self, features, record, hidden=None, depth=1, activation="silu", eps=1e-5, device=None, dtype=torch.float32):
+    def __init__(self, features, record, hidden=None, depth=1, activation="silu", eps=1e-5, device=None, dtype=torch.float32, heads=0, kv_heads=None,
+                 window=512):
         super().__init__()
         if activation not in _D.ACTIVATIONS:
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(_D.ACTIVATIONS)}")
@@ -119,13 +152,43 @@ class LeafDecoder(nn.Module):
         self.norms = nn.ModuleList(_Norm(features, eps, **kw) for _ in range(depth + 1))
         self.ffns = nn.ModuleList([_Ffn(features, hidden, features, activation, **kw) for _ in range(depth)]
                                   + [_Ffn(features, hidden, record, activation, **kw)])
+        self.window = window
+        if heads:
+            kv_heads = heads if kv_heads is None else kv_heads
+            if heads < 0 or kv_heads < 1 or features % heads or heads % kv_heads or window < 1:
+                raise ValueError(f"{features} features do not make {heads} heads for {kv_heads} heads of keys, or a window of {window} cells is none")
+            self.attends = nn.ModuleList(_Attend(features, heads, kv_heads, eps, **kw) for _ in range(depth))
+            # pairs of a head take turns among the three axes, from one turn over the tree to 2^8 (kept as whole numbers, whose type stays
+            # where a module's is changed)
+            pairs = torch.arange(features // heads // 2)
+            waves = 2 * math.pi * 2.0 ** (8.0 * (pairs // 3) / max(1, (len(pairs) + 2) // 3 - 1))
+            frequencies = torch.where(pairs % 3 == torch.arange(3)[:, None], waves, torch.zeros(())).float()
+            self.register_buffer("frequencies", frequencies.to(device).view(torch.int32), persistent=False)
 
-    def forward(self, x):
-        """(..., features) to (..., record), in the type of the weights."""
+    def forward(self, x, positions=None, offsets=None):
+        """(..., features) to (..., record), in the type of the weights.
+
+        :param positions: (rows, 3), of a decoder with heads: where the cells are, in tree coordinates
+        :param offsets: where the windows of a decoder with heads begin and end, as of `attention` (default: every `window` rows)
+        """
         x = x.to(self.norms[0].weight.dtype)
-        for norm, ffn in zip(self.norms[:-1], self.ffns[:-1]):
+        shape = x.shape
+        if self._attends():
+            if positions is None:
+                raise ValueError("a decoder with heads needs the positions of the cells")
+            x = x.reshape(-1, shape[-1])
+            if offsets is None:
+                rows = x.shape[0]
+                offsets = torch.arange(0, rows + self.window, self.window, device=x.device).clamp_(max=rows) if rows else None
+        for i, (norm, ffn) in enumerate(zip(self.norms[:-1], self.ffns[:-1])):
+            if self._attends():
+                x = self.attends[i](x, positions, self.frequencies.view(torch.float32), offsets)
             x = ffn(norm(x), residual=x)
-        return self.ffns[-1](self.norms[-1](x))
+        y = self.ffns[-1](self.norms[-1](x))
+        return y.reshape(*shape[:-1], y.shape[-1]) if self._attends() else y
+
+    def _attends(self):
+        return hasattr(self, "attends")
 
     def decode_tree(self, features, tree):
         """Writes the records of the features in the tree `features` into `tree`, a tree of the same structure (the same nodes, the
@@ -134,18 +197,20 @@ class LeafDecoder(nn.Module):
         if not features._divided_like(tree):
             raise ValueError("features and tree must have the same structure")
         source = _cells(features.data, features)
-        records = self(source.reshape(-1, features.data_dim))
+        rows = source.reshape(-1, features.data_dim)
+        records = self(rows, _cell_centres(features)) if self._attends() else self(rows)
         if records.shape[1] != tree.data_dim:
             raise ValueError(f"the decoder makes records of {records.shape[1]} numbers, the tree's have {tree.data_dim}")
         with torch.no_grad():
             _cells(tree.data, tree).copy_(records.view(*source.shape[:-1], -1))
         return records
 
-    def backward_through(self, features, tree, loss):
+    def backward_through(self, features, tree, loss, max_norm=None):
         """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
         adds the gradients of what it returns to those of the decoder's weights and of `features.data`, and to those of whatever else
         it was made of.  Returns the loss.  The records' gradient takes the decoder's type: in float16 what is below 2^-25 becomes zero,
-        so scale the loss there.  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
+        so scale the loss there.  With `max_norm` the gradients of the weights and of `features.data`, as they then stand, are clipped together
+        (`clip_grad_norm`).  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
         holds stays as it is.)"""
         if not (tree.data.requires_grad and tree.data.is_leaf):
             raise ValueError("tree.data does not require a gradient, or is computed from something else: that of the records has to come through it")
@@ -159,4 +224,6 @@ class LeafDecoder(nn.Module):
             tree.data.grad = kept
         if grad is not None and records.requires_grad:    # (None: the loss does not depend on the records)
             records.backward(_cells(grad, tree).reshape(records.shape).to(records.dtype))
+        if max_norm is not None:
+            clip_grad_norm([features.data, *self.parameters()], max_norm)
         return value.detach()

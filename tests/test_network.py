@@ -212,3 +212,24 @@ def test_the_bounds_of_attention_hold_for_torch_and_see_a_mistake(dtype, causal)
     sees_a_mistake(want, y.to(dtype))
     for name, got in zip("qkv", torch.autograd.grad(y, f, grad.float())):
         sees_a_mistake(wanted[name], got.to(dtype))
+
+
+def test_a_decoder_with_heads_is_a_module_like_others(tmp_path):
+    plain = svox.LeafDecoder(24, 4)
+    assert not any("attend" in n or "frequencies" in n for n in plain.state_dict())
+    decoder = svox.LeafDecoder(24, 4, depth=2, heads=4, kv_heads=2)
+    assert [tuple(p.shape) for p in decoder.attends[1].parameters()] == [(48, 24), (24, 24), (6,), (6,), (24,), (24,)]
+    assert "frequencies" not in decoder.state_dict() and set(plain.state_dict()) < set(decoder.state_dict())
+    torch.save(decoder.state_dict(), tmp_path / "decoder.pt")
+    other = svox.LeafDecoder(24, 4, depth=2, heads=4, kv_heads=2)
+    other.load_state_dict(torch.load(tmp_path / "decoder.pt", weights_only=True))
+    frequencies = decoder.frequencies.view(torch.float32)
+    assert frequencies.shape == (3, 3) and torch.equal(frequencies, torch.eye(3) * 2 * math.pi)
+    assert torch.equal(decoder.half().frequencies.view(torch.float32), frequencies) and decoder.attends[0].w_qkv.dtype == torch.float16
+    wide = svox.LeafDecoder(64, 4, heads=1).frequencies.view(torch.float32)
+    assert wide.shape == (3, 32) and wide.max() == wide[1, 31] == torch.tensor(2 * math.pi * 256) and (wide != 0).sum() == 32
+    for kw in ({"heads": 5}, {"heads": 4, "kv_heads": 3}, {"heads": -1}, {"heads": 4, "kv_heads": 0}, {"heads": 4, "window": 0}):
+        with pytest.raises(ValueError):
+            svox.LeafDecoder(24, 4, **kw)
+    with pytest.raises(ValueError, match="positions"):
+        decoder(torch.zeros(5, 24))
