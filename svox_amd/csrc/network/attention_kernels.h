@@ -116,11 +116,11 @@ template <class T, int DP, int N, int across>
 struct ForwardShape {
     static constexpr int down = 4 / across, rows = down * 32 * N;
     static constexpr int keys = across == 4 ? 128 : (sizeof(T) == 4 && DP == 128 ? 32 : 64), mine = keys / across, blocks = mine / 32;
-    static constexpr int stages = across == 4 ? 1 : 2;   // tiles in LDS
+    static constexpr int stages = across == 4 && sizeof(T) == 4 && DP == 128 ? 1 : 2;   // tiles in LDS
     static constexpr int tile = keys * DP;
 };
 
-template <class T, int DP, int N, int across, bool whole>
+template <class T, int DP, int N, int across, bool direct>
 __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_kernel(AttendArgs<T> p) {
     using S = ForwardShape<T, DP, N, across>;
     using F = Frag<T>;
@@ -129,14 +129,14 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     constexpr int join_numbers = across > 1 ? 4 * 32 * (DP + 2) : 0;   // floats
     constexpr int tile_bytes = 2 * S::stages * S::tile * (int)sizeof(T), join_bytes = join_numbers * 4;
     __shared__ __attribute__((aligned(16))) char lds[tile_bytes > join_bytes ? tile_bytes : join_bytes];
-    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    __shared__ int room[16];
+    __shared__ unsigned kinds[3][S::keys][DB];   // NaN, inf and -inf that were taken out of a tile of v
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
     const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32 * N;
 
     Span see[N];
     const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + S::rows, p.rows) - 1, see);
-    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
     const Spans block = spans_of_block(spans, room);
     const Span part = part_of(block, S::keys, place.split, p.splits);
     clip(see, part);
@@ -144,43 +144,45 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     Eight q[N][DP / 16];
 #pragma unroll
     for (int n = 0; n < N; ++n)
-        load_row<T, DP, whole>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
+        load_row<T, DP>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
 
     const float to2 = p.scale * kLog2E;
     f32x16 acc[N][DB];
     float m[N], l[N];
     T* const tiles = reinterpret_cast<T*>(lds);
-    const T* const k = p.k + place.head * p.k_head;
-    const T* const v = p.v + place.head * p.v_head;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         m[n] = -__builtin_inff(), l[n] = 0.0f;
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[n][db] = f32x16{};
     }
-    Stage<T, DP, S::keys, whole> ks, vs;
-    const auto load = [&](int k0) {
-        const int last = part.high - 1 - k0;
-        ks.load([&](int row) { return k + (k0 + (int64_t)row) * p.k_stride; }, last, p.dim);
-        vs.load([&](int row) { return v + (k0 + (int64_t)row) * p.v_stride; }, last, p.dim);
+    Loader<T, DP, S::keys, direct> ks(p.k + place.head * p.k_head, p.k_stride, 0, 1, p.dim), vs(p.v + place.head * p.v_head, p.v_stride, 0, 1, p.dim);
+    const auto load = [&](int k0, int stage) {
+        ks.load(k0, part.high - k0, tiles + stage * 2 * S::tile);
+        vs.load(k0, part.high - k0, tiles + (stage * 2 + 1) * S::tile);
     };
-    const auto store = [&](int stage, int k0) {
-        ks.store(tiles + stage * 2 * S::tile);
-        vs.store(tiles + (stage * 2 + 1) * S::tile);
-        if (block.masks(k0, S::keys) && vs.odd()) odd[stage] = k0;
-    };
-    __syncthreads();
-    if (part.low < part.high) {
-        load(part.low);
-        store(0, part.low);
+    const auto finish = [&](int stage) {
+        ks.finish(tiles + stage * 2 * S::tile);
+        vs.finish(tiles + (stage * 2 + 1) * S::tile);
         __syncthreads();
+    };
+    if (part.low < part.high) {
+        load(part.low, 0);
+        finish(0);
     }
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += S::keys) {
         const bool more = k0 + S::keys < part.high;
-        if (more) load(k0 + S::keys);
+        if (more && S::stages == 2) load(k0 + S::keys, stage ^ 1);
         const T* const kt = tiles + stage * 2 * S::tile;
         const T* const vt = kt + S::tile;
+        bool odd = false;
+        if (block.masks(k0, S::keys)) {
+            for (int i = (int)threadIdx.x; i < 3 * S::keys * DB; i += kAttendThreads) (&kinds[0][0][0])[i] = 0;
+            odd = take_out_odd<T, DP, S::keys>(tiles + (stage * 2 + 1) * S::tile, [&](int row, int column, float x) {
+                atomicOr(&kinds[x != x ? 0 : x > 0.0f ? 1 : 2][row][column / 32], 1u << column % 32);
+            });
+        }
         const int kw = k0 + wave % across * S::mine;   // this wavefront's keys
         if (kw < spans.high && kw + S::mine > spans.low && kw < part.high) {
             f32x16 s[KB][N];
@@ -243,18 +245,35 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int at = wave % across * S::mine + 32 * b + 16 * c;
-                    if (mask && odd[stage] == k0) accumulate_odd<T, DP, true>(acc, vt, at, e[b][c], see, k0 + at);
-                    else accumulate<T, DP, N>(acc, vt, at, e[b][c]);
+                    accumulate<T, DP, N>(acc, vt, at, e[b][c]);
                 }
+            if (odd) {
+                // (v's numbers that were taken out, for the lanes that see them: p is positive)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int kind = 0; kind < 3; ++kind) {
+                        unsigned which[DB] = {};
+#pragma unroll 1
+                        for (int i = wave % across * S::mine; i < (wave % across + 1) * S::mine; ++i)
+                            if (k0 + i >= see[n].low && k0 + i < see[n].high)
+#pragma unroll
+                                for (int db = 0; db < DB; ++db) which[db] |= kinds[kind][i][db];
+                        const float odd_one = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+#pragma unroll
+                        for (int db = 0; db < DB; ++db)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (which[db] >> (row_of(r) + 4 * h) & 1) acc[n][db][r] += odd_one;
+                    }
+            }
         }
         if constexpr (S::stages == 2) {
-            if (more) store(stage ^ 1, k0 + S::keys);
             stage ^= 1;
-            __syncthreads();
+            if (more) finish(stage);
         } else {
             __syncthreads();
-            if (more) store(0, k0 + S::keys);
-            __syncthreads();
+            if (more) load(k0 + S::keys, 0), finish(0);
         }
     }
 
@@ -263,6 +282,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     if constexpr (across > 1) {
         // the wavefronts' sums, joined by the first: every lane finds its own numbers of the others
         static_assert(across == 4 && N == 1, "all wavefronts share rows");
+        __syncthreads();
         float* const shared = reinterpret_cast<float*>(lds);
         const int lane = (int)threadIdx.x % kWave;
         constexpr int each = DB * 16 * kWave;   // numbers of a wavefront, then its maxima and sums
@@ -382,57 +402,58 @@ __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs
 }
 
 // ---- dq: rows as forward, through the keys they see
-template <class T, int DP, bool whole>
+template <class T, int DP, bool direct>
 __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_query_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
-    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    __shared__ int room[16];
+    __shared__ unsigned bad[keys / 32];   // keys that are not finite
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
     const int r0 = place.tile * rows, mine = r0 + wave * 32, row = min(mine + (int)threadIdx.x % 32, p.rows - 1);
 
     Span see[1];
     const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + rows, p.rows) - 1, see);
-    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
     const Spans block = spans_of_block(spans, room);
     const Span part = part_of(block, keys, place.split, p.splits);
     clip(see, part);
 
     Eight q[DP / 16], g[DP / 16];
-    load_row<T, DP, whole>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
-    load_row<T, DP, whole>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
+    load_row<T, DP>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
+    load_row<T, DP>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
     const float lse = p.lse[(int64_t)place.head * p.rows + row], delta = p.delta[(int64_t)place.head * p.rows + row];
     const float to2 = p.scale * kLog2E;
-    const T* const k = p.k + place.head * p.k_head;
-    const T* const v = p.v + place.head * p.v_head;
     f32x16 acc[1][DB];
+    float none = 0.0f;
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
-    Stage<T, DP, keys, whole> ks, vs;
-    const auto load = [&](int k0) {
-        const int last = part.high - 1 - k0;
-        ks.load([&](int row) { return k + (k0 + (int64_t)row) * p.k_stride; }, last, p.dim);
-        vs.load([&](int row) { return v + (k0 + (int64_t)row) * p.v_stride; }, last, p.dim);
+    Loader<T, DP, keys, direct> ks(p.k + place.head * p.k_head, p.k_stride, 0, 1, p.dim), vs(p.v + place.head * p.v_head, p.v_stride, 0, 1, p.dim);
+    const auto load = [&](int k0, int stage) {
+        ks.load(k0, part.high - k0, tiles + stage * 2 * tile);
+        vs.load(k0, part.high - k0, tiles + (stage * 2 + 1) * tile);
     };
-    const auto store = [&](int stage, int k0) {
-        ks.store(tiles + stage * 2 * tile);
-        vs.store(tiles + (stage * 2 + 1) * tile);
-        if (block.masks(k0, keys) && ks.odd()) odd[stage] = k0;
-    };
-    __syncthreads();
-    if (part.low < part.high) {
-        load(part.low);
-        store(0, part.low);
+    const auto finish = [&](int stage) {
+        ks.finish(tiles + stage * 2 * tile);
+        vs.finish(tiles + (stage * 2 + 1) * tile);
         __syncthreads();
+    };
+    if (part.low < part.high) {
+        load(part.low, 0);
+        finish(0);
     }
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += keys) {
         const bool more = k0 + keys < part.high;
-        if (more) load(k0 + keys);
+        if (more) load(k0 + keys, stage ^ 1);
         const T* const kt = tiles + stage * 2 * tile;
         const T* const vt = kt + tile;
+        bool odd = false;
+        if (block.masks(k0, keys)) {
+            if (threadIdx.x < keys / 32) bad[threadIdx.x] = 0;
+            odd = take_out_odd<T, DP, keys>(tiles + stage * 2 * tile, [&](int row, int, float) { atomicOr(&bad[row / 32], 1u << row % 32); });
+        }
         if (k0 < spans.high && k0 + keys > spans.low) {
             const bool mask = k0 < spans.all_low || k0 + keys > spans.all_high || k0 + keys > part.high;
 #pragma unroll
@@ -457,15 +478,18 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Eight e[1] = {F::pack(ds + 8 * c)};
-                    if (mask && odd[stage] == k0) accumulate_odd<T, DP, false>(acc, kt, 32 * b + 16 * c, e, see, k0 + 32 * b + 16 * c);
-                    else accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
+                    accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
                 }
             }
         }
-        if (more) store(stage ^ 1, k0 + keys);
+        if (odd)      // (whoever sees a key that is not finite has no gradient that is)
+            for (int i = 0; i < keys; ++i)
+                if ((bad[i / 32] >> i % 32 & 1) && k0 + i >= see[0].low && k0 + i < see[0].high) none = __builtin_nanf("");
         stage ^= 1;
-        __syncthreads();
+        if (more) finish(stage);
     }
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[0][db] += none;
     const int r = mine + (int)threadIdx.x % 32;
     if (r >= p.rows) return;
     if (p.splits > 1) {
@@ -477,63 +501,64 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 }
 
 // ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them
-template <class T, int DP, bool whole>
+template <class T, int DP, bool direct>
 __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
-    __shared__ int room[16], odd[2];   // odd: the tile of a stage that holds infinite numbers or NaN
+    __shared__ int room[16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
     const int j0 = place.tile * keys, mine = j0 + wave * 32, key = min(mine + (int)threadIdx.x % 32, p.keys - 1);
 
     Span see[1];
     const Spans spans = spans_of<1>(p.seq, false, mine, p.keys, p.group, j0, min(j0 + keys, p.keys) - 1, see);
-    if (threadIdx.x < 2) odd[threadIdx.x] = -1;
     const Spans block = spans_of_block(spans, room);
     const Span part = part_of(block, rows, place.split, p.splits);
     clip(see, part);
 
     Eight k[DP / 16], v[DP / 16];
-    load_row<T, DP, whole>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
-    load_row<T, DP, whole>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
+    load_row<T, DP>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
+    load_row<T, DP>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
     const float to2 = p.scale * kLog2E;
     const float* const lse = p.lse + (int64_t)place.head * p.rows;
     const float* const delta = p.delta + (int64_t)place.head * p.rows;
     f32x16 dk[1][DB], dv[1][DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) dk[0][db] = dv[0][db] = f32x16{};
-    Stage<T, DP, rows, whole> qs, gs;
+    Loader<T, DP, rows, direct> qs(p.q + (int64_t)place.head * p.group * p.q_head, p.q_stride, p.q_head, p.group, p.dim),
+        gs(p.grad + (int64_t)place.head * p.group * p.grad_head, p.grad_stride, p.grad_head, p.group, p.dim);
     float stat = 0.0f;
-    const auto load = [&](int i0) {
-        const int last = part.high - 1 - i0;
-        qs.load([&](int row) { return row_at(p.q, i0 + row, p.group, place.head, p.q_stride, p.q_head); }, last, p.dim);
-        gs.load([&](int row) { return row_at(p.grad, i0 + row, p.group, place.head, p.grad_stride, p.grad_head); }, last, p.dim);
+    const auto load = [&](int i0, int stage) {
         if ((int)threadIdx.x < 2 * rows) {
-            const int row = (int)threadIdx.x % rows, at = i0 + (row < last ? row : last);
+            const int at = min(i0 + (int)threadIdx.x % rows, part.high - 1);
             stat = (int)threadIdx.x < rows ? lse[at] : delta[at];
         }
+        qs.load(i0, part.high - i0, tiles + stage * 2 * tile);
+        gs.load(i0, part.high - i0, tiles + (stage * 2 + 1) * tile);
     };
-    const auto store = [&](int stage, int i0) {
-        qs.store(tiles + stage * 2 * tile);
-        gs.store(tiles + (stage * 2 + 1) * tile);
-        if (block.masks(i0, rows) && (qs.odd() || gs.odd())) odd[stage] = i0;
+    const auto finish = [&](int stage) {
+        qs.finish(tiles + stage * 2 * tile);
+        gs.finish(tiles + (stage * 2 + 1) * tile);
         if ((int)threadIdx.x < 2 * rows) shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
-    };
-    __syncthreads();
-    if (part.low < part.high) {
-        load(part.low);
-        store(0, part.low);
         __syncthreads();
+    };
+    if (part.low < part.high) {
+        load(part.low, 0);
+        finish(0);
     }
     int stage = 0;
     for (int i0 = part.low; i0 < part.high; i0 += rows) {
         const bool more = i0 + rows < part.high;
-        if (more) load(i0 + rows);
+        if (more) load(i0 + rows, stage ^ 1);
         const T* const qt = tiles + stage * 2 * tile;
         const T* const gt = qt + tile;
+        if (block.masks(i0, rows)) {
+            // (keys that see a row that is not finite have no gradient that is)
+            take_out_odd<T, DP, 2 * rows>(tiles + stage * 2 * tile, [&](int row, int, float) { shared[stage][0][row % rows] = __builtin_nanf(""); });
+        }
         if (i0 < spans.high && i0 + rows > spans.low) {
             const bool mask = i0 < spans.all_low || i0 + rows > spans.all_high || i0 + rows > part.high;
 #pragma unroll
@@ -568,19 +593,13 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
                 for (int c = 0; c < 2; ++c) {
                     const int at = 32 * b + 16 * c;
                     const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
-                    if (mask && odd[stage] == i0) {
-                        accumulate_odd<T, DP, true>(dv, gt, at, pe, see, i0 + at);
-                        accumulate_odd<T, DP, false>(dk, qt, at, pd, see, i0 + at);
-                    } else {
-                        accumulate<T, DP, 1>(dv, gt, at, pe);
-                        accumulate<T, DP, 1>(dk, qt, at, pd);
-                    }
+                    accumulate<T, DP, 1>(dv, gt, at, pe);
+                    accumulate<T, DP, 1>(dk, qt, at, pd);
                 }
             }
         }
-        if (more) store(stage ^ 1, i0 + rows);
         stage ^= 1;
-        __syncthreads();
+        if (more) finish(stage);
     }
     const int j = mine + (int)threadIdx.x % 32;
     if (j >= p.keys) return;

@@ -50,6 +50,20 @@ inline AttendPlan key_grad_plan(const SvoxAttention& s) {
     return {128, splits_for(blocks, likely_length(rows, s.sequences, 128, s.keys), 64), false};
 }
 
+// Whether tiles go from memory to LDS 16 bytes at a time: everything lies at whole numbers of 16 bytes, and no tile of up to 128 rows reaches
+// further than 32 bits count.
+inline bool direct_heads(const SvoxAttention& s, const void* x, int64_t stride, int64_t head, int64_t group) {
+    const int64_t size = s.dtype == SVOX_DECODER_F32 ? 4 : 2;
+    return (uintptr_t)x % 16 == 0 && s.dim * size % 16 == 0 && stride * size % 16 == 0 && head * size % 16 == 0 && 130 * stride + group * head < (int64_t)1 << 28;
+}
+inline bool direct_loads(const SvoxAttention& s) {
+    return direct_heads(s, s.q, s.q_stride, s.q_head, s.heads / s.kv_heads) && direct_heads(s, s.k, s.k_stride, s.k_head, 1) &&
+           direct_heads(s, s.v, s.v_stride, s.v_head, 1);
+}
+inline bool direct_loads(const SvoxAttention& s, const SvoxAttentionGrads& g) {
+    return direct_heads(s, g.grad, g.grad_stride, g.grad_head, s.heads / s.kv_heads);
+}
+
 // Whether the blocks of an XCD take tiles side by side: where many sequences share the keys out, so that one's stay in an XCD's cache.  The
 // tiles of few long ones differ in work where they are causal, and go round.
 inline bool in_runs(const SvoxAttention& s) { return s.sequences >= 16; }

@@ -6,7 +6,7 @@
 // As the order of a reduction is free as long as both operands have the same, those 16 numbers go into the next product as they lie in
 // the registers, eight to a fragment, and only the other operand is read in that order: no score passes through LDS.
 #pragma once
-#include "../decoder/common.h"
+#include "../decoder/tile.h"
 
 namespace svox_network {
 
@@ -104,56 +104,124 @@ struct Tile {
     }
 };
 
-// `rows` rows of memory on their way to a tile, through registers: the next tile's loads are in flight while this one is multiplied.
-// Rows from `last` on repeat it (whoever reads them knows that they are not there), numbers beyond a row are zeros.
-template <class T, int DP, int rows, bool whole>
-struct Stage {
-    using Shape = Tile<T, DP>;
-    static constexpr int each = rows * Shape::pieces / kAttendThreads;
-    static_assert(rows * Shape::pieces % kAttendThreads == 0, "as many pieces for every thread");
-    typename Few<T, Shape::V>::vector v[each];
+// `rows` rows of heads in memory on their way to a tile.  Row r of the tile is row `first` + r of what `group` heads of a token make up, the
+// token's rows side by side.  Rows from `left` on and numbers from `dim` on arrive as zeros.
+//
+// `direct`: from memory to LDS without a register, 16 bytes a lane, whose places follow one another there, so that it is the lane that takes
+// another piece of memory where pieces change places.  Everything lies at whole numbers of 16 bytes then.
+template <class T, int DP, int rows, bool direct>
+struct Loader;
 
-    template <class Row>
-    __device__ __forceinline__ void load(Row row_at, int last, int dim) {
+template <class T, int DP, int rows>
+struct Loader<T, DP, rows, true> {
+    using Shape = Tile<T, DP>;
+    static constexpr int V = Shape::V, each = rows * Shape::pieces / kAttendThreads;
+    static_assert(rows * Shape::pieces % kAttendThreads == 0, "as many pieces for every thread");
+    static constexpr unsigned range = 0x80000000u, outside = 0x80000000u;   // bytes: beyond the range the hardware delivers zeros
+    unsigned at[each];
+    const T* base;
+    int64_t stride, head_stride;
+    int group, dim;
+
+    __device__ __forceinline__ Loader(const T* x, int64_t stride_, int64_t head_stride_, int group_, int dim_)
+        : base(x), stride(stride_), head_stride(head_stride_), group(group_), dim(dim_) {
+        places(0);
+    }
+    __device__ __forceinline__ int row_of_load(int i) const { return (i * kAttendThreads + (int)threadIdx.x) / Shape::pieces; }
+    __device__ __forceinline__ void places(int first) {
+        const int begin = first % group;   // (0 but where a tile begins within a token)
 #pragma unroll
         for (int i = 0; i < each; ++i) {
-            const int piece = i * kAttendThreads + (int)threadIdx.x, row = piece / Shape::pieces, column = piece % Shape::pieces * Shape::V;
-            const T* const from = row_at(row < last ? row : last) + column;
-            if constexpr (whole) v[i] = load_few<T, Shape::V>(from);
-            else v[i] = load_some<T, Shape::V>(from, dim - column);
+            const int row = row_of_load(i), slot = (i * kAttendThreads + (int)threadIdx.x) % Shape::pieces;
+            const int column = (slot / Shape::ring * Shape::ring + ((slot % Shape::ring) ^ Shape::turn(row))) * V;
+            const int token = group == 1 ? row : (begin + row) / group, head = group == 1 ? 0 : (begin + row) % group;
+            at[i] = column < dim ? (unsigned)((token * stride + head * head_stride + column) * (int)sizeof(T)) : outside;
         }
     }
-    // whether one of this thread's numbers is infinite or NaN
-    __device__ __forceinline__ bool odd() const {
-        bool found = false;
+    __device__ __forceinline__ void load(int first, int left, T* lds) {
+        if (rows % group != 0) places(first);
+        const uint64_t from = (uint64_t)(base + first / group * stride);
+        const u32x4 buffer = {(unsigned)from, (unsigned)(from >> 32) & 0xffffu, range, 0x00020000u};
+        const int wave_first = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave * kWave);
+#pragma unroll
+        for (int i = 0; i < each; ++i)
+            load_to_lds(buffer, left >= rows || row_of_load(i) < left ? at[i] : outside, reinterpret_cast<u16*>(lds + (i * kAttendThreads + wave_first) * V));
+    }
+    // before the barrier behind which a tile is read
+    __device__ __forceinline__ void finish(T*) const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+};
+
+// Through registers: any alignment of the type's own.  The next tile's loads are in flight while this one is multiplied.
+template <class T, int DP, int rows>
+struct Loader<T, DP, rows, false> {
+    using Shape = Tile<T, DP>;
+    static constexpr int V = Shape::V, each = rows * Shape::pieces / kAttendThreads;
+    typename Few<T, V>::vector v[each];
+    const T* base;
+    int64_t stride, head_stride;
+    int group, dim;
+
+    __device__ __forceinline__ Loader(const T* x, int64_t stride_, int64_t head_stride_, int group_, int dim_)
+        : base(x), stride(stride_), head_stride(head_stride_), group(group_), dim(dim_) {}
+    __device__ __forceinline__ void load(int first, int left, T*) {
 #pragma unroll
         for (int i = 0; i < each; ++i) {
-            typedef unsigned Words __attribute__((ext_vector_type(4)));
-            // (an exponent of ones becomes a carry into the sign's place)
-            constexpr unsigned low = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu, sign = ~low;
-            constexpr unsigned one = sizeof(T) == 4 ? 0x00800000u : std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u;
-            const Words w = (__builtin_bit_cast(Words, v[i]) & low) + one;
-            found = found || ((w[0] | w[1] | w[2] | w[3]) & sign) != 0;
+            const int piece = i * kAttendThreads + (int)threadIdx.x, row = piece / Shape::pieces, column = piece % Shape::pieces * V;
+            const unsigned r = (unsigned)(first + row), token = r / (unsigned)group;
+            v[i] = load_some<T, V>(base + token * stride + (r - token * group) * head_stride + column, row < left ? dim - column : 0);
         }
-        return found;
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void finish(T* lds) const {
 #pragma unroll
         for (int i = 0; i < each; ++i) {
             const int piece = i * kAttendThreads + (int)threadIdx.x;
-            *reinterpret_cast<typename Few<T, Shape::V>::vector*>(lds + Shape::at(piece / Shape::pieces, piece % Shape::pieces)) = v[i];
+            *reinterpret_cast<typename Few<T, V>::vector*>(lds + Shape::at(piece / Shape::pieces, piece % Shape::pieces)) = v[i];
         }
     }
 };
 
+// Infinite numbers and NaN in a tile of which not every row is seen by every lane.  A score that is masked is 0, and 0 times what its row
+// holds is 0, unless that is one of these: they are taken out of the tile, and those who do see them are told otherwise.
+//
+// Found by all threads together; f(row, column, number) for each, by one thread.  The tile can be read when this returns.
+template <class T, int DP, int rows, class F>
+__device__ __forceinline__ bool take_out_odd(T* lds, F f) {
+    using Shape = Tile<T, DP>;
+    typedef unsigned Words __attribute__((ext_vector_type(4)));
+    typedef typename Few<T, Shape::V>::vector Piece;
+    constexpr int each = rows * Shape::pieces / kAttendThreads;
+    // (an exponent of ones becomes a carry into the sign's place)
+    constexpr unsigned low = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu, one = sizeof(T) == 4 ? 0x00800000u : std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u;
+    unsigned found = 0;
+#pragma unroll
+    for (int i = 0; i < each; ++i) {
+        const Words w = (reinterpret_cast<const Words*>(lds)[i * kAttendThreads + threadIdx.x] & low) + one;
+        found |= w[0] | w[1] | w[2] | w[3];
+    }
+    if (!__syncthreads_or((found & ~low) != 0)) return false;
+#pragma unroll 1
+    for (int i = 0; i < each; ++i) {
+        const int place = i * kAttendThreads + (int)threadIdx.x, row = place / Shape::pieces, slot = place % Shape::pieces;
+        const int column = (slot / Shape::ring * Shape::ring + ((slot % Shape::ring) ^ Shape::turn(row))) * Shape::V;
+#pragma unroll 1
+        for (int j = 0; j < Shape::V; ++j) {
+            const float v = (float)lds[place * Shape::V + j];
+            if (__builtin_fabsf(v) < __builtin_inff()) continue;
+            f(row, column + j, v);
+            lds[place * Shape::V + j] = (T)0.0f;
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
 // Fragments of a row in memory, as an operand that stays in registers: numbers 16 t + 8 half .. of `row`.
-template <class T, int DP, bool whole>
+template <class T, int DP>
 __device__ __forceinline__ void load_row(const T* row, int dim, typename Frag<T>::Eight (&out)[DP / 16]) {
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
         const int at = 16 * t + 8 * half_of();
-        if constexpr (whole) out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_few<T, 8>(row + at));
-        else out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_some<T, 8>(row + at, dim - at));
+        out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_some<T, 8>(row + at, dim - at));
     }
 }
 
@@ -250,19 +318,6 @@ __device__ __forceinline__ Spans spans_of_block(const Spans& s, int* room) {
             __builtin_amdgcn_readfirstlane(b.all_high)};
 }
 
-template <class T>
-__device__ __forceinline__ float number_of(typename Frag<T>::Eight a, int e) {
-    if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(T, (u16)a[e]);
-    else return a[e];
-}
-template <class T, class F>
-__device__ __forceinline__ typename Frag<T>::Eight ones_where(F f) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = f(e) ? 1.0f : 0.0f;
-    return Frag<T>::pack(v);
-}
-
 // acc += across rows r0 .. r0 + 15 of a tile times `b`
 template <class T, int DP, int N>
 __device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* lds, int r0, const typename Frag<T>::Eight (&b)[N]) {
@@ -271,45 +326,6 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* l
         const auto a = Tile<T, DP>::across(lds, r0, db);
 #pragma unroll
         for (int n = 0; n < N; ++n) acc[n][db] = Frag<T>::mma(a, b[n], acc[n][db]);
-    }
-}
-
-// The same of a tile that holds infinite numbers or NaN, in rows that not every lane sees.  A score that is masked is 0 in b, and 0 times
-// what its row holds is 0, unless that is infinite or NaN.  Such numbers are therefore taken out of the product, and what the lanes that do
-// see them get of them is found by products of ones: NaN of NaN, of infinite ones themselves if `infinite` (b's numbers are not negative),
-// else NaN as well.  (`first`: the tile's row r0 in the numbers that the spans count)
-template <class T, int DP, bool infinite, int N>
-__device__ __forceinline__ void accumulate_odd(f32x16 (&acc)[N][DP / 32], const T* lds, int r0, const typename Frag<T>::Eight (&b)[N], const Span (&see)[N],
-                                               int first) {
-    using Eight = typename Frag<T>::Eight;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const Eight seen = ones_where<T>([&](int e) {
-            const int row = first + row_of(e) + 4 * half_of();
-            return row >= see[n].low && row < see[n].high;
-        });
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-            const Eight a = Tile<T, DP>::across(lds, r0, db);
-            Eight finite = a;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(__builtin_fabsf(number_of<T>(a, e)) < __builtin_inff())) finite[e] = 0;
-            acc[n][db] = Frag<T>::mma(finite, b[n], acc[n][db]);
-#pragma unroll
-            for (int kind = 0; kind < (infinite ? 3 : 1); ++kind) {
-                const float inf = kind == 1 ? __builtin_inff() : -__builtin_inff();
-                const Eight ones = ones_where<T>([&](int e) {
-                    const float v = number_of<T>(a, e);
-                    return kind == 0 ? (infinite ? v != v : !(__builtin_fabsf(v) < __builtin_inff())) : v == inf;
-                });
-                const f32x16 count = Frag<T>::mma(ones, seen, f32x16{});
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (count[r] > 0.0f) acc[n][db][r] += kind == 0 ? __builtin_nanf("") : inf;
-                __builtin_amdgcn_sched_barrier(0);   // (one count at a time: this path is not to cost the others registers)
-            }
-        }
     }
 }
 

@@ -35,10 +35,10 @@ void launch(K kernel, AttendArgs<T> p, int64_t count, int size, int splits, bool
     p.runs = runs;
     hipLaunchKernelGGL(kernel, grid_of((int64_t)p.tiles * p.kv_heads * splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
 }
-template <bool whole>
+template <bool direct>
 void forward(const AttendArgs<T>& p, const AttendPlan& plan, bool runs, hipStream_t stream) {
-    if (plan.few) launch(attend_kernel<T, DP, 1, 4, whole>, p, p.rows, plan.rows, plan.splits, runs, stream);
-    else launch(attend_kernel<T, DP, 1, 1, whole>, p, p.rows, plan.rows, plan.splits, runs, stream);
+    if (plan.few) launch(attend_kernel<T, DP, 1, 4, direct>, p, p.rows, plan.rows, plan.splits, runs, stream);
+    else launch(attend_kernel<T, DP, 1, 1, direct>, p, p.rows, plan.rows, plan.splits, runs, stream);
 }
 
 }  // namespace
@@ -54,7 +54,7 @@ int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void*
         p.part = room.take<float>((int64_t)p.kv_heads * plan.splits * p.rows * DP);
         p.stats = room.take<f32x2>((int64_t)p.kv_heads * plan.splits * p.rows);
     }
-    if (s.dim == DP) forward<true>(p, plan, in_runs(s), stream);
+    if (direct_loads(s)) forward<true>(p, plan, in_runs(s), stream);
     else forward<false>(p, plan, in_runs(s), stream);
     if (plan.splits > 1) {
         p.splits = plan.splits;
@@ -74,7 +74,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     Room room(workspace);
     p.delta = room.take<float>((int64_t)p.kv_heads * p.rows);
     const AttendPlan of_q = query_grad_plan(s), of_k = key_grad_plan(s);
-    const bool whole = s.dim == DP, runs = in_runs(s);
+    const bool direct = s.dim == DP, runs = in_runs(s);
     if (p.rows > 0)
         hipLaunchKernelGGL((attend_delta_kernel<T>), dim3((unsigned)least(pieces((int64_t)p.rows * p.kv_heads, 16), 1 << 14)), dim3(kAttendThreads), 0, stream, p);
     char* const rest = room.at + room.used;
@@ -85,13 +85,13 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     };
     if (p.dq && p.rows > 0) {
         p.part = (float*)rest;
-        if (whole) launch(attend_query_grad_kernel<T, DP, true>, p, p.rows, of_q.rows, of_q.splits, runs, stream);
+        if (direct) launch(attend_query_grad_kernel<T, DP, true>, p, p.rows, of_q.rows, of_q.splits, runs, stream);
         else launch(attend_query_grad_kernel<T, DP, false>, p, p.rows, of_q.rows, of_q.splits, runs, stream);
         if (of_q.splits > 1) sum(p.part, p.rows, p.group, of_q.splits, p.scale, p.dq);
     }
     if ((p.dk || p.dv) && p.keys > 0) {
         p.part = (float*)rest;
-        if (whole) launch(attend_key_grad_kernel<T, DP, true>, p, p.keys, of_k.rows, of_k.splits, runs, stream);
+        if (direct) launch(attend_key_grad_kernel<T, DP, true>, p, p.keys, of_k.rows, of_k.splits, runs, stream);
         else launch(attend_key_grad_kernel<T, DP, false>, p, p.keys, of_k.rows, of_k.splits, runs, stream);
         if (of_k.splits > 1) {
             sum(p.part, p.keys, 1, of_k.splits, p.scale, p.dk);
