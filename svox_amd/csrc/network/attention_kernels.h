@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     Eight q[N][DP / 16];
 #pragma unroll
     for (int n = 0; n < N; ++n)
-        load_row<T, DP>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
+        load_row<T, DP, direct>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
 
     const float to2 = p.scale * kLog2E;
     f32x16 acc[N][DB];
@@ -421,8 +421,8 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     clip(see, part);
 
     Eight q[DP / 16], g[DP / 16];
-    load_row<T, DP>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
-    load_row<T, DP>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
+    load_row<T, DP, direct>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
+    load_row<T, DP, direct>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
     const float lse = p.lse[(int64_t)place.head * p.rows + row], delta = p.delta[(int64_t)place.head * p.rows + row];
     const float to2 = p.scale * kLog2E;
     f32x16 acc[1][DB];
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 
 // ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them
 template <class T, int DP, bool direct>
-__global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
@@ -520,8 +520,8 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
     clip(see, part);
 
     Eight k[DP / 16], v[DP / 16];
-    load_row<T, DP>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
-    load_row<T, DP>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
+    load_row<T, DP, direct>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
+    load_row<T, DP, direct>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
     const float to2 = p.scale * kLog2E;
     const float* const lse = p.lse + (int64_t)place.head * p.rows;
     const float* const delta = p.delta + (int64_t)place.head * p.rows;
@@ -563,12 +563,11 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
             const bool mask = i0 < spans.all_low || i0 + rows > spans.all_high || i0 + rows > part.high;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-                f32x16 s = {}, dp = {};
+                // (one product's fragments at a time: the sums and the fragments that stay take most of the registers)
+                f32x16 s = {}, dp;
 #pragma unroll
-                for (int t = 0; t < DP / 16; ++t) {
-                    s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
-                    dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
-                }
+                for (int t = 0; t < DP / 16; ++t) s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
+                __builtin_amdgcn_sched_barrier(0);
                 float e[16], ds[16];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -577,17 +576,22 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         e[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], to2, -from[j]));
-                        ds[4 * i + j] = e[4 * i + j] * (dp[4 * i + j] - less[j]);
+                        dp[4 * i + j] = -less[j];
                     }
                 }
+                const int low = see[0].low, high = see[0].high, first = i0 + 32 * b + 4 * h;
                 if (mask) {
-                    const int low = see[0].low, high = see[0].high;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = i0 + 32 * b + row_of(r) + 4 * h;
-                        const bool seen = row >= low && row < high;
-                        e[r] = seen ? e[r] : 0.0f, ds[r] = seen ? ds[r] : 0.0f;
-                    }
+                    for (int r = 0; r < 16; ++r) e[r] = first + row_of(r) >= low && first + row_of(r) < high ? e[r] : 0.0f;
+                }
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
+                if (mask) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] = first + row_of(r) >= low && first + row_of(r) < high ? ds[r] : 0.0f;
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -595,6 +599,7 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
                     const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
                     accumulate<T, DP, 1>(dv, gt, at, pe);
                     accumulate<T, DP, 1>(dk, qt, at, pd);
+                    
                 }
             }
         }

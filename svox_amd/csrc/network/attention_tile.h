@@ -215,13 +215,23 @@ __device__ __forceinline__ bool take_out_odd(T* lds, F f) {
     return true;
 }
 
-// Fragments of a row in memory, as an operand that stays in registers: numbers 16 t + 8 half .. of `row`.
-template <class T, int DP>
+// Fragments of a row in memory, as an operand that stays in registers: numbers 16 t + 8 half .. of `row`, zeros from `dim` on.
+template <class T, int DP, bool direct>
 __device__ __forceinline__ void load_row(const T* row, int dim, typename Frag<T>::Eight (&out)[DP / 16]) {
+    constexpr int V = 16 / (int)sizeof(T);
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
         const int at = 16 * t + 8 * half_of();
-        out[t] = __builtin_bit_cast(typename Frag<T>::Eight, load_some<T, 8>(row + at, dim - at));
+        typename Few<T, 8>::vector v = {};
+        if constexpr (direct) {     // (pieces are there as a whole or not at all)
+            if (V == 8 ? at < dim : at + V < dim) v = load_few<T, 8>(row + at);
+            else if (V < 8 && at < dim)
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = row[at + i];
+        } else {
+            v = load_some<T, 8>(row + at, dim - at);
+        }
+        out[t] = __builtin_bit_cast(typename Frag<T>::Eight, v);
     }
 }
 
