@@ -29,8 +29,10 @@ struct AttendArgs {
     Sequences seq;
     int rows, keys;                    // of a kv head
     int group, kv_heads, dim;
-    int tiles, splits;
-    int runs;                          // blocks of an XCD take tiles side by side, else heads go round the XCDs and the last tiles come first
+    int tiles;
+    int splits, steps;                 // blocks that may share a tile's other axis, and how many steps along it each is to have at least
+    int* used;                         // [kv head][tile]: how many of them did
+    int runs;                          // blocks of an XCD take a few tiles side by side, else heads go round the XCDs and the last tiles come first
     float scale;
 };
 
@@ -38,18 +40,19 @@ constexpr float kLog2E = 1.4426950408889634f;
 
 // The work of a block: a tile, a kv head, a part of the tile's other axis.
 struct Place {
-    int tile, head, split;
+    int tile, head, split;   // no tile: tile < 0
 };
+constexpr int kAttendRun = 8;
 template <class T>
 __device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
-    const unsigned id = blockIdx.x, unit = id / p.splits;
+    // (a tile's first blocks before all others: most tiles may need no more, and blocks go round the eight XCDs)
+    const unsigned units = gridDim.x / p.splits, unit = blockIdx.x % units;
     Place at;
-    at.split = id - unit * p.splits;
+    at.split = blockIdx.x / units;
     if (p.runs) {
-        const unsigned n = (unsigned)p.tiles * p.kv_heads, xcd = unit % 8, each = n / 8, left = n % 8;
-        const unsigned position = xcd * each + min(xcd, left) + unit / 8;
+        const unsigned xcd = unit % 8, i = unit / 8, position = (i / kAttendRun * 8 + xcd) * kAttendRun + i % kAttendRun;
         at.head = position / p.tiles;
-        at.tile = position - at.head * p.tiles;
+        at.tile = at.head < p.kv_heads ? (int)(position - at.head * p.tiles) : -1;
     } else {
         at.tile = unit / p.kv_heads;
         at.head = unit - at.tile * p.kv_heads;
@@ -57,13 +60,20 @@ __device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
     }
     return at;
 }
-// the tiles of `size` of a span that a split goes through: the first one's begin, and where the last one ends
-__device__ __forceinline__ Span part_of(const Spans& all, int size, int split, int splits) {
-    if (all.low >= all.high) return {0, 0};
-    if (splits == 1) return {all.low, all.high};
-    const int tiles = (all.high - all.low + size - 1) / size, each = (tiles + splits - 1) / splits;
-    const int64_t low = all.low + (int64_t)split * each * size, high = low + (int64_t)each * size;
-    return {(int)(low < all.high ? low : all.high), (int)(high < all.high ? high : all.high)};
+// A split's part of the tiles of `size` of a span.  How many blocks share it goes by its length, which only the GPU knows: as many as get
+// p.steps tiles each.
+struct Part {
+    Span span;
+    int used;
+};
+template <class T>
+__device__ __forceinline__ Part part_of(const AttendArgs<T>& p, const Spans& all, int size, const Place& place) {
+    if (all.low >= all.high) return {{0, 0}, 1};
+    const int tiles = (all.high - all.low + size - 1) / size, most = (tiles + p.steps - 1) / p.steps, used = most < p.splits ? most : p.splits;
+    if (used == 1) return {{all.low, all.high}, 1};
+    const int each = (tiles + used - 1) / used;
+    const int64_t low = all.low + (int64_t)place.split * each * size, high = low + (int64_t)each * size;
+    return {{(int)(low < all.high ? low : all.high), (int)(high < all.high ? high : all.high)}, used};
 }
 
 template <int N>
@@ -79,35 +89,30 @@ __device__ __forceinline__ const T* row_at(const T* x, int r, int group, int hea
     return x + (int64_t)token * stride + ((int64_t)head * group + (r - (int)token * group)) * head_stride;
 }
 
-// What the rows of a wavefront's lanes (row `first` + lane % 32 of each of N) see.  Rows that are not there see everything, so that
-// they never make a mask necessary.
+// What the rows of a wavefront's lanes (row `mine` + lane % 32 of each of N) see, all of them together, and those of its block together, rows
+// r0 .. r0 + rows - 1; of rows where `keys` is not set.  Rows that are not there see everything, so that they never make a mask necessary.
 template <int N>
-__device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int first, int count, int group, int low_row, int high_row, Span (&see)[N]) {
-    // the sequences of the block's first and last row
-    const Offsets& mine = keys ? s.q : s.k;
-    const int a = last_not_beyond(mine, keys ? low_row / group : low_row), b = last_not_beyond(mine, keys ? high_row / group : high_row);
-    Spans all{INT32_MAX, INT32_MIN, INT32_MIN, INT32_MAX};
+__device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int mine, int count, int r0, int rows, int group, Span (&see)[N], Spans& block) {
+    const int lane = (int)threadIdx.x % kWave, last = min(r0 + rows, count) - 1, there = min(mine + 32 * N, count) - mine;
+    const int per_token = keys ? group : 1, per_other = keys ? 1 : group;
+    Spans all{0, 0, INT32_MIN, INT32_MAX};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int r = first + 32 * n + (int)threadIdx.x % 32;
-        const bool there = r < count;
-        Span v{0, 0};
-        if (there) {
-            if (keys) {
-                v = s.keys_of(r / group, a, b);
-            } else {                                   // (of rows)
-                v = s.queries_of(r, a, b);
-                v.low *= group, v.high *= group;
-            }
+        // (the upper lanes look at the block's first and last row)
+        const int r = mine + 32 * n + lane % 32;
+        Span v = span_of(s, keys, (lane < 32 ? min(r, last) : lane == 32 ? r0 : last) / per_token, r0 / per_token, last / per_token);
+        v.low *= per_other, v.high *= per_other;
+        if (n == 0)
+            block = {__builtin_amdgcn_readlane(v.low, 32), __builtin_amdgcn_readlane(v.high, 33), __builtin_amdgcn_readlane(v.low, 33),
+                     __builtin_amdgcn_readlane(v.high, 32)};
+        const int here = min(there - 32 * n, 32);
+        if (here > 0) {
+            if (n == 0) all.low = __builtin_amdgcn_readlane(v.low, 0), all.all_high = __builtin_amdgcn_readlane(v.high, 0);
+            all.high = __builtin_amdgcn_readlane(v.high, here - 1), all.all_low = __builtin_amdgcn_readlane(v.low, here - 1);
         }
-        const bool some = v.low < v.high;
-        all.low = min(all.low, some ? v.low : INT32_MAX), all.high = max(all.high, some ? v.high : INT32_MIN);
-        if (!there) v = {INT32_MIN, INT32_MAX};
-        all.all_low = max(all.all_low, v.low), all.all_high = min(all.all_high, v.high);
-        see[n] = v;
+        v.low = __shfl(v.low, lane % 32, kWave), v.high = __shfl(v.high, lane % 32, kWave);
+        see[n] = r < count ? v : Span{INT32_MIN, INT32_MAX};
     }
-    all.low = least_of_wave(all.low), all.high = most_of_wave(-1 > all.high ? -1 : all.high);
-    all.all_low = most_of_wave(all.all_low < -1 ? -1 : all.all_low), all.all_high = least_of_wave(all.all_high);
     return all;
 }
 
@@ -129,16 +134,19 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     constexpr int join_numbers = across > 1 ? 4 * 32 * (DP + 2) : 0;   // floats
     constexpr int tile_bytes = 2 * S::stages * S::tile * (int)sizeof(T), join_bytes = join_numbers * 4;
     __shared__ __attribute__((aligned(16))) char lds[tile_bytes > join_bytes ? tile_bytes : join_bytes];
-    __shared__ int room[16];
     __shared__ unsigned kinds[3][S::keys][DB];   // NaN, inf and -inf that were taken out of a tile of v
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
+    if (place.tile < 0) return;
     const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32 * N;
 
     Span see[N];
-    const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + S::rows, p.rows) - 1, see);
-    const Spans block = spans_of_block(spans, room);
-    const Span part = part_of(block, S::keys, place.split, p.splits);
+    Spans block;
+    const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, r0, S::rows, p.group, see, block);
+    const Part share = part_of(p, block, S::keys, place);
+    if (place.split >= share.used) return;
+    if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
+    const Span part = share.span;
     clip(see, part);
 
     Eight q[N][DP / 16];
@@ -319,7 +327,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         if (r >= p.rows) continue;
         // (what a row that sees keys has, though all of its scores are -inf, is not what one that sees none has)
         const bool some = max(see[n].low, part.low) < see[n].high;
-        if (p.splits > 1) {
+        if (share.used > 1) {
             const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
             if (h == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
             if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f);
@@ -332,23 +340,63 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     }
 }
 
-// The splits' sums of a row, one joined row a block at a time: 32 lanes read a row's numbers, DP / 4 of them used, eight splits at once.
+template <class T>
+__device__ __forceinline__ void store_joined(const AttendArgs<T>& p, int64_t i, int head, int r, int lane, float most, float l, f32x4 sum) {
+    const bool some = most != -__builtin_inff();
+    const float factor = some ? 1.0f / l : 0.0f;
+    const int token = r / p.group;
+    T* const to = p.y + (((int64_t)token * p.kv_heads + head) * p.group + (r - token * p.group)) * p.dim;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (4 * lane + j < p.dim) to[4 * lane + j] = (T)(sum[j] * factor);
+    if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : __builtin_inff();
+}
+
+// The splits' sums of a row, where there are several: a row by as many lanes as its numbers are fours, one split after another.
 template <class T, int DP>
-__global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs<T> p, int rows) {
+    constexpr int lanes = DP / 4;
+    const int lane = (int)threadIdx.x % lanes;
+    const int64_t all = (int64_t)p.kv_heads * p.rows, step = (int64_t)gridDim.x * (kAttendThreads / lanes);
+    for (int64_t i = (int64_t)blockIdx.x * (kAttendThreads / lanes) + threadIdx.x / lanes; i < all; i += step) {
+        const int head = (int)(i / p.rows), r = (int)(i - (int64_t)head * p.rows);
+        const int used = p.used[head * p.tiles + r / rows];
+        if (used == 1) continue;
+        const int64_t first = (int64_t)head * p.splits * p.rows + r;
+        float most = -__builtin_inff(), l = 0.0f;
+        for (int s = 0; s < used; ++s) most = fmaxf(most, p.stats[first + (int64_t)s * p.rows][0]);
+        f32x4 sum = {};
+        for (int s = 0; s < used; ++s) {
+            const int64_t at = first + (int64_t)s * p.rows;
+            const f32x2 stat = p.stats[at];
+            if (stat[0] == -__builtin_inff()) continue;   // (nothing seen, nothing stored)
+            const float less = __builtin_amdgcn_exp2f(stat[0] - most);
+            l = __builtin_fmaf(stat[1], less, l);
+            sum += *reinterpret_cast<const f32x4*>(p.part + at * DP + 4 * lane) * less;
+        }
+        store_joined<T>(p, i, head, r, lane, most, l, sum);
+    }
+}
+// Of many splits: a row a block, as many splits at once as there are lanes for.
+template <class T, int DP>
+__global__ __launch_bounds__(kAttendThreads) void attend_join_many_kernel(AttendArgs<T> p, int rows) {
     constexpr int lanes = DP / 4, groups = kAttendThreads / lanes;
     __shared__ f32x4 room[kAttendThreads];
     __shared__ float sums[kAttendThreads];
     const int lane = (int)threadIdx.x % lanes, group = (int)threadIdx.x / lanes;
-    for (int64_t i = blockIdx.x; i < (int64_t)p.kv_heads * p.rows; i += gridDim.x) {
+    const int64_t all = (int64_t)p.kv_heads * p.rows, each = (all + gridDim.x - 1) / gridDim.x;
+    for (int64_t i = blockIdx.x * each; i < least((blockIdx.x + 1) * each, all); ++i) {
         const int head = (int)(i / p.rows), r = (int)(i - (int64_t)head * p.rows);
+        const int used = p.used[head * p.tiles + r / rows];
+        if (used == 1) continue;
         const int64_t first = (int64_t)head * p.splits * p.rows + r;
         float most = -__builtin_inff();
-        for (int s = (int)threadIdx.x % kWave; s < p.splits; s += kWave) most = fmaxf(most, p.stats[first + (int64_t)s * p.rows][0]);
+        for (int s = (int)threadIdx.x % kWave; s < used; s += kWave) most = fmaxf(most, p.stats[first + (int64_t)s * p.rows][0]);
 #pragma unroll
         for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d, kWave));
         f32x4 sum = {};
         float l = 0.0f;
-        for (int s = group; s < p.splits; s += groups) {
+        for (int s = group; s < used; s += groups) {
             const int64_t at = first + (int64_t)s * p.rows;
             const f32x2 stat = p.stats[at];
             if (stat[0] == -__builtin_inff()) continue;   // (nothing seen, nothing stored)
@@ -364,14 +412,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs<
         l = 0.0f;
         for (int g = 0; g < groups; ++g) l += sums[g];
         for (int g = 1; g < groups; ++g) sum += room[g * lanes + lane];
-        const bool some = most != -__builtin_inff();
-        const float factor = some ? 1.0f / l : 0.0f;
-        const int token = r / p.group;
-        T* const to = p.y + (((int64_t)token * p.kv_heads + head) * p.group + (r - token * p.group)) * p.dim;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (4 * lane + j < p.dim) to[4 * lane + j] = (T)(sum[j] * factor);
-        if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : __builtin_inff();
+        store_joined<T>(p, i, head, r, lane, most, l, sum);
     }
 }
 
@@ -408,16 +449,19 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
-    __shared__ int room[16];
     __shared__ unsigned bad[keys / 32];   // keys that are not finite
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
+    if (place.tile < 0) return;
     const int r0 = place.tile * rows, mine = r0 + wave * 32, row = min(mine + (int)threadIdx.x % 32, p.rows - 1);
 
     Span see[1];
-    const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, p.group, r0, min(r0 + rows, p.rows) - 1, see);
-    const Spans block = spans_of_block(spans, room);
-    const Span part = part_of(block, keys, place.split, p.splits);
+    Spans block;
+    const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, r0, rows, p.group, see, block);
+    const Part share = part_of(p, block, keys, place);
+    if (place.split >= share.used) return;
+    if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
+    const Span part = share.span;
     clip(see, part);
 
     Eight q[DP / 16], g[DP / 16];
@@ -492,7 +536,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     for (int db = 0; db < DB; ++db) acc[0][db] += none;
     const int r = mine + (int)threadIdx.x % 32;
     if (r >= p.rows) return;
-    if (p.splits > 1) {
+    if (share.used > 1) {
         store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f);
     } else {
         const unsigned token = (unsigned)r / (unsigned)p.group;
@@ -508,15 +552,18 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
-    __shared__ int room[16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
+    if (place.tile < 0) return;
     const int j0 = place.tile * keys, mine = j0 + wave * 32, key = min(mine + (int)threadIdx.x % 32, p.keys - 1);
 
     Span see[1];
-    const Spans spans = spans_of<1>(p.seq, false, mine, p.keys, p.group, j0, min(j0 + keys, p.keys) - 1, see);
-    const Spans block = spans_of_block(spans, room);
-    const Span part = part_of(block, rows, place.split, p.splits);
+    Spans block;
+    const Spans spans = spans_of<1>(p.seq, false, mine, p.keys, j0, keys, p.group, see, block);
+    const Part share = part_of(p, block, rows, place);
+    if (place.split >= share.used) return;
+    if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
+    const Span part = share.span;
     clip(see, part);
 
     Eight k[DP / 16], v[DP / 16];
@@ -563,11 +610,11 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
             const bool mask = i0 < spans.all_low || i0 + rows > spans.all_high || i0 + rows > part.high;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-                // (one product's fragments at a time: the sums and the fragments that stay take most of the registers)
+                // (heads of 128: one product's fragments at a time, as the sums and the fragments that stay take most of the registers)
                 f32x16 s = {}, dp;
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
-                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
                 float e[16], ds[16];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -586,7 +633,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
                 }
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
-                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
                 if (mask) {
@@ -608,7 +655,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     }
     const int j = mine + (int)threadIdx.x % 32;
     if (j >= p.keys) return;
-    if (p.splits > 1) {
+    if (share.used > 1) {
         float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
         store_row<float, DB>(at, DP, dk[0], 1.0f);
         store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], 1.0f);
@@ -619,21 +666,22 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     }
 }
 
-// The splits' sums of a gradient: [kv head][split][row][DP] to (tokens, kv heads, group, dim)
+// The splits' sums of a gradient, where there are several: [kv head][split][row][DP] to (tokens, kv heads, group, dim)
 template <class T, int DP>
-__global__ __launch_bounds__(kAttendThreads) void attend_sum_kernel(const float* part, int64_t rows, int kv_heads, int group, int dim, int splits, float factor,
-                                                                    T* to) {
+__global__ __launch_bounds__(kAttendThreads) void attend_sum_kernel(AttendArgs<T> p, const float* part, int64_t rows, int tile, int group, float factor, T* to) {
     constexpr int lanes = DP / 4;
     const int lane = (int)threadIdx.x % lanes;
-    const int64_t all = rows * kv_heads, step = (int64_t)gridDim.x * (kAttendThreads / lanes);
+    const int64_t all = rows * p.kv_heads, step = (int64_t)gridDim.x * (kAttendThreads / lanes);
     for (int64_t i = (int64_t)blockIdx.x * (kAttendThreads / lanes) + threadIdx.x / lanes; i < all; i += step) {
         const int64_t head = i / rows, r = i - head * rows, token = r / group;
+        const int used = p.used[head * p.tiles + r / tile];
+        if (used == 1) continue;
         f32x4 sum = {};
-        for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4*>(part + ((head * splits + s) * rows + r) * DP + 4 * lane);
-        T* const at = to + ((token * kv_heads + head) * group + (r - token * group)) * dim;
+        for (int s = 0; s < used; ++s) sum += *reinterpret_cast<const f32x4*>(part + ((head * p.splits + s) * rows + r) * DP + 4 * lane);
+        T* const at = to + ((token * p.kv_heads + head) * group + (r - token * group)) * p.dim;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (4 * lane + j < dim) at[4 * lane + j] = (T)(sum[j] * factor);
+            if (4 * lane + j < p.dim) at[4 * lane + j] = (T)(sum[j] * factor);
     }
 }
 

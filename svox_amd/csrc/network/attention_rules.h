@@ -13,20 +13,25 @@ using svox_decoder::pieces;
 inline int attend_width(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 struct AttendPlan {
-    int rows;      // of a block's tile
-    int splits;    // blocks that share a tile's other axis
+    int rows;            // of a block's tile
+    int splits, steps;   // blocks that may share a tile's other axis, and the least steps of each
     bool few;
 };
 
 constexpr int64_t kAttendBlocks = 512;   // two for each compute unit
 
-// Blocks for a tile's other axis, of which a tile sees `length` in all likelihood, `size` at a time: as many as fill the GPU, each with
-// two steps at least.
-inline int splits_for(int64_t blocks, int64_t length, int64_t size) {
-    if (blocks >= kAttendBlocks || blocks < 1) return 1;
-    const int64_t wanted = kAttendBlocks / blocks, most = length / (2 * size);
+// How a tile's other axis is split, `size` at a time.  What a tile sees of it only the GPU knows; in all likelihood it is `length`, and where
+// there are several sequences, or a causal one, it differs from tile to tile.  A block gets as many steps as leave two blocks for every
+// place on the GPU, two at least; as many blocks may share a tile as a tile of the whole axis would need, in launches of up to 4096 blocks.
+inline AttendPlan split(AttendPlan plan, int64_t blocks, int64_t length, int64_t whole, int64_t size) {
+    plan.splits = plan.steps = 1;
+    if (blocks < 1 || blocks >= 2 * kAttendBlocks) return plan;
+    const int64_t steps = pieces(length, size) * blocks / (2 * kAttendBlocks);
+    plan.steps = (int)(steps < 2 ? 2 : steps);
+    const int64_t wanted = pieces(pieces(whole, size), plan.steps), most = 8 * kAttendBlocks / blocks;
     const int64_t splits = wanted < most ? wanted : most;
-    return (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    plan.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    return plan;
 }
 // The part of `other` that a tile of `rows` out of `all` sees where sequences are of one length.
 inline int64_t likely_length(int64_t other, int64_t sequences, int64_t rows, int64_t all) {
@@ -37,17 +42,16 @@ inline int64_t likely_length(int64_t other, int64_t sequences, int64_t rows, int
 
 inline AttendPlan forward_plan(const SvoxAttention& s) {
     const int64_t rows = s.queries * (s.heads / s.kv_heads), blocks = pieces(rows, 128) * s.kv_heads;
-    if (blocks >= kAttendBlocks) return {128, 1, false};
-    const int64_t small = pieces(rows, 32) * s.kv_heads;
-    return {32, splits_for(small, likely_length(s.keys, s.sequences, 32, rows), 128), true};
+    if (blocks >= kAttendBlocks) return split({128, 1, 1, false}, blocks, likely_length(s.keys, s.sequences, 128, rows), s.keys, 64);
+    return split({32, 1, 1, true}, pieces(rows, 32) * s.kv_heads, likely_length(s.keys, s.sequences, 32, rows), s.keys, 128);
 }
 inline AttendPlan query_grad_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads), blocks = pieces(rows, 128) * s.kv_heads;
-    return {128, splits_for(blocks, likely_length(s.keys, s.sequences, 128, rows), 64), false};
+    const int64_t rows = s.queries * (s.heads / s.kv_heads);
+    return split({128, 1, 1, false}, pieces(rows, 128) * s.kv_heads, likely_length(s.keys, s.sequences, 128, rows), s.keys, 64);
 }
 inline AttendPlan key_grad_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads), blocks = pieces(s.keys, 128) * s.kv_heads;
-    return {128, splits_for(blocks, likely_length(rows, s.sequences, 128, s.keys), 64), false};
+    const int64_t rows = s.queries * (s.heads / s.kv_heads);
+    return split({128, 1, 1, false}, pieces(s.keys, 128) * s.kv_heads, likely_length(rows, s.sequences, 128, s.keys), rows, 64);
 }
 
 // Whether tiles go from memory to LDS 16 bytes at a time: everything lies at whole numbers of 16 bytes, and no tile of up to 128 rows reaches
@@ -64,19 +68,21 @@ inline bool direct_loads(const SvoxAttention& s, const SvoxAttentionGrads& g) {
     return direct_heads(s, g.grad, g.grad_stride, g.grad_head, s.heads / s.kv_heads);
 }
 
-// Whether the blocks of an XCD take tiles side by side: where many sequences share the keys out, so that one's stay in an XCD's cache.  The
-// tiles of few long ones differ in work where they are causal, and go round.
+// Whether the blocks of an XCD take a few tiles side by side: where many sequences share the keys out, so that one's stay in an XCD's cache.
+// Heads of few long sequences go round the XCDs instead.
 inline bool in_runs(const SvoxAttention& s) { return s.sequences >= 16; }
 
 inline int64_t attention_space(const SvoxAttention& s, bool backward) {
     const int64_t rows = s.queries * (s.heads / s.kv_heads), width = attend_width(s.dim);
     const auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    const auto space = [&](const AttendPlan& plan, int64_t count, int64_t numbers) {
+        return plan.splits > 1 ? whole(s.kv_heads * plan.splits * count * numbers * 4) + whole(s.kv_heads * pieces(count, plan.rows) * 4) : 0;
+    };
     if (!backward) {
-        const int64_t parts = forward_plan(s).splits;
-        return parts > 1 ? whole(s.kv_heads * parts * rows * width * 4) + whole(s.kv_heads * parts * rows * 8) : 0;
+        const AttendPlan plan = forward_plan(s);
+        return space(plan, rows, width) + (plan.splits > 1 ? whole(s.kv_heads * plan.splits * rows * 8) : 0);
     }
-    const int64_t of_q = query_grad_plan(s).splits, of_k = key_grad_plan(s).splits;
-    const int64_t q = of_q > 1 ? s.kv_heads * of_q * rows * width * 4 : 0, k = of_k > 1 ? 2 * s.kv_heads * of_k * s.keys * width * 4 : 0;
+    const int64_t q = space(query_grad_plan(s), rows, width), k = space(key_grad_plan(s), s.keys, 2 * width);
     return whole(s.kv_heads * rows * 4) + (q > k ? q : k);
 }
 

@@ -247,28 +247,19 @@ struct Offsets {
         return v < 0 ? 0 : v > total ? total : (int)v;
     }
 };
-// The last i with offsets(i) <= t, or -1: by the whole wavefront, 64 places at a time.  (At most n whatever the places hold.)
+// The last i with offsets(i) <= t, or 0: by the whole wavefront, 64 places at a time.  (At most n whatever the places hold.)
 __device__ __forceinline__ int last_not_beyond(const Offsets& o, int t) {
-    if (!o.at) return t < o.total ? 0 : 1;
+    if (!o.at) return 0;
     const int lane = (int)threadIdx.x % kWave;
     int low = 0, size = o.n + 1;
     while (true) {
         const int step = (size + kWave - 1) / kWave, at = lane * step;
         const int found = __popcll(__ballot(at < size && o(low + at) <= t));
-        if (found == 0) return low == 0 ? -1 : low;
+        if (found == 0) return low;
         low += (found - 1) * step;
         if (step == 1) return low;
         size = min(step, size - (found - 1) * step);
     }
-}
-// the sequence of t, which lies among low .. high
-__device__ __forceinline__ int sequence_of(const Offsets& o, int t, int low, int high) {
-    while (low < high) {
-        const int middle = (low + high + 1) / 2;
-        if (o(middle) <= t) low = middle;
-        else high = middle - 1;
-    }
-    return low;
 }
 
 struct Span {
@@ -277,56 +268,57 @@ struct Span {
 struct Sequences {
     Offsets q, k;
     int causal;
-    // of keys that query t sees, t's sequence among first .. last
-    __device__ __forceinline__ Span keys_of(int t, int first, int last) const {
-        const int s = sequence_of(q, t, max(first, 0), last);
-        if (s >= q.n) return {0, 0};
-        const int q0 = q(s), q1 = q(s + 1), k0 = k(s), k1 = max(k0, k(s + 1));
-        if (t < q0 || t >= q1) return {0, 0};
-        if (!causal) return {k0, k1};
-        const int64_t seen = (int64_t)(t - q0) + (k1 - k0) - (q1 - q0) + 1;
-        return {k0, k0 + (int)(seen < 0 ? 0 : seen > k1 - k0 ? k1 - k0 : seen)};
-    }
-    // of queries that see key t
-    __device__ __forceinline__ Span queries_of(int t, int first, int last) const {
-        const int s = sequence_of(k, t, max(first, 0), last);
-        if (s >= k.n) return {0, 0};
-        const int q0 = q(s), q1 = max(q0, q(s + 1)), k0 = k(s), k1 = k(s + 1);
-        if (t < k0 || t >= k1) return {0, 0};
-        if (!causal) return {q0, q1};
-        const int64_t hidden = (int64_t)(t - k0) - ((k1 - k0) - (q1 - q0));
-        return {q0 + (int)(hidden < 0 ? 0 : hidden > q1 - q0 ? q1 - q0 : hidden), q1};
-    }
 };
+// What every lane's token `t` sees of the other axis; `keys`: t is a query, else a key.  A lane's tokens are none before `first` and none beyond
+// `last`.  Where sequences are in order, spans do not go back from token to token, also those that are empty.
+__device__ __forceinline__ Span span_of(const Sequences& s, bool keys, int t, int first, int last) {
+    const Offsets &mine = keys ? s.q : s.k, &other = keys ? s.k : s.q;
+    const int lane = (int)threadIdx.x % kWave, a = last_not_beyond(mine, first);
+    // the places from the first token's sequence on, one a lane: those of all tokens in all likelihood
+    const int place = min(a + lane, mine.n), mine_at = mine(place), other_at = other(place);
+    int m0, m1, o0, o1;
+    if (__builtin_amdgcn_readlane(mine_at, 1) > last) {
+        m0 = __builtin_amdgcn_readlane(mine_at, 0), m1 = __builtin_amdgcn_readlane(mine_at, 1);
+        o0 = __builtin_amdgcn_readlane(other_at, 0), o1 = __builtin_amdgcn_readlane(other_at, 1);
+    } else if (a + kWave - 1 >= mine.n || __builtin_amdgcn_readlane(mine_at, kWave - 1) > last) {
+        int i = 0;
+#pragma unroll
+        for (int d = kWave / 2; d > 0; d /= 2) {
+            const int there = __shfl(mine_at, i + d, kWave);   // (by all lanes)
+            if (i + d < kWave - 1 && there <= t) i += d;
+        }
+        m0 = __shfl(mine_at, i, kWave), m1 = __shfl(mine_at, i + 1, kWave);
+        o0 = __shfl(other_at, i, kWave), o1 = __shfl(other_at, i + 1, kWave);
+    } else {
+        int low = a, high = mine.n;
+        while (low < high) {
+            const int middle = (low + high + 1) / 2;
+            if (mine(middle) <= t) low = middle;
+            else high = middle - 1;
+        }
+        const int next = min(low + 1, mine.n);
+        m0 = mine(low), m1 = mine(next), o0 = other(low), o1 = other(next);
+    }
+    o1 = max(o0, o1);
+    if (t < m0) return {o0, o0};
+    if (t >= m1) return {o1, o1};
+    if (!s.causal) return {o0, o1};
+    const int ends = (o1 - o0) - (m1 - m0);   // (the places are counted from the sequences' ends)
+    if (keys) {
+        const int64_t seen = (int64_t)(t - m0) + ends + 1;
+        return {o0, o0 + (int)(seen < 0 ? 0 : seen > o1 - o0 ? o1 - o0 : seen)};
+    }
+    const int64_t hidden = (int64_t)(t - m0) + ends;   // (mine are keys: ends is of queries less keys)
+    return {o0 + (int)(hidden < 0 ? 0 : hidden > o1 - o0 ? o1 - o0 : hidden), o1};
+}
 
-// What the lanes of a wavefront see: the span of all, and the one that every lane sees whole.
+// What a wavefront's lanes, or a block's, see: the span of all, and the one that every lane sees whole.
 struct Spans {
     int low, high;            // of all; none: low >= high
     int all_low, all_high;
     // whether some lane does not see all of the `n` from `first` on
     __device__ __forceinline__ bool masks(int first, int n) const { return first < all_low || first + n > all_high; }
 };
-__device__ __forceinline__ int least_of_wave(int v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) v = min(v, __shfl_xor(v, d, kWave));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int most_of_wave(int v) { return -least_of_wave(-v); }
-
-// of every wavefront's spans the block's
-__device__ __forceinline__ Spans spans_of_block(const Spans& s, int* room) {
-    const int wave = (int)threadIdx.x / kWave;
-    if (threadIdx.x % kWave == 0) room[4 * wave] = s.low, room[4 * wave + 1] = s.high, room[4 * wave + 2] = s.all_low, room[4 * wave + 3] = s.all_high;
-    __syncthreads();
-    Spans b{room[0], room[1], room[2], room[3]};
-#pragma unroll
-    for (int w = 1; w < kAttendThreads / kWave; ++w) {
-        b.low = min(b.low, room[4 * w]), b.high = max(b.high, room[4 * w + 1]);
-        b.all_low = max(b.all_low, room[4 * w + 2]), b.all_high = min(b.all_high, room[4 * w + 3]);
-    }
-    return {__builtin_amdgcn_readfirstlane(b.low), __builtin_amdgcn_readfirstlane(b.high), __builtin_amdgcn_readfirstlane(b.all_low),
-            __builtin_amdgcn_readfirstlane(b.all_high)};
-}
 
 // acc += across rows r0 .. r0 + 15 of a tile times `b`
 template <class T, int DP, int N>

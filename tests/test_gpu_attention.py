@@ -302,3 +302,31 @@ def test_two_streams_at_once(gpu):
     for (y, grads), several in zip(want, got):
         for y2, grads2 in several:
             assert torch.equal(y, y2) and all(torch.equal(grads[n], grads2[n]) for n in grads)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("d", [32, 64, 128, 24])
+def test_heads_that_begin_anywhere(gpu, d, dtype):
+    """Whole and partial widths whose numbers do not lie at whole numbers of 16 bytes, or rows of which do not."""
+    g = torch.Generator().manual_seed(13)
+    for shift, more in ((1, 0), (0, 1), (8, 8), (2, 6)):
+        wide = normal(g, 140, 6 * d + shift + more, dtype=dtype)
+        q, k, v = wide[:, shift:shift + 6 * d].split([2 * d, 2 * d, 2 * d], dim=1)
+        grads = normal(g, 140, 2 * d + shift + more, dtype=dtype)[:, shift:shift + 2 * d].unflatten(1, (2, d))
+        check({"q": q.unflatten(1, (2, d)), "k": k.unflatten(1, (2, d)), "v": v.unflatten(1, (2, d))}, grads, packed([100, 3, 37]), causal=True)
+        grads = normal(g, 140, 2, d, dtype=dtype)
+        check({"q": q.unflatten(1, (2, d)), "k": k.unflatten(1, (2, d)), "v": v.unflatten(1, (2, d))}, grads)
+
+
+def test_tiles_that_are_shared_out_and_tiles_that_are_not(gpu):
+    """Sequences of very different lengths: long ones' tiles are split and joined, short ones' are not, forward and backward."""
+    for lengths, h, g, d in [([2000, 3, 0, 10, 1500, 1], 2, 1, 64), ([1, 3000], 3, 1, 16), ([5] * 30 + [2500], 1, 1, 128)]:
+        x, grad = inputs(sum(lengths), sum(lengths), h, g, d, torch.float16, seed=sum(lengths))
+        check(x, grad, packed(lengths), causal=True)
+        check(x, grad, packed(lengths))
+    of_q, of_k = [1, 3, 0, 2], [4000, 5, 60, 900]
+    x, grad = inputs(sum(of_q), sum(of_k), 8, 2, 64, torch.bfloat16, seed=1)
+    check(x, grad, packed(of_q), packed(of_k), causal=True)
+    of_q, of_k = [4000, 5, 60, 900], [1, 3, 0, 2]
+    x, grad = inputs(sum(of_q), sum(of_k), 2, 2, 64, torch.bfloat16, seed=1)
+    check(x, grad, packed(of_q), packed(of_k))
