@@ -32,7 +32,7 @@ struct AttendArgs {
     int tiles;
     int splits, steps;                 // blocks that may share a tile's other axis, and how many steps along it each is to have at least
     int* used;                         // [kv head][tile]: how many of them did
-    int runs;                          // blocks of an XCD take a few tiles side by side, else heads go round the XCDs and the last tiles come first
+    int runs, last_first;              // blocks of an XCD take a few tiles side by side, else heads go round the XCDs; the last tiles come first
     float scale;
 };
 
@@ -50,14 +50,16 @@ __device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
     Place at;
     at.split = blockIdx.x / units;
     if (p.runs) {
-        const unsigned xcd = unit % 8, i = unit / 8, position = (i / kAttendRun * 8 + xcd) * kAttendRun + i % kAttendRun;
+        // (each time round the XCDs one further: sequences of a power of two would otherwise give one XCD all of their last tiles)
+        const unsigned i = unit / 8, round = i / kAttendRun, xcd = (unit + round) % 8, position = (round * 8 + xcd) * kAttendRun + i % kAttendRun;
         at.head = position / p.tiles;
-        at.tile = at.head < p.kv_heads ? (int)(position - at.head * p.tiles) : -1;
+        at.tile = position - at.head * p.tiles;
+        if (at.head >= p.kv_heads) return {-1, 0, 0};
     } else {
         at.tile = unit / p.kv_heads;
         at.head = unit - at.tile * p.kv_heads;
-        if (p.seq.causal) at.tile = p.tiles - 1 - at.tile;
     }
+    if (p.last_first) at.tile = p.tiles - 1 - at.tile;
     return at;
 }
 // A split's part of the tiles of `size` of a span.  How many blocks share it goes by its length, which only the GPU knows: as many as get
@@ -116,6 +118,18 @@ __device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int min
     return all;
 }
 
+// A lane's 16 scores whose rows lie below `low`, or from `high` on (counted from the first of them), become `v`.
+template <class Scores>
+__device__ __forceinline__ void hide_below(Scores& s, int low, float v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = row_of(r) < low ? v : s[r];
+}
+template <class Scores>
+__device__ __forceinline__ void hide_from(Scores& s, int high, float v) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = row_of(r) < high ? s[r] : v;
+}
+
 // ---- forward.  Four wavefronts, of which `across` share rows and take a part of every tile's keys each.
 template <class T, int DP, int N, int across>
 struct ForwardShape {
@@ -134,6 +148,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     constexpr int join_numbers = across > 1 ? 4 * 32 * (DP + 2) : 0;   // floats
     constexpr int tile_bytes = 2 * S::stages * S::tile * (int)sizeof(T), join_bytes = join_numbers * 4;
     __shared__ __attribute__((aligned(16))) char lds[tile_bytes > join_bytes ? tile_bytes : join_bytes];
+    __shared__ int found[2];                     // the tile of a stage that holds infinite numbers or NaN
     __shared__ unsigned kinds[3][S::keys][DB];   // NaN, inf and -inf that were taken out of a tile of v
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -169,14 +184,17 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         ks.load(k0, part.high - k0, tiles + stage * 2 * S::tile);
         vs.load(k0, part.high - k0, tiles + (stage * 2 + 1) * S::tile);
     };
-    const auto finish = [&](int stage) {
+    const auto finish = [&](int stage, int k0) {
         ks.finish(tiles + stage * 2 * S::tile);
         vs.finish(tiles + (stage * 2 + 1) * S::tile);
+        if (block.masks(k0, S::keys) && holds_odd<T, DP, S::keys>(tiles + (stage * 2 + 1) * S::tile)) found[stage] = k0;
         __syncthreads();
     };
+    if (threadIdx.x < 2) found[threadIdx.x] = -1;
+    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
-        finish(0);
+        finish(0, part.low);
     }
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += S::keys) {
@@ -184,10 +202,10 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         if (more && S::stages == 2) load(k0 + S::keys, stage ^ 1);
         const T* const kt = tiles + stage * 2 * S::tile;
         const T* const vt = kt + S::tile;
-        bool odd = false;
-        if (block.masks(k0, S::keys)) {
+        const bool odd = block.masks(k0, S::keys) && found[stage] == k0;
+        if (odd) {
             for (int i = (int)threadIdx.x; i < 3 * S::keys * DB; i += kAttendThreads) (&kinds[0][0][0])[i] = 0;
-            odd = take_out_odd<T, DP, S::keys>(tiles + (stage * 2 + 1) * S::tile, [&](int row, int column, float x) {
+            take_out_odd<T, DP, S::keys>(tiles + (stage * 2 + 1) * S::tile, [&](int row, int column, float x) {
                 atomicOr(&kinds[x != x ? 0 : x > 0.0f ? 1 : 2][row][column / 32], 1u << column % 32);
             });
         }
@@ -205,19 +223,18 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                     for (int n = 0; n < N; ++n) s[b][n] = F::mma(a, q[n][t], s[b][n]);
                 }
             }
-            const bool mask = kw < spans.all_low || kw + S::mine > spans.all_high || kw + S::mine > part.high;
-            if (mask) {
+            // (the tile's end lies beyond what some lane sees, if it lies beyond the part)
+            if (kw < spans.all_low) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const int low = see[n].low, high = see[n].high;
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int b = 0; b < KB; ++b)
+                    for (int b = 0; b < KB; ++b) hide_below(s[b][n], see[n].low - kw - 32 * b - 4 * h, -__builtin_inff());
+            }
+            if (kw + S::mine > min(spans.all_high, part.high)) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int key = kw + 32 * b + row_of(r) + 4 * h;
-                            s[b][n][r] = key >= low && key < high ? s[b][n][r] : -__builtin_inff();
-                        }
-                }
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) hide_from(s[b][n], see[n].high - kw - 32 * b - 4 * h, -__builtin_inff());
             }
             Eight e[KB][2][N];
 #pragma unroll
@@ -278,10 +295,10 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         }
         if constexpr (S::stages == 2) {
             stage ^= 1;
-            if (more) finish(stage);
+            if (more) finish(stage, k0 + S::keys);
         } else {
             __syncthreads();
-            if (more) load(k0 + S::keys, 0), finish(0);
+            if (more) load(k0 + S::keys, 0), finish(0, k0 + S::keys);
         }
     }
 
@@ -449,6 +466,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
+    __shared__ int found[2];              // the tile of a stage that holds infinite numbers or NaN
     __shared__ unsigned bad[keys / 32];   // keys that are not finite
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -478,14 +496,17 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         ks.load(k0, part.high - k0, tiles + stage * 2 * tile);
         vs.load(k0, part.high - k0, tiles + (stage * 2 + 1) * tile);
     };
-    const auto finish = [&](int stage) {
+    const auto finish = [&](int stage, int k0) {
         ks.finish(tiles + stage * 2 * tile);
         vs.finish(tiles + (stage * 2 + 1) * tile);
+        if (block.masks(k0, keys) && holds_odd<T, DP, keys>(tiles + stage * 2 * tile)) found[stage] = k0;
         __syncthreads();
     };
+    if (threadIdx.x < 2) found[threadIdx.x] = -1;
+    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
-        finish(0);
+        finish(0, part.low);
     }
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += keys) {
@@ -493,13 +514,12 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         if (more) load(k0 + keys, stage ^ 1);
         const T* const kt = tiles + stage * 2 * tile;
         const T* const vt = kt + tile;
-        bool odd = false;
-        if (block.masks(k0, keys)) {
+        const bool odd = block.masks(k0, keys) && found[stage] == k0;
+        if (odd) {
             if (threadIdx.x < keys / 32) bad[threadIdx.x] = 0;
-            odd = take_out_odd<T, DP, keys>(tiles + stage * 2 * tile, [&](int row, int, float) { atomicOr(&bad[row / 32], 1u << row % 32); });
+            take_out_odd<T, DP, keys>(tiles + stage * 2 * tile, [&](int row, int, float) { atomicOr(&bad[row / 32], 1u << row % 32); });
         }
         if (k0 < spans.high && k0 + keys > spans.low) {
-            const bool mask = k0 < spans.all_low || k0 + keys > spans.all_high || k0 + keys > part.high;
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
                 f32x16 s = {}, dp = {};
@@ -511,14 +531,8 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                 float ds[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to2, -lse)) * (dp[r] - delta);
-                if (mask) {
-                    const int low = see[0].low, high = see[0].high;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int key = k0 + 32 * b + row_of(r) + 4 * h;
-                        ds[r] = key >= low && key < high ? ds[r] : 0.0f;
-                    }
-                }
+                if (k0 < spans.all_low) hide_below(ds, see[0].low - k0 - 32 * b - 4 * h, 0.0f);
+                if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see[0].high - k0 - 32 * b - 4 * h, 0.0f);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Eight e[1] = {F::pack(ds + 8 * c)};
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
             for (int i = 0; i < keys; ++i)
                 if ((bad[i / 32] >> i % 32 & 1) && k0 + i >= see[0].low && k0 + i < see[0].high) none = __builtin_nanf("");
         stage ^= 1;
-        if (more) finish(stage);
+        if (more) finish(stage, k0 + keys);
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[0][db] += none;
@@ -551,6 +565,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
+    __shared__ int found[2];   // the tile of a stage that holds infinite numbers or NaN
     __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -586,15 +601,18 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
         qs.load(i0, part.high - i0, tiles + stage * 2 * tile);
         gs.load(i0, part.high - i0, tiles + (stage * 2 + 1) * tile);
     };
-    const auto finish = [&](int stage) {
+    const auto finish = [&](int stage, int i0) {
         qs.finish(tiles + stage * 2 * tile);
         gs.finish(tiles + (stage * 2 + 1) * tile);
+        if (block.masks(i0, rows) && holds_odd<T, DP, 2 * rows>(tiles + stage * 2 * tile)) found[stage] = i0;
         if ((int)threadIdx.x < 2 * rows) shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
         __syncthreads();
     };
+    if (threadIdx.x < 2) found[threadIdx.x] = -1;
+    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
-        finish(0);
+        finish(0, part.low);
     }
     int stage = 0;
     for (int i0 = part.low; i0 < part.high; i0 += rows) {
@@ -602,12 +620,11 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
         if (more) load(i0 + rows, stage ^ 1);
         const T* const qt = tiles + stage * 2 * tile;
         const T* const gt = qt + tile;
-        if (block.masks(i0, rows)) {
+        if (block.masks(i0, rows) && found[stage] == i0) {
             // (keys that see a row that is not finite have no gradient that is)
             take_out_odd<T, DP, 2 * rows>(tiles + stage * 2 * tile, [&](int row, int, float) { shared[stage][0][row % rows] = __builtin_nanf(""); });
         }
         if (i0 < spans.high && i0 + rows > spans.low) {
-            const bool mask = i0 < spans.all_low || i0 + rows > spans.all_high || i0 + rows > part.high;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 // (heads of 128: one product's fragments at a time, as the sums and the fragments that stay take most of the registers)
@@ -626,20 +643,17 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
                         dp[4 * i + j] = -less[j];
                     }
                 }
-                const int low = see[0].low, high = see[0].high, first = i0 + 32 * b + 4 * h;
-                if (mask) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) e[r] = first + row_of(r) >= low && first + row_of(r) < high ? e[r] : 0.0f;
-                }
+                const bool below = i0 < spans.all_low, beyond = i0 + rows > min(spans.all_high, part.high);
+                const int low = see[0].low - i0 - 32 * b - 4 * h, high = see[0].high - i0 - 32 * b - 4 * h;
+                if (below) hide_below(e, low, 0.0f);
+                if (beyond) hide_from(e, high, 0.0f);
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
                 if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
-                if (mask) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) ds[r] = first + row_of(r) >= low && first + row_of(r) < high ? ds[r] : 0.0f;
-                }
+                if (below) hide_below(ds, low, 0.0f);
+                if (beyond) hide_from(ds, high, 0.0f);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int at = 32 * b + 16 * c;
@@ -651,7 +665,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
             }
         }
         stage ^= 1;
-        if (more) finish(stage);
+        if (more) finish(stage, i0 + rows);
     }
     const int j = mine + (int)threadIdx.x % 32;
     if (j >= p.keys) return;

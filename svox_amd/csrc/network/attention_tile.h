@@ -183,36 +183,35 @@ struct Loader<T, DP, rows, false> {
 // Infinite numbers and NaN in a tile of which not every row is seen by every lane.  A score that is masked is 0, and 0 times what its row
 // holds is 0, unless that is one of these: they are taken out of the tile, and those who do see them are told otherwise.
 //
-// Found by all threads together; f(row, column, number) for each, by one thread.  The tile can be read when this returns.
-template <class T, int DP, int rows, class F>
-__device__ __forceinline__ bool take_out_odd(T* lds, F f) {
-    using Shape = Tile<T, DP>;
+// Whether the pieces of a tile that this wavefront's threads have loaded hold any; before the barrier behind which the tile is read.
+template <class T, int DP, int rows>
+__device__ __forceinline__ bool holds_odd(const T* lds) {
     typedef unsigned Words __attribute__((ext_vector_type(4)));
-    typedef typename Few<T, Shape::V>::vector Piece;
-    constexpr int each = rows * Shape::pieces / kAttendThreads;
     // (an exponent of ones becomes a carry into the sign's place)
     constexpr unsigned low = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu, one = sizeof(T) == 4 ? 0x00800000u : std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u;
     unsigned found = 0;
 #pragma unroll
-    for (int i = 0; i < each; ++i) {
-        const Words w = (reinterpret_cast<const Words*>(lds)[i * kAttendThreads + threadIdx.x] & low) + one;
+    for (int i = 0; i < rows * Tile<T, DP>::pieces / kAttendThreads; ++i) {
+        const int place = i * kAttendThreads + (int)threadIdx.x;
+        const Words w = (*reinterpret_cast<const Words*>(lds + Tile<T, DP>::at(place / Tile<T, DP>::pieces, place % Tile<T, DP>::pieces)) & low) + one;
         found |= w[0] | w[1] | w[2] | w[3];
     }
-    if (!__syncthreads_or((found & ~low) != 0)) return false;
+    return __any((found & ~low) != 0);
+}
+// Takes them out, all threads together; f(row, column, number) for each, by one thread.  The tile can be read when this returns.
+template <class T, int DP, int rows, class F>
+__device__ __forceinline__ void take_out_odd(T* lds, F f) {
+    __syncthreads();
 #pragma unroll 1
-    for (int i = 0; i < each; ++i) {
-        const int place = i * kAttendThreads + (int)threadIdx.x, row = place / Shape::pieces, slot = place % Shape::pieces;
-        const int column = (slot / Shape::ring * Shape::ring + ((slot % Shape::ring) ^ Shape::turn(row))) * Shape::V;
-#pragma unroll 1
-        for (int j = 0; j < Shape::V; ++j) {
-            const float v = (float)lds[place * Shape::V + j];
-            if (__builtin_fabsf(v) < __builtin_inff()) continue;
-            f(row, column + j, v);
-            lds[place * Shape::V + j] = (T)0.0f;
-        }
+    for (int i = (int)threadIdx.x; i < rows * DP; i += kAttendThreads) {
+        const int row = i / DP, column = i % DP;
+        T* const at = lds + Tile<T, DP>::at(row, column / Tile<T, DP>::V) + column % Tile<T, DP>::V;
+        const float v = (float)*at;
+        if (__builtin_fabsf(v) < __builtin_inff()) continue;
+        f(row, column, v);
+        *at = (T)0.0f;
     }
     __syncthreads();
-    return true;
 }
 
 // Fragments of a row in memory, as an operand that stays in registers: numbers 16 t + 8 half .. of `row`, zeros from `dim` on.

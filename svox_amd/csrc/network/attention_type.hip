@@ -26,6 +26,7 @@ AttendArgs<T> args(const SvoxAttention& s) {
     p.keys = (int)s.keys;
     p.dim = s.dim;
     p.scale = s.scale;
+    p.last_first = s.causal;   // (the last queries see most, as the first keys are seen by most)
     return p;
 }
 template <class K>
@@ -100,6 +101,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     }
     if ((p.dk || p.dv) && p.keys > 0) {
         Room mine = room;
+        p.last_first = 0;
         if (of_k.splits > 1) {
             p.used = mine.take<int>(p.kv_heads * pieces(p.keys, of_k.rows));
             p.part = mine.take<float>(2 * (int64_t)p.kv_heads * of_k.splits * p.keys * DP);
