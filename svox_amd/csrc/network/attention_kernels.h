@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     constexpr int join_numbers = across > 1 ? 4 * 32 * (DP + 2) : 0;   // floats
     constexpr int tile_bytes = 2 * S::stages * S::tile * (int)sizeof(T), join_bytes = join_numbers * 4;
     __shared__ __attribute__((aligned(16))) char lds[tile_bytes > join_bytes ? tile_bytes : join_bytes];
-    __shared__ int found[2];                     // the tile of a stage that holds infinite numbers or NaN
+    __shared__ int found[2];                     // the tile of a stage that holds infinite numbers or NaN (or chance: it is looked at once more)
     __shared__ unsigned kinds[3][S::keys][DB];   // NaN, inf and -inf that were taken out of a tile of v
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -170,12 +170,21 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         load_row<T, DP, direct>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
 
     const float to2 = p.scale * kLog2E;
-    f32x16 acc[N][DB];
+    // Narrow heads: vector instructions, the exponentials first of all, are what bounds them (64 scores some 36 cycles, their products 8 to 16): the
+    // exponentials' sum is one more product, with ones, of which a lane's first number is kept.
+    constexpr bool by_product = sizeof(T) == 2 && DP <= 64;
+    f32x16 acc[N][DB], ones_acc[N];
     float m[N], l[N];
+    Eight ones;
+    if constexpr (by_product) {
+        const float one[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+        ones = F::pack(one);
+    }
     T* const tiles = reinterpret_cast<T*>(lds);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         m[n] = -__builtin_inff(), l[n] = 0.0f;
+        ones_acc[n] = f32x16{};
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[n][db] = f32x16{};
     }
@@ -190,12 +199,13 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         if (block.masks(k0, S::keys) && holds_odd<T, DP, S::keys>(tiles + (stage * 2 + 1) * S::tile)) found[stage] = k0;
         __syncthreads();
     };
-    if (threadIdx.x < 2) found[threadIdx.x] = -1;
-    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
         finish(0, part.low);
     }
+    // vmcnt(0).  What stays in registers has arrived; the compiler, which does not see the tiles' loads, would else wait for it where it is first
+    // used in the loop, and for the next tile with it.
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += S::keys) {
         const bool more = k0 + S::keys < part.high;
@@ -244,11 +254,12 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                 for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][n][r]);
-                most = fmaxf(most, other_half(most));
+                most = most_of_halves(most);
                 const float from = most == -__builtin_inff() ? 0.0f : most * to2;   // (nothing seen yet: exponentials of -inf are 0)
                 if (__any(most != m[n])) {
                     const float less = __builtin_amdgcn_exp2f(__builtin_fmaf(m[n], to2, -from));
-                    l[n] *= less;
+                    if constexpr (by_product) ones_acc[n][0] *= less;
+                    else l[n] *= less;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) acc[n][db] *= less;
                     m[n] = most;
@@ -259,7 +270,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][r], to2, -from));
-                        l[n] += x[r];
+                        if constexpr (!by_product) l[n] += x[r];
                     }
                     e[b][0][n] = F::pack(x);
                     e[b][1][n] = F::pack(x + 8);
@@ -271,6 +282,9 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                 for (int c = 0; c < 2; ++c) {
                     const int at = wave % across * S::mine + 32 * b + 16 * c;
                     accumulate<T, DP, N>(acc, vt, at, e[b][c]);
+                    if constexpr (by_product)
+#pragma unroll
+                        for (int n = 0; n < N; ++n) ones_acc[n] = F::mma(ones, e[b][c][n], ones_acc[n]);
                 }
             if (odd) {
                 // (v's numbers that were taken out, for the lanes that see them: p is positive)
@@ -303,7 +317,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     }
 
 #pragma unroll
-    for (int n = 0; n < N; ++n) l[n] += other_half(l[n]);
+    for (int n = 0; n < N; ++n) l[n] = by_product ? ones_acc[n][0] : sum_of_halves(l[n]);
     if constexpr (across > 1) {
         // the wavefronts' sums, joined by the first: every lane finds its own numbers of the others
         static_assert(across == 4 && N == 1, "all wavefronts share rows");
@@ -413,13 +427,16 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_many_kernel(Attend
         for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d, kWave));
         f32x4 sum = {};
         float l = 0.0f;
+#pragma unroll 4
         for (int s = group; s < used; s += groups) {
             const int64_t at = first + (int64_t)s * p.rows;
             const f32x2 stat = p.stats[at];
-            if (stat[0] == -__builtin_inff()) continue;   // (nothing seen, nothing stored)
+            const f32x4 part = *reinterpret_cast<const f32x4*>(p.part + at * DP + 4 * lane);
+            const bool some = stat[0] != -__builtin_inff();   // (else nothing was seen, and nothing stored)
             const float less = __builtin_amdgcn_exp2f(stat[0] - most);
-            l = __builtin_fmaf(stat[1], less, l);
-            sum += *reinterpret_cast<const f32x4*>(p.part + at * DP + 4 * lane) * less;
+            l += some ? stat[1] * less : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += some ? part[j] * less : 0.0f;
         }
         __syncthreads();
         room[threadIdx.x] = sum;
@@ -433,7 +450,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_many_kernel(Attend
     }
 }
 
-// delta: a row's sum of do o, by sixteen lanes
+// delta: a row's sum of do o, by sixteen lanes; where dq, whose kernel computes it too, is not asked for
 template <class T>
 __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs<T> p) {
     constexpr int V = 16 / (int)sizeof(T);
@@ -466,7 +483,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
-    __shared__ int found[2];              // the tile of a stage that holds infinite numbers or NaN
+    __shared__ int found[2];              // the tile of a stage that holds infinite numbers or NaN, or none
     __shared__ unsigned bad[keys / 32];   // keys that are not finite
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -485,7 +502,17 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     Eight q[DP / 16], g[DP / 16];
     load_row<T, DP, direct>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
     load_row<T, DP, direct>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
-    const float lse = p.lse[(int64_t)place.head * p.rows + row], delta = p.delta[(int64_t)place.head * p.rows + row];
+    const float lse = p.lse[(int64_t)place.head * p.rows + row];
+    float delta = 0.0f;
+    {
+        Eight o[DP / 16];
+        const unsigned token = (unsigned)row / (unsigned)p.group;
+        load_row<T, DP, direct>(p.out + (((int64_t)token * p.kv_heads + place.head) * p.group + (row - (int)token * p.group)) * p.dim, p.dim, o);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) delta += dot<T>(o[t], g[t]);
+        delta = sum_of_halves(delta);
+    }
+    if (place.split == 0 && h == 0 && mine + (int)threadIdx.x % 32 < p.rows) p.delta[(int64_t)place.head * p.rows + row] = delta;
     const float to2 = p.scale * kLog2E;
     f32x16 acc[1][DB];
     float none = 0.0f;
@@ -502,12 +529,13 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         if (block.masks(k0, keys) && holds_odd<T, DP, keys>(tiles + stage * 2 * tile)) found[stage] = k0;
         __syncthreads();
     };
-    if (threadIdx.x < 2) found[threadIdx.x] = -1;
-    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
         finish(0, part.low);
     }
+    // vmcnt(0).  What stays in registers has arrived; the compiler, which does not see the tiles' loads, would else wait for it where it is first
+    // used in the loop, and for the next tile with it.
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     int stage = 0;
     for (int k0 = part.low; k0 < part.high; k0 += keys) {
         const bool more = k0 + keys < part.high;
@@ -565,7 +593,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
-    __shared__ int found[2];   // the tile of a stage that holds infinite numbers or NaN
+    __shared__ int found[2];   // the tile of a stage that holds infinite numbers or NaN, or none
     __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
@@ -608,12 +636,13 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
         if ((int)threadIdx.x < 2 * rows) shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
         __syncthreads();
     };
-    if (threadIdx.x < 2) found[threadIdx.x] = -1;
-    __syncthreads();
     if (part.low < part.high) {
         load(part.low, 0);
         finish(0, part.low);
     }
+    // vmcnt(0).  What stays in registers has arrived; the compiler, which does not see the tiles' loads, would else wait for it where it is first
+    // used in the loop, and for the next tile with it.
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     int stage = 0;
     for (int i0 = part.low; i0 < part.high; i0 += rows) {
         const bool more = i0 + rows < part.high;

@@ -22,15 +22,15 @@ constexpr int64_t kAttendBlocks = 512;   // two for each compute unit
 
 // How a tile's other axis is split, `size` at a time.  What a tile sees of it only the GPU knows; in all likelihood it is `length`, and where
 // there are several sequences, or a causal one, it differs from tile to tile.  A block gets as many steps as leave two blocks for every
-// place on the GPU, two at least; as many blocks may share a tile as a tile of the whole axis would need, in launches of up to 4096 blocks.
+// place on the GPU; as many blocks may share a tile as a tile of the whole axis would need, in launches of up to 4096 blocks.
 inline AttendPlan split(AttendPlan plan, int64_t blocks, int64_t length, int64_t whole, int64_t size) {
     plan.splits = plan.steps = 1;
     if (blocks < 1 || blocks >= 2 * kAttendBlocks) return plan;
     const int64_t steps = pieces(length, size) * blocks / (2 * kAttendBlocks);
-    plan.steps = (int)(steps < 2 ? 2 : steps);
+    plan.steps = (int)(steps < 1 ? 1 : steps);
     const int64_t wanted = pieces(pieces(whole, size), plan.steps), most = 8 * kAttendBlocks / blocks;
     const int64_t splits = wanted < most ? wanted : most;
-    plan.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+    plan.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
     return plan;
 }
 // The part of `other` that a tile of `rows` out of `all` sees where sequences are of one length.

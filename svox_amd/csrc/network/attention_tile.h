@@ -46,6 +46,16 @@ struct Frag<float> {
     static __device__ __forceinline__ Eight pack(const float* v) { return (Eight){v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}; }
 };
 
+// the sum of the products of two fragments' numbers
+template <class T>
+__device__ __forceinline__ float dot(typename Frag<T>::Eight a, typename Frag<T>::Eight b) {
+    const auto x = __builtin_bit_cast(typename Frag<T>::Numbers, a), y = __builtin_bit_cast(typename Frag<T>::Numbers, b);
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)x[e], (float)y[e], sum);
+    return sum;
+}
+
 // row of a result's number r, and of a fragment's number e that holds results
 __device__ __forceinline__ constexpr int row_of(int r) { return (r & 3) + 8 * (r >> 2); }
 
@@ -330,8 +340,15 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* l
     }
 }
 
-// the other half's number
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, kWave); }
+// the sum, and the larger, of a lane's number and that of the lane 32 away
+__device__ __forceinline__ float sum_of_halves(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+__device__ __forceinline__ float most_of_halves(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
 
 // A row of a result, a lane's 16 numbers of every 32: to memory as `V`, times `factor`.
 template <class V, int DB>

@@ -82,7 +82,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     p.delta = room.take<float>((int64_t)p.kv_heads * p.rows);
     const AttendPlan of_q = query_grad_plan(s), of_k = key_grad_plan(s);
     const bool direct = direct_loads(s) && direct_loads(s, g), runs = in_runs(s);
-    if (p.rows > 0)
+    if (p.rows > 0 && !p.dq)
         hipLaunchKernelGGL((attend_delta_kernel<T>), dim3((unsigned)least(pieces((int64_t)p.rows * p.kv_heads, 16), 1 << 14)), dim3(kAttendThreads), 0, stream, p);
     const auto sum = [&](const float* part, int64_t rows, const AttendPlan& plan, int group, float factor, T* to) {
         if (to)

@@ -21,7 +21,7 @@ namespace svox_network {
 
 using namespace svox_decoder;
 
-constexpr int kRotateThreads = 256, kRotateRows = 16, kRotateMostDim = 256, kRotateMostBlocks = 1024;
+constexpr int kRotateThreads = 256, kRotateTurns = 2048, kRotateMostDim = 256, kRotateMostBlocks = 1024;
 
 template <class T>
 constexpr int kRotatePairs = 16 / (int)sizeof(T);
@@ -140,7 +140,7 @@ template <class T, int lanes, bool interleaved, bool backward>
 __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p) {
     constexpr int W = kRotatePairs<T>, groups = kRotateThreads / lanes;
     constexpr bool accurate = sizeof(T) == 4;
-    __shared__ float2 turns[kRotateRows * kRotateMostDim / 2];
+    __shared__ float2 turns[kRotateTurns];
     __shared__ float sums[backward ? kRotateThreads * 2 * W : 1];
     const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, pairs = p.rotated / 2;
     const RotatePiece piece = piece_of<W>(lane, p.dim, p.rotated);
@@ -234,18 +234,21 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
     }
 }
 
-// The weights' gradients: columns of [blocks][2 dim], 16 to a block, by 16 threads each.
+// The weights' gradients: columns of [blocks][2 dim], 16 to a block, by 64 threads each.  (1024 rows of 256: 29 us by 16 threads, XX by 64.)
 template <class T>
-__global__ __launch_bounds__(256) void rotate_join_kernel(const float* part, int blocks, int dim, T* q_weight, T* k_weight) {
-    __shared__ float room[256];
+__global__ __launch_bounds__(1024) void rotate_join_kernel(const float* part, int blocks, int dim, T* q_weight, T* k_weight) {
+    __shared__ float room[1024];
     const int column = blockIdx.x * 16 + threadIdx.x % 16, from = threadIdx.x / 16;
     float sum = 0.0f;
     if (column < 2 * dim)
-        for (int b = from; b < blocks; b += 16) sum += part[(int64_t)b * 2 * dim + column];
+#pragma unroll 8
+        for (int b = from; b < blocks; b += 64) sum += part[(int64_t)b * 2 * dim + column];
     room[threadIdx.x] = sum;
-    __syncthreads();
+    for (int n = 32; n > 0; n /= 2) {
+        __syncthreads();
+        if (from < n) room[threadIdx.x] = sum += room[threadIdx.x + n * 16];
+    }
     if (from != 0 || column >= 2 * dim) return;
-    for (int i = 1; i < 16; ++i) sum += room[i * 16 + threadIdx.x];
     T* const to = column < dim ? q_weight : k_weight;
     if (to) to[column < dim ? column : column - dim] = (T)sum;
 }

@@ -17,10 +17,12 @@ int lanes_of(const SvoxRotateHeads& s) {
     while (lanes < pieces_of(s)) lanes *= 2;
     return lanes;
 }
-// rows of a block at a time: enough heads for four of every lane group
+// Rows of a block at a time: enough of them for two keys' heads of every lane group, as far as LDS holds their angles, and as long as there are
+// rows for all blocks.  (262 144 rows of 8 + 2 heads of 32: 16 rows 105 us, 64 rows 98.)
 int rows_at_once(const SvoxRotateHeads& s) {
-    const int64_t rows = pieces(4 * kRotateThreads / lanes_of(s), (int64_t)s.heads + s.kv_heads);
-    return (int)(rows < kRotateRows ? rows : kRotateRows);
+    int64_t rows = pieces(2 * kRotateThreads / lanes_of(s), (int64_t)s.kv_heads);
+    rows = least(least(rows, kRotateTurns / (s.rotated < 2 ? 1 : s.rotated / 2)), pieces(s.rows, 1024));
+    return (int)(rows < 1 ? 1 : rows);
 }
 RotateArgs<T> args(const SvoxRotateHeads& s) {
     RotateArgs<T> p{};
@@ -81,7 +83,7 @@ int launch_rotate_backward<T>(const SvoxRotateHeads& s, const void* grad_q, cons
     if (s.interleaved) launch<true, true>(p, lanes_of(s), blocks, stream);
     else launch<false, true>(p, lanes_of(s), blocks, stream);
     if (part)
-        hipLaunchKernelGGL((rotate_join_kernel<T>), dim3((unsigned)pieces(2 * s.dim, 16)), dim3(256), 0, stream, part, blocks, s.dim, (T*)out_q_weight,
+        hipLaunchKernelGGL((rotate_join_kernel<T>), dim3((unsigned)pieces(2 * s.dim, 16)), dim3(1024), 0, stream, part, blocks, s.dim, (T*)out_q_weight,
                            (T*)out_k_weight);
     return check_launch("rotate_heads_backward");
 }
