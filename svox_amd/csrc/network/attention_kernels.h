@@ -221,6 +221,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
         }
         const int kw = k0 + wave % across * S::mine;   // this wavefront's keys
         if (kw < spans.high && kw + S::mine > spans.low && kw < part.high) {
+            if constexpr (DP == 128) __builtin_amdgcn_s_setprio(1);   // (the other wavefront of the SIMD has exponentials to compute meanwhile: 633 -> 600 us)
             f32x16 s[KB][N];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
@@ -233,6 +234,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                     for (int n = 0; n < N; ++n) s[b][n] = F::mma(a, q[n][t], s[b][n]);
                 }
             }
+            if constexpr (DP == 128) __builtin_amdgcn_s_setprio(0);
             // (the tile's end lies beyond what some lane sees, if it lies beyond the part)
             if (kw < spans.all_low) {
 #pragma unroll
@@ -594,7 +596,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ int found[2];   // the tile of a stage that holds infinite numbers or NaN, or none
-    __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and delta of a tile's rows
+    __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and -delta of a tile's rows
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
     if (place.tile < 0) return;
@@ -609,9 +611,15 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     const Span part = share.span;
     clip(see, part);
 
+    // (heads of 128: six of the eight fragments of v stay in LDS.  The registers that would be missing lay in memory, and to load them again was to wait for
+    // the next tile too: 1460 -> 1390 us for 16 384 causal rows, 8 heads.)
+    constexpr int kept = sizeof(T) == 2 && DP == 128 ? 2 : DP / 16;
+    __shared__ Eight rest[kept < DP / 16 ? DP / 16 - kept : 1][kept < DP / 16 ? kAttendThreads : 1];
     Eight k[DP / 16], v[DP / 16];
     load_row<T, DP, direct>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
     load_row<T, DP, direct>(p.v + (int64_t)key * p.v_stride + place.head * p.v_head, p.dim, v);
+#pragma unroll
+    for (int t = kept; t < DP / 16; ++t) rest[t - kept][threadIdx.x] = v[t];
     const float to2 = p.scale * kLog2E;
     const float* const lse = p.lse + (int64_t)place.head * p.rows;
     const float* const delta = p.delta + (int64_t)place.head * p.rows;
@@ -624,7 +632,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     const auto load = [&](int i0, int stage) {
         if ((int)threadIdx.x < 2 * rows) {
             const int at = min(i0 + (int)threadIdx.x % rows, part.high - 1);
-            stat = (int)threadIdx.x < rows ? lse[at] : delta[at];
+            stat = (int)threadIdx.x < rows ? lse[at] : -delta[at];
         }
         qs.load(i0, part.high - i0, tiles + stage * 2 * tile);
         gs.load(i0, part.high - i0, tiles + (stage * 2 + 1) * tile);
@@ -669,7 +677,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         e[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], to2, -from[j]));
-                        dp[4 * i + j] = -less[j];
+                        dp[4 * i + j] = less[j];
                     }
                 }
                 const bool below = i0 < spans.all_low, beyond = i0 + rows > min(spans.all_high, part.high);
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
                 if (below) hide_below(e, low, 0.0f);
                 if (beyond) hide_from(e, high, 0.0f);
 #pragma unroll
-                for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), v[t], dp);
+                for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), t < kept ? v[t] : rest[t < kept ? 0 : t - kept][threadIdx.x], dp);
                 if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
