@@ -36,7 +36,7 @@ struct AttendArgs {
     float scale;
 };
 
-constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLog2E = 1.4426950408889634f, kNoSum = 3.0e38f;   // (the lse of a row that sees no key)
 
 // The work of a block: a tile, a kv head, a part of the tile's other axis.
 struct Place {
@@ -155,6 +155,10 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     if (place.tile < 0) return;
     const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32 * N;
 
+    Eight q[N][DP / 16];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        load_row<T, DP, direct>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
     Span see[N];
     Spans block;
     const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, r0, S::rows, p.group, see, block);
@@ -163,11 +167,6 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
     const Span part = share.span;
     clip(see, part);
-
-    Eight q[N][DP / 16];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        load_row<T, DP, direct>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
 
     const float to2 = p.scale * kLog2E;
     // Narrow heads: vector instructions, the exponentials first of all, are what bounds them (64 scores some 36 cycles, their products 8 to 16): the
@@ -229,6 +228,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                 for (int n = 0; n < N; ++n) s[b][n] = f32x16{};
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
+                    if (sizeof(T) == 4 && 16 * t >= p.dim) break;   // (float32's products are dear)
                     const Eight a = Tile<T, DP>::along(kt, wave % across * S::mine + 32 * b, t);
 #pragma unroll
                     for (int n = 0; n < N; ++n) s[b][n] = F::mma(a, q[n][t], s[b][n]);
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
             const unsigned token = (unsigned)r / (unsigned)p.group;
             store_row<T, DB>(p.y + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[n],
                              some ? 1.0f / l[n] : 0.0f);
-            if (p.lse && h == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : __builtin_inff();
+            if (p.lse && h == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : kNoSum;
         }
     }
 }
@@ -382,7 +382,7 @@ __device__ __forceinline__ void store_joined(const AttendArgs<T>& p, int64_t i, 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (4 * lane + j < p.dim) to[4 * lane + j] = (T)(sum[j] * factor);
-    if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : __builtin_inff();
+    if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : kNoSum;
 }
 
 // The splits' sums of a row, where there are several: a row by as many lanes as its numbers are fours, one split after another.
@@ -492,6 +492,9 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     if (place.tile < 0) return;
     const int r0 = place.tile * rows, mine = r0 + wave * 32, row = min(mine + (int)threadIdx.x % 32, p.rows - 1);
 
+    Eight q[DP / 16], g[DP / 16];
+    load_row<T, DP, direct>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
+    load_row<T, DP, direct>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
     Span see[1];
     Spans block;
     const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, r0, rows, p.group, see, block);
@@ -501,9 +504,6 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     const Span part = share.span;
     clip(see, part);
 
-    Eight q[DP / 16], g[DP / 16];
-    load_row<T, DP, direct>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
-    load_row<T, DP, direct>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
     const float lse = p.lse[(int64_t)place.head * p.rows + row];
     float delta = 0.0f;
     {
@@ -555,6 +555,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
                 f32x16 s = {}, dp = {};
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
+                    if (sizeof(T) == 4 && 16 * t >= p.dim) break;
                     s = F::mma(Tile<T, DP>::along(kt, 32 * b, t), q[t], s);
                     dp = F::mma(Tile<T, DP>::along(vt, 32 * b, t), g[t], dp);
                 }
@@ -640,8 +641,11 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
     const auto finish = [&](int stage, int i0) {
         qs.finish(tiles + stage * 2 * tile);
         gs.finish(tiles + (stage * 2 + 1) * tile);
-        if (block.masks(i0, rows) && holds_odd<T, DP, 2 * rows>(tiles + stage * 2 * tile)) found[stage] = i0;
-        if ((int)threadIdx.x < 2 * rows) shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
+        // (where q or the gradient of a row is not finite, one of these is not)
+        if ((int)threadIdx.x < 2 * rows) {
+            shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
+            if (!(__builtin_fabsf(stat) < __builtin_inff())) found[stage] = i0;
+        }
         __syncthreads();
     };
     if (part.low < part.high) {
@@ -667,7 +671,10 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
                 // (heads of 128: one product's fragments at a time, as the sums and the fragments that stay take most of the registers)
                 f32x16 s = {}, dp;
 #pragma unroll
-                for (int t = 0; t < DP / 16; ++t) s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
+                for (int t = 0; t < DP / 16; ++t) {
+                    if (sizeof(T) == 4 && 16 * t >= p.dim) break;
+                    s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
+                }
                 if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
                 float e[16], ds[16];
 #pragma unroll
@@ -685,7 +692,10 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) 
                 if (below) hide_below(e, low, 0.0f);
                 if (beyond) hide_from(e, high, 0.0f);
 #pragma unroll
-                for (int t = 0; t < DP / 16; ++t) dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), t < kept ? v[t] : rest[t < kept ? 0 : t - kept][threadIdx.x], dp);
+                for (int t = 0; t < DP / 16; ++t) {
+                    if (sizeof(T) == 4 && 16 * t >= p.dim) break;
+                    dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), t < kept ? v[t] : rest[t < kept ? 0 : t - kept][threadIdx.x], dp);
+                }
                 if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];

@@ -22,13 +22,14 @@ constexpr int64_t kAttendBlocks = 512;   // two for each compute unit
 
 // How a tile's other axis is split, `size` at a time.  What a tile sees of it only the GPU knows; in all likelihood it is `length`, and where
 // there are several sequences, or a causal one, it differs from tile to tile.  A block gets as many steps as leave two blocks for every
-// place on the GPU; as many blocks may share a tile as a tile of the whole axis would need, in launches of up to 4096 blocks.
+// place on the GPU, two at least; as many blocks may share a tile as a tile of the whole axis would need, in launches of up to 2048 blocks (one that
+// finds nothing left to do costs two microseconds of its place).
 inline AttendPlan split(AttendPlan plan, int64_t blocks, int64_t length, int64_t whole, int64_t size) {
     plan.splits = plan.steps = 1;
     if (blocks < 1 || blocks >= 2 * kAttendBlocks) return plan;
     const int64_t steps = pieces(length, size) * blocks / (2 * kAttendBlocks);
-    plan.steps = (int)(steps < 1 ? 1 : steps);
-    const int64_t wanted = pieces(pieces(whole, size), plan.steps), most = 8 * kAttendBlocks / blocks;
+    plan.steps = (int)(steps < 2 ? 2 : steps);
+    const int64_t wanted = pieces(pieces(whole, size), plan.steps), most = 4 * kAttendBlocks / blocks;
     const int64_t splits = wanted < most ? wanted : most;
     plan.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
     return plan;
@@ -68,9 +69,9 @@ inline bool direct_loads(const SvoxAttention& s, const SvoxAttentionGrads& g) {
     return direct_heads(s, g.grad, g.grad_stride, g.grad_head, s.heads / s.kv_heads);
 }
 
-// Whether the blocks of an XCD take a few tiles side by side: where many sequences share the keys out, so that one's stay in an XCD's cache.
-// Heads of few long sequences go round the XCDs instead.
-inline bool in_runs(const SvoxAttention& s) { return s.sequences >= 16; }
+// Whether the blocks of an XCD take a few tiles side by side: where many sequences share the keys out, so that one's stay in an XCD's cache, and
+// there are tiles for all XCDs.  Heads of few long sequences go round the XCDs instead.
+inline bool in_runs(const SvoxAttention& s, int64_t tiles) { return s.sequences >= 16 && tiles * s.kv_heads >= kAttendBlocks; }
 
 inline int64_t attention_space(const SvoxAttention& s, bool backward) {
     const int64_t rows = s.queries * (s.heads / s.kv_heads), width = attend_width(s.dim);

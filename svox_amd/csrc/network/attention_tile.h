@@ -282,13 +282,24 @@ struct Sequences {
 // `last`.  Where sequences are in order, spans do not go back from token to token, also those that are empty.
 __device__ __forceinline__ Span span_of(const Sequences& s, bool keys, int t, int first, int last) {
     const Offsets &mine = keys ? s.q : s.k, &other = keys ? s.k : s.q;
-    const int lane = (int)threadIdx.x % kWave, a = last_not_beyond(mine, first);
-    // the places from the first token's sequence on, one a lane: those of all tokens in all likelihood
-    const int place = min(a + lane, mine.n), mine_at = mine(place), other_at = other(place);
+    const int lane = (int)threadIdx.x % kWave;
+    // 64 places, one a lane, about where sequences of one length would have the first token's, or all of them: it is among them as a rule, and nothing
+    // has to be looked for first
+    const int guess = (int)((int64_t)first * mine.n / max(mine.total, 1)) - kWave / 2;
+    int a = max(0, min(guess, mine.n + 1 - kWave));
+    int place = min(a + lane, mine.n), mine_at = mine(place), other_at = other(place);
+    int found = __popcll(__ballot(mine_at <= first)) - 1;
+    if (found < 0 ? a > 0 : (found == kWave - 1 && a + found < mine.n) || (__builtin_amdgcn_readlane(mine_at, kWave - 1) <= last && a + kWave - 1 < mine.n)) {
+        a = last_not_beyond(mine, first);
+        place = min(a + lane, mine.n), mine_at = mine(place), other_at = other(place);
+        found = 0;
+    }
+    found = max(found, 0);
     int m0, m1, o0, o1;
-    if (__builtin_amdgcn_readlane(mine_at, 1) > last) {
-        m0 = __builtin_amdgcn_readlane(mine_at, 0), m1 = __builtin_amdgcn_readlane(mine_at, 1);
-        o0 = __builtin_amdgcn_readlane(other_at, 0), o1 = __builtin_amdgcn_readlane(other_at, 1);
+    const int next = min(found + 1, kWave - 1);
+    if (__builtin_amdgcn_readlane(mine_at, next) > last) {
+        m0 = __builtin_amdgcn_readlane(mine_at, found), m1 = __builtin_amdgcn_readlane(mine_at, next);
+        o0 = __builtin_amdgcn_readlane(other_at, found), o1 = __builtin_amdgcn_readlane(other_at, next);
     } else if (a + kWave - 1 >= mine.n || __builtin_amdgcn_readlane(mine_at, kWave - 1) > last) {
         int i = 0;
 #pragma unroll
@@ -305,8 +316,8 @@ __device__ __forceinline__ Span span_of(const Sequences& s, bool keys, int t, in
             if (mine(middle) <= t) low = middle;
             else high = middle - 1;
         }
-        const int next = min(low + 1, mine.n);
-        m0 = mine(low), m1 = mine(next), o0 = other(low), o1 = other(next);
+        const int after = min(low + 1, mine.n);
+        m0 = mine(low), m1 = mine(after), o0 = other(low), o1 = other(after);
     }
     o1 = max(o0, o1);
     if (t < m0) return {o0, o0};

@@ -30,18 +30,18 @@ AttendArgs<T> args(const SvoxAttention& s) {
     return p;
 }
 template <class K>
-void launch(K kernel, AttendArgs<T>& p, int64_t count, const AttendPlan& plan, bool runs, hipStream_t stream) {
+void launch(K kernel, AttendArgs<T>& p, const SvoxAttention& s, int64_t count, const AttendPlan& plan, hipStream_t stream) {
     p.tiles = (int)pieces(count, plan.rows);
     p.splits = plan.splits;
     p.steps = plan.steps;
-    p.runs = runs;
+    p.runs = in_runs(s, p.tiles);
     const int64_t units = (int64_t)p.tiles * p.kv_heads;
-    hipLaunchKernelGGL(kernel, grid_of((runs ? svox_decoder::up_to(units, 8 * kAttendRun) : units) * plan.splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
+    hipLaunchKernelGGL(kernel, grid_of((p.runs ? svox_decoder::up_to(units, 8 * kAttendRun) : units) * plan.splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
 }
 template <bool direct>
-void forward(AttendArgs<T>& p, const AttendPlan& plan, bool runs, hipStream_t stream) {
-    if (plan.few) launch(attend_kernel<T, DP, 1, 4, direct>, p, p.rows, plan, runs, stream);
-    else launch(attend_kernel<T, DP, 1, 1, direct>, p, p.rows, plan, runs, stream);
+void forward(AttendArgs<T>& p, const SvoxAttention& s, const AttendPlan& plan, hipStream_t stream) {
+    if (plan.few) launch(attend_kernel<T, DP, 1, 4, direct>, p, s, p.rows, plan, stream);
+    else launch(attend_kernel<T, DP, 1, 1, direct>, p, s, p.rows, plan, stream);
 }
 
 }  // namespace
@@ -58,11 +58,11 @@ int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void*
         p.stats = room.take<f32x2>((int64_t)p.kv_heads * plan.splits * p.rows);
         p.used = room.take<int>(p.kv_heads * pieces(p.rows, plan.rows));
     }
-    if (direct_loads(s)) forward<true>(p, plan, in_runs(s), stream);
-    else forward<false>(p, plan, in_runs(s), stream);
-    // (one row after another by 1 to 16 splits, 8 rows of 64 by 257 splits: 180 us and 9 by blocks, 12 and 40 by lanes)
+    if (direct_loads(s)) forward<true>(p, s, plan, stream);
+    else forward<false>(p, s, plan, stream);
+    // (240 000 rows of up to 2 splits: 180 us by blocks, 13 by lanes; 32 rows of 12 splits: 5 us by blocks, 12 by lanes)
     const int64_t joined = (int64_t)p.kv_heads * p.rows;
-    if (plan.splits > 16)
+    if (plan.splits > 16 || (plan.splits > 1 && joined <= 4096))
         hipLaunchKernelGGL((attend_join_many_kernel<T, DP>), dim3((unsigned)least(joined, 4096)), dim3(kAttendThreads), 0, stream, p, plan.rows);
     else if (plan.splits > 1)
         hipLaunchKernelGGL((attend_join_kernel<T, DP>), dim3((unsigned)least(pieces(joined, kAttendThreads / (DP / 4)), 1 << 14)), dim3(kAttendThreads), 0, stream, p,
@@ -81,7 +81,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     Room room(workspace);
     p.delta = room.take<float>((int64_t)p.kv_heads * p.rows);
     const AttendPlan of_q = query_grad_plan(s), of_k = key_grad_plan(s);
-    const bool direct = direct_loads(s) && direct_loads(s, g), runs = in_runs(s);
+    const bool direct = direct_loads(s) && direct_loads(s, g);
     if (p.rows > 0 && !p.dq)
         hipLaunchKernelGGL((attend_delta_kernel<T>), dim3((unsigned)least(pieces((int64_t)p.rows * p.kv_heads, 16), 1 << 14)), dim3(kAttendThreads), 0, stream, p);
     const auto sum = [&](const float* part, int64_t rows, const AttendPlan& plan, int group, float factor, T* to) {
@@ -95,8 +95,8 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.used = mine.take<int>(p.kv_heads * pieces(p.rows, of_q.rows));
             p.part = mine.take<float>((int64_t)p.kv_heads * of_q.splits * p.rows * DP);
         }
-        if (direct) launch(attend_query_grad_kernel<T, DP, true>, p, p.rows, of_q, runs, stream);
-        else launch(attend_query_grad_kernel<T, DP, false>, p, p.rows, of_q, runs, stream);
+        if (direct) launch(attend_query_grad_kernel<T, DP, true>, p, s, p.rows, of_q, stream);
+        else launch(attend_query_grad_kernel<T, DP, false>, p, s, p.rows, of_q, stream);
         if (of_q.splits > 1) sum(p.part, p.rows, of_q, p.group, p.scale, p.dq);
     }
     if ((p.dk || p.dv) && p.keys > 0) {
@@ -106,8 +106,8 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.used = mine.take<int>(p.kv_heads * pieces(p.keys, of_k.rows));
             p.part = mine.take<float>(2 * (int64_t)p.kv_heads * of_k.splits * p.keys * DP);
         }
-        if (direct) launch(attend_key_grad_kernel<T, DP, true>, p, p.keys, of_k, runs, stream);
-        else launch(attend_key_grad_kernel<T, DP, false>, p, p.keys, of_k, runs, stream);
+        if (direct) launch(attend_key_grad_kernel<T, DP, true>, p, s, p.keys, of_k, stream);
+        else launch(attend_key_grad_kernel<T, DP, false>, p, s, p.keys, of_k, stream);
         if (of_k.splits > 1) {
             sum(p.part, p.keys, of_k, 1, p.scale, p.dk);
             sum(p.part + (int64_t)p.kv_heads * of_k.splits * p.keys * DP, p.keys, of_k, 1, 1.0f, p.dv);
