@@ -72,6 +72,7 @@ def _network_units():
                    [f"-DSVOX_DECODER_TYPE={of}", f"-DSVOX_ATTEND_WIDTH={width}"])
     for of in DECODER_TYPES:
         yield f"rotate_{of.lower()}", os.path.join("network", "rotate_type.hip"), [f"-DSVOX_DECODER_TYPE={of}"]
+    yield "order", os.path.join("network", "attention_order.hip"), []
     yield "clip", os.path.join("network", "clip.hip"), []
     yield "network", os.path.join("network", "network.hip"), []
 

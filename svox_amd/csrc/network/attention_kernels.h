@@ -32,6 +32,7 @@ struct AttendArgs {
     int tiles;
     int splits, steps;                 // blocks that may share a tile's other axis, and how many steps along it each is to have at least
     int* used;                         // [kv head][tile]: how many of them did
+    const int* order;                  // tiles, those with the most to do first, or NULL
     int runs, last_first;              // blocks of an XCD take a few tiles side by side, else heads go round the XCDs; the last tiles come first
     float scale;
 };
@@ -49,6 +50,10 @@ __device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
     const unsigned units = gridDim.x / p.splits, unit = blockIdx.x % units;
     Place at;
     at.split = blockIdx.x / units;
+    if (p.order) {
+        const unsigned i = unit / p.kv_heads;
+        return {p.order[i], (int)(unit - i * p.kv_heads), at.split};
+    }
     if (p.runs) {
         // (each time round the XCDs one further: sequences of a power of two would otherwise give one XCD all of their last tiles)
         const unsigned i = unit / 8, round = i / kAttendRun, xcd = (unit + round) % 8, position = (round * 8 + xcd) * kAttendRun + i % kAttendRun;

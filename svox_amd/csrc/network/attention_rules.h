@@ -16,6 +16,7 @@ struct AttendPlan {
     int rows;            // of a block's tile
     int splits, steps;   // blocks that may share a tile's other axis, and the least steps of each
     bool few;
+    bool ordered;        // tiles in the order of what they have to do, which a launch of its own finds out
 };
 
 constexpr int64_t kAttendBlocks = 512;   // two for each compute unit
@@ -34,6 +35,13 @@ inline AttendPlan split(AttendPlan plan, int64_t blocks, int64_t length, int64_t
     plan.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
     return plan;
 }
+// Whether tiles are to be put in order: where sequences may differ in length, the blocks are more than the GPU has places for but not so many that the
+// last ones matter little, and each has enough to do for the launch, some six microseconds, to pay.  (Its places are in LDS: up to 4095 sequences.)
+inline AttendPlan ordered(AttendPlan plan, const SvoxAttention& s, int64_t tiles, int64_t length) {
+    const int64_t blocks = tiles * s.kv_heads;
+    plan.ordered = s.sequences >= 2 && s.sequences < 4096 && blocks >= kAttendBlocks / 2 && blocks < 8 * kAttendBlocks && length >= 256;
+    return plan;
+}
 // The part of `other` that a tile of `rows` out of `all` sees where sequences are of one length.
 inline int64_t likely_length(int64_t other, int64_t sequences, int64_t rows, int64_t all) {
     const int64_t sequences_of_tile = all > 0 ? 1 + (rows * sequences - 1) / all : 1;
@@ -42,17 +50,20 @@ inline int64_t likely_length(int64_t other, int64_t sequences, int64_t rows, int
 }
 
 inline AttendPlan forward_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads), blocks = pieces(rows, 128) * s.kv_heads;
-    if (blocks >= kAttendBlocks) return split({128, 1, 1, false}, blocks, likely_length(s.keys, s.sequences, 128, rows), s.keys, 64);
-    return split({32, 1, 1, true}, pieces(rows, 32) * s.kv_heads, likely_length(s.keys, s.sequences, 32, rows), s.keys, 128);
+    const int64_t rows = s.queries * (s.heads / s.kv_heads), tiles = pieces(rows, 128);
+    if (tiles * s.kv_heads >= kAttendBlocks) {
+        const int64_t length = likely_length(s.keys, s.sequences, 128, rows);
+        return ordered(split({128, 1, 1, false, false}, tiles * s.kv_heads, length, s.keys, 64), s, tiles, length);
+    }
+    return split({32, 1, 1, true, false}, pieces(rows, 32) * s.kv_heads, likely_length(s.keys, s.sequences, 32, rows), s.keys, 128);
 }
 inline AttendPlan query_grad_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads);
-    return split({128, 1, 1, false}, pieces(rows, 128) * s.kv_heads, likely_length(s.keys, s.sequences, 128, rows), s.keys, 64);
+    const int64_t rows = s.queries * (s.heads / s.kv_heads), tiles = pieces(rows, 128), length = likely_length(s.keys, s.sequences, 128, rows);
+    return ordered(split({128, 1, 1, false, false}, tiles * s.kv_heads, length, s.keys, 64), s, tiles, length);
 }
 inline AttendPlan key_grad_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads);
-    return split({128, 1, 1, false}, pieces(s.keys, 128) * s.kv_heads, likely_length(rows, s.sequences, 128, s.keys), rows, 64);
+    const int64_t rows = s.queries * (s.heads / s.kv_heads), tiles = pieces(s.keys, 128), length = likely_length(rows, s.sequences, 128, s.keys);
+    return ordered(split({128, 1, 1, false, false}, tiles * s.kv_heads, length, rows, 64), s, tiles, length);
 }
 
 // Whether tiles go from memory to LDS 16 bytes at a time: everything lies at whole numbers of 16 bytes, and no tile of up to 128 rows reaches
@@ -79,12 +90,14 @@ inline int64_t attention_space(const SvoxAttention& s, bool backward) {
     const auto space = [&](const AttendPlan& plan, int64_t count, int64_t numbers) {
         return plan.splits > 1 ? whole(s.kv_heads * plan.splits * count * numbers * 4) + whole(s.kv_heads * pieces(count, plan.rows) * 4) : 0;
     };
+    const auto order = [&](const AttendPlan& plan, int64_t count) { return plan.ordered ? whole(pieces(count, plan.rows) * 4) : 0; };
     if (!backward) {
         const AttendPlan plan = forward_plan(s);
-        return space(plan, rows, width) + (plan.splits > 1 ? whole(s.kv_heads * plan.splits * rows * 8) : 0);
+        return order(plan, rows) + space(plan, rows, width) + (plan.splits > 1 ? whole(s.kv_heads * plan.splits * rows * 8) : 0);
     }
-    const int64_t q = space(query_grad_plan(s), rows, width), k = space(key_grad_plan(s), s.keys, 2 * width);
-    return whole(s.kv_heads * rows * 4) + (q > k ? q : k);
+    const AttendPlan of_q = query_grad_plan(s), of_k = key_grad_plan(s);
+    const int64_t q = space(of_q, rows, width), k = space(of_k, s.keys, 2 * width);
+    return whole(s.kv_heads * rows * 4) + order(of_q, rows) + order(of_k, s.keys) + (q > k ? q : k);
 }
 
 }  // namespace svox_network

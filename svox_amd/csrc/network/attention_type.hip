@@ -1,5 +1,6 @@
 // attention_type.hip -- the attention kernels of one type (SVOX_DECODER_TYPE) for heads of up to SVOX_ATTEND_WIDTH numbers, and their launches.
 #include "attention_kernels.h"
+#include "attention_order.h"
 #include "attention_rules.h"
 #include "entry.h"
 
@@ -34,9 +35,14 @@ void launch(K kernel, AttendArgs<T>& p, const SvoxAttention& s, int64_t count, c
     p.tiles = (int)pieces(count, plan.rows);
     p.splits = plan.splits;
     p.steps = plan.steps;
-    p.runs = in_runs(s, p.tiles);
+    p.runs = !p.order && in_runs(s, p.tiles);
     const int64_t units = (int64_t)p.tiles * p.kv_heads;
     hipLaunchKernelGGL(kernel, grid_of((p.runs ? svox_decoder::up_to(units, 8 * kAttendRun) : units) * plan.splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
+}
+// One axis of the launch that puts tiles in order.
+OrderArgs::Axis order_axis(const AttendArgs<T>& p, const AttendPlan& plan, bool keys, int* to) {
+    const int count = keys ? p.rows : p.keys;
+    return {to, (int)pieces(count, plan.rows), count, plan.rows, p.group, keys};
 }
 template <bool direct>
 void forward(AttendArgs<T>& p, const SvoxAttention& s, const AttendPlan& plan, hipStream_t stream) {
@@ -57,6 +63,12 @@ int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void*
         p.part = room.take<float>((int64_t)p.kv_heads * plan.splits * p.rows * DP);
         p.stats = room.take<f32x2>((int64_t)p.kv_heads * plan.splits * p.rows);
         p.used = room.take<int>(p.kv_heads * pieces(p.rows, plan.rows));
+    }
+    if (plan.ordered) {
+        OrderArgs o{p.seq, {}};
+        o.axis[0] = order_axis(p, plan, true, room.take<int>(pieces(p.rows, plan.rows)));
+        p.order = o.axis[0].to;
+        launch_order(o, 1, stream);
     }
     if (direct_loads(s)) forward<true>(p, s, plan, stream);
     else forward<false>(p, s, plan, stream);
@@ -84,6 +96,14 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     const bool direct = direct_loads(s) && direct_loads(s, g);
     if (p.rows > 0 && !p.dq)
         hipLaunchKernelGGL((attend_delta_kernel<T>), dim3((unsigned)least(pieces((int64_t)p.rows * p.kv_heads, 16), 1 << 14)), dim3(kAttendThreads), 0, stream, p);
+    const int* order[2] = {};
+    {
+        OrderArgs o{p.seq, {}};
+        int n = 0;
+        if (of_q.ordered && p.dq && p.rows > 0) order[0] = (o.axis[n++] = order_axis(p, of_q, true, room.take<int>(pieces(p.rows, of_q.rows)))).to;
+        if (of_k.ordered && (p.dk || p.dv) && p.keys > 0) order[1] = (o.axis[n++] = order_axis(p, of_k, false, room.take<int>(pieces(p.keys, of_k.rows)))).to;
+        if (n > 0) launch_order(o, n, stream);
+    }
     const auto sum = [&](const float* part, int64_t rows, const AttendPlan& plan, int group, float factor, T* to) {
         if (to)
             hipLaunchKernelGGL((attend_sum_kernel<T, DP>), dim3((unsigned)least(pieces(rows * p.kv_heads, kAttendThreads / (DP / 4)), 1 << 14)), dim3(kAttendThreads),
@@ -95,6 +115,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.used = mine.take<int>(p.kv_heads * pieces(p.rows, of_q.rows));
             p.part = mine.take<float>((int64_t)p.kv_heads * of_q.splits * p.rows * DP);
         }
+        p.order = order[0];
         if (direct) launch(attend_query_grad_kernel<T, DP, true>, p, s, p.rows, of_q, stream);
         else launch(attend_query_grad_kernel<T, DP, false>, p, s, p.rows, of_q, stream);
         if (of_q.splits > 1) sum(p.part, p.rows, of_q, p.group, p.scale, p.dq);
@@ -106,6 +127,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.used = mine.take<int>(p.kv_heads * pieces(p.keys, of_k.rows));
             p.part = mine.take<float>(2 * (int64_t)p.kv_heads * of_k.splits * p.keys * DP);
         }
+        p.order = order[1];
         if (direct) launch(attend_key_grad_kernel<T, DP, true>, p, s, p.keys, of_k, stream);
         else launch(attend_key_grad_kernel<T, DP, false>, p, s, p.keys, of_k, stream);
         if (of_k.splits > 1) {
