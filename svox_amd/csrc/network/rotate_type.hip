@@ -18,7 +18,7 @@ int lanes_of(const SvoxRotateHeads& s) {
     return lanes;
 }
 // Rows of a block at a time: enough of them for two keys' heads of every lane group, as far as LDS holds their angles, and as long as there are
-// rows for all blocks.  (262 144 rows of 8 + 2 heads of 32: 16 rows 105 us, 64 rows 98.)
+// rows for all blocks.  (262 144 rows of 8 + 2 heads of 32: 16 rows 105 us, 64 rows and more 98.)
 int rows_at_once(const SvoxRotateHeads& s) {
     int64_t rows = pieces(2 * kRotateThreads / lanes_of(s), (int64_t)s.kv_heads);
     rows = least(least(rows, kRotateTurns / (s.rotated < 2 ? 1 : s.rotated / 2)), pieces(s.rows, 1024));
