@@ -596,7 +596,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
 
 // ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them
 template <class T, int DP, bool direct>
-__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 32 ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64 && !direct) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
