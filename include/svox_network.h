@@ -94,12 +94,14 @@ typedef struct SvoxAttention {
     float scale;                 /* > 0 */
 } SvoxAttention;
 
-/* out (queries, heads, dim); lse (queries * heads floats) or NULL: what svox_attention_backward needs of the scores' sums. */
-int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* out (queries, heads, dim).  What svox_attention_backward needs besides, or NULL: lse (queries * heads floats), of the scores' sums; rest
+ * (queries, heads, dim), what rounding to 16 bits took from out. */
+int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* rest, void* workspace, int64_t workspace_bytes, void* stream);
 
 typedef struct SvoxAttentionGrads {
     const void* out;                      /* what svox_attention left */
     const float* lse;
+    const void* rest;                     /* or NULL: 0 */
     const void* grad;                     /* of out, (queries, heads, dim) */
     int64_t grad_stride, grad_head;       /* from row to row and from head to head */
     void *q, *k, *v;                      /* where the gradients go, dense; NULL where one is not wanted */

@@ -33,7 +33,7 @@ class AttentionC(ctypes.Structure):
 
 
 class AttentionGradsC(ctypes.Structure):
-    _fields_ = [("out", c_void_p), ("lse", c_void_p), ("grad", c_void_p), ("grad_stride", c_int64), ("grad_head", c_int64), ("q", c_void_p),
+    _fields_ = [("out", c_void_p), ("lse", c_void_p), ("rest", c_void_p), ("grad", c_void_p), ("grad_stride", c_int64), ("grad_head", c_int64), ("q", c_void_p),
                 ("k", c_void_p), ("v", c_void_p)]
 
 
@@ -49,7 +49,7 @@ SIGNATURES = {
     "svox_rotate_heads_backward": (
         ctypes.c_int, [P(RotateHeadsC), c_void_p, c_void_p, P(c_int64), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "svox_rotate_heads_workspace_bytes": (c_int64, [P(RotateHeadsC), c_int32]),
-    "svox_attention": (ctypes.c_int, [P(AttentionC), c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "svox_attention": (ctypes.c_int, [P(AttentionC), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "svox_attention_backward": (ctypes.c_int, [P(AttentionC), P(AttentionGradsC), c_void_p, c_int64, c_void_p]),
     "svox_attention_workspace_bytes": (c_int64, [P(AttentionC), c_int32]),
 }

@@ -21,6 +21,7 @@ template <class T>
 struct AttendArgs {
     const T *q, *k, *v, *out, *grad;   // out (tokens, heads, dim) dense
     T* y;                              // forward: the result
+    T* rest;                           // what rounding took from the result, as `out`, or NULL
     T *dq, *dk, *dv;                   // dense
     float *lse, *delta;                // [kv head][row]: log2 of the sum of exponentials, and its sum of do o
     float* part;                       // where the work of a tile is split: [kv head][split][row][DP] (keys and values: two of them)
@@ -133,6 +134,13 @@ template <class Scores>
 __device__ __forceinline__ void hide_from(Scores& s, int high, float v) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = row_of(r) < high ? s[r] : v;
+}
+
+// What is left of a number that is rounded to T.  The backward pass takes delta from both: with the rounded result alone delta was off by a
+// part in 2^11 (f16), for all of a row's keys alike, and dq and dk with it (1659 causal rows of 64: 1.54 times the error of one rounding, 1.42 so).
+template <class T>
+__device__ __forceinline__ float left_of(float v) {
+    return v - (float)(T)v;
 }
 
 // ---- forward.  Four wavefronts, of which `across` share rows and take a part of every tile's keys each.
@@ -371,8 +379,16 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
             if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f);
         } else {
             const unsigned token = (unsigned)r / (unsigned)p.group;
-            store_row<T, DB>(p.y + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[n],
-                             some ? 1.0f / l[n] : 0.0f);
+            const int64_t to = (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim;
+            const float factor = some ? 1.0f / l[n] : 0.0f;
+            store_row<T, DB>(p.y + to, p.dim, acc[n], factor);
+            if (p.rest) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[n][db][i] = left_of<T>(acc[n][db][i] * factor);
+                store_row<T, DB>(p.rest + to, p.dim, acc[n], 1.0f);
+            }
             if (p.lse && h == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : kNoSum;
         }
     }
@@ -383,10 +399,13 @@ __device__ __forceinline__ void store_joined(const AttendArgs<T>& p, int64_t i, 
     const bool some = most != -__builtin_inff();
     const float factor = some ? 1.0f / l : 0.0f;
     const int token = r / p.group;
-    T* const to = p.y + (((int64_t)token * p.kv_heads + head) * p.group + (r - token * p.group)) * p.dim;
+    const int64_t to = (((int64_t)token * p.kv_heads + head) * p.group + (r - token * p.group)) * p.dim + 4 * lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (4 * lane + j < p.dim) to[4 * lane + j] = (T)(sum[j] * factor);
+        if (4 * lane + j < p.dim) {
+            p.y[to + j] = (T)(sum[j] * factor);
+            if (p.rest) p.rest[to + j] = (T)left_of<T>(sum[j] * factor);
+        }
     if (p.lse && lane == 0) p.lse[i] = some ? most + __builtin_amdgcn_logf(l) : kNoSum;
 }
 
@@ -457,29 +476,33 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_many_kernel(Attend
     }
 }
 
-// delta: a row's sum of do o, by sixteen lanes; where dq, whose kernel computes it too, is not asked for
-template <class T>
+// delta of row `row`, whose gradient is g: its sum of do o, by two lanes
+template <class T, int DP, bool direct>
+__device__ __forceinline__ float delta_of(const AttendArgs<T>& p, int row, int head, const typename Frag<T>::Eight (&g)[DP / 16]) {
+    typename Frag<T>::Eight o[DP / 16];
+    const unsigned token = (unsigned)row / (unsigned)p.group;
+    const int64_t at = (((int64_t)token * p.kv_heads + head) * p.group + (row - (int)token * p.group)) * p.dim;
+    load_row<T, DP, direct>(p.out + at, p.dim, o);
+    float delta = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) delta += dot<T>(o[t], g[t]);
+    if (p.rest) {
+        load_row<T, DP, direct>(p.rest + at, p.dim, o);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) delta += dot<T>(o[t], g[t]);
+    }
+    return sum_of_halves(delta);
+}
+// Where dq, whose kernel computes it too, is not asked for.
+template <class T, int DP>
 __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs<T> p) {
-    constexpr int V = 16 / (int)sizeof(T);
-    const int lane = (int)threadIdx.x % 16;
-    const int64_t all = (int64_t)p.rows * p.kv_heads;
-    // (in memory's order: token, kv head, head of the group)
-    for (int64_t first = (int64_t)blockIdx.x * 16; first < all; first += (int64_t)gridDim.x * 16) {
-        const int64_t i = first + threadIdx.x / 16;
-        if (i >= all) continue;
-        const int64_t heads = (int64_t)p.kv_heads * p.group, token = i / heads;
-        const int head = (int)(i - token * heads);
-        const T* const o = p.out + i * p.dim;
-        const T* const g = p.grad + token * p.grad_stride + head * p.grad_head;
-        float sum = 0.0f;
-        for (int c = lane * V; c < p.dim; c += 16 * V) {
-            const auto a = load_some<T, V>(o + c, p.dim - c), b = load_some<T, V>(g + c, p.dim - c);
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum = __builtin_fmaf((float)a[j], (float)b[j], sum);
-        }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) sum += __shfl_xor(sum, d, kWave);
-        if (lane == 0) p.delta[(int64_t)(head / p.group) * p.rows + token * p.group + head % p.group] = sum;
+    const int64_t tiles = ((int64_t)p.rows + 127) / 128;
+    for (int64_t i = blockIdx.x; i < tiles * p.kv_heads; i += gridDim.x) {
+        const int head = (int)(i / tiles), mine = (int)(i - head * tiles) * 128 + (int)threadIdx.x / kWave * 32 + (int)threadIdx.x % 32, row = min(mine, p.rows - 1);
+        typename Frag<T>::Eight g[DP / 16];
+        load_row<T, DP, false>(row_at(p.grad, row, p.group, head, p.grad_stride, p.grad_head), p.dim, g);
+        const float delta = delta_of<T, DP, false>(p, row, head, g);
+        if (half_of() == 0 && mine < p.rows) p.delta[(int64_t)head * p.rows + row] = delta;
     }
 }
 
@@ -510,15 +533,7 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     clip(see, part);
 
     const float lse = p.lse[(int64_t)place.head * p.rows + row];
-    float delta = 0.0f;
-    {
-        Eight o[DP / 16];
-        const unsigned token = (unsigned)row / (unsigned)p.group;
-        load_row<T, DP, direct>(p.out + (((int64_t)token * p.kv_heads + place.head) * p.group + (row - (int)token * p.group)) * p.dim, p.dim, o);
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) delta += dot<T>(o[t], g[t]);
-        delta = sum_of_halves(delta);
-    }
+    const float delta = delta_of<T, DP, direct>(p, row, place.head, g);
     if (place.split == 0 && h == 0 && mine + (int)threadIdx.x % 32 < p.rows) p.delta[(int64_t)place.head * p.rows + row] = delta;
     const float to2 = p.scale * kLog2E;
     f32x16 acc[1][DB];

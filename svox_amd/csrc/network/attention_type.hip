@@ -53,10 +53,11 @@ void forward(AttendArgs<T>& p, const SvoxAttention& s, const AttendPlan& plan, h
 }  // namespace
 
 template <>
-int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void* workspace, hipStream_t stream) {
+int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void* rest, void* workspace, hipStream_t stream) {
     AttendArgs<T> p = args(s);
     p.y = (T*)out;
     p.lse = lse;
+    p.rest = (T*)rest;
     const AttendPlan plan = forward_plan(s);
     Room room(workspace);
     if (plan.splits > 1) {
@@ -89,13 +90,14 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
     p.grad = (const T*)g.grad;
     p.grad_stride = g.grad_stride, p.grad_head = g.grad_head;
     p.lse = const_cast<float*>(g.lse);
+    p.rest = (T*)const_cast<void*>(g.rest);
     p.dq = (T*)g.q, p.dk = (T*)g.k, p.dv = (T*)g.v;
     Room room(workspace);
     p.delta = room.take<float>((int64_t)p.kv_heads * p.rows);
     const AttendPlan of_q = query_grad_plan(s), of_k = key_grad_plan(s);
     const bool direct = direct_loads(s) && direct_loads(s, g);
     if (p.rows > 0 && !p.dq)
-        hipLaunchKernelGGL((attend_delta_kernel<T>), dim3((unsigned)least(pieces((int64_t)p.rows * p.kv_heads, 16), 1 << 14)), dim3(kAttendThreads), 0, stream, p);
+        hipLaunchKernelGGL((attend_delta_kernel<T, DP>), dim3((unsigned)least(pieces(p.rows, 128) * p.kv_heads, 1 << 14)), dim3(kAttendThreads), 0, stream, p);
     const int* order[2] = {};
     {
         OrderArgs o{p.seq, {}};

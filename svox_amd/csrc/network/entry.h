@@ -25,7 +25,7 @@ int rotate_backward_blocks(const SvoxRotateHeads& s);   // each with a row of pa
 
 // (defined for every type and width in attention_type.hip)
 template <class T, int width>
-int launch_attention(const SvoxAttention& s, void* out, float* lse, void* workspace, hipStream_t stream);
+int launch_attention(const SvoxAttention& s, void* out, float* lse, void* rest, void* workspace, hipStream_t stream);
 template <class T, int width>
 int launch_attention_backward(const SvoxAttention& s, const SvoxAttentionGrads& grads, void* workspace, hipStream_t stream);
 

@@ -208,12 +208,12 @@ SVOX_API int64_t svox_attention_workspace_bytes(const SvoxAttention* spec, int32
     return attention_space(*spec, backward != 0);
 }
 
-SVOX_API int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+SVOX_API int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* rest, void* workspace, int64_t workspace_bytes, void* stream) {
     SVOX_TRY(check_attention(spec));
     if (spec->queries == 0) return SVOX_OK;
     if (!out) return fail(SVOX_ERR_NULL_POINTER, "out is NULL");
     SVOX_TRY(check_space(workspace, workspace_bytes, attention_space(*spec, false)));
-    SVOX_BY_TYPE_AND_WIDTH(*spec, return (launch_attention<T, width>(*spec, out, lse, workspace, (hipStream_t)stream)));
+    SVOX_BY_TYPE_AND_WIDTH(*spec, return (launch_attention<T, width>(*spec, out, lse, rest, workspace, (hipStream_t)stream)));
 }
 
 SVOX_API int svox_attention_backward(const SvoxAttention* spec, const SvoxAttentionGrads* grads, void* workspace, int64_t workspace_bytes, void* stream) {

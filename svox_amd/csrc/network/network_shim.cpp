@@ -299,19 +299,21 @@ Attend dense_heads(Attend a) {
     a.q = heads_of(a.q), a.k = heads_of(a.k), a.v = heads_of(a.v);
     return a;
 }
-Tensor attention_forward(const Attend& a, Tensor* lse) {
+// `lse` and `rest`: what a backward pass needs; rest only of 16-bit types
+Tensor attention_forward(const Attend& a, Tensor* lse, Tensor* rest) {
     const On on(a.q);
     Tensor y = make_like(a.q);
     if (lse) *lse = make({a.q.size(0) * a.q.size(1)}, at::kFloat, a.q);
+    if (rest && a.q.scalar_type() != at::kFloat) *rest = make_like(a.q);
     const SvoxAttention s = attention_spec(a);
     const int64_t bytes = status(lib.svox_attention_workspace_bytes(&s, 0), "attention");
     const Tensor space = bytes_on(a.q, bytes);
-    status(lib.svox_attention(&s, y.data_ptr(), lse ? (float*)lse->data_ptr() : nullptr, at_or_null(space), bytes, on.stream), "attention");
+    status(lib.svox_attention(&s, y.data_ptr(), lse ? (float*)lse->data_ptr() : nullptr, rest ? at_or_null(*rest) : nullptr, at_or_null(space), bytes, on.stream), "attention");
     return y;
 }
 
 struct AttendNode : torch::autograd::Node {
-    SavedVariable saved_[5], out_, lse_;   // q, k, v and the offsets
+    SavedVariable saved_[5], out_, lse_, rest_;   // q, k, v and the offsets
     bool causal = false;
     double scale = 0.0;
 
@@ -321,6 +323,7 @@ struct AttendNode : torch::autograd::Node {
         for (SavedVariable& v : saved_) v.reset_data();
         out_.reset_data();
         lse_.reset_data();
+        rest_.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
@@ -328,7 +331,7 @@ struct AttendNode : torch::autograd::Node {
         if (!grads[0].defined()) return out;
         once("attention", grads[0]);
         Attend a{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), causal, scale};
-        const Tensor y = out_.unpack(shared_from_this()), lse = lse_.unpack();
+        const Tensor y = out_.unpack(shared_from_this()), lse = lse_.unpack(), rest = rest_.unpack();
         const On on(a.q);
         check_like(grads[0], a.q, "grad_output", "q");
         a = dense_heads(a);
@@ -340,6 +343,7 @@ struct AttendNode : torch::autograd::Node {
         SvoxAttentionGrads g{};
         g.out = y.data_ptr();
         g.lse = (const float*)lse.data_ptr();
+        g.rest = at_or_null(rest);
         g.grad = dy.data_ptr();
         g.grad_stride = dy.stride(0), g.grad_head = dy.stride(1);
         g.q = at_or_null(out[0]), g.k = at_or_null(out[1]), g.v = at_or_null(out[2]);
@@ -384,16 +388,17 @@ Tensor attention(Attend a) {
     if (!(a.scale > 0.0) || std::isinf(a.scale)) fail("scale must be > 0 and finite, got " + std::to_string(a.scale));
     make_contiguous(a.offsets);
     make_contiguous(a.key_offsets);
-    if (!wants_node({&q, &k, &v}, "attention")) return attention_forward(dense_heads(a), nullptr);
+    if (!wants_node({&q, &k, &v}, "attention")) return attention_forward(dense_heads(a), nullptr, nullptr);
     const auto node = node_of<AttendNode>(q, k, v);
-    Tensor lse, y;
+    Tensor lse, rest, y;
     {
         const at::AutoDispatchBelowADInplaceOrView guard;
-        y = attention_forward(dense_heads(a), &lse);
+        y = attention_forward(dense_heads(a), &lse, &rest);
     }
     const Tensor* const saved[5] = {&q, &k, &v, &a.offsets, &a.key_offsets};
     for (int i = 0; i < 5; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
     node->lse_ = SavedVariable(lse, false);
+    node->rest_ = SavedVariable(rest, false);
     node->causal = a.causal;
     node->scale = a.scale;
     torch::autograd::set_history(y, node);

@@ -103,23 +103,23 @@ def test_argument_errors_of_attention_come_before_anything_touches_a_device():
     def grads(**kw):
         return with_fields(N.AttentionGradsC(out=16, lse=16, grad=16, grad_stride=32, grad_head=8, q=16, k=16, v=16), kw)
 
-    assert lib.svox_attention(None, 16, None, 16, 1 << 20, None) == -1
+    assert lib.svox_attention(None, 16, None, None, 16, 1 << 20, None) == -1
     for kw, rc in [({"dtype": 3}, -3), ({"queries": -1}, -2), ({"keys": -1}, -2), ({"heads": 0}, -2), ({"kv_heads": 0}, -2), ({"heads": 5}, -2), ({"dim": 0}, -2),
                    ({"dim": 129}, -4), ({"scale": 0.0}, -2), ({"scale": -1.0}, -2), ({"scale": math.nan}, -2), ({"scale": math.inf}, -2), ({"sequences": 0}, -2),
                    ({"sequences": 2}, -1), ({"key_offsets": 16}, -1), ({"offsets": 16}, -2), ({"q": None}, -1), ({"k": None}, -1), ({"v": None}, -1),
                    ({"queries": 1 << 30, "offsets": 16, "key_offsets": 16}, -4), ({"keys": 1 << 31}, -4), ({"heads": 1 << 20, "queries": 1 << 11}, -4),
                    ({"q_stride": -1}, -2), ({"v_head": -8}, -2), ({"k_stride": 1 << 45}, -2)]:
-        assert lib.svox_attention(spec(**kw), 16, None, 16, 1 << 40, None) == rc, kw
+        assert lib.svox_attention(spec(**kw), 16, None, None, 16, 1 << 40, None) == rc, kw
         assert lib.svox_attention_backward(spec(**kw), grads(), 16, 1 << 40, None) == rc, kw
         assert lib.svox_network_last_error()
-    assert lib.svox_attention(spec(), None, None, 16, 1 << 20, None) == -1
-    assert lib.svox_attention(spec(queries=0, q=None), None, None, None, 0, None) == 0
+    assert lib.svox_attention(spec(), None, None, None, 16, 1 << 20, None) == -1
+    assert lib.svox_attention(spec(queries=0, q=None), None, None, None, None, 0, None) == 0
     long = spec(keys=100000)
     least = lib.svox_attention_workspace_bytes(long, 0)
     assert least > 0 and lib.svox_attention_workspace_bytes(spec(), 0) == 0
-    assert lib.svox_attention(long, 16, None, None, least, None) == -1
-    assert lib.svox_attention(long, 16, None, 16, least - 1, None) == -2
-    assert lib.svox_attention(long, 16, None, 8, least, None) == -2
+    assert lib.svox_attention(long, 16, None, None, None, least, None) == -1
+    assert lib.svox_attention(long, 16, None, None, 16, least - 1, None) == -2
+    assert lib.svox_attention(long, 16, None, None, 8, least, None) == -2
     least = lib.svox_attention_workspace_bytes(spec(), 1)
     assert least > 0
     assert lib.svox_attention_backward(spec(), None, 16, least, None) == -1
