@@ -108,7 +108,8 @@ __device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int min
     for (int n = 0; n < N; ++n) {
         // (the upper lanes look at the block's first and last row)
         const int r = mine + 32 * n + lane % 32;
-        Span v = span_of(s, keys, (lane < 32 ? min(r, last) : lane == 32 ? r0 : last) / per_token, r0 / per_token, last / per_token);
+        const int looked = lane < 32 ? min(r, last) : lane == 32 ? r0 : last;
+        Span v = per_token == 1 ? span_of(s, keys, looked, r0, last) : span_of(s, keys, looked / per_token, r0 / per_token, last / per_token);
         v.low *= per_other, v.high *= per_other;
         if (n == 0)
             block = {__builtin_amdgcn_readlane(v.low, 32), __builtin_amdgcn_readlane(v.high, 33), __builtin_amdgcn_readlane(v.low, 33),
@@ -506,12 +507,13 @@ __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs
     }
 }
 
-// ---- dq: rows as forward, through the keys they see
+// ---- dq: rows as forward, through the keys they see.  (float32, heads of 32: tiles of 32 keys leave registers for four wavefronts a SIMD, 64 for
+// three: 512 windows of 64 cells, 4 heads of 16, 34 -> 28 us; heads of 64 lose as much as they gain, those of 128 have room for no more.)
 template <class T, int DP, bool direct>
 __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_query_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
-    constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP == 128 ? 32 : 64, tile = keys * DP, KB = keys / 32;
+    constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP != 64 ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ int found[2];              // the tile of a stage that holds infinite numbers or NaN, or none
     __shared__ unsigned bad[keys / 32];   // keys that are not finite
@@ -609,12 +611,13 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     }
 }
 
-// ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them
+// ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them.  (Rows of a tile, 32 or 64: float32 with heads of 32 437 -> 400 us
+// by 32, with heads of 64 2600 -> 2820; heads of 128 have registers for 32.)
 template <class T, int DP, bool direct>
 __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64 && !direct) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
-    constexpr int DB = DP / 32, keys = 128, rows = DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
+    constexpr int DB = DP / 32, keys = 128, rows = (sizeof(T) == 4 && DP == 32) || DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ int found[2];   // the tile of a stage that holds infinite numbers or NaN, or none
     __shared__ __attribute__((aligned(16))) float shared[2][2][rows];   // lse and -delta of a tile's rows

@@ -250,6 +250,7 @@ struct Offsets {
     const void* at;   // or NULL: one sequence, 0 .. total
     int wide, n;
     int total;
+    float each;       // sequences to a token, in the mean
     __device__ __forceinline__ int operator()(int i) const {
         if (!at) return i == 0 ? 0 : total;
         const int64_t v = wide ? ((const int64_t*)at)[i] : (int64_t)((const int32_t*)at)[i];
@@ -285,7 +286,7 @@ __device__ __forceinline__ Span span_of(const Sequences& s, bool keys, int t, in
     const int lane = (int)threadIdx.x % kWave;
     // 64 places, one a lane, about where sequences of one length would have the first token's, or all of them: it is among them as a rule, and nothing
     // has to be looked for first
-    const int guess = (int)((int64_t)first * mine.n / max(mine.total, 1)) - kWave / 2;
+    const int guess = (int)((float)first * mine.each) - kWave / 2;
     int a = max(0, min(guess, mine.n + 1 - kWave));
     int place = min(a + lane, mine.n), mine_at = mine(place), other_at = other(place);
     int found = __popcll(__ballot(mine_at <= first)) - 1;

@@ -18,8 +18,12 @@ AttendArgs<T> args(const SvoxAttention& s) {
     p.k_stride = s.k_stride, p.k_head = s.k_head;
     p.v_stride = s.v_stride, p.v_head = s.v_head;
     const void* const keys = s.key_offsets ? s.key_offsets : s.offsets;
-    p.seq.q = {s.offsets, s.wide_offsets, s.offsets ? (int)s.sequences : 1, (int)s.queries};
-    p.seq.k = {keys, s.wide_offsets, keys ? (int)s.sequences : 1, (int)s.keys};
+    const auto offsets = [&](const void* at, int64_t total) {
+        const int n = at ? (int)s.sequences : 1;
+        return Offsets{at, s.wide_offsets, n, (int)total, total > 0 ? (float)n / (float)total : 0.0f};
+    };
+    p.seq.q = offsets(s.offsets, s.queries);
+    p.seq.k = offsets(keys, s.keys);
     p.seq.causal = s.causal;
     p.group = s.heads / s.kv_heads;
     p.kv_heads = s.kv_heads;
