@@ -58,14 +58,14 @@ def rotate_heads(q, k, positions, frequencies, q_weight=None, k_weight=None, int
 def clip_norm(tensors, max_norm):
     """The norm of all numbers of many tensors together, and the tensors scaled to `max_norm` where it is larger.
 
-    :param tensors: float32, float16 or bfloat16 tensors of one GPU, of any shapes and also of different types
+    :param tensors: float32, float16 or bfloat16 tensors of one GPU, of any shapes and also of different types, or one of them
     :param max_norm: >= 0
     :return: the norm, a float32 tensor without dimensions, and a list of new tensors: x * (max_norm / norm) where the norm exceeds max_norm
         and is finite, else copies of x
 
     The squares are summed in 64 bits and in an order of their own.  Nothing waits for the GPU.  Not differentiable.
     """
-    tensors = list(tensors)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.zeros(()), []
     return (_native or _calls()).clip_norm(tensors, max_norm)

@@ -76,6 +76,10 @@ def test_bounds_at_the_ends(gpu):
     assert norm == 0 and torch.equal(y, zero)
     assert svox.clip_norm([], 1.0)[1] == [] and svox.clip_grad_norm([], 1.0) == 0
     assert svox.clip_norm([zero[:0]], 1.0)[0] == 0
+    norm, out = svox.clip_norm(x, 1.0)
+    assert len(out) == 1 and torch.equal(out[0], svox.clip_norm([x], 1.0)[1][0])
+    norm, (a, b) = svox.clip_norm([x, x], 1.0)     # (twice is twice)
+    assert torch.equal(a, b) and a.data_ptr() != b.data_ptr() and abs(float(norm) - float(x.norm()) * 2 ** 0.5) <= 1e-4
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])

@@ -123,3 +123,52 @@ def test_offsets_of_any_kind_with_tiles_in_order(gpu):
         y = svox.attention(t["q"], t["k"], t["v"], torch.tensor(offsets, device=gpu), causal=True)
         grads = torch.autograd.grad(y, list(t.values()), torch.ones_like(y))
         assert all(torch.isfinite(v).all() for v in (y, *grads))
+
+
+def test_a_graph_that_is_kept_gives_the_same_gradients_again(gpu):
+    x, grad = inputs(300, 300, 4, 2, 64, torch.bfloat16, seed=10)
+    leaves = [v.requires_grad_() for v in x.values()]
+    y = svox.attention(*leaves, packed([200, 0, 100]))
+    first = torch.autograd.grad(y, leaves, grad, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, grad)))
+    with pytest.raises(RuntimeError, match="second time|already been freed"):
+        torch.autograd.grad(y, leaves, grad)
+
+
+def test_sequences_without_any_key(gpu):
+    x, grad = inputs(50, 0, 4, 2, 32, torch.float16)
+    y, grads = step(x, grad, packed([20, 30]), packed([0, 0]), causal=True)
+    assert not y.any() and not grads["q"].any() and grads["k"].shape == (0, 2, 32)
+    x, grad = inputs(0, 50, 4, 2, 32, torch.float16)
+    y, grads = step(x, grad, packed([0, 0]), packed([20, 30]))
+    assert y.shape == (0, 4, 32) and not grads["k"].any() and not grads["v"].any()
+
+
+def test_calls_from_two_threads(gpu):
+    """Each with a stream of its own; errors of one thread are not the other's."""
+    import threading
+
+    sets = [inputs(500 + i, 2000, 4, 2, 64, torch.bfloat16, seed=i) for i in range(2)]
+    want = [step(x, grad) for x, grad in sets]
+    torch.cuda.synchronize()
+    got, errors = [[], []], [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i].append(step(*sets[i]))
+                try:
+                    svox.attention(sets[i][0]["q"], sets[i][0]["k"], sets[i][0]["v"], scale=-1.0 - i)
+                except RuntimeError as e:
+                    errors[i].append(str(e))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(errors[i]) == 5 and all(f"{-1.0 - i:.6f}" in e for e in errors[i])
+        for y, grads in got[i]:
+            assert torch.equal(y, want[i][0]) and all(torch.equal(grads[n], want[i][1][n]) for n in grads)
