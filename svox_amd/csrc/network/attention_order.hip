@@ -4,8 +4,8 @@
 namespace svox_network {
 
 // The tiles of rows (queries') or keys by what they have to do, most first: blocks that start late then have little to do.  (61 causal sequences of
-// up to 1659 rows, 8 heads of 64: forward 86 -> 71 us, dq 113 -> 93, dk and dv 175 -> 157, this launch 6 to 7 for each pass.)  One block for each of both; the places are in LDS.  Tiles that have as much to do come in any order, which
-// changes nothing but when they are computed.
+// up to 1659 rows, 8 heads of 64: forward 86 -> 71 us, dq 113 -> 93, dk and dv 175 -> 157, this launch 6 to 7 for each pass.)  One block for each of
+// both; the places are in LDS.  Tiles that have as much to do come in any order, which changes nothing but when they are computed.
 constexpr int kOrderThreads = 1024, kOrderPlaces = 4096, kOrderBuckets = 1024;
 
 __global__ __launch_bounds__(kOrderThreads) void attend_order_kernel(OrderArgs p) {
