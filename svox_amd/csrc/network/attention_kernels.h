@@ -183,8 +183,8 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     clip(see, part);
 
     const float to2 = p.scale * kLog2E;
-    // Narrow heads: vector instructions are what bounds them (a product of 32 rows, 32 keys and 32 numbers takes 16 cycles, its 16 scores to a lane some
-    // 100 for exponentials, maxima and rounding): the exponentials' sum is one more product, with ones, of which a lane's first number is kept
+    // Narrow heads: vector instructions are what bounds them (32 rows, 64 keys of 32 numbers: 115 of them, of which 32 are exponentials at half the rate,
+    // some 590 cycles; 8 products of 32 cycles): the exponentials' sum is one more product, with ones, of which a lane's first number is kept
     // (512 windows of 512 cells, 4 heads of 32: 154 -> 149 us).
     constexpr bool by_product = sizeof(T) == 2 && DP <= 64;
     f32x16 acc[N][DB], ones_acc[N];
@@ -668,10 +668,10 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
     const auto finish = [&](int stage, int i0) {
         qs.finish(tiles + stage * 2 * tile);
         gs.finish(tiles + (stage * 2 + 1) * tile);
-        // (where q or the gradient of a row is not finite, one of these is not)
+        // (where q or the gradient of a row is not finite, one of these is not, or the row sees no key)
         if ((int)threadIdx.x < 2 * rows) {
             shared[stage][threadIdx.x / rows][threadIdx.x % rows] = stat;
-            if (!(__builtin_fabsf(stat) < __builtin_inff())) found[stage] = i0;
+            if (!(__builtin_fabsf(stat) < kNoSum)) found[stage] = i0;
         }
         __syncthreads();
     };
@@ -734,7 +734,6 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
                     const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
                     accumulate<T, DP, 1>(dv, gt, at, pe);
                     accumulate<T, DP, 1>(dk, qt, at, pd);
-                    
                 }
             }
         }

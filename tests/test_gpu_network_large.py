@@ -172,3 +172,20 @@ def test_calls_from_two_threads(gpu):
         assert len(errors[i]) == 5 and all(f"{-1.0 - i:.6f}" in e for e in errors[i])
         for y, grads in got[i]:
             assert torch.equal(y, want[i][0]) and all(torch.equal(grads[n], want[i][1][n]) for n in grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_rows_between_that_see_nothing(gpu, d, bad, dtype):
+    """Whatever the queries of a sequence without keys hold, and the keys of one without queries, between others of the same tiles."""
+    for queries, keys, names in (([40, 5, 40], [40, 0, 40], ("q", "grad")), ([40, 0, 40], [40, 5, 40], ("k", "v"))):
+        x, grad = inputs(sum(queries), sum(keys), 4, 2, d, dtype, seed=11)
+        clean_y, clean = step(x, grad, packed(queries), packed(keys))
+        for name in names:
+            broken, dy = {n: v.clone() for n, v in x.items()}, grad.clone()
+            (dy if name == "grad" else broken[name])[40:45, :, 1:4] = bad
+            y, grads = step(broken, dy, packed(queries), packed(keys))
+            assert torch.equal(y, clean_y), name
+            assert torch.equal(grads["q"], clean["q"]), name
+            assert torch.equal(grads["k"], clean["k"]) and torch.equal(grads["v"], clean["v"]), name
