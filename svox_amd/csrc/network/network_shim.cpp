@@ -91,7 +91,7 @@ Tensor clip_norm(const std::vector<Tensor>& all, double max_norm, std::vector<Te
     return clip(table, all[0], max_norm, "clip_norm");
 }
 
-// Gradients where they lie.  What two of them share, whole, is one gradient; what overlaps otherwise is refused.
+// Gradients where they lie.  What two of them share, whole, is one gradient; those that reach into one another otherwise are refused.
 Tensor clip_in_place(const std::vector<Tensor>& all, double max_norm) {
     const char* const name = "clip_grad_norm";
     check_clipped(all, name, max_norm);
@@ -120,7 +120,7 @@ Tensor clip_in_place(const std::vector<Tensor>& all, double max_norm) {
         if (!once.empty() && p.from < once.back().to) {
             const Tensor &a = *once.back().x, &b = *p.x;
             if (p.from == once.back().from && a.sizes() == b.sizes() && a.strides() == b.strides() && a.scalar_type() == b.scalar_type()) continue;
-            fail("svox.clip_grad_norm: two gradients share memory");
+            fail("svox.clip_grad_norm: two gradients share memory, or one lies between the numbers of another");
         }
         once.push_back(p);
     }
