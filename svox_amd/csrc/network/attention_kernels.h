@@ -153,8 +153,10 @@ struct ForwardShape {
     static constexpr int tile = keys * DP;
 };
 
+// (float32, heads of 32: registers for four wavefronts a SIMD rather than three: 512 windows of 64 cells, 4 heads of 16, 36 -> 30 us; 8 of 4096 644 -> 625.)
 template <class T, int DP, int N, int across, bool direct>
-__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 && DP == 32 && across == 1 && direct ? 4 : 2)
+void attend_kernel(AttendArgs<T> p) {
     using S = ForwardShape<T, DP, N, across>;
     using F = Frag<T>;
     using Eight = typename F::Eight;
@@ -374,27 +376,27 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int r = mine + 32 * n + (int)threadIdx.x % 32;
+        const int thread = thread_again(), half = thread / 32 % 2, r = mine + 32 * n + thread % 32;
         if (r >= p.rows) continue;
         // (what a row that sees keys has, though all of its scores are -inf, is not what one that sees none has)
         const bool some = max(see[n].low, part.low) < see[n].high;
         if (share.used > 1) {
             const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
-            if (h == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
-            if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f);
+            if (half == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
+            if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f, half);
         } else {
-            const unsigned token = (unsigned)r / (unsigned)p.group;
+            const unsigned token = (unsigned)r / again(p.group);
             const int64_t to = (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim;
             const float factor = some ? 1.0f / l[n] : 0.0f;
-            store_row<T, DB>(p.y + to, p.dim, acc[n], factor);
+            store_row<T, DB>(p.y + to, p.dim, acc[n], factor, half);
             if (p.rest) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[n][db][i] = left_of<T>(acc[n][db][i] * factor);
-                store_row<T, DB>(p.rest + to, p.dim, acc[n], 1.0f);
+                store_row<T, DB>(p.rest + to, p.dim, acc[n], 1.0f, half);
             }
-            if (p.lse && h == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : kNoSum;
+            if (p.lse && half == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : kNoSum;
         }
     }
 }
@@ -513,8 +515,11 @@ __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs
 
 // ---- dq: rows as forward, through the keys they see.  (float32, heads of 32: tiles of 32 keys leave registers for four wavefronts a SIMD, 64 for
 // three: 512 windows of 64 cells, 4 heads of 16, 34 -> 28 us; heads of 64 lose as much as they gain, those of 128 have room for no more.)
+// (Heads of 64 in 16 bits: registers for three wavefronts a SIMD rather than two, 536 -> 472 us for 16 384 causal rows, 8 heads; with two of the four
+// fragments of g in LDS as good.)
 template <class T, int DP, bool direct>
-__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_query_grad_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 2 && DP == 64 && direct ? 3 : 2)
+void attend_query_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP != 64 ? 32 : 64, tile = keys * DP, KB = keys / 32;
@@ -605,20 +610,25 @@ __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) 
     }
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[0][db] += none;
-    const int r = mine + (int)threadIdx.x % 32;
+    const int thread = thread_again(), half = thread / 32 % 2, r = mine + thread % 32;
     if (r >= p.rows) return;
     if (share.used > 1) {
-        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f);
+        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f, half);
     } else {
-        const unsigned token = (unsigned)r / (unsigned)p.group;
-        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale);
+        const unsigned token = (unsigned)r / again(p.group);
+        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale, half);
     }
 }
 
 // ---- dk and dv: a tile of keys, 32 to a wavefront, through the rows that see them.  (Rows of a tile, 32 or 64: float32 with heads of 32 437 -> 400 us
 // by 32, with heads of 64 2600 -> 2820; heads of 128 have registers for 32.)
+// How many wavefronts share a SIMD: four with heads of 32, three with heads of 64 in 16 bits, and some of v's fragments in LDS for it (`kept`), where
+// registers alone left three and two: float32 512 windows of 64 cells, 4 heads of 16, 42 -> 30 us, 8 of 4096, heads of 32, 1330 -> 1220 (16 384 causal
+// rows 2650 -> 2840: all blocks start at once, the long with the short); bfloat16 windows of 1024, 4 heads of 32, 72 -> 62; heads of 64, 16 384 causal rows
+// 786 -> 752, 61 sequences of f16 154 -> 140.
 template <class T, int DP, bool direct>
-__global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64 && !direct) ? 1 : 2) void attend_key_grad_kernel(AttendArgs<T> p) {
+__global__ __launch_bounds__(kAttendThreads, DP == 32 ? (direct ? 4 : 2) : sizeof(T) == 4 ? 1 : DP == 64 ? (direct ? 3 : 2) : direct ? 2 : 1)
+void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, keys = 128, rows = (sizeof(T) == 4 && DP == 32) || DP == 128 ? 32 : 64, tile = rows * DP, RB = rows / 32;
@@ -639,9 +649,9 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
     const Span part = share.span;
     clip(see, part);
 
-    // (heads of 128: six of the eight fragments of v stay in LDS.  The registers that would be missing lay in memory, and to load them again was to wait for
-    // the next tile too: 1460 -> 1390 us for 16 384 causal rows, 8 heads.)
-    constexpr int kept = sizeof(T) == 2 && DP == 128 ? 2 : DP / 16;
+    // (Fragments of v that stay in registers; the others stay in LDS.  Heads of 128: registers that were missing lay in memory, and to load them again was to
+    // wait for the next tile too: 1460 -> 1390 us for 16 384 causal rows, 8 heads.)
+    constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? 1 : 2;
     __shared__ Eight rest[kept < DP / 16 ? DP / 16 - kept : 1][kept < DP / 16 ? kAttendThreads : 1];
     Eight k[DP / 16], v[DP / 16];
     load_row<T, DP, direct>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
@@ -740,16 +750,16 @@ __global__ __launch_bounds__(kAttendThreads, (sizeof(T) == 4 ? DP > 32 : DP > 64
         stage ^= 1;
         if (more) finish(stage, i0 + rows);
     }
-    const int j = mine + (int)threadIdx.x % 32;
+    const int thread = thread_again(), half = thread / 32 % 2, j = mine + thread % 32;
     if (j >= p.keys) return;
     if (share.used > 1) {
         float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
-        store_row<float, DB>(at, DP, dk[0], 1.0f);
-        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], 1.0f);
+        store_row<float, DB>(at, DP, dk[0], 1.0f, half);
+        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], 1.0f, half);
     } else {
         const int64_t at = ((int64_t)j * p.kv_heads + place.head) * p.dim;
-        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale);
-        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], 1.0f);
+        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale, half);
+        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], 1.0f, half);
     }
 }
 

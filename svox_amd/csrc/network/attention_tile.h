@@ -208,12 +208,25 @@ __device__ __forceinline__ bool holds_odd(const T* lds) {
     }
     return __any((found & ~low) != 0);
 }
+
+// threadIdx.x, and a number that is the same for all, from which what is needed behind a loop, or seldom within, is found once more: the
+// compiler would else keep it in registers throughout.
+__device__ __forceinline__ int thread_again() {
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+__device__ __forceinline__ unsigned again(unsigned v) {
+    asm volatile("" : "+s"(v));
+    return v;
+}
+
 // Takes them out, all threads together; f(row, column, number) for each, by one thread.  The tile can be read when this returns.
 template <class T, int DP, int rows, class F>
 __device__ __forceinline__ void take_out_odd(T* lds, F f) {
     __syncthreads();
 #pragma unroll 1
-    for (int i = (int)threadIdx.x; i < rows * DP; i += kAttendThreads) {
+    for (int i = thread_again(); i < rows * DP; i += kAttendThreads) {
         const int row = i / DP, column = i % DP;
         T* const at = lds + Tile<T, DP>::at(row, column / Tile<T, DP>::V) + column % Tile<T, DP>::V;
         const float v = (float)*at;
@@ -364,12 +377,12 @@ __device__ __forceinline__ float most_of_halves(float v) {
 
 // A row of a result, a lane's 16 numbers of every 32: to memory as `V`, times `factor`.
 template <class V, int DB>
-__device__ __forceinline__ void store_row(V* row, int dim, const f32x16 (&acc)[DB], float factor) {
+__device__ __forceinline__ void store_row(V* row, int dim, const f32x16 (&acc)[DB], float factor, int half) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int at = db * 32 + 8 * i + 4 * half_of();
+            const int at = db * 32 + 8 * i + 4 * half;
             const f32x4 v = {acc[db][4 * i] * factor, acc[db][4 * i + 1] * factor, acc[db][4 * i + 2] * factor, acc[db][4 * i + 3] * factor};
             if (at + 4 <= dim) {
                 store_few<V, 4>(row + at, __builtin_convertvector(v, typename Few<V, 4>::vector));
