@@ -650,8 +650,8 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     clip(see, part);
 
     // (Fragments of v that stay in registers; the others stay in LDS.  Heads of 128: registers that were missing lay in memory, and to load them again was to
-    // wait for the next tile too: 1460 -> 1390 us for 16 384 causal rows, 8 heads.)
-    constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? 1 : 2;
+    // wait for the next tile too: 1460 -> 1380 us for 16 384 causal rows, 8 heads.)
+    constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? 1 : 4;
     __shared__ Eight rest[kept < DP / 16 ? DP / 16 - kept : 1][kept < DP / 16 ? kAttendThreads : 1];
     Eight k[DP / 16], v[DP / 16];
     load_row<T, DP, direct>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);

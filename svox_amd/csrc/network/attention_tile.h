@@ -61,20 +61,25 @@ __device__ __forceinline__ constexpr int row_of(int r) { return (r & 3) + 8 * (r
 
 __device__ __forceinline__ int half_of() { return (int)threadIdx.x / 32 % 2; }
 
-// A tile of rows of DP numbers in LDS.  The 16-byte pieces of a row lie in an order that depends on the row, so that both the eight
-// lanes that read eight rows at a time and the sixteen that read four rows across find them in different banks.
+// A tile of rows of DP numbers in LDS.  The 16-byte pieces of a row lie in an order that depends on the row, so that lanes that read a piece of
+// different rows, and those that read four rows across, find them in different banks.  Rows of 256 bytes fill the banks: sixteen pieces change places, for
+// sixteen rows, and reads take half as long as with eight (16 384 causal rows of bfloat16, 8 heads: forward 586 -> 576 us, dq 864 -> 848, dk and dv, which
+// wait for one product after another, 1380 either way).  Narrower rows and float32's: eight, as what sixteen save in LDS they cost in registers (heads
+// of 64: dk and dv 84 -> 86 us).
 template <class T, int DP>
 struct Tile {
     static constexpr int V = 16 / (int)sizeof(T), pieces = DP / V;   // numbers of a piece, pieces of a row
-    static constexpr int ring = pieces < 8 ? pieces : 8;              // pieces that change places
+    static constexpr bool sixteen = sizeof(T) == 2 && DP == 128;
+    static constexpr int most = sixteen ? 16 : 8, ring = pieces < most ? pieces : most;   // pieces that change places
     static __device__ __forceinline__ int turn(int row) {
-        if constexpr (pieces == 4) return (row & 2) | (row >> 2 & 1);
+        if constexpr (sixteen) return (row & 3) << 2 | (row >> 1 & 2) | (row >> 3 & 1);   // (eight rows on, the lowest bit is another)
+        else if constexpr (pieces == 4) return (row & 2) | (row >> 2 & 1);
         else return (row & 3) << 1 | (row >> 2 & 1);
     }
     // (what is the same for all lanes stands by itself: it goes into the instructions' own offsets)
     static __device__ __forceinline__ int at(int row, int piece) { return row * DP + piece / ring * ring * V + ((piece % ring) ^ turn(row)) * V; }
 
-    // numbers 16 t + 8 half .. of row r0 + lane % 32; r0 a whole number of 8
+    // numbers 16 t + 8 half .. of row r0 + lane % 32; r0 a whole number of 16
     static __device__ __forceinline__ typename Frag<T>::Eight along(const T* lds, int r0, int t) {
         const int row = (int)threadIdx.x % 32, h = half_of(), turned = turn(row);
         const T* const from = lds + row * DP;
@@ -92,11 +97,12 @@ struct Tile {
         const int lane = (int)threadIdx.x % kWave, h = half_of();
         if constexpr (sizeof(T) == 2) {
             const int l = lane & 15, row = 4 * h + (l >> 2), piece = (lane >> 3 & 2) + (l >> 1 & 1);   // of the first 32 columns
-            const T* const from = lds + row * DP + (l & 1) * 4 + ((4 * db % ring) ^ (piece ^ turn(row))) * V;
+            const T* const from = lds + row * DP + (l & 1) * 4;
+            const int turned = piece ^ turn(row);
             u16x8 both;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(from + (r0 + 8 * half) * DP + 4 * db / ring * ring * V));
+                const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsFour*)(from + (r0 + 8 * half) * DP + 4 * db / ring * ring * V + ((4 * db % ring ^ (sixteen ? half : 0)) ^ turned) * V));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) both[half * 4 + i] = (u16)four[i];
             }
