@@ -277,13 +277,14 @@ void attend_kernel(AttendArgs<T> p) {
                 // The maximum that exponentials are relative to need not be the largest score: any will do whose exponentials stay in range.  It is moved, and
                 // the sums with it, where a row's has grown by more than 2^8 (a wavefront's 32 rows find new maxima in two tiles of three of a
                 // long sequence: 16 384 causal rows, 8 heads of 128 581 -> 550 us).
-                if (__any((most - m[n]) * to2 > 8.0f)) {
-                    const float less = __builtin_amdgcn_exp2f((m[n] - most) * to2);   // (-inf at first; NaN where both are infinite: so is the row)
-                    if constexpr (by_product) ones_acc[n][0] *= m[n] == most ? 1.0f : less;
-                    else l[n] *= m[n] == most ? 1.0f : less;
+                const bool grown = (most - m[n]) * to2 > 8.0f;      // (not where both are infinite: exponentials of -inf are 0, and the row of an inf is NaN)
+                if (__any(grown)) {
+                    const float less = grown ? __builtin_amdgcn_exp2f((m[n] - most) * to2) : 1.0f;
+                    if constexpr (by_product) ones_acc[n][0] *= less;
+                    else l[n] *= less;
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) acc[n][db] *= m[n] == most ? 1.0f : less;
-                    m[n] = most;
+                    for (int db = 0; db < DB; ++db) acc[n][db] *= less;
+                    m[n] = grown ? most : m[n];      // (each row by itself: no row has other bits for what its neighbours hold)
                 }
                 const float from = m[n] == -__builtin_inff() ? 0.0f : m[n] * to2;   // (nothing seen yet: exponentials of -inf are 0)
 #pragma unroll

@@ -189,3 +189,25 @@ def test_rows_between_that_see_nothing(gpu, d, bad, dtype):
             assert torch.equal(y, clean_y), name
             assert torch.equal(grads["q"], clean["q"]), name
             assert torch.equal(grads["k"], clean["k"]) and torch.equal(grads["v"], clean["v"]), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [32, 33, 64, 128])
+def test_what_other_sequences_hold_in_larger_launches(gpu, d, causal, dtype):
+    """Tiles of 128 rows that hold several sequences, of which one is not finite."""
+    lengths = [1 + 37 * i % 170 for i in range(103)]
+    rows, first = sum(lengths), sum(lengths[:50])
+    x, grad = inputs(rows, rows, 8, 8, d, dtype, seed=12)
+    offsets, mine = packed(lengths), slice(first, first + lengths[50])
+    others = torch.ones(rows, dtype=torch.bool)
+    others[mine] = False
+    clean_y, clean = step(x, grad, offsets, causal=causal)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for name in ("q", "k", "v", "grad"):
+            broken, dy = {n: v.clone() for n, v in x.items()}, grad.clone()
+            (dy if name == "grad" else broken[name])[mine, :, d // 2] = bad
+            y, grads = step(broken, dy, offsets, causal=causal)
+            assert torch.equal(y[others], clean_y[others]), name
+            assert all(torch.equal(grads[n][others], clean[n][others]) for n in grads), name
+            assert not torch.isfinite(grads[{"grad": "v", "v": "q"}.get(name, name)][mine]).all(), name
