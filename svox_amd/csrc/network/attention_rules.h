@@ -49,12 +49,16 @@ inline int64_t likely_length(int64_t other, int64_t sequences, int64_t rows, int
     return length < other ? length : other;
 }
 
+// Tiles of 128 rows where there are enough of them for the GPU, or where keys are read so often that rows of a tile matter more than places: from
+// some number of scores on, which are dearest where heads are wide, and in float32.  (Tiles of 32 rows and of 128, us, bfloat16: 8192 rows of one head of
+// 128, 1024 keys 48, 32; 4096 rows, 512 keys 21, 22; 4096 rows of 8 heads of 64, 4096 keys 81, 68; 2048 rows, 2048 keys 36, 37; 16 384 rows of 2 heads of
+// 32, 4096 keys 49, 49; 8192 rows, 2048 keys 24, 30.  float32: 1024 rows of 8 heads of 64, 1024 keys 52, 41; 512 rows, 512 keys 21, 25.)
 inline AttendPlan forward_plan(const SvoxAttention& s) {
-    const int64_t rows = s.queries * (s.heads / s.kv_heads), tiles = pieces(rows, 128);
-    if (tiles * s.kv_heads >= kAttendBlocks) {
-        const int64_t length = likely_length(s.keys, s.sequences, 128, rows);
+    const int64_t rows = s.queries * (s.heads / s.kv_heads), tiles = pieces(rows, 128), length = likely_length(s.keys, s.sequences, 128, rows);
+    const int width = attend_width(s.dim), dear = s.dtype == SVOX_DECODER_F32 || width == 128 ? 22 : width == 64 ? 26 : 27;
+    const bool many = rows >= 256 && length >= ((int64_t)1 << dear) / (rows * s.kv_heads);
+    if (tiles * s.kv_heads >= kAttendBlocks || many)
         return ordered(split({128, 1, 1, false, false}, tiles * s.kv_heads, length, s.keys, 64), s, tiles, length);
-    }
     return split({32, 1, 1, true, false}, pieces(rows, 32) * s.kv_heads, likely_length(s.keys, s.sequences, 32, rows), s.keys, 128);
 }
 inline AttendPlan query_grad_plan(const SvoxAttention& s) {

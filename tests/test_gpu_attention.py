@@ -330,3 +330,12 @@ def test_tiles_that_are_shared_out_and_tiles_that_are_not(gpu):
     of_q, of_k = [4000, 5, 60, 900], [1, 3, 0, 2]
     x, grad = inputs(sum(of_q), sum(of_k), 2, 2, 64, torch.bfloat16, seed=1)
     check(x, grad, packed(of_q), packed(of_k))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d,t,n", [(128, 1100, 1200), (113, 1100, 1200), (60, 2900, 2910), (128, 400, 400)])
+def test_rows_between_few_and_many(gpu, d, t, n, causal, dtype):
+    """Too few tiles for the GPU, but keys enough for tiles of 128 rows, or not."""
+    x, grad = inputs(t, n, 8, 1 if d > 64 else 2, d, dtype, seed=13)
+    check(x, grad, packed([t - 300, 0, 300]), packed([n - 350, 50, 300]), causal=causal)
