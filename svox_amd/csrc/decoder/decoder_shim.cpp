@@ -39,22 +39,22 @@ Tensor norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, d
 }
 
 struct NormNode : torch::autograd::Node {
-    SavedVariable x_, weight_, stats_;
+    Kept x_, weight_, stats_;
     double eps = 0.0;
 
     std::string name() const override { return "SvoxLayerNormBackward"; }
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
-        x_.reset_data();
-        weight_.reset_data();
-        stats_.reset_data();
+        x_.reset();
+        weight_.reset();
+        stats_.reset();
     }
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(3);
         if (!grads[0].defined()) return out;
         once("layer_norm", grads[0]);
-        const Tensor x = x_.unpack(), weight = weight_.unpack(), stats = stats_.unpack();
+        const Tensor x = x_.take("layer_norm"), weight = weight_.take_contiguous("layer_norm"), stats = stats_.take_contiguous("layer_norm");
         const On on(x);
         check_like(grads[0], x, "grad_output");
         const Rows rows = rows_of(x), dy = rows_of(grads[0]);
@@ -88,9 +88,9 @@ Tensor layer_norm(const Tensor& x, Tensor weight, Tensor bias, double eps) {
         const at::AutoDispatchBelowADInplaceOrView guard;
         y = norm_forward(x, weight, bias, eps, &stats);
     }
-    node->x_ = SavedVariable(x, false);
-    node->weight_ = SavedVariable(weight, false);
-    node->stats_ = SavedVariable(stats, false);
+    node->x_.keep(x);
+    node->weight_.keep(weight);
+    node->stats_.keep(stats);
     node->eps = eps;
     torch::autograd::set_history(y, node);
     return y;
@@ -141,20 +141,21 @@ Tensor ffn_forward(const Ffn& f, int32_t activation) {
 }
 
 struct FfnNode : torch::autograd::Node {
-    SavedVariable saved_[6];   // x, w_gate, w_up, w_down, b_gate, b_up
+    Kept saved_[6];   // x, w_gate, w_up, w_down, b_gate, b_up
     int32_t activation = 0;
 
     std::string name() const override { return "SvoxGatedFfnBackward"; }
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable& v : saved_) v.reset_data();
+        for (Kept& v : saved_) v.reset();
     }
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(8);
         if (!grads[0].defined()) return out;
         once("gated_ffn", grads[0]);
-        const Ffn f{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), saved_[5].unpack(), Tensor(), Tensor()};
+        const auto kept = [&](int i) { return saved_[i].take_contiguous("gated_ffn"); };
+        const Ffn f{saved_[0].take("gated_ffn"), kept(1), kept(2), kept(3), kept(4), kept(5), Tensor(), Tensor()};
         const On on(f.x);
         check_like(grads[0], f.x, "grad_output");
         if (task_should_compute_output(7)) out[7] = grads[0];
@@ -207,7 +208,7 @@ Tensor gated_ffn(Ffn& f, int64_t activation) {
         y = ffn_forward(f, (int32_t)activation);
     }
     const Tensor* const saved[6] = {&f.x, &f.w_gate, &f.w_up, &f.w_down, &f.b_gate, &f.b_up};
-    for (int i = 0; i < 6; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
+    for (int i = 0; i < 6; ++i) node->saved_[i].keep(*saved[i]);
     node->activation = (int32_t)activation;
     torch::autograd::set_history(y, node);
     return y;

@@ -178,20 +178,21 @@ std::pair<Tensor, Tensor> rotate_forward(const Heads& h) {
 }
 
 struct RotateNode : torch::autograd::Node {
-    SavedVariable saved_[6];   // q, k, positions, frequencies and the weights
+    Kept saved_[6];   // q, k, positions, frequencies and the weights
     bool interleaved = false;
     double eps = 0.0;
 
     std::string name() const override { return "SvoxRotateHeadsBackward"; }
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable& v : saved_) v.reset_data();
+        for (Kept& v : saved_) v.reset();
     }
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(4);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        Heads h{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), saved_[5].unpack(), interleaved, eps};
+        const auto kept = [&](int i) { return saved_[i].take_contiguous("rotate_heads"); };
+        Heads h{saved_[0].take("rotate_heads"), saved_[1].take("rotate_heads"), kept(2), kept(3), kept(4), kept(5), interleaved, eps};
         const On on(h.q);
         h.q = heads_of(h.q), h.k = heads_of(h.k);
         for (int i = 0; i < 2; ++i) {
@@ -261,7 +262,7 @@ std::pair<Tensor, Tensor> rotate_heads(Heads h) {
     }
     if (!wants) return y;
     const Tensor* const saved[6] = {&q, &k, &h.positions, &h.frequencies, &h.q_weight, &h.k_weight};
-    for (int i = 0; i < 6; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
+    for (int i = 0; i < 6; ++i) node->saved_[i].keep(*saved[i]);
     node->interleaved = h.interleaved;
     node->eps = h.eps;
     torch::autograd::set_history(std::vector<Tensor>{y.first, y.second}, node);
@@ -313,25 +314,26 @@ Tensor attention_forward(const Attend& a, Tensor* lse, Tensor* rest) {
 }
 
 struct AttendNode : torch::autograd::Node {
-    SavedVariable saved_[5], out_, lse_, rest_;   // q, k, v and the offsets
+    Kept saved_[5], out_, lse_, rest_;   // q, k, v and the offsets
     bool causal = false;
     double scale = 0.0;
 
     std::string name() const override { return "SvoxAttentionBackward"; }
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable& v : saved_) v.reset_data();
-        out_.reset_data();
-        lse_.reset_data();
-        rest_.reset_data();
+        for (Kept& v : saved_) v.reset();
+        out_.reset();
+        lse_.reset();
+        rest_.reset();
     }
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         variable_list out(3);
         if (!grads[0].defined()) return out;
         once("attention", grads[0]);
-        Attend a{saved_[0].unpack(), saved_[1].unpack(), saved_[2].unpack(), saved_[3].unpack(), saved_[4].unpack(), causal, scale};
-        const Tensor y = out_.unpack(shared_from_this()), lse = lse_.unpack(), rest = rest_.unpack();
+        const auto kept = [&](int i) { return saved_[i].take("attention"); };
+        Attend a{kept(0), kept(1), kept(2), saved_[3].take_contiguous("attention"), saved_[4].take_contiguous("attention"), causal, scale};
+        const Tensor y = out_.take_contiguous("attention", shared_from_this()), lse = lse_.take_contiguous("attention"), rest = rest_.take_contiguous("attention");
         const On on(a.q);
         check_like(grads[0], a.q, "grad_output", "q");
         a = dense_heads(a);
@@ -396,13 +398,13 @@ Tensor attention(Attend a) {
         y = attention_forward(dense_heads(a), &lse, &rest);
     }
     const Tensor* const saved[5] = {&q, &k, &v, &a.offsets, &a.key_offsets};
-    for (int i = 0; i < 5; ++i) node->saved_[i] = SavedVariable(*saved[i], false);
-    node->lse_ = SavedVariable(lse, false);
-    node->rest_ = SavedVariable(rest, false);
+    for (int i = 0; i < 5; ++i) node->saved_[i].keep(*saved[i]);
+    node->lse_.keep(lse);
+    node->rest_.keep(rest);
     node->causal = a.causal;
     node->scale = a.scale;
     torch::autograd::set_history(y, node);
-    node->out_ = SavedVariable(y, true);
+    node->out_.keep(y, true);
     return y;
 }
 

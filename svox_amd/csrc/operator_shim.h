@@ -146,6 +146,39 @@ void make_contiguous(Tensor& x) {
     if (!x.is_contiguous()) x = x.contiguous();
 }
 
+// A tensor kept for the backward pass.  Hooks on saved tensors may give back another in its place: one of another device, type or shape is refused,
+// any strides can be.
+struct Kept {
+    SavedVariable saved;
+    at::DimVector shape;
+    at::ScalarType type = at::kFloat;
+    at::Device device = at::kCPU;
+    bool defined = false;
+
+    void keep(const Tensor& x, bool is_output = false) {
+        saved = SavedVariable(x, is_output);
+        defined = x.defined();
+        if (!defined) return;
+        shape.assign(x.sizes().begin(), x.sizes().end());
+        type = x.scalar_type();
+        device = x.device();
+    }
+    Tensor take(const char* name, std::shared_ptr<torch::autograd::Node> node = nullptr) const {
+        const Tensor x = saved.unpack(std::move(node));
+        if (!defined) return Tensor();
+        if (!x.defined() || x.layout() != at::kStrided || x.device() != device || x.scalar_type() != type || x.sizes() != at::IntArrayRef(shape))
+            fail(std::string("svox.") + name + ": a hook on saved tensors gave back another tensor than a " + dtype_text(type) + " one of shape " + shape_text(shape) + " on " +
+                 device.str());
+        return x;
+    }
+    Tensor take_contiguous(const char* name, std::shared_ptr<torch::autograd::Node> node = nullptr) const {
+        Tensor x = take(name, std::move(node));
+        make_contiguous(x);
+        return x;
+    }
+    void reset() { saved.reset_data(); }
+};
+
 // ---- called from Python with positional arguments
 struct WrongType {
     const char* name;
