@@ -40,6 +40,14 @@ struct AttendArgs {
 
 constexpr float kLog2E = 1.4426950408889634f, kNoSum = 3.0e38f;   // (the lse of a row that sees no key)
 
+// Powers of two that keep the operands of products away from where float16's numbers run out (bfloat16 has float32's): from 2^-14 down they have fewer
+// bits, from 2^-25 down none.  p of a row of n keys is some 1 / n: dv takes it times 2^14, of 65 536 at most four times what p can be (dv of 20
+// rows of 8 heads over 262 144 keys: 10.4 times the error of one rounding without it, 1.4 with it).
+template <class T>
+constexpr int kRaised = std::is_same_v<T, F16> ? 14 : 0;
+template <class T>
+constexpr float kLowered = std::is_same_v<T, F16> ? 0x1p-14f : 1.0f;
+
 // The work of a block: a tile, a kv head, a part of the tile's other axis.
 struct Place {
     int tile, head, split;   // no tile: tile < 0
@@ -671,7 +679,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     const auto load = [&](int i0, int stage) {
         if ((int)threadIdx.x < 2 * rows) {
             const int at = min(i0 + (int)threadIdx.x % rows, part.high - 1);
-            stat = (int)threadIdx.x < rows ? lse[at] : -delta[at];
+            stat = (int)threadIdx.x < rows ? lse[at] - (float)kRaised<T> : -delta[at];
         }
         qs.load(i0, part.high - i0, tiles + stage * 2 * tile);
         gs.load(i0, part.high - i0, tiles + (stage * 2 + 1) * tile);
@@ -736,7 +744,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                 }
                 if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
+                for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r] * kLowered<T>;
                 if (below) hide_below(ds, low, 0.0f);
                 if (beyond) hide_from(ds, high, 0.0f);
 #pragma unroll
@@ -756,11 +764,11 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     if (share.used > 1) {
         float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
         store_row<float, DB>(at, DP, dk[0], 1.0f, half);
-        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], 1.0f, half);
+        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], kLowered<T>, half);
     } else {
         const int64_t at = ((int64_t)j * p.kv_heads + place.head) * p.dim;
         if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale, half);
-        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], 1.0f, half);
+        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], kLowered<T>, half);
     }
 }
 
