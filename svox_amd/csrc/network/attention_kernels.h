@@ -11,7 +11,8 @@
 // The backward pass computes scores twice, once for dq and once for dk and dv: seven products where one pass with atomic sums of dq
 // would do with five, but sums in a fixed order, the same call the same bits.
 //
-// Scores and their exponentials, sums, maxima and results are in 32 bits.  p and ds are rounded to 16-bit operands where the type has 16 bits.
+// Scores and their exponentials, sums, maxima and results are in 32 bits.  p and ds are rounded to 16-bit operands where the type has 16 bits, as the matrix
+// cores take them (in 32 bits they take seven times as long): a sum of many is off by what one rounding is, in the mean.
 #pragma once
 #include "attention_tile.h"
 
@@ -47,6 +48,28 @@ template <class T>
 constexpr int kRaised = std::is_same_v<T, F16> ? 14 : 0;
 template <class T>
 constexpr float kLowered = std::is_same_v<T, F16> ? 0x1p-14f : 1.0f;
+// ds, which may be anything, each row of dq and each key of dk takes times a power of two of its own, `up`: from kMostUp on, with which no number of
+// float16 leaves float32's range, down to where the largest so far lies below 2^15, each time by as much as brings it to 2^14; the sum goes along.
+// (Gradients of some 1e-3, 200 rows over 32 768 keys: dq 22.6 times the error of one rounding without it, 1.01 with it.  It is 61 sequences' dq in 85 ->
+// 94 us, dk and dv in 143 -> 162.)
+template <class T>
+constexpr bool kOwnScale = std::is_same_v<T, F16>;
+constexpr float kMostUp = 0x1p80f;
+template <int DB>
+__device__ __forceinline__ float fit(float (&ds)[16], float& up, f32x16 (&acc)[DB]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, __builtin_fabsf(ds[r]));
+    if (!__any(most > 0x1p15f)) return 1.0f;
+    most = most_of_halves(most);      // (the halves share the sum)
+    const float less = most > 0x1p15f && most < __builtin_inff() ? __builtin_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(most)) : 1.0f;
+    up *= less;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] *= less;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] *= less;
+    return less;
+}
 
 // The work of a block: a tile, a kv head, a part of the tile's other axis.
 struct Place {
@@ -553,11 +576,18 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
     clip(see, part);
 
     const float lse = p.lse[(int64_t)place.head * p.rows + row];
-    const float delta = delta_of<T, DP, direct>(p, row, place.head, g);
+    float delta = delta_of<T, DP, direct>(p, row, place.head, g);
     if (place.split == 0 && h == 0 && mine + (int)threadIdx.x % 32 < p.rows) p.delta[(int64_t)place.head * p.rows + row] = delta;
+    // (registers for float16's `fit`: 32 keys at a time, or a fragment of g in LDS)
+    constexpr bool one_by_one = kOwnScale<T> && DP == 64;
+    constexpr int kept = kOwnScale<T> && DP == 128 && !direct ? DP / 16 - 1 : DP / 16;
+    __shared__ Eight rest[kept < DP / 16 ? DP / 16 - kept : 1][kept < DP / 16 ? kAttendThreads : 1];
+#pragma unroll
+    for (int t = kept; t < DP / 16; ++t) rest[t - kept][threadIdx.x] = g[t];
     const float to2 = p.scale * kLog2E;
     f32x16 acc[1][DB];
-    float none = 0.0f;
+    float none = 0.0f, up = kOwnScale<T> ? kMostUp : 1.0f;
+    delta *= up;
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
     Loader<T, DP, keys, direct> ks(p.k + place.head * p.k_head, p.k_stride, 0, 1, p.dim), vs(p.v + place.head * p.v_head, p.v_stride, 0, 1, p.dim);
@@ -590,20 +620,25 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
             take_out_odd<T, DP, keys>(tiles + stage * 2 * tile, [&](int row, int, float) { atomicOr(&bad[row / 32], 1u << row % 32); });
         }
         if (k0 < spans.high && k0 + keys > spans.low) {
-#pragma unroll
+#pragma unroll one_by_one ? 1 : KB
             for (int b = 0; b < KB; ++b) {
                 f32x16 s = {}, dp = {};
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     if (sizeof(T) == 4 && 16 * t >= p.dim) break;
                     s = F::mma(Tile<T, DP>::along(kt, 32 * b, t), q[t], s);
-                    dp = F::mma(Tile<T, DP>::along(vt, 32 * b, t), g[t], dp);
+                    dp = F::mma(Tile<T, DP>::along(vt, 32 * b, t), t < kept ? g[t] : rest[t < kept ? 0 : t - kept][threadIdx.x], dp);
                 }
                 float ds[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to2, -lse)) * (dp[r] - delta);
+                for (int r = 0; r < 16; ++r) {
+                    const float p_r = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], to2, -lse));
+                    if constexpr (kOwnScale<T>) ds[r] = p_r * __builtin_fmaf(dp[r], up, -delta);
+                    else ds[r] = p_r * (dp[r] - delta);
+                }
                 if (k0 < spans.all_low) hide_below(ds, see[0].low - k0 - 32 * b - 4 * h, 0.0f);
                 if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see[0].high - k0 - 32 * b - 4 * h, 0.0f);
+                if constexpr (kOwnScale<T>) delta *= fit(ds, up, acc[0]);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Eight e[1] = {F::pack(ds + 8 * c)};
@@ -622,10 +657,10 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
     const int thread = thread_again(), half = thread / 32 % 2, r = mine + thread % 32;
     if (r >= p.rows) return;
     if (share.used > 1) {
-        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f, half);
+        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f / up, half);
     } else {
         const unsigned token = (unsigned)r / again(p.group);
-        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale, half);
+        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale / up, half);
     }
 }
 
@@ -660,7 +695,9 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
 
     // (Fragments of v that stay in registers; the others stay in LDS.  Heads of 128: registers that were missing lay in memory, and to load them again was to
     // wait for the next tile too: 1460 -> 1380 us for 16 384 causal rows, 8 heads.)
-    constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? 1 : 4;
+    constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? (kOwnScale<T> ? 0 : 1) : kOwnScale<T> ? 2 : 4;
+    // (float16: `fit` needs some as well, and has them by 32 rows at a time and more of v in LDS)
+    constexpr bool one_by_one = kOwnScale<T> && DP <= 64;
     __shared__ Eight rest[kept < DP / 16 ? DP / 16 - kept : 1][kept < DP / 16 ? kAttendThreads : 1];
     Eight k[DP / 16], v[DP / 16];
     load_row<T, DP, direct>(p.k + (int64_t)key * p.k_stride + place.head * p.k_head, p.dim, k);
@@ -675,7 +712,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     for (int db = 0; db < DB; ++db) dk[0][db] = dv[0][db] = f32x16{};
     Loader<T, DP, rows, direct> qs(p.q + (int64_t)place.head * p.group * p.q_head, p.q_stride, p.q_head, p.group, p.dim),
         gs(p.grad + (int64_t)place.head * p.group * p.grad_head, p.grad_stride, p.grad_head, p.group, p.dim);
-    float stat = 0.0f;
+    float stat = 0.0f, up = kOwnScale<T> ? kMostUp * kLowered<T> : 1.0f;
     const auto load = [&](int i0, int stage) {
         if ((int)threadIdx.x < 2 * rows) {
             const int at = min(i0 + (int)threadIdx.x % rows, part.high - 1);
@@ -712,7 +749,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
             take_out_odd<T, DP, 2 * rows>(tiles + stage * 2 * tile, [&](int row, int, float) { shared[stage][0][row % rows] = __builtin_nanf(""); });
         }
         if (i0 < spans.high && i0 + rows > spans.low) {
-#pragma unroll
+#pragma unroll one_by_one ? 1 : RB
             for (int b = 0; b < RB; ++b) {
                 // (heads of 128: one product's fragments at a time, as the sums and the fragments that stay take most of the registers)
                 f32x16 s = {}, dp;
@@ -721,7 +758,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                     if (sizeof(T) == 4 && 16 * t >= p.dim) break;
                     s = F::mma(Tile<T, DP>::along(qt, 32 * b, t), k[t], s);
                 }
-                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                if constexpr (DP == 128 || one_by_one) __builtin_amdgcn_sched_barrier(0);
                 float e[16], ds[16];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -740,13 +777,14 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     if (sizeof(T) == 4 && 16 * t >= p.dim) break;
-                    dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), t < kept ? v[t] : rest[t < kept ? 0 : t - kept][threadIdx.x], dp);
+                    dp = F::mma(Tile<T, DP>::along(gt, 32 * b, t), t < kept ? v[t] : rest[t < kept ? 0 : t - kept][one_by_one ? thread_again() : (int)threadIdx.x], dp);
                 }
-                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                if constexpr (DP == 128 || one_by_one) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r] * kLowered<T>;
+                for (int r = 0; r < 16; ++r) ds[r] = kOwnScale<T> ? e[r] * dp[r] * up : e[r] * dp[r];
                 if (below) hide_below(ds, low, 0.0f);
                 if (beyond) hide_from(ds, high, 0.0f);
+                if constexpr (kOwnScale<T>) (void)fit(ds, up, dk[0]);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int at = 32 * b + 16 * c;
@@ -763,11 +801,11 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     if (j >= p.keys) return;
     if (share.used > 1) {
         float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
-        store_row<float, DB>(at, DP, dk[0], 1.0f, half);
+        store_row<float, DB>(at, DP, dk[0], kLowered<T> / up, half);
         store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], kLowered<T>, half);
     } else {
         const int64_t at = ((int64_t)j * p.kv_heads + place.head) * p.dim;
-        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale, half);
+        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale * kLowered<T> / up, half);
         if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], kLowered<T>, half);
     }
 }

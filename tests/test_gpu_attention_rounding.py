@@ -68,3 +68,79 @@ def test_values_gradients_over_long_rows(gpu, t, n, h, kv_heads, d, dtype):
     got = step(x, grad)
     assert roundings(got[0], want[0]) <= TWO
     assert roundings(got[3], want[3]) <= TWO
+
+
+SHAPES = [(200, 4096, 2, 1, 64), (200, 32768, 2, 1, 128), (70, 20011, 4, 2, 33), (300, 9000, 2, 2, 32), (40, 33000, 3, 1, 100)]
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=name_of)
+@pytest.mark.parametrize("size", [1e-3, 1.0, 300.0])
+@pytest.mark.parametrize("t,n,h,kv_heads,d", SHAPES)
+def test_gradients_of_every_size_over_long_rows(gpu, t, n, h, kv_heads, d, size, dtype):
+    """Influences of single scores, some 1 / keys of the gradient's, below what float16 holds, or beyond it."""
+    x, grad = inputs(t, n, h, kv_heads, d, dtype, seed=n, size=size)
+    for got, want in zip(step(x, grad), exact(*x, grad)):
+        assert roundings(got, want) <= TWO
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=name_of)
+@pytest.mark.parametrize("size", [1e-4, 1.0, 4000.0])
+@pytest.mark.parametrize("d,kv_heads", [(16, 2), (32, 1), (64, 1), (128, 2), (100, 1)])
+def test_gradients_of_every_size_of_causal_rows(gpu, d, kv_heads, size, dtype):
+    """Few keys to a row and many."""
+    x, grad = inputs(1500, 1500, 2, kv_heads, d, dtype, seed=d, size=size)
+    want = exact(*x, grad, causal=True)
+    assert all(float(w.abs().max()) < torch.finfo(torch.float16).max for w in want)
+    for got, w in zip(step(x, grad, causal=True), want):
+        assert roundings(got, w) <= TWO
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 33])
+@pytest.mark.parametrize("falling", [False, True])
+def test_sizes_that_differ_from_row_to_row_and_along_a_row(gpu, d, falling):
+    """Rows' gradients of all sizes from 2^-9 to 2^9, in either order, so that sums over rows grow by 2^18 on their way, and so do values along the keys:
+    each row is as exact as if it were alone, and so is each key whose values are small."""
+    t, n = 600, 5000
+    x, grad = inputs(t, n, 2, 1, d, torch.float16, seed=d)
+    along = 2.0 ** torch.linspace(9, -9, t, device="cuda:0") if falling else 2.0 ** torch.linspace(-9, 9, t, device="cuda:0")
+    grad = (grad * along[:, None, None]).half()
+    got, want = step(x, grad), exact(*x, grad)
+    for a, b in zip(got, want):
+        assert roundings(a, b) <= TWO
+    for a in range(0, t, 50):
+        assert roundings(got[1][a:a + 50], want[1][a:a + 50]) <= TWO
+    x[2] = (x[2] * (2.0 ** torch.linspace(5 if falling else -5, -5 if falling else 5, n, device="cuda:0"))[:, None, None]).half()
+    grad = (grad / along[:, None, None]).half()
+    got, want = step(x, grad), exact(*x, grad)
+    for a, b in zip(got, want):
+        assert roundings(a, b) <= TWO
+
+
+def test_rows_do_not_depend_on_what_their_neighbours_are(gpu):
+    """Bit for bit, where the other sequences' gradients and values are 2^12 times as large or as small."""
+    lengths = [30, 50, 7, 90, 41]
+    offsets = torch.tensor([0, 30, 80, 87, 177, 218], device="cuda:0")
+    for d in (32, 64, 128, 33):
+        x, grad = inputs(218, 218, 4, 2, d, torch.float16, seed=d, size=1e-2)
+        mine = slice(80, 87)
+        clean = step(x, grad, offsets=offsets, causal=True)
+        for factor in (2.0 ** 12, 2.0 ** -12):
+            other, dy = [v.clone() for v in x], grad * factor
+            other[2] = other[2] * factor
+            for v, w in ((other[2], x[2]), (dy, grad)):
+                v[mine] = w[mine]
+            for a, b in zip(clean, step(other, dy, offsets=offsets, causal=True)):
+                assert torch.equal(a[mine], b[mine])
+    assert sum(lengths) == 218
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 33])
+def test_influences_beyond_float16(gpu, d):
+    """do . v beyond 65 504 for keys so small that no gradient is."""
+    x, grad = inputs(700, 700, 2, 1, d, torch.float16, seed=d, size=4000.0)
+    x[0], x[1], x[2] = x[0] / 16, x[1] / 64, x[2] * 8
+    want = exact(*x, grad, causal=True)
+    assert all(float(w.abs().max()) < torch.finfo(torch.float16).max for w in want[1:])
+    assert float((grad[:, 0].double() @ x[2][:, 0].double().t().contiguous()).abs().max()) > 2 * torch.finfo(torch.float16).max
+    for got, w in zip(step(x, grad, causal=True), want):
+        assert roundings(got, w) <= TWO
