@@ -26,7 +26,7 @@ struct AttendArgs {
     T *dq, *dk, *dv;                   // dense
     float *lse, *delta;                // [kv head][row]: log2 of the sum of exponentials, and its sum of do o
     float* part;                       // where the work of a tile is split: [kv head][split][row][DP] (keys and values: two of them)
-    f32x2* stats;                      // [kv head][split][row]: maximum (of base 2) and sum
+    f32x2* stats;                      // [kv head][split][row]: maximum (of base 2), less kForwardRaised, and sum
     int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, grad_stride, grad_head;
     Sequences seq;
     int rows, keys;                    // of a kv head
@@ -46,6 +46,13 @@ constexpr float kLog2E = 1.4426950408889634f, kNoSum = 3.0e38f;   // (the lse of
 // rows of 8 heads over 262 144 keys: 10.4 times the error of one rounding without it, 1.4 with it).
 template <class T>
 constexpr int kRaised = std::is_same_v<T, F16> ? 14 : 0;
+// The forward pass takes exponentials times 2^8, relative to a maximum that may lag behind by 2^4 (other types: 2^8): one that is 2^-22 of the largest has
+// all of its bits still.  (8192 keys, all but the first 13 below it and their values 100 times its: 6.5 to 20 times the error of one rounding without it, at
+// most 1.8 with it; the time is the same.)
+template <class T>
+constexpr int kForwardRaised = std::is_same_v<T, F16> ? 8 : 0;
+template <class T>
+constexpr int kLag = std::is_same_v<T, F16> ? 4 : 8;
 template <class T>
 constexpr float kLowered = std::is_same_v<T, F16> ? 0x1p-14f : 1.0f;
 // ds, which may be anything, each row of dq and each key of dk takes times a power of two of its own, `up`: from kMostUp on, with which no number of
@@ -306,9 +313,9 @@ void attend_kernel(AttendArgs<T> p) {
                     for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][n][r]);
                 most = most_of_halves(most);
                 // The maximum that exponentials are relative to need not be the largest score: any will do whose exponentials stay in range.  It is moved, and
-                // the sums with it, where a row's has grown by more than 2^8 (a wavefront's 32 rows find new maxima in two tiles of three of a
+                // the sums with it, where a row's has grown by more than 2^kLag (a wavefront's 32 rows find new maxima in two tiles of three of a
                 // long sequence: 16 384 causal rows, 8 heads of 128 581 -> 550 us).
-                const bool grown = (most - m[n]) * to2 > 8.0f;      // (not where both are infinite: exponentials of -inf are 0, and the row of an inf is NaN)
+                const bool grown = (most - m[n]) * to2 > (float)kLag<T>;      // (not where both are infinite: exponentials of -inf are 0, and the row of an inf is NaN)
                 if (__any(grown)) {
                     const float less = grown ? __builtin_amdgcn_exp2f((m[n] - most) * to2) : 1.0f;
                     if constexpr (by_product) ones_acc[n][0] *= less;
@@ -317,7 +324,7 @@ void attend_kernel(AttendArgs<T> p) {
                     for (int db = 0; db < DB; ++db) acc[n][db] *= less;
                     m[n] = grown ? most : m[n];      // (each row by itself: no row has other bits for what its neighbours hold)
                 }
-                const float from = m[n] == -__builtin_inff() ? 0.0f : m[n] * to2;   // (nothing seen yet: exponentials of -inf are 0)
+                const float from = m[n] == -__builtin_inff() ? 0.0f : m[n] * to2 - (float)kForwardRaised<T>;   // (nothing seen yet: exponentials of -inf are 0)
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     float x[16];
@@ -414,7 +421,7 @@ void attend_kernel(AttendArgs<T> p) {
         const bool some = max(see[n].low, part.low) < see[n].high;
         if (share.used > 1) {
             const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
-            if (half == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
+            if (half == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2 - (float)kForwardRaised<T>, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
             if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f, half);
         } else {
             const unsigned token = (unsigned)r / again(p.group);
@@ -428,7 +435,7 @@ void attend_kernel(AttendArgs<T> p) {
                     for (int i = 0; i < 16; ++i) acc[n][db][i] = left_of<T>(acc[n][db][i] * factor);
                 store_row<T, DB>(p.rest + to, p.dim, acc[n], 1.0f, half);
             }
-            if (p.lse && half == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n])) : kNoSum;
+            if (p.lse && half == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n]) - (float)kForwardRaised<T>) : kNoSum;
         }
     }
 }

@@ -144,3 +144,22 @@ def test_influences_beyond_float16(gpu, d):
     assert float((grad[:, 0].double() @ x[2][:, 0].double().t().contiguous()).abs().max()) > 2 * torch.finfo(torch.float16).max
     for got, w in zip(step(x, grad, causal=True), want):
         assert roundings(got, w) <= TWO
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=name_of)
+@pytest.mark.parametrize("d", [32, 64, 128, 33])
+def test_a_row_of_small_exponentials(gpu, d, dtype):
+    """Each e^-8 to e^-15 of the first, times values 100 times as large, in rows that no blocks share.  They are alike and rounded alike, by half a step,
+    which is 2^-p of them at most (p bits); the root of the mean square of one rounding of the result is 2^-p-1 / sqrt(3) of it at least, and the
+    result is rounded itself: at most sqrt(1 + 12) roundings, if they are all of the row.  A sum of 4096 numbers one after another, a lane's, is off by
+    4096 2^-24 of itself at most, two roundings of float16.  Together less than 6."""
+    g = torch.Generator().manual_seed(d)
+    t, n = 16384, 8192
+    q, k = torch.ones(t, 8, d, device="cuda:0", dtype=dtype), torch.zeros(n, 1, d, device="cuda:0", dtype=dtype)
+    v = (100 * torch.linspace(0.7, 1.3, d) + torch.randn(n, 1, d, generator=g)).to("cuda:0").to(dtype)     # (so that results lie anywhere between steps)
+    v[0] = 1
+    for below in (8.0, 9.5, 10.4, 11.0, 12.0, 13.0, 14.2, 15.0):
+        k.fill_(-below * d ** -0.5)
+        k[0] = 0
+        want = exact(q[:1, :1], k, v, torch.zeros_like(q[:1, :1]))[0]
+        assert roundings(svox.attention(q, k, v), want.expand(t, 8, d)) <= 6.0, below
