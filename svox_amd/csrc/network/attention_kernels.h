@@ -183,19 +183,19 @@ __device__ __forceinline__ float left_of(float v) {
 }
 
 // ---- forward.  Four wavefronts, of which `across` share rows and take a part of every tile's keys each.
-template <class T, int DP, int N, int across>
+template <class T, int DP, int N, int across, bool narrow>
 struct ForwardShape {
     static constexpr int down = 4 / across, rows = down * 32 * N;
-    static constexpr int keys = across == 4 ? 128 : (sizeof(T) == 4 && DP == 128 ? 32 : 64), mine = keys / across, blocks = mine / 32;
+    static constexpr int keys = across == 4 ? 128 : (narrow ? 32 : 64), mine = keys / across, blocks = mine / 32;
     static constexpr int stages = across == 4 && sizeof(T) == 4 && DP == 128 ? 1 : 2;   // tiles in LDS
     static constexpr int tile = keys * DP;
 };
 
 // (float32, heads of 32: registers for four wavefronts a SIMD rather than three: 512 windows of 64 cells, 4 heads of 16, 36 -> 30 us; 8 of 4096 644 -> 625.)
-template <class T, int DP, int N, int across, bool direct>
-__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 && DP == 32 && across == 1 && direct ? 4 : 2)
+template <class T, int DP, int N, int across, bool direct, bool far>
+__global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 && DP == 32 && across == 1 && direct ? (far ? 3 : 4) : 2)
 void attend_kernel(AttendArgs<T> p) {
-    using S = ForwardShape<T, DP, N, across>;
+    using S = ForwardShape<T, DP, N, across, sizeof(T) == 4 && (DP == 128 || (far && DP == 64 && !direct))>;
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, KB = S::blocks;
@@ -325,28 +325,34 @@ void attend_kernel(AttendArgs<T> p) {
                     m[n] = grown ? most : m[n];      // (each row by itself: no row has other bits for what its neighbours hold)
                 }
                 const float from = m[n] == -__builtin_inff() ? 0.0f : m[n] * to2 - (float)kForwardRaised<T>;   // (nothing seen yet: exponentials of -inf are 0)
+                float sum = 0.0f;      // (of this step alone: one addition a step to what may be the sum of very many)
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
                     float x[16];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][r], to2, -from));
-                        if constexpr (!by_product) l[n] += x[r];
+                        if constexpr (!by_product) sum += x[r];
                     }
                     e[b][0][n] = F::pack(x);
                     e[b][1][n] = F::pack(x + 8);
                 }
+                if constexpr (!by_product) l[n] += sum;
             }
+            if constexpr (far) {
+                accumulate_apart<DP, N>(acc, vt, wave % across * S::mine, e);
+            } else {
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int at = wave % across * S::mine + 32 * b + 16 * c;
-                    accumulate<T, DP, N>(acc, vt, at, e[b][c]);
-                    if constexpr (by_product)
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = wave % across * S::mine + 32 * b + 16 * c;
+                        accumulate<T, DP, N>(acc, vt, at, e[b][c]);
+                        if constexpr (by_product)
 #pragma unroll
-                        for (int n = 0; n < N; ++n) ones_acc[n] = F::mma(ones, e[b][c][n], ones_acc[n]);
-                }
+                            for (int n = 0; n < N; ++n) ones_acc[n] = F::mma(ones, e[b][c][n], ones_acc[n]);
+                    }
+            }
             if (odd) {
                 // (v's numbers that were taken out, for the lanes that see them: p is positive)
 #pragma unroll
@@ -556,12 +562,12 @@ __global__ __launch_bounds__(kAttendThreads) void attend_delta_kernel(AttendArgs
 // three: 512 windows of 64 cells, 4 heads of 16, 34 -> 28 us; heads of 64 lose as much as they gain, those of 128 have room for no more.)
 // (Heads of 64 in 16 bits: registers for three wavefronts a SIMD rather than two, 536 -> 472 us for 16 384 causal rows, 8 heads; with two of the four
 // fragments of g in LDS as good.)
-template <class T, int DP, bool direct>
+template <class T, int DP, bool direct, bool far>
 __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 2 && DP == 64 && direct ? 3 : 2)
 void attend_query_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
-    constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && DP != 64 ? 32 : 64, tile = keys * DP, KB = keys / 32;
+    constexpr int DB = DP / 32, rows = 128, keys = sizeof(T) == 4 && (DP != 64 || (far && !direct)) ? 32 : 64, tile = keys * DP, KB = keys / 32;
     __shared__ __attribute__((aligned(16))) T tiles[4 * tile];
     __shared__ int found[2];              // the tile of a stage that holds infinite numbers or NaN, or none
     __shared__ unsigned bad[keys / 32];   // keys that are not finite
@@ -646,10 +652,15 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
                 if (k0 < spans.all_low) hide_below(ds, see[0].low - k0 - 32 * b - 4 * h, 0.0f);
                 if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see[0].high - k0 - 32 * b - 4 * h, 0.0f);
                 if constexpr (kOwnScale<T>) delta *= fit(ds, up, acc[0]);
+                if constexpr (far) {
+                    const Eight e[1][2][1] = {{{F::pack(ds)}, {F::pack(ds + 8)}}};
+                    accumulate_apart<DP, 1>(acc, kt, 32 * b, e);
+                } else {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const Eight e[1] = {F::pack(ds + 8 * c)};
-                    accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
+                    for (int c = 0; c < 2; ++c) {
+                        const Eight e[1] = {F::pack(ds + 8 * c)};
+                        accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
+                    }
                 }
             }
         }
@@ -677,8 +688,8 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
 // registers alone left three and two: float32 512 windows of 64 cells, 4 heads of 16, 42 -> 30 us, 8 of 4096, heads of 32, 1330 -> 1220 (16 384 causal
 // rows 2650 -> 2840: all blocks start at once, the long with the short); bfloat16 windows of 1024, 4 heads of 32, 72 -> 62; heads of 64, 16 384 causal rows
 // 786 -> 752, 61 sequences of f16 154 -> 140.
-template <class T, int DP, bool direct>
-__global__ __launch_bounds__(kAttendThreads, DP == 32 ? (direct ? 4 : 2) : sizeof(T) == 4 ? 1 : DP == 64 ? (direct ? 3 : 2) : direct ? 2 : 1)
+template <class T, int DP, bool direct, bool far>
+__global__ __launch_bounds__(kAttendThreads, DP == 32 ? (direct ? (far ? 3 : 4) : 2) : sizeof(T) == 4 ? 1 : DP == 64 ? (direct ? 3 : 2) : direct ? 2 : 1)
 void attend_key_grad_kernel(AttendArgs<T> p) {
     using F = Frag<T>;
     using Eight = typename F::Eight;
@@ -792,12 +803,19 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                 if (below) hide_below(ds, low, 0.0f);
                 if (beyond) hide_from(ds, high, 0.0f);
                 if constexpr (kOwnScale<T>) (void)fit(ds, up, dk[0]);
+                if constexpr (far) {
+                    const Eight pe[1][2][1] = {{{F::pack(e)}, {F::pack(e + 8)}}}, pd[1][2][1] = {{{F::pack(ds)}, {F::pack(ds + 8)}}};
+                    accumulate_apart<DP, 1>(dv, gt, 32 * b, pe);
+                    if constexpr (DP == 32) __builtin_amdgcn_sched_barrier(0);
+                    accumulate_apart<DP, 1>(dk, qt, 32 * b, pd);
+                } else {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int at = 32 * b + 16 * c;
-                    const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
-                    accumulate<T, DP, 1>(dv, gt, at, pe);
-                    accumulate<T, DP, 1>(dk, qt, at, pd);
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = 32 * b + 16 * c;
+                        const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
+                        accumulate<T, DP, 1>(dv, gt, at, pe);
+                        accumulate<T, DP, 1>(dk, qt, at, pd);
+                    }
                 }
             }
         }

@@ -371,6 +371,26 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* l
     }
 }
 
+// The same of 32 KB rows from r0 on for float32, whose sums have no fewer bits than the result: these products are added up by themselves and then to acc, so
+// that a sum over very many rows is not one addition after another.
+template <int DP, int N, int KB>
+__device__ __forceinline__ void accumulate_apart(f32x16 (&acc)[N][DP / 32], const float* lds, int r0, const Frag<float>::Eight (&e)[KB][2][N]) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+        f32x16 sum[N] = {};
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const auto a = Tile<float, DP>::across(lds, r0 + 32 * b + 16 * c, db);
+#pragma unroll
+                for (int n = 0; n < N; ++n) sum[n] = Frag<float>::mma(a, e[b][c][n], sum[n]);
+            }
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n][db] += sum[n];
+    }
+}
+
 // the sum, and the larger, of a lane's number and that of the lane 32 away
 __device__ __forceinline__ float sum_of_halves(float v) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -48,10 +48,12 @@ OrderArgs::Axis order_axis(const AttendArgs<T>& p, const AttendPlan& plan, bool 
     const int count = keys ? p.rows : p.keys;
     return {to, (int)pieces(count, plan.rows), count, plan.rows, p.group, keys};
 }
-template <bool direct>
-void forward(AttendArgs<T>& p, const SvoxAttention& s, const AttendPlan& plan, hipStream_t stream) {
-    if (plan.few) launch(attend_kernel<T, DP, 1, 4, direct>, p, s, p.rows, plan, stream);
-    else launch(attend_kernel<T, DP, 1, 1, direct>, p, s, p.rows, plan, stream);
+// f(std::bool_constant of `direct`, of plan.far), of which 16-bit types have no kernels
+template <class F>
+void with_kind(bool direct, const AttendPlan& plan, F f) {
+    if constexpr (sizeof(T) == 4)
+        if (plan.far) return direct ? f(std::true_type(), std::true_type()) : f(std::false_type(), std::true_type());
+    direct ? f(std::true_type(), std::false_type()) : f(std::false_type(), std::false_type());
 }
 
 }  // namespace
@@ -75,8 +77,14 @@ int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void*
         p.order = o.axis[0].to;
         launch_order(o, 1, stream);
     }
-    if (direct_loads(s)) forward<true>(p, s, plan, stream);
-    else forward<false>(p, s, plan, stream);
+    if (plan.few) {
+        if (direct_loads(s)) launch(attend_kernel<T, DP, 1, 4, true, false>, p, s, p.rows, plan, stream);
+        else launch(attend_kernel<T, DP, 1, 4, false, false>, p, s, p.rows, plan, stream);
+    } else {
+        with_kind(direct_loads(s), plan, [&](auto direct, auto far) {
+            launch(attend_kernel<T, DP, 1, 1, decltype(direct)::value, decltype(far)::value>, p, s, p.rows, plan, stream);
+        });
+    }
     // (240 000 rows of up to 2 splits: 180 us by blocks, 13 by lanes; 32 rows of 12 splits: 5 us by blocks, 12 by lanes)
     const int64_t joined = (int64_t)p.kv_heads * p.rows;
     if (plan.splits > 16 || (plan.splits > 1 && joined <= 4096))
@@ -122,8 +130,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.part = mine.take<float>((int64_t)p.kv_heads * of_q.splits * p.rows * DP);
         }
         p.order = order[0];
-        if (direct) launch(attend_query_grad_kernel<T, DP, true>, p, s, p.rows, of_q, stream);
-        else launch(attend_query_grad_kernel<T, DP, false>, p, s, p.rows, of_q, stream);
+        with_kind(direct, of_q, [&](auto d, auto far) { launch(attend_query_grad_kernel<T, DP, decltype(d)::value, decltype(far)::value>, p, s, p.rows, of_q, stream); });
         if (of_q.splits > 1) sum(p.part, p.rows, of_q, p.group, p.scale, p.dq);
     }
     if ((p.dk || p.dv) && p.keys > 0) {
@@ -134,8 +141,7 @@ int launch_attention_backward<T, DP>(const SvoxAttention& s, const SvoxAttention
             p.part = mine.take<float>(2 * (int64_t)p.kv_heads * of_k.splits * p.keys * DP);
         }
         p.order = order[1];
-        if (direct) launch(attend_key_grad_kernel<T, DP, true>, p, s, p.keys, of_k, stream);
-        else launch(attend_key_grad_kernel<T, DP, false>, p, s, p.keys, of_k, stream);
+        with_kind(direct, of_k, [&](auto d, auto far) { launch(attend_key_grad_kernel<T, DP, decltype(d)::value, decltype(far)::value>, p, s, p.keys, of_k, stream); });
         if (of_k.splits > 1) {
             sum(p.part, p.keys, of_k, 1, p.scale, p.dk);
             sum(p.part + (int64_t)p.kv_heads * of_k.splits * p.keys * DP, p.keys, of_k, 1, 1.0f, p.dv);

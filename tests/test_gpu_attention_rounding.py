@@ -163,3 +163,16 @@ def test_a_row_of_small_exponentials(gpu, d, dtype):
         k[0] = 0
         want = exact(q[:1, :1], k, v, torch.zeros_like(q[:1, :1]))[0]
         assert roundings(svox.attention(q, k, v), want.expand(t, 8, d)) <= 6.0, below
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 30, 50, 99])
+def test_long_sums_in_32_bits(gpu, d):
+    """float32: a row's sums go over 65 536 keys in tiles of 32 or more, a key's over 16 384 rows.  An addition is a rounding of what the sum is by then: of
+    n / 32 one after another each of two sums (a row's exponentials and their products with values) has the root of n / 64 roundings' error, those within
+    a tile, a score's and an exponential's are some 200 more, a logarithm of a sum of some 2^14 as many again.  Twice the root of all of them, as they
+    are not all by themselves; of n / 4 or n / 2 additions one after another it would be more than that."""
+    t, n, h = 16384, 65536, 8
+    x, grad = inputs(t, n, h, h, d, torch.float32, seed=d)
+    got, want = step(x, grad), exact(*(v[:, :1] for v in (*x, grad)))
+    for name, a, b, along in zip(("y", "q", "k", "v"), got, want, (n, n, t, t)):
+        assert roundings(a[:, :1], b) <= 2 * math.sqrt(400 + along / 32), name
