@@ -137,7 +137,7 @@ class LeafDecoder(nn.Module):
     :param features: numbers of a leaf's features
     :param record: numbers of a record (`tree.data_dim`)
     :param hidden: hidden units of every block (default: four for each feature)
-    :param heads: heads of the attention in every block; 0: cells are decoded by themselves
+    :param heads: heads of the attention in every block, of up to 128 features each; 0: cells are decoded by themselves
     :param kv_heads: heads of its keys and values (default: as many)
     :param window: cells of a window: consecutive ones, which lie near one another in space, as a node's children follow one another
     """
@@ -157,6 +157,8 @@ class LeafDecoder(nn.Module):
             kv_heads = heads if kv_heads is None else kv_heads
             if heads < 0 or kv_heads < 1 or features % heads or heads % kv_heads or window < 1:
                 raise ValueError(f"{features} features do not make {heads} heads for {kv_heads} heads of keys, or a window of {window} cells is none")
+            if features // heads > 128:
+                raise ValueError(f"{features} features make heads of {features // heads} numbers of {heads} heads, more than the 128 that attention takes")
             self.attends = nn.ModuleList(_Attend(features, heads, kv_heads, eps, **kw) for _ in range(depth))
             # pairs of a head take turns among the three axes, from one turn over the tree to 2^8 (kept as whole numbers, whose type stays
             # where a module's is changed)
