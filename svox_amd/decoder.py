@@ -207,13 +207,18 @@ class LeafDecoder(nn.Module):
             _cells(tree.data, tree).copy_(records.view(*source.shape[:-1], -1))
         return records
 
-    def backward_through(self, features, tree, loss, max_norm=None):
+    def backward_through(self, features, tree, loss, max_norm=None, with_norm=False):
         """One pass of training: decodes `features` into `tree`, calls `loss` (a function of no arguments that renders `tree`) and
         adds the gradients of what it returns to those of the decoder's weights and of `features.data`, and to those of whatever else
         it was made of.  Returns the loss.  The records' gradient takes the decoder's type: in float16 what is below 2^-25 becomes zero,
         so scale the loss there.  With `max_norm` the gradients of the weights and of `features.data`, as they then stand, are clipped together
-        (`clip_grad_norm`).  (`tree.data` has to require its gradient, which is that of the records; what `tree.data.grad`
-        holds stays as it is.)"""
+        (`clip_grad_norm`); where their norm is not finite they stay as they are.  `with_norm` returns (loss, norm before), by which the caller
+        tells a batch whose step it had better leave out.  (`tree.data` has to require its gradient, which is that of the records; what
+        `tree.data.grad` holds stays as it is.)"""
+        if with_norm and max_norm is None:
+            raise ValueError("with_norm is the norm that max_norm bounds: give both")
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"max_norm must be >= 0, got {max_norm}")
         if not (tree.data.requires_grad and tree.data.is_leaf):
             raise ValueError("tree.data does not require a gradient, or is computed from something else: that of the records has to come through it")
         records = self.decode_tree(features, tree)
@@ -226,6 +231,7 @@ class LeafDecoder(nn.Module):
             tree.data.grad = kept
         if grad is not None and records.requires_grad:    # (None: the loss does not depend on the records)
             records.backward(_cells(grad, tree).reshape(records.shape).to(records.dtype))
-        if max_norm is not None:
-            clip_grad_norm([features.data, *self.parameters()], max_norm)
-        return value.detach()
+        if max_norm is None:
+            return value.detach()
+        norm = clip_grad_norm([features.data, *self.parameters()], max_norm)
+        return (value.detach(), norm) if with_norm else value.detach()
