@@ -219,6 +219,8 @@ class LeafDecoder(nn.Module):
             raise ValueError("with_norm is the norm that max_norm bounds: give both")
         if max_norm is not None and not max_norm >= 0:
             raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+        if max_norm is not None and features.data.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"gradients of {features.data.dtype} cannot be clipped: features need float32, float16 or bfloat16 for max_norm")
         if not (tree.data.requires_grad and tree.data.is_leaf):
             raise ValueError("tree.data does not require a gradient, or is computed from something else: that of the records has to come through it")
         records = self.decode_tree(features, tree)

@@ -22,6 +22,14 @@ def test_a_step_whose_norm_cannot_be_bounded_is_refused_before_it_begins():
             decoder.backward_through(None, None, None, **kw)
 
 
+def test_features_whose_gradients_cannot_be_clipped_are_refused_before_the_step_begins():
+    features, tree = svox.N3Tree(data_format=None, data_dim=8, dtype=torch.float64), svox.N3Tree(data_format="SH1")
+    called = []
+    with pytest.raises(ValueError, match="float64"):
+        svox.LeafDecoder(8, tree.data_dim, hidden=8).backward_through(features, tree, lambda: called.append(1), max_norm=1.0)
+    assert not called and features.data.grad is None
+
+
 @pytest.mark.gpu
 def test_a_step_tells_its_norm(gpu):
     """The norm of the gradients before they are clipped; where a batch has none that is finite, the step says so and leaves them as they are."""
