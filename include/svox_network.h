@@ -56,7 +56,7 @@ typedef struct SvoxRotateHeads {
     const float* frequencies;           /* (axes, rotated / 2) */
     int64_t rows;                       /* >= 0 */
     int64_t q_stride, q_head, k_stride, k_head;   /* from row to row and from head to head */
-    int32_t heads, kv_heads;            /* >= 1 and >= 0 */
+    int32_t heads, kv_heads;            /* >= 1 */
     int32_t dim;                        /* 1 .. 256 */
     int32_t rotated;                    /* even, 0 .. dim */
     int32_t axes;                       /* 1 .. 4 */
@@ -85,7 +85,8 @@ typedef struct SvoxAttention {
     const void *q, *k, *v;       /* (queries, heads, dim), (keys, kv_heads, dim) twice; a head's numbers lie side by side */
     const void* offsets;         /* (sequences + 1) int32, or int64 where wide_offsets; NULL: one sequence of all */
     const void* key_offsets;     /* the same of the keys; NULL: as offsets */
-    int64_t queries, keys;       /* >= 0; queries * heads / kv_heads and keys < 2^31 - 2^10 */
+    int64_t queries, keys;       /* >= 0; queries * heads / kv_heads and keys < 2^31 - 2^10, queries * heads and keys * kv_heads < 2^31 - 2^13 where
+                                  * the rows, or keys, of a kv head count in whole 128s */
     int64_t sequences;           /* >= 1 (1 without offsets) */
     int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;   /* from row to row and from head to head */
     int32_t heads, kv_heads;     /* heads a multiple of kv_heads */

@@ -14,6 +14,7 @@
 // Scores and their exponentials, sums, maxima and results are in 32 bits.  p and ds are rounded to 16-bit operands where the type has 16 bits, as the matrix
 // cores take them (in 32 bits they take seven times as long): a sum of many is off by what one rounding is, in the mean.
 #pragma once
+#include "attention_rules.h"
 #include "attention_tile.h"
 
 namespace svox_network {
@@ -82,7 +83,6 @@ __device__ __forceinline__ float fit(float (&ds)[16], float& up, f32x16 (&acc)[D
 struct Place {
     int tile, head, split;   // no tile: tile < 0
 };
-constexpr int kAttendRun = 8;
 template <class T>
 __device__ __forceinline__ Place place_of_block(const AttendArgs<T>& p) {
     // (a tile's first blocks before all others: most tiles may need no more, and blocks go round the eight XCDs)

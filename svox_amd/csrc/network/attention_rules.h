@@ -92,6 +92,10 @@ inline bool direct_loads(const SvoxAttention& s, const SvoxAttentionGrads& g) {
 // there are tiles for all XCDs.  Heads of few long sequences go round the XCDs instead.
 inline bool in_runs(const SvoxAttention& s, int64_t tiles) { return s.sequences >= 16 && tiles * s.kv_heads >= kAttendBlocks; }
 
+// Tiles that blocks of an XCD take side by side, and the blocks of `units` tiles of heads in such runs for all eight XCDs.
+constexpr int kAttendRun = 8;
+inline int64_t in_whole_runs(int64_t units) { return svox_decoder::up_to(units, 8 * kAttendRun); }
+
 inline int64_t attention_space(const SvoxAttention& s, bool backward) {
     const int64_t rows = s.queries * (s.heads / s.kv_heads), width = attend_width(s.dim);
     const auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };

@@ -41,7 +41,7 @@ void launch(K kernel, AttendArgs<T>& p, const SvoxAttention& s, int64_t count, c
     p.steps = plan.steps;
     p.runs = !p.order && in_runs(s, p.tiles);
     const int64_t units = (int64_t)p.tiles * p.kv_heads;
-    hipLaunchKernelGGL(kernel, grid_of((p.runs ? svox_decoder::up_to(units, 8 * kAttendRun) : units) * plan.splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
+    hipLaunchKernelGGL(kernel, grid_of((p.runs ? in_whole_runs(units) : units) * plan.splits, kAttendThreads), dim3(kAttendThreads), 0, stream, p);
 }
 // One axis of the launch that puts tiles in order.
 OrderArgs::Axis order_axis(const AttendArgs<T>& p, const AttendPlan& plan, bool keys, int* to) {

@@ -121,11 +121,12 @@ int check_attention(const SvoxAttention* s) {
     if (!s->offsets && (s->key_offsets || s->sequences != 1)) return fail(SVOX_ERR_NULL_POINTER, "offsets is NULL");
     if (s->offsets && !s->key_offsets && s->queries != s->keys)
         return fail(SVOX_ERR_BAD_SHAPE, "without key_offsets there must be as many keys as queries, got %lld and %lld", (long long)s->keys, (long long)s->queries);
-    // (rows of a kv head are counted in 32 bits, and a launch has fewer than 2^24 blocks of 32 of them and more)
+    // (rows of a kv head are counted in 32 bits, and a launch has fewer than 2^24 blocks of 128 of them, also where their number is made a whole one of runs)
     const int64_t most = INT32_MAX - 1024, rows = s->heads / s->kv_heads;
     if (s->keys > most || s->queries > most / rows) return fail(SVOX_ERR_UNSUPPORTED, "queries * heads / kv_heads and keys must be < 2^31 - 2^10");
-    if ((svox_decoder::pieces(s->queries * rows, 128) + 1) * s->kv_heads >= 1 << 24 || (svox_decoder::pieces(s->keys, 128) + 1) * s->kv_heads >= 1 << 24)
-        return fail(SVOX_ERR_UNSUPPORTED, "queries * heads and keys * kv_heads must be < 2^31");
+    for (const int64_t tiles : {svox_decoder::pieces(s->queries * rows, 128), svox_decoder::pieces(s->keys, 128)})
+        if ((tiles + 1) * s->kv_heads >= 1 << 24 || (in_runs(*s, tiles) && in_whole_runs(tiles * s->kv_heads) >= 1 << 24))
+            return fail(SVOX_ERR_UNSUPPORTED, "queries * heads and keys * kv_heads must be < 2^31 - 2^13");
     SVOX_TRY(check_heads("q", s->q, s->queries, s->heads, s->q_stride, s->q_head));
     SVOX_TRY(check_heads("k", s->k, s->keys, s->kv_heads, s->k_stride, s->k_head));
     return check_heads("v", s->v, s->keys, s->kv_heads, s->v_stride, s->v_head);
