@@ -122,11 +122,7 @@ __device__ __forceinline__ Part part_of(const AttendArgs<T>& p, const Spans& all
     return {{(int)(low < all.high ? low : all.high), (int)(high < all.high ? high : all.high)}, used};
 }
 
-template <int N>
-__device__ __forceinline__ void clip(Span (&see)[N], const Span& part) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) see[n].high = min(see[n].high, part.high);
-}
+__device__ __forceinline__ void clip(Span& see, const Span& part) { see.high = min(see.high, part.high); }
 
 // rows r of `x`, (tokens, heads, dim) with strides
 template <class T>
@@ -135,31 +131,23 @@ __device__ __forceinline__ const T* row_at(const T* x, int r, int group, int hea
     return x + (int64_t)token * stride + ((int64_t)head * group + (r - (int)token * group)) * head_stride;
 }
 
-// What the rows of a wavefront's lanes (row `mine` + lane % 32 of each of N) see, all of them together, and those of its block together, rows
+// What the rows of a wavefront's lanes (row `mine` + lane % 32) see, all of them together, and those of its block together, rows
 // r0 .. r0 + rows - 1; of rows where `keys` is not set.  Rows that are not there see everything, so that they never make a mask necessary.
-template <int N>
-__device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int mine, int count, int r0, int rows, int group, Span (&see)[N], Spans& block) {
-    const int lane = (int)threadIdx.x % kWave, last = min(r0 + rows, count) - 1, there = min(mine + 32 * N, count) - mine;
+__device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int mine, int count, int r0, int rows, int group, Span& see, Spans& block) {
+    const int lane = (int)threadIdx.x % kWave, last = min(r0 + rows, count) - 1, here = min(mine + 32, count) - mine;
     const int per_token = keys ? group : 1, per_other = keys ? 1 : group;
+    // (the upper lanes look at the block's first and last row)
+    const int r = mine + lane % 32, looked = lane < 32 ? min(r, last) : lane == 32 ? r0 : last;
+    Span v = per_token == 1 ? span_of(s, keys, looked, r0, last) : span_of(s, keys, looked / per_token, r0 / per_token, last / per_token);
+    v.low *= per_other, v.high *= per_other;
+    block = {__builtin_amdgcn_readlane(v.low, 32), __builtin_amdgcn_readlane(v.high, 33), __builtin_amdgcn_readlane(v.low, 33),
+             __builtin_amdgcn_readlane(v.high, 32)};
     Spans all{0, 0, INT32_MIN, INT32_MAX};
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        // (the upper lanes look at the block's first and last row)
-        const int r = mine + 32 * n + lane % 32;
-        const int looked = lane < 32 ? min(r, last) : lane == 32 ? r0 : last;
-        Span v = per_token == 1 ? span_of(s, keys, looked, r0, last) : span_of(s, keys, looked / per_token, r0 / per_token, last / per_token);
-        v.low *= per_other, v.high *= per_other;
-        if (n == 0)
-            block = {__builtin_amdgcn_readlane(v.low, 32), __builtin_amdgcn_readlane(v.high, 33), __builtin_amdgcn_readlane(v.low, 33),
-                     __builtin_amdgcn_readlane(v.high, 32)};
-        const int here = min(there - 32 * n, 32);
-        if (here > 0) {
-            if (n == 0) all.low = __builtin_amdgcn_readlane(v.low, 0), all.all_high = __builtin_amdgcn_readlane(v.high, 0);
-            all.high = __builtin_amdgcn_readlane(v.high, here - 1), all.all_low = __builtin_amdgcn_readlane(v.low, here - 1);
-        }
-        v.low = __shfl(v.low, lane % 32, kWave), v.high = __shfl(v.high, lane % 32, kWave);
-        see[n] = r < count ? v : Span{INT32_MIN, INT32_MAX};
-    }
+    if (here > 0)
+        all = {__builtin_amdgcn_readlane(v.low, 0), __builtin_amdgcn_readlane(v.high, here - 1), __builtin_amdgcn_readlane(v.low, here - 1),
+               __builtin_amdgcn_readlane(v.high, 0)};
+    v.low = __shfl(v.low, lane % 32, kWave), v.high = __shfl(v.high, lane % 32, kWave);
+    see = r < count ? v : Span{INT32_MIN, INT32_MAX};
     return all;
 }
 
@@ -183,19 +171,19 @@ __device__ __forceinline__ float left_of(float v) {
 }
 
 // ---- forward.  Four wavefronts, of which `across` share rows and take a part of every tile's keys each.
-template <class T, int DP, int N, int across, bool narrow>
+template <class T, int DP, int across, bool narrow>
 struct ForwardShape {
-    static constexpr int down = 4 / across, rows = down * 32 * N;
+    static constexpr int down = 4 / across, rows = down * 32;
     static constexpr int keys = across == 4 ? 128 : (narrow ? 32 : 64), mine = keys / across, blocks = mine / 32;
     static constexpr int stages = across == 4 && sizeof(T) == 4 && DP == 128 ? 1 : 2;   // tiles in LDS
     static constexpr int tile = keys * DP;
 };
 
 // (float32, heads of 32: registers for four wavefronts a SIMD rather than three: 512 windows of 64 cells, 4 heads of 16, 36 -> 30 us; 8 of 4096 644 -> 625.)
-template <class T, int DP, int N, int across, bool direct, bool far>
+template <class T, int DP, int across, bool direct, bool far>
 __global__ __launch_bounds__(kAttendThreads, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 && DP == 32 && across == 1 && direct ? (far ? 3 : 4) : 2)
 void attend_kernel(AttendArgs<T> p) {
-    using S = ForwardShape<T, DP, N, across, sizeof(T) == 4 && (DP == 128 || (far && DP == 64 && !direct))>;
+    using S = ForwardShape<T, DP, across, sizeof(T) == 4 && (DP == 128 || (far && DP == 64 && !direct))>;
     using F = Frag<T>;
     using Eight = typename F::Eight;
     constexpr int DB = DP / 32, KB = S::blocks;
@@ -207,15 +195,13 @@ void attend_kernel(AttendArgs<T> p) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), h = half_of();
     const Place place = place_of_block(p);
     if (place.tile < 0) return;
-    const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32 * N;
+    const int r0 = place.tile * S::rows, mine = r0 + wave / across * 32;
 
-    Eight q[N][DP / 16];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        load_row<T, DP, direct>(row_at(p.q, min(mine + 32 * n + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q[n]);
-    Span see[N];
+    Eight q[DP / 16];
+    load_row<T, DP, direct>(row_at(p.q, min(mine + (int)threadIdx.x % 32, p.rows - 1), p.group, place.head, p.q_stride, p.q_head), p.dim, q);
+    Span see;
     Spans block;
-    const Spans spans = spans_of<N>(p.seq, true, mine, p.rows, r0, S::rows, p.group, see, block);
+    const Spans spans = spans_of(p.seq, true, mine, p.rows, r0, S::rows, p.group, see, block);
     const Part share = part_of(p, block, S::keys, place);
     if (place.split >= share.used) return;
     if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
@@ -227,8 +213,8 @@ void attend_kernel(AttendArgs<T> p) {
     // some 590 cycles; 8 products of 32 cycles): the exponentials' sum is one more product, with ones, of which a lane's first number is kept
     // (512 windows of 512 cells, 4 heads of 32: 154 -> 149 us).
     constexpr bool by_product = sizeof(T) == 2 && DP <= 64;
-    f32x16 acc[N][DB], ones_acc[N];
-    float m[N], l[N];
+    f32x16 acc[DB], ones_acc = {};
+    float m = -__builtin_inff(), l = 0.0f;
     Eight ones;
     if constexpr (by_product) {
         const float one[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
@@ -236,12 +222,7 @@ void attend_kernel(AttendArgs<T> p) {
     }
     T* const tiles = reinterpret_cast<T*>(lds);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        m[n] = -__builtin_inff(), l[n] = 0.0f;
-        ones_acc[n] = f32x16{};
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[n][db] = f32x16{};
-    }
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
     Loader<T, DP, S::keys, direct> ks(p.k + place.head * p.k_head, p.k_stride, 0, 1, p.dim), vs(p.v + place.head * p.v_head, p.v_stride, 0, 1, p.dim);
     const auto load = [&](int k0, int stage) {
         ks.load(k0, part.high - k0, tiles + stage * 2 * S::tile);
@@ -276,102 +257,88 @@ void attend_kernel(AttendArgs<T> p) {
         const int kw = k0 + wave % across * S::mine;   // this wavefront's keys
         if (kw < spans.high && kw + S::mine > spans.low && kw < part.high) {
             if constexpr (DP == 128) __builtin_amdgcn_s_setprio(1);   // (the other wavefront of the SIMD has exponentials to compute meanwhile: 633 -> 600 us)
-            f32x16 s[KB][N];
+            f32x16 s[KB];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-#pragma unroll
-                for (int n = 0; n < N; ++n) s[b][n] = f32x16{};
+                s[b] = f32x16{};
 #pragma unroll
                 for (int t = 0; t < DP / 16; ++t) {
                     if (sizeof(T) == 4 && 16 * t >= p.dim) break;   // (float32's products are dear)
-                    const Eight a = Tile<T, DP>::along(kt, wave % across * S::mine + 32 * b, t);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) s[b][n] = F::mma(a, q[n][t], s[b][n]);
+                    s[b] = F::mma(Tile<T, DP>::along(kt, wave % across * S::mine + 32 * b, t), q[t], s[b]);
                 }
             }
             if constexpr (DP == 128) __builtin_amdgcn_s_setprio(0);
             // (the tile's end lies beyond what some lane sees, if it lies beyond the part)
             if (kw < spans.all_low) {
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) hide_below(s[b][n], see[n].low - kw - 32 * b - 4 * h, -__builtin_inff());
+                for (int b = 0; b < KB; ++b) hide_below(s[b], see.low - kw - 32 * b - 4 * h, -__builtin_inff());
             }
             if (kw + S::mine > min(spans.all_high, part.high)) {
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) hide_from(s[b][n], see[n].high - kw - 32 * b - 4 * h, -__builtin_inff());
+                for (int b = 0; b < KB; ++b) hide_from(s[b], see.high - kw - 32 * b - 4 * h, -__builtin_inff());
             }
-            Eight e[KB][2][N];
+            Eight e[KB][2];
+            float most = m;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                float most = m[n];
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
+                for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][r]);
+            most = most_of_halves(most);
+            // The maximum that exponentials are relative to need not be the largest score: any will do whose exponentials stay in range.  It is moved, and
+            // the sums with it, where a row's has grown by more than 2^kLag (a wavefront's 32 rows find new maxima in two tiles of three of a
+            // long sequence: 16 384 causal rows, 8 heads of 128 581 -> 550 us).
+            const bool grown = (most - m) * to2 > (float)kLag<T>;      // (not where both are infinite: exponentials of -inf are 0, and the row of an inf is NaN)
+            if (__any(grown)) {
+                const float less = grown ? __builtin_amdgcn_exp2f((m - most) * to2) : 1.0f;
+                if constexpr (by_product) ones_acc[0] *= less;
+                else l *= less;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][n][r]);
-                most = most_of_halves(most);
-                // The maximum that exponentials are relative to need not be the largest score: any will do whose exponentials stay in range.  It is moved, and
-                // the sums with it, where a row's has grown by more than 2^kLag (a wavefront's 32 rows find new maxima in two tiles of three of a
-                // long sequence: 16 384 causal rows, 8 heads of 128 581 -> 550 us).
-                const bool grown = (most - m[n]) * to2 > (float)kLag<T>;      // (not where both are infinite: exponentials of -inf are 0, and the row of an inf is NaN)
-                if (__any(grown)) {
-                    const float less = grown ? __builtin_amdgcn_exp2f((m[n] - most) * to2) : 1.0f;
-                    if constexpr (by_product) ones_acc[n][0] *= less;
-                    else l[n] *= less;
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) acc[n][db] *= less;
-                    m[n] = grown ? most : m[n];      // (each row by itself: no row has other bits for what its neighbours hold)
-                }
-                const float from = m[n] == -__builtin_inff() ? 0.0f : m[n] * to2 - (float)kForwardRaised<T>;   // (nothing seen yet: exponentials of -inf are 0)
-                float sum = 0.0f;      // (of this step alone: one addition a step to what may be the sum of very many)
-#pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    float x[16];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][n][r], to2, -from));
-                        if constexpr (!by_product) sum += x[r];
-                    }
-                    e[b][0][n] = F::pack(x);
-                    e[b][1][n] = F::pack(x + 8);
-                }
-                if constexpr (!by_product) l[n] += sum;
+                for (int db = 0; db < DB; ++db) acc[db] *= less;
+                m = grown ? most : m;      // (each row by itself: no row has other bits for what its neighbours hold)
             }
+            const float from = m == -__builtin_inff() ? 0.0f : m * to2 - (float)kForwardRaised<T>;   // (nothing seen yet: exponentials of -inf are 0)
+            float sum = 0.0f;      // (of this step alone: one addition a step to what may be the sum of very many)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                float x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], to2, -from));
+                    if constexpr (!by_product) sum += x[r];
+                }
+                e[b][0] = F::pack(x);
+                e[b][1] = F::pack(x + 8);
+            }
+            if constexpr (!by_product) l += sum;
             if constexpr (far) {
-                accumulate_apart<DP, N>(acc, vt, wave % across * S::mine, e);
+                accumulate_apart<DP>(acc, vt, wave % across * S::mine, e);
             } else {
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int at = wave % across * S::mine + 32 * b + 16 * c;
-                        accumulate<T, DP, N>(acc, vt, at, e[b][c]);
-                        if constexpr (by_product)
-#pragma unroll
-                            for (int n = 0; n < N; ++n) ones_acc[n] = F::mma(ones, e[b][c][n], ones_acc[n]);
+                        accumulate<T, DP>(acc, vt, at, e[b][c]);
+                        if constexpr (by_product) ones_acc = F::mma(ones, e[b][c], ones_acc);
                     }
             }
             if (odd) {
                 // (v's numbers that were taken out, for the lanes that see them: p is positive)
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int kind = 0; kind < 3; ++kind) {
-                        unsigned which[DB] = {};
+                for (int kind = 0; kind < 3; ++kind) {
+                    unsigned which[DB] = {};
 #pragma unroll 1
-                        for (int i = wave % across * S::mine; i < (wave % across + 1) * S::mine; ++i)
-                            if (k0 + i >= see[n].low && k0 + i < see[n].high)
+                    for (int i = wave % across * S::mine; i < (wave % across + 1) * S::mine; ++i)
+                        if (k0 + i >= see.low && k0 + i < see.high)
 #pragma unroll
-                                for (int db = 0; db < DB; ++db) which[db] |= kinds[kind][i][db];
-                        const float odd_one = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+                            for (int db = 0; db < DB; ++db) which[db] |= kinds[kind][i][db];
+                    const float odd_one = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
 #pragma unroll
-                        for (int db = 0; db < DB; ++db)
+                    for (int db = 0; db < DB; ++db)
 #pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                if (which[db] >> (row_of(r) + 4 * h) & 1) acc[n][db][r] += odd_one;
-                    }
+                        for (int r = 0; r < 16; ++r)
+                            if (which[db] >> (row_of(r) + 4 * h) & 1) acc[db][r] += odd_one;
+                }
             }
         }
         if constexpr (S::stages == 2) {
@@ -383,11 +350,10 @@ void attend_kernel(AttendArgs<T> p) {
         }
     }
 
-#pragma unroll
-    for (int n = 0; n < N; ++n) l[n] = by_product ? ones_acc[n][0] : sum_of_halves(l[n]);
+    l = by_product ? ones_acc[0] : sum_of_halves(l);
     if constexpr (across > 1) {
         // the wavefronts' sums, joined by the first: every lane finds its own numbers of the others
-        static_assert(across == 4 && N == 1, "all wavefronts share rows");
+        static_assert(across == 4, "all wavefronts share rows");
         __syncthreads();
         float* const shared = reinterpret_cast<float*>(lds);
         const int lane = (int)threadIdx.x % kWave;
@@ -397,52 +363,49 @@ void attend_kernel(AttendArgs<T> p) {
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) own[(db * 16 + r) * kWave + lane] = acc[0][db][r];
-        if (lane < 32) own[each + lane] = m[0], own[each + 32 + lane] = l[0];
+            for (int r = 0; r < 16; ++r) own[(db * 16 + r) * kWave + lane] = acc[db][r];
+        if (lane < 32) own[each + lane] = m, own[each + 32 + lane] = l;
         __syncthreads();
         if (wave != 0) return;
-        float most = m[0];
+        float most = m;
         for (int w = 1; w < 4; ++w) most = fmaxf(most, shared[w * (each + 64) + each + lane % 32]);
         const float from = most == -__builtin_inff() ? 0.0f : most;
-        l[0] = 0.0f;
+        l = 0.0f;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
+        for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
         for (int w = 0; w < 4; ++w) {
             const float* const other = shared + w * (each + 64);
             if (other[each + lane % 32] == -__builtin_inff() && other[each + 32 + lane % 32] == 0.0f) continue;
             const float less = __builtin_amdgcn_exp2f((other[each + lane % 32] - from) * to2);
-            l[0] = __builtin_fmaf(other[each + 32 + lane % 32], less, l[0]);
+            l = __builtin_fmaf(other[each + 32 + lane % 32], less, l);
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[0][db][r] = __builtin_fmaf(other[(db * 16 + r) * kWave + lane], less, acc[0][db][r]);
+                for (int r = 0; r < 16; ++r) acc[db][r] = __builtin_fmaf(other[(db * 16 + r) * kWave + lane], less, acc[db][r]);
         }
-        m[0] = most;
+        m = most;
     }
+    const int thread = thread_again(), half = thread / 32 % 2, r = mine + thread % 32;
+    if (r >= p.rows) return;
+    // (what a row that sees keys has, though all of its scores are -inf, is not what one that sees none has)
+    const bool some = max(see.low, part.low) < see.high;
+    if (share.used > 1) {
+        const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
+        if (half == 0) p.stats[at] = f32x2{some ? fmaxf(m * to2 - (float)kForwardRaised<T>, -3.0e38f) : -__builtin_inff(), some ? l : 0.0f};
+        if (some) store_row<float, DB>(p.part + at * DP, DP, acc, 1.0f, half);
+    } else {
+        const unsigned token = (unsigned)r / again(p.group);
+        const int64_t to = (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim;
+        const float factor = some ? 1.0f / l : 0.0f;
+        store_row<T, DB>(p.y + to, p.dim, acc, factor, half);
+        if (p.rest) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const int thread = thread_again(), half = thread / 32 % 2, r = mine + 32 * n + thread % 32;
-        if (r >= p.rows) continue;
-        // (what a row that sees keys has, though all of its scores are -inf, is not what one that sees none has)
-        const bool some = max(see[n].low, part.low) < see[n].high;
-        if (share.used > 1) {
-            const int64_t at = ((int64_t)place.head * p.splits + place.split) * p.rows + r;
-            if (half == 0) p.stats[at] = f32x2{some ? fmaxf(m[n] * to2 - (float)kForwardRaised<T>, -3.0e38f) : -__builtin_inff(), some ? l[n] : 0.0f};
-            if (some) store_row<float, DB>(p.part + at * DP, DP, acc[n], 1.0f, half);
-        } else {
-            const unsigned token = (unsigned)r / again(p.group);
-            const int64_t to = (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim;
-            const float factor = some ? 1.0f / l[n] : 0.0f;
-            store_row<T, DB>(p.y + to, p.dim, acc[n], factor, half);
-            if (p.rest) {
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[n][db][i] = left_of<T>(acc[n][db][i] * factor);
-                store_row<T, DB>(p.rest + to, p.dim, acc[n], 1.0f, half);
-            }
-            if (p.lse && half == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m[n], to2, __builtin_amdgcn_logf(l[n]) - (float)kForwardRaised<T>) : kNoSum;
+                for (int i = 0; i < 16; ++i) acc[db][i] = left_of<T>(acc[db][i] * factor);
+            store_row<T, DB>(p.rest + to, p.dim, acc, 1.0f, half);
         }
+        if (p.lse && half == 0) p.lse[(int64_t)place.head * p.rows + r] = some ? __builtin_fmaf(m, to2, __builtin_amdgcn_logf(l) - (float)kForwardRaised<T>) : kNoSum;
     }
 }
 
@@ -579,9 +542,9 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
     Eight q[DP / 16], g[DP / 16];
     load_row<T, DP, direct>(row_at(p.q, row, p.group, place.head, p.q_stride, p.q_head), p.dim, q);
     load_row<T, DP, direct>(row_at(p.grad, row, p.group, place.head, p.grad_stride, p.grad_head), p.dim, g);
-    Span see[1];
+    Span see;
     Spans block;
-    const Spans spans = spans_of<1>(p.seq, true, mine, p.rows, r0, rows, p.group, see, block);
+    const Spans spans = spans_of(p.seq, true, mine, p.rows, r0, rows, p.group, see, block);
     const Part share = part_of(p, block, keys, place);
     if (place.split >= share.used) return;
     if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
@@ -598,11 +561,11 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
 #pragma unroll
     for (int t = kept; t < DP / 16; ++t) rest[t - kept][threadIdx.x] = g[t];
     const float to2 = p.scale * kLog2E;
-    f32x16 acc[1][DB];
+    f32x16 acc[DB];
     float none = 0.0f, up = kOwnScale<T> ? kMostUp : 1.0f;
     delta *= up;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[0][db] = f32x16{};
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
     Loader<T, DP, keys, direct> ks(p.k + place.head * p.k_head, p.k_stride, 0, 1, p.dim), vs(p.v + place.head * p.v_head, p.v_stride, 0, 1, p.dim);
     const auto load = [&](int k0, int stage) {
         ks.load(k0, part.high - k0, tiles + stage * 2 * tile);
@@ -649,36 +612,35 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
                     if constexpr (kOwnScale<T>) ds[r] = p_r * __builtin_fmaf(dp[r], up, -delta);
                     else ds[r] = p_r * (dp[r] - delta);
                 }
-                if (k0 < spans.all_low) hide_below(ds, see[0].low - k0 - 32 * b - 4 * h, 0.0f);
-                if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see[0].high - k0 - 32 * b - 4 * h, 0.0f);
-                if constexpr (kOwnScale<T>) delta *= fit(ds, up, acc[0]);
+                if (k0 < spans.all_low) hide_below(ds, see.low - k0 - 32 * b - 4 * h, 0.0f);
+                if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see.high - k0 - 32 * b - 4 * h, 0.0f);
+                if constexpr (kOwnScale<T>) delta *= fit(ds, up, acc);
                 if constexpr (far) {
-                    const Eight e[1][2][1] = {{{F::pack(ds)}, {F::pack(ds + 8)}}};
-                    accumulate_apart<DP, 1>(acc, kt, 32 * b, e);
+                    const Eight e[1][2] = {{F::pack(ds), F::pack(ds + 8)}};
+                    accumulate_apart<DP>(acc, kt, 32 * b, e);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const Eight e[1] = {F::pack(ds + 8 * c)};
-                        accumulate<T, DP, 1>(acc, kt, 32 * b + 16 * c, e);
+                        accumulate<T, DP>(acc, kt, 32 * b + 16 * c, F::pack(ds + 8 * c));
                     }
                 }
             }
         }
         if (odd)      // (whoever sees a key that is not finite has no gradient that is)
             for (int i = 0; i < keys; ++i)
-                if ((bad[i / 32] >> i % 32 & 1) && k0 + i >= see[0].low && k0 + i < see[0].high) none = __builtin_nanf("");
+                if ((bad[i / 32] >> i % 32 & 1) && k0 + i >= see.low && k0 + i < see.high) none = __builtin_nanf("");
         stage ^= 1;
         if (more) finish(stage, k0 + keys);
     }
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[0][db] += none;
+    for (int db = 0; db < DB; ++db) acc[db] += none;
     const int thread = thread_again(), half = thread / 32 % 2, r = mine + thread % 32;
     if (r >= p.rows) return;
     if (share.used > 1) {
-        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc[0], 1.0f / up, half);
+        store_row<float, DB>(p.part + (((int64_t)place.head * p.splits + place.split) * p.rows + r) * DP, DP, acc, 1.0f / up, half);
     } else {
         const unsigned token = (unsigned)r / again(p.group);
-        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc[0], p.scale / up, half);
+        store_row<T, DB>(p.dq + (((int64_t)token * p.kv_heads + place.head) * p.group + (r - (int)token * p.group)) * p.dim, p.dim, acc, p.scale / up, half);
     }
 }
 
@@ -702,9 +664,9 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     if (place.tile < 0) return;
     const int j0 = place.tile * keys, mine = j0 + wave * 32, key = min(mine + (int)threadIdx.x % 32, p.keys - 1);
 
-    Span see[1];
+    Span see;
     Spans block;
-    const Spans spans = spans_of<1>(p.seq, false, mine, p.keys, j0, keys, p.group, see, block);
+    const Spans spans = spans_of(p.seq, false, mine, p.keys, j0, keys, p.group, see, block);
     const Part share = part_of(p, block, rows, place);
     if (place.split >= share.used) return;
     if (p.splits > 1 && place.split == 0 && threadIdx.x == 0) p.used[place.head * p.tiles + place.tile] = share.used;
@@ -725,9 +687,9 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     const float to2 = p.scale * kLog2E;
     const float* const lse = p.lse + (int64_t)place.head * p.rows;
     const float* const delta = p.delta + (int64_t)place.head * p.rows;
-    f32x16 dk[1][DB], dv[1][DB];
+    f32x16 dk[DB], dv[DB];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) dk[0][db] = dv[0][db] = f32x16{};
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
     Loader<T, DP, rows, direct> qs(p.q + (int64_t)place.head * p.group * p.q_head, p.q_stride, p.q_head, p.group, p.dim),
         gs(p.grad + (int64_t)place.head * p.group * p.grad_head, p.grad_stride, p.grad_head, p.group, p.dim);
     float stat = 0.0f, up = kOwnScale<T> ? kMostUp * kLowered<T> : 1.0f;
@@ -789,7 +751,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                     }
                 }
                 const bool below = i0 < spans.all_low, beyond = i0 + rows > min(spans.all_high, part.high);
-                const int low = see[0].low - i0 - 32 * b - 4 * h, high = see[0].high - i0 - 32 * b - 4 * h;
+                const int low = see.low - i0 - 32 * b - 4 * h, high = see.high - i0 - 32 * b - 4 * h;
                 if (below) hide_below(e, low, 0.0f);
                 if (beyond) hide_from(e, high, 0.0f);
 #pragma unroll
@@ -802,19 +764,19 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                 for (int r = 0; r < 16; ++r) ds[r] = kOwnScale<T> ? e[r] * dp[r] * up : e[r] * dp[r];
                 if (below) hide_below(ds, low, 0.0f);
                 if (beyond) hide_from(ds, high, 0.0f);
-                if constexpr (kOwnScale<T>) (void)fit(ds, up, dk[0]);
+                if constexpr (kOwnScale<T>) (void)fit(ds, up, dk);
                 if constexpr (far) {
-                    const Eight pe[1][2][1] = {{{F::pack(e)}, {F::pack(e + 8)}}}, pd[1][2][1] = {{{F::pack(ds)}, {F::pack(ds + 8)}}};
-                    accumulate_apart<DP, 1>(dv, gt, 32 * b, pe);
+                    const Eight pe[1][2] = {{F::pack(e), F::pack(e + 8)}}, pd[1][2] = {{F::pack(ds), F::pack(ds + 8)}};
+                    accumulate_apart<DP>(dv, gt, 32 * b, pe);
                     if constexpr (DP == 32) __builtin_amdgcn_sched_barrier(0);
-                    accumulate_apart<DP, 1>(dk, qt, 32 * b, pd);
+                    accumulate_apart<DP>(dk, qt, 32 * b, pd);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int at = 32 * b + 16 * c;
-                        const Eight pe[1] = {F::pack(e + 8 * c)}, pd[1] = {F::pack(ds + 8 * c)};
-                        accumulate<T, DP, 1>(dv, gt, at, pe);
-                        accumulate<T, DP, 1>(dk, qt, at, pd);
+                        const Eight pe = F::pack(e + 8 * c), pd = F::pack(ds + 8 * c);
+                        accumulate<T, DP>(dv, gt, at, pe);
+                        accumulate<T, DP>(dk, qt, at, pd);
                     }
                 }
             }
@@ -826,12 +788,12 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     if (j >= p.keys) return;
     if (share.used > 1) {
         float* const at = p.part + (((int64_t)place.head * p.splits + place.split) * p.keys + j) * DP;
-        store_row<float, DB>(at, DP, dk[0], kLowered<T> / up, half);
-        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv[0], kLowered<T>, half);
+        store_row<float, DB>(at, DP, dk, kLowered<T> / up, half);
+        store_row<float, DB>(at + (int64_t)p.kv_heads * p.splits * p.keys * DP, DP, dv, kLowered<T>, half);
     } else {
         const int64_t at = ((int64_t)j * p.kv_heads + place.head) * p.dim;
-        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk[0], p.scale * kLowered<T> / up, half);
-        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv[0], kLowered<T>, half);
+        if (p.dk) store_row<T, DB>(p.dk + at, p.dim, dk, p.scale * kLowered<T> / up, half);
+        if (p.dv) store_row<T, DB>(p.dv + at, p.dim, dv, kLowered<T>, half);
     }
 }
 

@@ -361,33 +361,24 @@ struct Spans {
 };
 
 // acc += across rows r0 .. r0 + 15 of a tile times `b`
-template <class T, int DP, int N>
-__device__ __forceinline__ void accumulate(f32x16 (&acc)[N][DP / 32], const T* lds, int r0, const typename Frag<T>::Eight (&b)[N]) {
+template <class T, int DP>
+__device__ __forceinline__ void accumulate(f32x16 (&acc)[DP / 32], const T* lds, int r0, typename Frag<T>::Eight b) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) {
-        const auto a = Tile<T, DP>::across(lds, r0, db);
-#pragma unroll
-        for (int n = 0; n < N; ++n) acc[n][db] = Frag<T>::mma(a, b[n], acc[n][db]);
-    }
+    for (int db = 0; db < DP / 32; ++db) acc[db] = Frag<T>::mma(Tile<T, DP>::across(lds, r0, db), b, acc[db]);
 }
 
 // The same of 32 KB rows from r0 on for float32, whose sums have no fewer bits than the result: these products are added up by themselves and then to acc, so
 // that a sum over very many rows is not one addition after another.
-template <int DP, int N, int KB>
-__device__ __forceinline__ void accumulate_apart(f32x16 (&acc)[N][DP / 32], const float* lds, int r0, const Frag<float>::Eight (&e)[KB][2][N]) {
+template <int DP, int KB>
+__device__ __forceinline__ void accumulate_apart(f32x16 (&acc)[DP / 32], const float* lds, int r0, const Frag<float>::Eight (&e)[KB][2]) {
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) {
-        f32x16 sum[N] = {};
+        f32x16 sum = {};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const auto a = Tile<float, DP>::across(lds, r0 + 32 * b + 16 * c, db);
-#pragma unroll
-                for (int n = 0; n < N; ++n) sum[n] = Frag<float>::mma(a, e[b][c][n], sum[n]);
-            }
-#pragma unroll
-        for (int n = 0; n < N; ++n) acc[n][db] += sum[n];
+            for (int c = 0; c < 2; ++c) sum = Frag<float>::mma(Tile<float, DP>::across(lds, r0 + 32 * b + 16 * c, db), e[b][c], sum);
+        acc[db] += sum;
     }
 }
 

@@ -78,11 +78,11 @@ int launch_attention<T, DP>(const SvoxAttention& s, void* out, float* lse, void*
         launch_order(o, 1, stream);
     }
     if (plan.few) {
-        if (direct_loads(s)) launch(attend_kernel<T, DP, 1, 4, true, false>, p, s, p.rows, plan, stream);
-        else launch(attend_kernel<T, DP, 1, 4, false, false>, p, s, p.rows, plan, stream);
+        if (direct_loads(s)) launch(attend_kernel<T, DP, 4, true, false>, p, s, p.rows, plan, stream);
+        else launch(attend_kernel<T, DP, 4, false, false>, p, s, p.rows, plan, stream);
     } else {
         with_kind(direct_loads(s), plan, [&](auto direct, auto far) {
-            launch(attend_kernel<T, DP, 1, 1, decltype(direct)::value, decltype(far)::value>, p, s, p.rows, plan, stream);
+            launch(attend_kernel<T, DP, 1, decltype(direct)::value, decltype(far)::value>, p, s, p.rows, plan, stream);
         });
     }
     // (240 000 rows of up to 2 splits: 180 us by blocks, 13 by lanes; 32 rows of 12 splits: 5 us by blocks, 12 by lanes)
