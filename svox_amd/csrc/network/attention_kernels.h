@@ -151,6 +151,10 @@ __device__ __forceinline__ Spans spans_of(const Sequences& s, bool keys, int min
     return all;
 }
 
+// `place`, an end of what a lane sees, counted from `from`: modulo 2^32, as the ends of rows that are not there are those of the integers, and what it
+// then is does not matter.
+__device__ __forceinline__ int from_place(int place, int from) { return (int)((unsigned)place - (unsigned)from); }
+
 // A lane's 16 scores whose rows lie below `low`, or from `high` on (counted from the first of them), become `v`.
 template <class Scores>
 __device__ __forceinline__ void hide_below(Scores& s, int low, float v) {
@@ -271,11 +275,11 @@ void attend_kernel(AttendArgs<T> p) {
             // (the tile's end lies beyond what some lane sees, if it lies beyond the part)
             if (kw < spans.all_low) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b) hide_below(s[b], see.low - kw - 32 * b - 4 * h, -__builtin_inff());
+                for (int b = 0; b < KB; ++b) hide_below(s[b], from_place(see.low, kw + 32 * b + 4 * h), -__builtin_inff());
             }
             if (kw + S::mine > min(spans.all_high, part.high)) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b) hide_from(s[b], see.high - kw - 32 * b - 4 * h, -__builtin_inff());
+                for (int b = 0; b < KB; ++b) hide_from(s[b], from_place(see.high, kw + 32 * b + 4 * h), -__builtin_inff());
             }
             Eight e[KB][2];
             float most = m;
@@ -612,8 +616,8 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
                     if constexpr (kOwnScale<T>) ds[r] = p_r * __builtin_fmaf(dp[r], up, -delta);
                     else ds[r] = p_r * (dp[r] - delta);
                 }
-                if (k0 < spans.all_low) hide_below(ds, see.low - k0 - 32 * b - 4 * h, 0.0f);
-                if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, see.high - k0 - 32 * b - 4 * h, 0.0f);
+                if (k0 < spans.all_low) hide_below(ds, from_place(see.low, k0 + 32 * b + 4 * h), 0.0f);
+                if (k0 + keys > min(spans.all_high, part.high)) hide_from(ds, from_place(see.high, k0 + 32 * b + 4 * h), 0.0f);
                 if constexpr (kOwnScale<T>) delta *= fit(ds, up, acc);
                 if constexpr (far) {
                     const Eight e[1][2] = {{F::pack(ds), F::pack(ds + 8)}};
@@ -751,7 +755,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
                     }
                 }
                 const bool below = i0 < spans.all_low, beyond = i0 + rows > min(spans.all_high, part.high);
-                const int low = see.low - i0 - 32 * b - 4 * h, high = see.high - i0 - 32 * b - 4 * h;
+                const int low = from_place(see.low, i0 + 32 * b + 4 * h), high = from_place(see.high, i0 + 32 * b + 4 * h);
                 if (below) hide_below(e, low, 0.0f);
                 if (beyond) hide_from(e, high, 0.0f);
 #pragma unroll
