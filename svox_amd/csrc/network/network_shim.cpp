@@ -46,6 +46,7 @@ void check_clipped(const std::vector<Tensor>& all, const char* name, double max_
     for (const Tensor& x : all) {
         if (!x.is_cuda()) fail("every tensor must be a CUDA tensor");
         if (x.layout() != at::kStrided) fail("every tensor must be a dense tensor");
+        if (!x.has_storage()) fail("every tensor must have memory of its own: transforms of functions (vmap, torch.func) are not supported");
         if (x.device() != all[0].device()) fail("every tensor must be on the same device, got " + all[0].device().str() + " and " + x.device().str());
         dtype_code(x, "every tensor");
         if (x._fw_grad(0).defined()) fail(std::string("svox.") + name + " has no derivatives in forward mode");
