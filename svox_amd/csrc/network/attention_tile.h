@@ -332,7 +332,7 @@ __device__ __forceinline__ Span span_of(const Sequences& s, bool keys, int t, in
     } else {
         int low = a, high = mine.n;
         while (low < high) {
-            const int middle = (low + high + 1) / 2;
+            const int middle = low + (high - low + 1) / 2;      // (there may be more than 2^30 sequences)
             if (mine(middle) <= t) low = middle;
             else high = middle - 1;
         }
