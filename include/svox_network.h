@@ -96,7 +96,7 @@ typedef struct SvoxAttention {
 } SvoxAttention;
 
 /* out (queries, heads, dim).  What svox_attention_backward needs besides, or NULL: lse (queries * heads floats), of the scores' sums; rest
- * (queries, heads, dim), what rounding to 16 bits took from out. */
+ * (queries, heads, dim), what rounding to 16 bits took from out (of float16 times 2^11). */
 int svox_attention(const SvoxAttention* spec, void* out, float* lse, void* rest, void* workspace, int64_t workspace_bytes, void* stream);
 
 typedef struct SvoxAttentionGrads {

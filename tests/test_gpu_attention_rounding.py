@@ -176,3 +176,14 @@ def test_long_sums_in_32_bits(gpu, d):
     got, want = step(x, grad), exact(*(v[:, :1] for v in (*x, grad)))
     for name, a, b, along in zip(("y", "q", "k", "v"), got, want, (n, n, t, t)):
         assert roundings(a[:, :1], b) <= 2 * math.sqrt(400 + along / 32), name
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=name_of)
+@pytest.mark.parametrize("n,d", [(300, 64), (4000, 32), (4000, 128), (2000, 33)])
+@pytest.mark.parametrize("values", [1e-2, 1e-4, 1e-5])
+def test_small_values_and_large_gradients(gpu, n, d, values, dtype):
+    """A loss that is scaled, as float16 asks for, over values whose mean float16 holds a few bits of: the influences of scores are of both's product."""
+    x, grad = inputs(300, n, 2, 1, d, dtype, seed=d, size=2000.0)
+    x[2] = (x[2].float() * values).to(dtype)
+    for got, want in zip(step(x, grad), exact(*x, grad)):
+        assert roundings(got, want) <= TWO
