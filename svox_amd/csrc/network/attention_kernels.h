@@ -58,8 +58,8 @@ template <class T>
 constexpr float kLowered = std::is_same_v<T, F16> ? 0x1p-14f : 1.0f;
 // ds, which may be anything, each row of dq and each key of dk takes times a power of two of its own, `up`: from kMostUp on, with which no number of
 // float16 leaves float32's range, down to where the largest so far lies below 2^15, each time by as much as brings it to 2^14; the sum goes along.
-// (Gradients of some 1e-3, 200 rows over 32 768 keys: dq 22.6 times the error of one rounding without it, 1.01 with it.  It is 61 sequences' dq in 85 ->
-// 94 us, dk and dv in 143 -> 162.)
+// (Gradients of some 1e-3, 200 rows over 32 768 keys: dq 22.6 times the error of one rounding without it, 1.01 with it.  61 sequences' dq takes
+// 85 -> 93 us for it, dk and dv 143 -> 161.)
 template <class T>
 constexpr bool kOwnScale = std::is_same_v<T, F16>;
 constexpr float kMostUp = 0x1p80f;
@@ -659,7 +659,7 @@ void attend_query_grad_kernel(AttendArgs<T> p) {
 // How many wavefronts share a SIMD: four with heads of 32, three with heads of 64 in 16 bits, and some of v's fragments in LDS for it (`kept`), where
 // registers alone left three and two: float32 512 windows of 64 cells, 4 heads of 16, 42 -> 30 us, 8 of 4096, heads of 32, 1330 -> 1220 (16 384 causal
 // rows 2650 -> 2840: all blocks start at once, the long with the short); bfloat16 windows of 1024, 4 heads of 32, 72 -> 62; heads of 64, 16 384 causal rows
-// 786 -> 752, 61 sequences of f16 154 -> 140.
+// 786 -> 752, 61 sequences of f16 154 -> 140 (with `fit` 161).
 template <class T, int DP, bool direct, bool far>
 __global__ __launch_bounds__(kAttendThreads, DP == 32 ? (direct ? (far ? 3 : 4) : 2) : sizeof(T) == 4 ? 1 : DP == 64 ? (direct ? 3 : 2) : direct ? 2 : 1)
 void attend_key_grad_kernel(AttendArgs<T> p) {
@@ -684,7 +684,7 @@ void attend_key_grad_kernel(AttendArgs<T> p) {
     clip(see, part);
 
     // (Fragments of v that stay in registers; the others stay in LDS.  Heads of 128: registers that were missing lay in memory, and to load them again was to
-    // wait for the next tile too: 1460 -> 1380 us for 16 384 causal rows, 8 heads.)
+    // wait for the next tile too: 1460 -> 1380 us for 16 384 causal rows, 8 heads, by that alone; 1228 with all that came since.)
     constexpr int kept = DP == 32 ? 1 : sizeof(T) == 4 ? DP / 16 : DP == 64 ? (kOwnScale<T> ? 0 : 1) : kOwnScale<T> ? 2 : 4;
     // (float16: `fit` needs some as well, and has them by 32 rows at a time and more of v in LDS)
     constexpr bool one_by_one = kOwnScale<T> && DP <= 64;

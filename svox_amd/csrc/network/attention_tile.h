@@ -63,8 +63,8 @@ __device__ __forceinline__ int half_of() { return (int)threadIdx.x / 32 % 2; }
 
 // A tile of rows of DP numbers in LDS.  The 16-byte pieces of a row lie in an order that depends on the row, so that lanes that read a piece of
 // different rows, and those that read four rows across, find them in different banks.  Rows of 256 bytes fill the banks: sixteen pieces change places, for
-// sixteen rows, and reads take half as long as with eight (16 384 causal rows of bfloat16, 8 heads: forward 586 -> 576 us, dq 864 -> 848, dk and dv, which
-// wait for one product after another, 1380 either way).  Narrower rows and float32's: eight, as what sixteen save in LDS they cost in registers (heads
+// sixteen rows, and reads take half as long as with eight (16 384 causal rows of bfloat16, 8 heads, by that alone: forward 586 -> 576 us, dq 864 -> 848, dk and dv,
+// which wait for one product after another, as before; with all that came since, under the profiler, 531, 776 and 1228).  Narrower rows and float32's: eight, as what sixteen save in LDS they cost in registers (heads
 // of 64: dk and dv 84 -> 86 us).
 template <class T, int DP>
 struct Tile {

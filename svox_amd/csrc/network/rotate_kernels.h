@@ -144,8 +144,8 @@ __device__ __forceinline__ float sum_over_lanes(float v) {
     return v;
 }
 
-// Measured, bfloat16: 131 072 rows of 8 + 4 heads of 128 158 us (805 MB, 5.1 TB/s; a copy of 2 GiB 4.9), their gradients 281 us (1.2 GB, 4.3 TB/s);
-// 262 144 rows of 8 + 2 heads of 32 91 us (338 MB, 3.7 TB/s: the angles of 16 pairs a row, three axes each, are a quarter of the instructions).
+// Measured under the profiler, bfloat16: 131 072 rows of 8 + 4 heads of 128 160 us (805 MB, 5.0 TB/s; a copy of 2 GiB 4.9), their gradients 288 us (1.2 GB,
+// 4.2 TB/s); 262 144 rows of 8 + 2 heads of 32 91 us (339 MB, 3.7 TB/s: the angles of 16 pairs a row, three axes each, are a quarter of the instructions).
 template <class T, int lanes, bool interleaved, bool backward>
 __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateArgs<T> p) {
     constexpr int W = kRotatePairs<T>, groups = kRotateThreads / lanes;

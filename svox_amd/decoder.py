@@ -139,7 +139,8 @@ class LeafDecoder(nn.Module):
     :param hidden: hidden units of every block (default: four for each feature)
     :param heads: heads of the attention in every block, of up to 128 features each; 0: cells are decoded by themselves
     :param kv_heads: heads of its keys and values (default: as many)
-    :param window: cells of a window: consecutive ones, which lie near one another in space, as a node's children follow one another
+    :param window: cells of a window: consecutive ones, which lie near one another in space, as a node's children follow one another.  Cells that
+        are divided are among them: their records nobody reads, but the leaves of their window see their features
     """
 
     def __init__(self, features, record, hidden=None, depth=1, activation="silu", eps=1e-5, device=None, dtype=torch.float32, heads=0, kv_heads=None,
