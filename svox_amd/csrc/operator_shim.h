@@ -59,8 +59,8 @@ int32_t dtype_code(const Tensor& x, const char* name) {
 }
 void check_like(const Tensor& x, const Tensor& with, const char* name, const char* of = "x") {
     if (!x.is_cuda()) fail(std::string(name) + " must be a CUDA tensor");
-    if (!x.has_storage()) fail(std::string(name) + " has no memory of its own: transforms of functions (vmap, torch.func) are not supported");
     if (x.layout() != at::kStrided) fail(std::string(name) + " must be a dense tensor");
+    if (!x.has_storage()) fail(std::string(name) + " has no memory of its own: transforms of functions (vmap, torch.func) are not supported");
     if (x.device() != with.device()) fail(std::string(name) + " must be on the device of " + of + " (" + with.device().str() + "), got " + x.device().str());
     if (x.scalar_type() != with.scalar_type())
         fail("expected scalar type " + dtype_text(with.scalar_type()) + " for " + name + " but found " + dtype_text(x.scalar_type()));

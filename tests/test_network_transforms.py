@@ -67,3 +67,11 @@ def test_second_derivatives_are_refused(gpu):
         leaf = torch.randn(3, 2, 8, device=gpu, requires_grad=True)
         with pytest.raises(RuntimeError, match="cannot be differentiated again"):
             torch.autograd.grad(call(leaf).sum(), leaf, create_graph=True)
+
+
+def test_tensors_that_are_not_dense_are_named_so(gpu):
+    x = torch.randn(3, 2, 8, device=gpu)
+    for call in (lambda: svox.attention(x, x.to_sparse(), x), lambda: svox.rotate_heads(x.to_sparse(), x, torch.zeros(3, device=gpu), torch.zeros(4, device=gpu)),
+                 lambda: svox.layer_norm(x.to_sparse()), lambda: svox.clip_norm([x.to_sparse()], 1.0)):
+        with pytest.raises(RuntimeError, match="dense"):
+            call()
