@@ -99,10 +99,11 @@ class _Attend(nn.Module):
 
     def forward(self, x, positions, frequencies, offsets):
         wide, narrow = self.heads * self.dim, self.kv_heads * self.dim
-        q, k, v = nn.functional.linear(self.norm(x), self.w_qkv).split([wide, narrow, narrow], dim=1)
         heads = lambda t: t.unflatten(1, (-1, self.dim))  # noqa: E731
-        q, k = rotate_heads(heads(q), heads(k), positions, frequencies, self.q_weight, self.k_weight)
-        return torch.addmm(x, attention(q, k, heads(v), offsets).flatten(1), self.w_out.t())
+        with torch.autocast(x.device.type, enabled=False):      # (a decoder is of its weights' type, whatever a caller has torch's products in)
+            q, k, v = nn.functional.linear(self.norm(x), self.w_qkv).split([wide, narrow, narrow], dim=1)
+            q, k = rotate_heads(heads(q), heads(k), positions, frequencies, self.q_weight, self.k_weight)
+            return torch.addmm(x, attention(q, k, heads(v), offsets).flatten(1), self.w_out.t())
 
 
 def _cell_centres(tree):

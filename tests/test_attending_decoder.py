@@ -67,3 +67,16 @@ def test_the_widest_heads_run(gpu):
     y = decoder(torch.randn(35, 256, device=gpu), torch.rand(35, 3, device=gpu))
     y.sum().backward()
     assert y.shape == (35, 28) and all(torch.isfinite(p.grad).all() for p in decoder.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [0, 2])
+def test_a_decoder_is_of_its_weights_type_under_autocast(gpu, heads):
+    decoder = svox.LeafDecoder(32, 28, hidden=64, device=gpu, heads=heads, window=10)
+    x, positions = torch.randn(35, 32, device=gpu), torch.rand(35, 3, device=gpu)
+    want = decoder(x, positions)
+    wanted = torch.autograd.grad(want.sum(), list(decoder.parameters()))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = decoder(x, positions)
+    assert got.dtype == torch.float32 and torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got.sum(), list(decoder.parameters())), wanted))
