@@ -78,3 +78,16 @@ def test_other_tensors_are_refused(gpu, name):
             unpack = lambda p: change(p[1]) if p[0] == i else p[1]  # noqa: E731
             with pytest.raises(RuntimeError, match="hook on saved tensors"):
                 gradients(call, inputs, pack, unpack)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_checkpoints_compute_the_same_again(gpu, name):
+    """Nothing is kept but the inputs; the operator runs again for its backward pass."""
+    from torch.utils.checkpoint import checkpoint
+
+    call, inputs = operators(torch.bfloat16)[name]
+    want = gradients(call, inputs, same, same)
+    leaves = [x.detach().requires_grad_() for x in inputs]
+    y = checkpoint(call, *leaves, use_reentrant=False)
+    grad = torch.randn(y.shape, generator=torch.Generator().manual_seed(1)).to(y.dtype).to(y.device)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, grad)))
